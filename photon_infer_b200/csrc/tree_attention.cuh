@@ -1,0 +1,78 @@
+// What the kernels of tree attention share: the sizes of a call, and which keys a node of a drafted tree sees.
+//
+// A request's nodes are its last tokens: with n nodes and a context of L tokens (the nodes counted), node i is key base + i, base =
+// L - n.  Node t sees the cached keys j < base with j > pos(t) - window, and the nodes i whose bit is set in its mask and whose
+// place on their path, pos(i), is within the window.  A bit at or behind n says nothing.
+#pragma once
+#include "common.cuh"
+
+struct TreeParams {
+  const void* q; long q_stride;                    // [T, n_q * d] view
+  void* out; long out_stride;                      // [T, n_q * d]
+  const void* k_cache; const void* v_cache;        // [num_pages, n_kv, page_size, d]
+  const int* block_table; int max_pages;           // [S, max_pages]
+  const int* cu_tokens;                            // [S + 1] first node of each request
+  const int* context_lens;                         // [S] keys of each request, its nodes counted
+  const int* positions;                            // [T]
+  const int* tree_mask; int mask_words;            // [T, mask_words]: bit i of a row: the node sees node i of its request
+  int S, T, max_tokens, n_q, n_kv, group, d, page_size, num_pages, window;
+  float scale;
+  const float* sinks;                              // [n_q] or null
+  float softcap;                                   // 0: off
+  int* err;
+};
+
+// The request's node range and first key that is a node, kept inside the call's arrays whatever the tables say.
+struct TreeRequest { int tok0, n, base; };
+__device__ __forceinline__ TreeRequest tree_request(const TreeParams& P, int s) {
+  TreeRequest r;
+  const int a = P.cu_tokens[s], b = P.cu_tokens[s + 1];
+  r.tok0 = max(0, min(a, P.T));
+  r.n = max(0, min(min(b, P.T) - r.tok0, P.max_tokens));
+  r.base = max(0, P.context_lens[s] - r.n);
+  return r;
+}
+
+// 32 keys from `key0` on, as bits: those that the node at row `t` of the step may see.  lo: first cached key inside its window.
+__device__ __forceinline__ uint32_t tree_visible32(const TreeParams& P, const TreeRequest& r, int t, int key0, int lo) {
+  const int i0 = key0 - r.base;                    // place of the first of them among the nodes
+  uint32_t bits = 0;
+  if (i0 < 0) {                                    // cached keys: lo <= key < base
+    const int past = min(32, -i0), skip = max(0, min(lo - key0, past));
+    bits = (past >= 32 ? 0xffffffffu : (1u << past) - 1u);
+    bits &= skip >= 32 ? 0u : (0xffffffffu << skip);
+  }
+  if (i0 > -32 && i0 < r.n) {                      // nodes
+    const int* row = P.tree_mask + (size_t)t * P.mask_words;
+    uint32_t m;
+    if (i0 < 0) {
+      m = (uint32_t)row[0] << (-i0);
+      if (r.n + (-i0) < 32) m &= (1u << (r.n - i0)) - 1u;
+    } else {
+      const int w = i0 >> 5, sh = i0 & 31;
+      const uint32_t a = w < P.mask_words ? (uint32_t)row[w] : 0u, b = w + 1 < P.mask_words ? (uint32_t)row[w + 1] : 0u;
+      m = __funnelshift_r(a, b, sh);
+      if (r.n - i0 < 32) m &= (1u << (r.n - i0)) - 1u;
+    }
+    if (P.window > 0) {
+      const int pos = P.positions[t];
+      for (uint32_t left = m; left != 0; left &= left - 1) {
+        const int u = __ffs(left) - 1;
+        if (P.positions[r.tok0 + i0 + u] <= pos - P.window) m &= ~(1u << u);
+      }
+    }
+    bits |= m;
+  }
+  return bits;
+}
+
+// The cache row (of d numbers) of a key, or -1 where its page is missing, which is recorded.
+__device__ __forceinline__ long long tree_row(const TreeParams& P, const int* table, int g, int key, int tok0) {
+  const int pidx = key / P.page_size;
+  const int page = pidx < P.max_pages ? table[pidx] : -1;
+  if (page < 0 || page >= P.num_pages) {
+    report_error(P.err, PHOTON_DEV_BAD_PAGE, tok0, key, page);
+    return -1;
+  }
+  return ((long long)page * P.n_kv + g) * P.page_size + (key - pidx * P.page_size);
+}

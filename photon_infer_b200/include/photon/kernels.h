@@ -564,6 +564,37 @@ PHOTON_EXPORT int photon_gemm_tc2_qkv(const void* x, long ldx, const void* W, lo
                         int table_positions, void* k_cache, void* v_cache, int n_q, int n_kv, int d, int page_size,
                         long num_slots, int* err, cudaStream_t stream);
 
+/* ------------------------------------------------------------------ tree_attention.cu: trees of drafted tokens over the paged cache */
+/* The nodes of request s are its tokens cu_tokens[s] .. cu_tokens[s + 1] - 1 of the step and the last of its context_lens[s] keys.  Node t sees
+ * the keys before the nodes (with a window those at positions > positions[t] - window) and the nodes i of its request whose bit i is set in
+ * tree_mask[t][0 .. mask_words - 1] (within the window as well); positions[t]: its place on its path.  A row that sees no key is zero.
+ * sinks (float [n_q], may be null), softcap (0: off): as in photon_paged_attention_ex.  d <= 256.  splits > 1 shares a request's keys out over that
+ * many blocks: part_o float [T * n_q * splits * d], part_ml float [T * n_q * splits * 2]. */
+PHOTON_EXPORT int photon_tree_attention(const void* q, long q_stride, void* out, long out_stride, int dtype, const void* k_cache,
+                          const void* v_cache, const int* block_table, int max_pages, const int* cu_tokens,
+                          const int* context_lens, const int* positions, const int* tree_mask, int mask_words, int S, int T,
+                          int max_tokens_per_seq, int n_q, int n_kv, int d, int page_size, int num_pages, int window,
+                          float scale, const float* sinks, float softcap, int splits, float* part_o, float* part_ml,
+                          int* err, cudaStream_t stream);
+
+/* ------------------------------------------------------------------ tree_accept.cu */
+/* From node 0 of each request on: the token that the node's logits (float [T, V], row stride ld) give, greedily or with temperature[s] > 0 by
+ * uniforms[t] as photon_sample does, then the first child (parents [T]: indices into the request's nodes, below the node's own; -1 for node 0) with that
+ * token.  path, sampled [S, D]: the nodes gone through and the tokens they gave, -1 behind the last; counts [S].  Stops after D nodes. */
+PHOTON_EXPORT int photon_tree_accept(const float* logits, long ld, const int* tokens, const int* parents, const int* cu_tokens, int S, int T,
+                       int max_tokens_per_seq, int V, const float* temperature, const float* uniforms, int* path, int* counts,
+                       int* sampled, int D, cudaStream_t stream);
+
+/* ------------------------------------------------------------------ cache_rows.cu */
+/* kv [planes][num_pages][n_kv][page_size][d].  Key base + path[s][j] of request s goes to key base + j for 0 < j < counts[s], base = context_lens[s]
+ * minus the request's nodes; paths ascend. */
+PHOTON_EXPORT int photon_cache_keep(void* kv, int dtype, int planes, int num_pages, int n_kv, int page_size, int d, const int* block_table,
+                      int max_pages, const int* cu_tokens, const int* context_lens, const int* path, const int* counts, int S,
+                      int D, int* err, cudaStream_t stream);
+/* kv [planes][num_pages][page_elems]: page pairs[i][0] onto page pairs[i][1] in every plane.  No page is written twice, or both read and written. */
+PHOTON_EXPORT int photon_cache_copy_pages(void* kv, int dtype, int planes, int num_pages, long page_elems, const int* pairs, int count, int* err,
+                            cudaStream_t stream);
+
 /* ------------------------------------------------------------------ sampling.cu */
 /* Per row: first maximum where temperature is null or <= 0, else the first index whose running sum of
  * softmax(logits / temperature) reaches u.  scratch: float [rows * 128] for V > 16384, else may be null. */

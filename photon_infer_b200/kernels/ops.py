@@ -2519,6 +2519,139 @@ def moe_gemv(x: torch.Tensor, x_div: int, ids: torch.Tensor, weight: torch.Tenso
              int(glu), act, _ptr(weights), float(limit), float(slope), _stream()), "moe_gemv")
 
 
+# ----------------------------------------------------------------------------- trees of drafted tokens
+
+def _check_step(what: str, num_seqs: int, cu_tokens: torch.Tensor, context_lens: Optional[torch.Tensor], block_table: Optional[torch.Tensor]) -> None:
+    _int32(cu_tokens, "cu_tokens")
+    covered = cu_tokens.numel() > num_seqs
+    if context_lens is not None:
+        _int32(context_lens, "context_lens")
+        covered = covered and context_lens.numel() >= num_seqs
+    if block_table is not None:
+        _int32(block_table, "block_table")
+        covered = covered and block_table.dim() == 2 and block_table.shape[0] >= num_seqs and block_table.shape[1] > 0
+    if num_seqs < 0 or not covered:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: cu_tokens, context_lens and block_table must cover every request")
+
+
+def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
+                   cu_tokens: torch.Tensor, context_lens: torch.Tensor, positions: torch.Tensor, tree_mask: torch.Tensor, num_seqs: int,
+                   max_tokens_per_seq: int, max_keys: int, n_q: int, n_kv: int, head_dim: int, window: Optional[int], scale: float,
+                   err: Optional[torch.Tensor], sink: Optional[torch.Tensor] = None, softcap: Optional[float] = None) -> None:
+    """Attention of the nodes of drafted trees over the paged cache.  The tokens ``cu_tokens[s] .. cu_tokens[s + 1]`` of the step are the
+    nodes of request ``s`` (at most ``max_tokens_per_seq``) and the last of its ``context_lens[s]`` keys (at most ``max_keys``): node ``i``
+    is stored behind the request's cached tokens at ``base + i``.  A node sees the cached tokens, and the nodes ``i`` whose bit is set in its row of
+    ``tree_mask`` (int32 ``[T, words]``, bit ``i % 32`` of word ``i // 32``: itself and what it descends from).  ``positions [T]``: its place on its path
+    (``base`` plus its depth); with a ``window`` it sees what lies at positions ``> positions[t] - window``.  A row that sees nothing is zero.
+    ``q [T, n_q * d]`` may be a view with a row stride; ``sink``, ``softcap``: as in ``paged_attention``."""
+    _check_sink(sink, n_q)
+    _cuda(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, positions, tree_mask, err)
+    T = q.shape[0]
+    if q.dim() != 2 or q.shape[1] != n_q * head_dim or q.stride(1) != 1 or out.shape != q.shape or out.stride(1) != 1:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: q and out must be [T, n_q * head_dim] with contiguous rows")
+    if out.dtype != q.dtype or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
+        raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: q, out and the caches must share one dtype")
+    if n_kv <= 0 or n_q % n_kv or not 1 <= head_dim <= 256:
+        raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, f"tree_attention: {n_q}/{n_kv} heads of {head_dim} are not supported (up to 256 numbers)")
+    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != n_kv or k_cache.shape[3] != head_dim \
+            or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: the caches must be contiguous [pages, n_kv, page_size, head_dim]")
+    _check_step("tree_attention", num_seqs, cu_tokens, context_lens, block_table)
+    _int32(positions, "positions")
+    _int32(tree_mask, "tree_mask")
+    if positions.numel() < T or tree_mask.dim() != 2 or tree_mask.shape[0] < T or tree_mask.shape[1] * 32 < max_tokens_per_seq:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: positions [T] and tree_mask [T, words] with a bit for every node")
+    if not scale > 0 or (softcap is not None and softcap < 0) or (window is not None and window < 0):
+        raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: the scale must be positive, softcap and window not negative")
+    keys = max_keys if not window else min(max_keys, window + max_tokens_per_seq)
+    splits = _tree_splits(num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv), keys, sm_count(q.device))
+    part = torch.empty(T * n_q * splits * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
+    f = _fn("tree_attention", "photon_tree_attention",
+            [c_void_p, c_long, c_void_p, c_long, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
+             c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
+    _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _dtype_code(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[1],
+             _ptr(cu_tokens), _ptr(context_lens), _ptr(positions), _ptr(tree_mask), tree_mask.shape[1], int(num_seqs), T,
+             int(max_tokens_per_seq), n_q, n_kv, head_dim, k_cache.shape[2], k_cache.shape[0], int(window or 0), float(scale), _ptr(sink),
+             float(softcap or 0.0), splits, _ptr(part), _ptr(part[T * n_q * splits * head_dim:] if splits > 1 else None), _ptr(err),
+             _stream()), "tree_attention")
+    if splits > 1:
+        global _launch_count
+        _launch_count += 1
+
+
+def _tree_splits(num_seqs: int, n_kv: int, rows: int, keys: int, sms: int) -> int:
+    """Shares of a request's keys for the general kernel: about four blocks an SM, none with less than two tiles of 32 keys."""
+    blocks = max(1, num_seqs * n_kv * -(-rows // 32))
+    return max(1, min(4 * sms // blocks, keys // 64, 64))
+
+
+def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Tensor, num_seqs: int,
+                max_tokens_per_seq: int, path: torch.Tensor, counts: torch.Tensor, sampled: torch.Tensor,
+                temperature: Optional[torch.Tensor] = None, uniforms: Optional[torch.Tensor] = None,
+                err: Optional[torch.Tensor] = None) -> None:
+    """The drafted tokens that each request keeps.  From node 0 (the request's last token) on: the token that the node's row of ``logits``
+    (float32 ``[T, V]``) gives, as ``sample`` gives it with ``temperature[s]`` and ``uniforms[t]`` (greedily without them), then the first
+    child with that token.  ``tokens``, ``parents`` (int32 ``[T]``): each node's token and its parent among the request's nodes, an earlier one; -1 for
+    node 0.  ``path``, ``sampled`` (int32 ``[S, D]``): the nodes gone through and the tokens they gave, -1 behind the last of ``counts [S]``; the walk
+    ends after ``D`` nodes."""
+    _cuda(logits, tokens, parents, cu_tokens, path, counts, sampled, temperature, uniforms, err)
+    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or logits.shape[1] < 1:
+        raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_accept: logits must be float32 [T, V] with unit inner stride")
+    T, V = logits.shape
+    for name, t in (("tokens", tokens), ("parents", parents), ("path", path), ("counts", counts), ("sampled", sampled)):
+        _int32(t, name)
+    _check_step("tree_accept", num_seqs, cu_tokens, None, None)
+    if tokens.numel() < T or parents.numel() < T:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_accept: tokens and parents must have one entry per row of logits")
+    if path.dim() != 2 or path.shape[0] < num_seqs or path.shape[1] < 1 or sampled.shape != path.shape or counts.numel() < num_seqs:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_accept: path and sampled must be [requests, depth], counts [requests]")
+    if temperature is not None and (uniforms is None or any(t.dtype != torch.float32 or not t.is_contiguous() for t in (temperature, uniforms))
+                                    or temperature.numel() < num_seqs or uniforms.numel() < T):
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_accept: temperature [requests] and uniforms [T] must be contiguous float32")
+    f = _fn("tree_accept", "photon_tree_accept",
+            [c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
+             c_void_p])
+    _check(f(_ptr(logits), logits.stride(0), _ptr(tokens), _ptr(parents), _ptr(cu_tokens), int(num_seqs), T, int(max_tokens_per_seq), V,
+             _ptr(temperature), _ptr(uniforms), _ptr(path), _ptr(counts), _ptr(sampled), path.shape[1], _stream()), "tree_accept")
+
+
+def _check_pool(what: str, kv: torch.Tensor) -> int:
+    if kv.dim() != 6 or not kv.is_contiguous() or kv.numel() == 0:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: the pools must be contiguous [entries, planes, pages, n_kv, page_size, d]")
+    return kv.shape[0] * kv.shape[1]
+
+
+def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Tensor, context_lens: torch.Tensor, path: torch.Tensor,
+               counts: torch.Tensor, num_seqs: int, err: Optional[torch.Tensor]) -> None:
+    """The accepted nodes' rows move behind the request's cached tokens, in every entry and plane of a cache group's pools ``kv [entries,
+    planes, pages, n_kv, page_size, d]``: key ``base + path[s, j]`` of request ``s`` goes to key ``base + j`` for ``0 < j < counts[s]``, with ``base =
+    context_lens[s]`` minus the request's nodes of the step.  ``path`` and ``counts`` as ``tree_accept`` leaves them (paths ascend)."""
+    _cuda(kv, block_table, cu_tokens, context_lens, path, counts, err)
+    planes = _check_pool("cache_keep", kv)
+    _check_step("cache_keep", num_seqs, cu_tokens, context_lens, block_table)
+    _int32(path, "path")
+    _int32(counts, "counts")
+    if path.dim() != 2 or path.shape[0] < num_seqs or counts.numel() < num_seqs:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_keep: path must be [requests, depth], counts [requests]")
+    f = _fn("cache_rows", "photon_cache_keep",
+            [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p])
+    _check(f(_ptr(kv), _dtype_code(kv), planes, kv.shape[2], kv.shape[3], kv.shape[4], kv.shape[5], _ptr(block_table), block_table.shape[1],
+             _ptr(cu_tokens), _ptr(context_lens), _ptr(path), _ptr(counts), int(num_seqs), path.shape[1], _ptr(err), _stream()), "cache_keep")
+
+
+def cache_copy_pages(kv: torch.Tensor, pairs: torch.Tensor, err: Optional[torch.Tensor]) -> None:
+    """Page ``pairs[i, 0]`` onto page ``pairs[i, 1]`` (int32 ``[N, 2]``) in every entry and plane of a cache group's pools ``kv [entries, planes,
+    pages, n_kv, page_size, d]``.  No page may be written twice, or be both read and written.  A page outside the pool is left out and recorded in ``err``."""
+    _cuda(kv, pairs, err)
+    planes = _check_pool("cache_copy_pages", kv)
+    _int32(pairs, "pairs")
+    if pairs.dim() != 2 or pairs.shape[1] != 2:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_copy_pages: pairs must be [pages, 2]")
+    f = _fn("cache_rows", "photon_cache_copy_pages", [c_void_p, c_int, c_int, c_int, c_long, c_void_p, c_int, c_void_p, c_void_p])
+    _check(f(_ptr(kv), _dtype_code(kv), planes, kv.shape[2], kv.shape[3] * kv.shape[4] * kv.shape[5], _ptr(pairs), pairs.shape[0], _ptr(err),
+             _stream()), "cache_copy_pages")
+
+
 # ----------------------------------------------------------------------------- sampling
 
 def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor], u: Optional[torch.Tensor],
