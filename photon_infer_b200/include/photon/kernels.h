@@ -577,6 +577,17 @@ PHOTON_EXPORT int photon_tree_attention(const void* q, long q_stride, void* out,
                           float scale, const float* sinks, float softcap, int splits, float* part_o, float* part_ml,
                           int* err, cudaStream_t stream);
 
+/* ------------------------------------------------------------------ tree_attention_tc.cu: the same on tcgen05, bfloat16, d 64 or 128 */
+/* At most 128 query heads per key/value head, pages of 8, 16, 32 or a multiple of 64 tokens, 16-byte aligned rows; positions[t] = the request's cached
+ * tokens plus the node's depth.  blocks: the grid, at most as many as the chip holds at once.  scratch: as many floats as the function before says. */
+PHOTON_EXPORT long photon_tree_attention_tc_scratch(int max_tokens_per_seq, int n_q, int n_kv, int d, int blocks);
+PHOTON_EXPORT int photon_tree_attention_tc(const void* q, long q_stride, void* out, long out_stride, const void* k_cache, const void* v_cache,
+                             const int* block_table, int max_pages, const int* cu_tokens, const int* context_lens,
+                             const int* positions, const int* tree_mask, int mask_words, int S, int T, int max_tokens_per_seq,
+                             int n_q, int n_kv, int d, int page_size, int num_pages, int window, float scale,
+                             const float* sinks, float softcap, int blocks, float* scratch, long scratch_floats, int* err,
+                             cudaStream_t stream);
+
 /* ------------------------------------------------------------------ tree_accept.cu */
 /* From node 0 of each request on: the token that the node's logits (float [T, V], row stride ld) give, greedily or with temperature[s] > 0 by
  * uniforms[t] as photon_sample does, then the first child (parents [T]: indices into the request's nodes, below the node's own; -1 for node 0) with that

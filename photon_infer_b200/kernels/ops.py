@@ -2564,7 +2564,23 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     if not scale > 0 or (softcap is not None and softcap < 0) or (window is not None and window < 0):
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: the scale must be positive, softcap and window not negative")
     keys = max_keys if not window else min(max_keys, window + max_tokens_per_seq)
-    splits = _tree_splits(num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv), keys, sm_count(q.device))
+    group = n_q // n_kv
+    if tree_attention_tc_supported(q, out, k_cache, v_cache, group):
+        tile_rows = 128 // group * group
+        units = num_seqs * n_kv * -(-max_tokens_per_seq * group // (2 * tile_rows))
+        blocks = max(1, min(sm_count(q.device), units * (-(-keys // 128) + 1)))
+        rows = min(-(-max_tokens_per_seq * group // 32) * 32, -(-2 * tile_rows // 32) * 32)
+        scratch = torch.empty(2 * blocks * rows * (head_dim + 2), dtype=torch.float32, device=q.device)
+        f = _fn("tree_attention_tc", "photon_tree_attention_tc",
+                [c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
+                 c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_float, c_int, c_void_p, c_long, c_void_p, c_void_p])
+        _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[1],
+                 _ptr(cu_tokens), _ptr(context_lens), _ptr(positions), _ptr(tree_mask), tree_mask.shape[1], int(num_seqs), T,
+                 int(max_tokens_per_seq), n_q, n_kv, head_dim, k_cache.shape[2], k_cache.shape[0], int(window or 0), float(scale), _ptr(sink),
+                 float(softcap or 0.0), blocks, _ptr(scratch), scratch.numel(), _ptr(err), _stream()), "tree_attention")
+        _count_launches(1)
+        return
+    splits = _tree_splits(num_seqs, n_kv, max_tokens_per_seq * group, keys, sm_count(q.device))
     part = torch.empty(T * n_q * splits * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
     f = _fn("tree_attention", "photon_tree_attention",
             [c_void_p, c_long, c_void_p, c_long, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
@@ -2575,8 +2591,23 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
              float(softcap or 0.0), splits, _ptr(part), _ptr(part[T * n_q * splits * head_dim:] if splits > 1 else None), _ptr(err),
              _stream()), "tree_attention")
     if splits > 1:
-        global _launch_count
-        _launch_count += 1
+        _count_launches(1)
+
+
+def _count_launches(n: int) -> None:
+    """Kernels that an entry point launched beside the one that ``_check`` counts."""
+    global _launch_count
+    _launch_count += n
+
+
+def tree_attention_tc_supported(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, group: int) -> bool:
+    """Whether the tcgen05 kernel takes the call: bfloat16, heads of 64 or 128, up to 128 of them per key/value head, pages of 8, 16, 32 or a
+    multiple of 64 tokens, rows and caches that TMA can read."""
+    pages, n_kv, page_size, d = k_cache.shape
+    return (q.dtype == torch.bfloat16 and d in (64, 128) and group <= 128
+            and page_size % 8 == 0 and (64 % page_size == 0 or page_size % 64 == 0)
+            and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and pages * n_kv * page_size <= 0x7fffff00
+            and all(t.data_ptr() % 16 == 0 for t in (q, out, k_cache, v_cache)))
 
 
 def _tree_splits(num_seqs: int, n_kv: int, rows: int, keys: int, sms: int) -> int:
