@@ -31,7 +31,7 @@ BASE_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-shared", "-Xcompiler", "-fPIC"
               "-Xcompiler", "-fvisibility=hidden"]
 ALL_MODULES = ("elementwise", "rope_kv", "qk_norm", "attention", "attention_rows", "latent", "hyper", "gla", "delta", "delta_chunked", "attention_talk", "attention_diff", "linrec", "linrec_segments", "linrec_chunks", "row_norms", "moe", "gemm_f32", "gemm_f32_tc", "gemm_skinny", "gemm_skinny_fused",
                "gemm_skinny_static",
-               "gemm_tc", "gemm_tc2", "sampling", "tree_attention", "tree_attention_tc", "tree_accept", "cache_rows")
+               "gemm_tc", "gemm_tc2", "sampling", "tree_attention", "tree_attention_tc", "tree_attention_few", "tree_accept", "cache_rows")
 
 _loaded: Dict[Tuple[str, Tuple[Tuple[str, str], ...]], ctypes.CDLL] = {}
 _lock = threading.Lock()

@@ -245,38 +245,29 @@ tree_join_kernel(const TreeParams P, const TreeShares H) {
 template <typename T, int D>
 static int tree_launch(const TreeParams& P, const TreeShares& H, long blocks, cudaStream_t stream) {
   const size_t smem = (size_t)(TG_ROWS * (D + 4) + TG_KEYS * (D + 4) + TG_KEYS * D + TG_ROWS * TG_PS) * sizeof(float);
-  cudaError_t e = cudaFuncSetAttribute(tree_attention_kernel<T, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-  if (e != cudaSuccess) return (int)e;
+  static bool ready[64] = {};                      // the limit is set once a device
+  const int set = tree_smem_limit((const void*)tree_attention_kernel<T, D>, (int)smem, ready);
+  if (set != 0) return set;
   int st = launch_pdl(tree_attention_kernel<T, D>, dim3((unsigned)blocks), dim3(TG_THREADS), smem, stream, P, H);
   if (st != 0 || H.splits == 1) return st;
   return launch_pdl(tree_join_kernel<T>, dim3((unsigned)(((long)P.T * P.n_q + 3) / 4)), dim3(128), 0, stream, P, H);
 }
 
-PHOTON_API int photon_tree_attention(const void* q, long q_stride, void* out, long out_stride, int dtype, const void* k_cache,
-                                     const void* v_cache, const int* block_table, int max_pages, const int* cu_tokens,
-                                     const int* context_lens, const int* positions, const int* tree_mask, int mask_words, int S, int T,
-                                     int max_tokens_per_seq, int n_q, int n_kv, int d, int page_size, int num_pages, int window,
-                                     float scale, const float* sinks, float softcap, int splits, float* part_o, float* part_ml,
-                                     int* err, cudaStream_t stream) {
-  if (S <= 0 || T <= 0 || max_tokens_per_seq <= 0) return 0;
-  if (softcap < 0.f || splits < 1 || mask_words < 1 || page_size <= 0 || num_pages <= 0 || max_pages <= 0) return PHOTON_ERR_ARGUMENT;
-  if (dtype != PHOTON_F32 && dtype != PHOTON_BF16) return PHOTON_ERR_ARGUMENT;
-  if (n_kv <= 0 || n_q <= 0 || n_q % n_kv || d <= 0 || d > 256 || !(scale > 0.f)) return PHOTON_ERR_UNSUPPORTED;
-  if (splits > 1 && (part_o == nullptr || part_ml == nullptr)) return PHOTON_ERR_ARGUMENT;
+PHOTON_API int photon_tree_attention(const photon_tree_call* call, cudaStream_t stream) {
+  if (call->S <= 0 || call->T <= 0 || call->max_tokens_per_seq <= 0) return 0;
   TreeParams P;
-  P.q = q; P.q_stride = q_stride; P.out = out; P.out_stride = out_stride; P.k_cache = k_cache; P.v_cache = v_cache;
-  P.block_table = block_table; P.max_pages = max_pages; P.cu_tokens = cu_tokens; P.context_lens = context_lens;
-  P.positions = positions; P.tree_mask = tree_mask; P.mask_words = mask_words; P.S = S; P.T = T; P.max_tokens = max_tokens_per_seq;
-  P.n_q = n_q; P.n_kv = n_kv; P.group = n_q / n_kv; P.d = d; P.page_size = page_size; P.num_pages = num_pages;
-  P.window = window > 0 ? window : 0; P.scale = scale; P.sinks = sinks; P.softcap = softcap; P.err = err;
+  const int st = tree_params(call, P);
+  if (st != 0) return st;
+  const long rows = (long)P.T * P.n_q * call->parts;
+  if (call->parts > 1 && (call->scratch == nullptr || call->scratch_floats < rows * (P.d + 2))) return PHOTON_ERR_ARGUMENT;
   TreeShares H;
-  H.part_o = part_o; H.part_ml = part_ml; H.splits = splits;
-  H.row_tiles = (int)(((long)max_tokens_per_seq * P.group + TG_ROWS - 1) / TG_ROWS);
-  const long blocks = (long)S * H.row_tiles * n_kv * splits;
+  H.part_o = call->scratch; H.part_ml = call->scratch + rows * P.d; H.splits = call->parts;
+  H.row_tiles = (int)(((long)P.max_tokens * P.group + TG_ROWS - 1) / TG_ROWS);
+  const long blocks = (long)P.S * H.row_tiles * P.n_kv * H.splits;
   if (blocks > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
-  if (dtype == PHOTON_F32)
-    return d <= 64 ? tree_launch<float, 64>(P, H, blocks, stream) : d <= 128 ? tree_launch<float, 128>(P, H, blocks, stream)
-                                                                              : tree_launch<float, 256>(P, H, blocks, stream);
-  return d <= 64 ? tree_launch<bf16, 64>(P, H, blocks, stream) : d <= 128 ? tree_launch<bf16, 128>(P, H, blocks, stream)
-                                                                          : tree_launch<bf16, 256>(P, H, blocks, stream);
+  if (call->dtype == PHOTON_F32)
+    return P.d <= 64 ? tree_launch<float, 64>(P, H, blocks, stream) : P.d <= 128 ? tree_launch<float, 128>(P, H, blocks, stream)
+                                                                                : tree_launch<float, 256>(P, H, blocks, stream);
+  return P.d <= 64 ? tree_launch<bf16, 64>(P, H, blocks, stream) : P.d <= 128 ? tree_launch<bf16, 128>(P, H, blocks, stream)
+                                                                              : tree_launch<bf16, 256>(P, H, blocks, stream);
 }

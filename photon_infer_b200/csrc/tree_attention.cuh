@@ -76,3 +76,27 @@ __device__ __forceinline__ long long tree_row(const TreeParams& P, const int* ta
   }
   return ((long long)page * P.n_kv + g) * P.page_size + (key - pidx * P.page_size);
 }
+
+// Dynamic shared memory of a kernel, asked for once a device.
+static int tree_smem_limit(const void* kernel, int bytes, bool (&ready)[64]) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e == cudaSuccess && (dev < 0 || dev >= 64 || !ready[dev])) {
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess && dev >= 0 && dev < 64) ready[dev] = true;
+  }
+  return (int)e;
+}
+
+// The call's arguments as the kernels take them; 0 or the error that refuses them.
+static int tree_params(const photon_tree_call* c, TreeParams& P) {
+  if (c->softcap < 0.f || c->mask_words < 1 || c->page_size <= 0 || c->num_pages <= 0 || c->max_pages <= 0 || c->parts < 1) return PHOTON_ERR_ARGUMENT;
+  if (c->dtype != PHOTON_F32 && c->dtype != PHOTON_BF16) return PHOTON_ERR_ARGUMENT;
+  if (c->n_kv <= 0 || c->n_q <= 0 || c->n_q % c->n_kv || c->d <= 0 || c->d > 256 || !(c->scale > 0.f)) return PHOTON_ERR_UNSUPPORTED;
+  P.q = c->q; P.q_stride = c->q_stride; P.out = c->out; P.out_stride = c->out_stride; P.k_cache = c->k_cache; P.v_cache = c->v_cache;
+  P.block_table = c->block_table; P.max_pages = c->max_pages; P.cu_tokens = c->cu_tokens; P.context_lens = c->context_lens;
+  P.positions = c->positions; P.tree_mask = c->tree_mask; P.mask_words = c->mask_words; P.S = c->S; P.T = c->T; P.max_tokens = c->max_tokens_per_seq;
+  P.n_q = c->n_q; P.n_kv = c->n_kv; P.group = c->n_q / c->n_kv; P.d = c->d; P.page_size = c->page_size; P.num_pages = c->num_pages;
+  P.window = c->window > 0 ? c->window : 0; P.scale = c->scale; P.sinks = c->sinks; P.softcap = c->softcap; P.err = c->err;
+  return 0;
+}

@@ -619,9 +619,10 @@ tree_join_tc_kernel(const TtParams P, int blocks, int chunks) {
 
 template <int D>
 static int tt_launch(TtParams& P, const CUtensorMap& mq, const CUtensorMap& mk, const CUtensorMap& mv, int blocks, int chunks, cudaStream_t stream) {
-  cudaError_t e = cudaFuncSetAttribute(tree_attention_tc_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tt<D>::SMEM);
-  if (e != cudaSuccess) return (int)e;
-  int st = launch_pdl(tree_attention_tc_kernel<D>, dim3(blocks), dim3(TT_THREADS), (size_t)Tt<D>::SMEM, stream, mq, mk, mv, P);
+  static bool ready[64] = {};                      // the limit is set once a device
+  int st = tree_smem_limit((const void*)tree_attention_tc_kernel<D>, Tt<D>::SMEM, ready);
+  if (st != 0) return st;
+  st = launch_pdl(tree_attention_tc_kernel<D>, dim3(blocks), dim3(TT_THREADS), (size_t)Tt<D>::SMEM, stream, mq, mk, mv, P);
   if (st != 0) return st;
   return launch_pdl(tree_join_tc_kernel<D>, dim3((unsigned)((long)P.t.S * P.t.n_kv * chunks)), dim3(256), 0, stream, P, blocks, chunks);
 }
@@ -636,59 +637,51 @@ PHOTON_API long photon_tree_attention_tc_scratch(int max_tokens_per_seq, int n_q
   return 2L * blocks * tt_part_rows(max_tokens_per_seq, n_q / n_kv) * (d + 2);
 }
 
-PHOTON_API int photon_tree_attention_tc(const void* q, long q_stride, void* out, long out_stride, const void* k_cache, const void* v_cache,
-                                        const int* block_table, int max_pages, const int* cu_tokens, const int* context_lens,
-                                        const int* positions, const int* tree_mask, int mask_words, int S, int T, int max_tokens_per_seq,
-                                        int n_q, int n_kv, int d, int page_size, int num_pages, int window, float scale,
-                                        const float* sinks, float softcap, int blocks, float* scratch, long scratch_floats, int* err,
-                                        cudaStream_t stream) {
-  if (S <= 0 || T <= 0 || max_tokens_per_seq <= 0) return 0;
-  if (softcap < 0.f || mask_words < 1 || num_pages <= 0 || max_pages <= 0 || blocks < 1) return PHOTON_ERR_ARGUMENT;
-  if ((d != 64 && d != 128) || n_kv <= 0 || n_q <= 0 || n_q % n_kv || n_q / n_kv > 128 || !(scale > 0.f)) return PHOTON_ERR_UNSUPPORTED;
+PHOTON_API int photon_tree_attention_tc(const photon_tree_call* call, cudaStream_t stream) {
+  if (call->S <= 0 || call->T <= 0 || call->max_tokens_per_seq <= 0) return 0;
+  TtParams P;
+  TreeParams& t = P.t;
+  int st = tree_params(call, t);
+  if (st != 0) return st;
+  const int G = t.group, d = t.d, page_size = t.page_size;
+  if (call->dtype != PHOTON_BF16 || (d != 64 && d != 128) || G > 128) return PHOTON_ERR_UNSUPPORTED;
   if (page_size < 8 || (page_size & 7) || !((64 % page_size) == 0 || (page_size % 64) == 0)) return PHOTON_ERR_UNSUPPORTED;
-  if (((uintptr_t)q & 15) || (q_stride & 7) || ((uintptr_t)k_cache & 15) || ((uintptr_t)v_cache & 15) || ((uintptr_t)out & 15) || (out_stride & 7))
+  if (((uintptr_t)t.q & 15) || (t.q_stride & 7) || ((uintptr_t)t.k_cache & 15) || ((uintptr_t)t.v_cache & 15) || ((uintptr_t)t.out & 15) || (t.out_stride & 7))
     return PHOTON_ERR_UNSUPPORTED;
-  const long total_rows = (long)num_pages * n_kv * page_size;
+  const long total_rows = (long)t.num_pages * t.n_kv * page_size;
   if (total_rows > 0x7fffff00L) return PHOTON_ERR_UNSUPPORTED;
-  const int G = n_q / n_kv;
-  if (scratch == nullptr || scratch_floats < photon_tree_attention_tc_scratch(max_tokens_per_seq, n_q, n_kv, d, blocks)) return PHOTON_ERR_ARGUMENT;
+  if (call->scratch == nullptr || call->scratch_floats < photon_tree_attention_tc_scratch(t.max_tokens, t.n_q, t.n_kv, d, call->parts)) return PHOTON_ERR_ARGUMENT;
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return PHOTON_ERR_UNSUPPORTED;
-  TtParams P;
   P.tile_nodes = 128 / G; P.tile_rows = P.tile_nodes * G;
   P.box_rows = page_size < 64 ? page_size : (page_size % 128 == 0 ? 128 : 64);
   P.total_rows = (int)total_rows;
   CUtensorMap map_q, map_k, map_v;
   {
-    cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)n_q, (cuuint64_t)T};
-    cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)q_stride * 2};
+    cuuint64_t dims[3] = {(cuuint64_t)d, (cuuint64_t)t.n_q, (cuuint64_t)t.T};
+    cuuint64_t strides[2] = {(cuuint64_t)d * 2, (cuuint64_t)t.q_stride * 2};
     cuuint32_t box[3] = {64, (cuuint32_t)G, (cuuint32_t)P.tile_nodes};
     cuuint32_t estr[3] = {1, 1, 1};
-    CUresult r = fn(&map_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr,
+    CUresult r = fn(&map_q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(t.q), dims, strides, box, estr,
                     CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                     CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return PHOTON_ERR_ARGUMENT;
   }
-  int st = make_map(&map_k, k_cache, total_rows, d, d, P.box_rows);
+  st = make_map(&map_k, t.k_cache, total_rows, d, d, P.box_rows);
   if (st != 0) return st;
-  st = make_map(&map_v, v_cache, total_rows, d, d, P.box_rows);
+  st = make_map(&map_v, t.v_cache, total_rows, d, d, P.box_rows);
   if (st != 0) return st;
-  TreeParams& t = P.t;
-  t.q = q; t.q_stride = q_stride; t.out = out; t.out_stride = out_stride; t.k_cache = k_cache; t.v_cache = v_cache;
-  t.block_table = block_table; t.max_pages = max_pages; t.cu_tokens = cu_tokens; t.context_lens = context_lens;
-  t.positions = positions; t.tree_mask = tree_mask; t.mask_words = mask_words; t.S = S; t.T = T; t.max_tokens = max_tokens_per_seq;
-  t.n_q = n_q; t.n_kv = n_kv; t.group = G; t.d = d; t.page_size = page_size; t.num_pages = num_pages;
-  t.window = window > 0 ? window : 0; t.scale = scale; t.sinks = sinks; t.softcap = softcap; t.err = err;
   P.page_shift = -1;
   for (int sh = 0; sh < 20; ++sh) if ((1 << sh) == page_size) P.page_shift = sh;
-  P.scale_log2 = scale * TT_LOG2E; P.cap_in = 0.f;
-  if (softcap > 0.f) { P.cap_in = scale / softcap; P.scale_log2 = TT_LOG2E; }
-  P.part_rows = tt_part_rows(max_tokens_per_seq, G);
-  P.part_o = scratch;
-  P.part_ml = scratch + 2L * blocks * P.part_rows * d;
+  P.scale_log2 = t.scale * TT_LOG2E; P.cap_in = 0.f;
+  if (t.softcap > 0.f) { P.cap_in = t.scale / t.softcap; P.scale_log2 = TT_LOG2E; }
+  P.part_rows = tt_part_rows(t.max_tokens, G);
+  P.part_o = call->scratch;
+  P.part_ml = call->scratch + 2L * call->parts * P.part_rows * d;
   // 32 rows a block of the second kernel
-  const long most = (long)max_tokens_per_seq * G, span = 2L * P.tile_rows;
+  const long most = (long)t.max_tokens * G, span = 2L * P.tile_rows;
   const long chunks = most / span * ((span + 31) / 32) + (most % span + 31) / 32;
-  if ((long)S * n_kv * chunks > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
-  return d == 64 ? tt_launch<64>(P, map_q, map_k, map_v, blocks, (int)chunks, stream) : tt_launch<128>(P, map_q, map_k, map_v, blocks, (int)chunks, stream);
+  if ((long)t.S * t.n_kv * chunks > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
+  return d == 64 ? tt_launch<64>(P, map_q, map_k, map_v, call->parts, (int)chunks, stream)
+                 : tt_launch<128>(P, map_q, map_k, map_v, call->parts, (int)chunks, stream);
 }

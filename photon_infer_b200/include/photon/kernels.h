@@ -567,26 +567,31 @@ PHOTON_EXPORT int photon_gemm_tc2_qkv(const void* x, long ldx, const void* W, lo
 /* ------------------------------------------------------------------ tree_attention.cu: trees of drafted tokens over the paged cache */
 /* The nodes of request s are its tokens cu_tokens[s] .. cu_tokens[s + 1] - 1 of the step and the last of its context_lens[s] keys.  Node t sees
  * the keys before the nodes (with a window those at positions > positions[t] - window) and the nodes i of its request whose bit i is set in
- * tree_mask[t][0 .. mask_words - 1] (within the window as well); positions[t]: its place on its path.  A row that sees no key is zero.
- * sinks (float [n_q], may be null), softcap (0: off): as in photon_paged_attention_ex.  d <= 256.  splits > 1 shares a request's keys out over that
- * many blocks: part_o float [T * n_q * splits * d], part_ml float [T * n_q * splits * 2]. */
-PHOTON_EXPORT int photon_tree_attention(const void* q, long q_stride, void* out, long out_stride, int dtype, const void* k_cache,
-                          const void* v_cache, const int* block_table, int max_pages, const int* cu_tokens,
-                          const int* context_lens, const int* positions, const int* tree_mask, int mask_words, int S, int T,
-                          int max_tokens_per_seq, int n_q, int n_kv, int d, int page_size, int num_pages, int window,
-                          float scale, const float* sinks, float softcap, int splits, float* part_o, float* part_ml,
-                          int* err, cudaStream_t stream);
+ * tree_mask[t][0 .. mask_words - 1] (within the window as well); positions[t]: its place on its path, the cached tokens plus its depth.  A row that sees
+ * no key is zero.  The arguments come as one structure: a caller that launches every layer builds it in a microsecond. */
+typedef struct {
+  const void* q; void* out;             /* [T, n_q * d], rows q_stride and out_stride apart */
+  const void* k_cache; const void* v_cache;
+  const int* block_table; const int* cu_tokens; const int* context_lens; const int* positions; const int* tree_mask;
+  const float* sinks;                   /* [n_q] or null: as in photon_paged_attention_ex */
+  float* scratch; int* err;
+  long q_stride, out_stride, scratch_floats;
+  int dtype, max_pages, mask_words, S, T, max_tokens_per_seq, n_q, n_kv, d, page_size, num_pages, window;
+  int parts;                            /* tree_attention.cu: shares of a request's keys; tree_attention_tc.cu: blocks of the grid */
+  float scale, softcap;                 /* softcap 0: off */
+} photon_tree_call;
+/* Either type, d <= 256.  parts > 1: scratch of T * n_q * parts * (d + 2) floats. */
+PHOTON_EXPORT int photon_tree_attention(const photon_tree_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ tree_attention_tc.cu: the same on tcgen05, bfloat16, d 64 or 128 */
-/* At most 128 query heads per key/value head, pages of 8, 16, 32 or a multiple of 64 tokens, 16-byte aligned rows; positions[t] = the request's cached
- * tokens plus the node's depth.  blocks: the grid, at most as many as the chip holds at once.  scratch: as many floats as the function before says. */
+/* At most 128 query heads per key/value head, pages of 8, 16, 32 or a multiple of 64 tokens, 16-byte aligned rows.  parts: the grid, at most as many blocks
+ * as the chip holds at once; scratch: as many floats as the first function says. */
 PHOTON_EXPORT long photon_tree_attention_tc_scratch(int max_tokens_per_seq, int n_q, int n_kv, int d, int blocks);
-PHOTON_EXPORT int photon_tree_attention_tc(const void* q, long q_stride, void* out, long out_stride, const void* k_cache, const void* v_cache,
-                             const int* block_table, int max_pages, const int* cu_tokens, const int* context_lens,
-                             const int* positions, const int* tree_mask, int mask_words, int S, int T, int max_tokens_per_seq,
-                             int n_q, int n_kv, int d, int page_size, int num_pages, int window, float scale,
-                             const float* sinks, float softcap, int blocks, float* scratch, long scratch_floats, int* err,
-                             cudaStream_t stream);
+PHOTON_EXPORT int photon_tree_attention_tc(const photon_tree_call* call, cudaStream_t stream);
+
+/* ------------------------------------------------------------------ tree_attention_few.cu: the same for few rows, bfloat16, d 64 or 128 */
+/* max_tokens_per_seq * n_q / n_kv <= 64; 16-byte aligned rows and caches.  parts: blocks of a cluster that share a request's keys, 1, 2, 4 or 8; no scratch. */
+PHOTON_EXPORT int photon_tree_attention_few(const photon_tree_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ tree_accept.cu */
 /* From node 0 of each request on: the token that the node's logits (float [T, V], row stride ld) give, greedily or with temperature[s] > 0 by

@@ -10,7 +10,8 @@ from __future__ import annotations
 import ctypes
 import functools
 import os
-from ctypes import c_float, c_int, c_long, c_void_p
+import struct
+from ctypes import c_char_p, c_float, c_int, c_long, c_void_p
 from typing import Optional
 
 import torch
@@ -34,10 +35,10 @@ _sm_counts = {}
 
 def sm_count(device) -> int:
     """Streaming multiprocessors of ``device`` (asked once)."""
-    key = (device.type, device.index)
-    if key not in _sm_counts:
-        _sm_counts[key] = torch.cuda.get_device_properties(device).multi_processor_count
-    return _sm_counts[key]
+    n = _sm_counts.get(device)
+    if n is None:
+        n = _sm_counts[device] = torch.cuda.get_device_properties(device).multi_processor_count
+    return n
 
 
 def _dtype_code(t: torch.Tensor) -> int:
@@ -76,6 +77,16 @@ def _check(status: int, what: str) -> None:
 
 
 _sigs_done = set()
+_plain_fns = {}
+
+
+def _plain_fn(module: str, name: str, argtypes):
+    """``_fn`` of a module without definitions, looked up in one step: for entry points whose launches the host pays for."""
+    key = (load_module, module, name)
+    f = _plain_fns.get(key)
+    if f is None:
+        f = _plain_fns[key] = _fn(module, name, argtypes)
+    return f
 
 
 def _fn(module: str, name: str, argtypes, defines=None, restype=c_int):
@@ -2523,15 +2534,20 @@ def moe_gemv(x: torch.Tensor, x_div: int, ids: torch.Tensor, weight: torch.Tenso
 
 def _check_step(what: str, num_seqs: int, cu_tokens: torch.Tensor, context_lens: Optional[torch.Tensor], block_table: Optional[torch.Tensor]) -> None:
     _int32(cu_tokens, "cu_tokens")
-    covered = cu_tokens.numel() > num_seqs
+    covered = 0 <= num_seqs < cu_tokens.numel()
     if context_lens is not None:
         _int32(context_lens, "context_lens")
         covered = covered and context_lens.numel() >= num_seqs
     if block_table is not None:
         _int32(block_table, "block_table")
-        covered = covered and block_table.dim() == 2 and block_table.shape[0] >= num_seqs and block_table.shape[1] > 0
-    if num_seqs < 0 or not covered:
+        covered = covered and block_table.dim() == 2 and block_table.shape[0] >= num_seqs and block_table.numel() > 0
+    if not covered:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: cu_tokens, context_lens and block_table must cover every request")
+
+
+#: photon_tree_call: pointers, strides and the scratch's size, sizes, scale and bound
+_TREE_CALL = struct.Struct("15q13i2f4x")
+_CALL_ARGS = [c_char_p, c_void_p]
 
 
 def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor,
@@ -2544,54 +2560,49 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     ``tree_mask`` (int32 ``[T, words]``, bit ``i % 32`` of word ``i // 32``: itself and what it descends from).  ``positions [T]``: its place on its path
     (``base`` plus its depth); with a ``window`` it sees what lies at positions ``> positions[t] - window``.  A row that sees nothing is zero.
     ``q [T, n_q * d]`` may be a view with a row stride; ``sink``, ``softcap``: as in ``paged_attention``."""
-    _check_sink(sink, n_q)
     _cuda(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, positions, tree_mask, err)
-    T = q.shape[0]
-    if q.dim() != 2 or q.shape[1] != n_q * head_dim or q.stride(1) != 1 or out.shape != q.shape or out.stride(1) != 1:
-        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: q and out must be [T, n_q * head_dim] with contiguous rows")
-    if out.dtype != q.dtype or k_cache.dtype != q.dtype or v_cache.dtype != q.dtype:
-        raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: q, out and the caches must share one dtype")
-    if n_kv <= 0 or n_q % n_kv or not 1 <= head_dim <= 256:
+    if sink is not None:
+        _check_sink(sink, n_q)
+    if n_kv <= 0 or n_q <= 0 or n_q % n_kv or not 1 <= head_dim <= 256:
         raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, f"tree_attention: {n_q}/{n_kv} heads of {head_dim} are not supported (up to 256 numbers)")
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.shape[1] != n_kv or k_cache.shape[3] != head_dim \
-            or not k_cache.is_contiguous() or not v_cache.is_contiguous():
+    dtype, cache = q.dtype, k_cache.shape
+    if q.dim() != 2 or out.shape != q.shape or q.shape[1] != n_q * head_dim:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: q and out must be [T, n_q * head_dim]")
+    T, (q_stride, q_inner), (out_stride, out_inner) = q.shape[0], q.stride(), out.stride()
+    if (q_inner != 1 or out_inner != 1) and T:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: rows of q and out must be contiguous")
+    if out.dtype != dtype or k_cache.dtype != dtype or v_cache.dtype != dtype:
+        raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: q, out and the caches must share one dtype")
+    if len(cache) != 4 or v_cache.shape != cache or cache[1] != n_kv or cache[3] != head_dim or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: the caches must be contiguous [pages, n_kv, page_size, head_dim]")
     _check_step("tree_attention", num_seqs, cu_tokens, context_lens, block_table)
     _int32(positions, "positions")
     _int32(tree_mask, "tree_mask")
-    if positions.numel() < T or tree_mask.dim() != 2 or tree_mask.shape[0] < T or tree_mask.shape[1] * 32 < max_tokens_per_seq:
+    words = tree_mask.shape[1] if tree_mask.dim() == 2 else 0
+    if positions.numel() < T or tree_mask.numel() < T * words or words * 32 < max_tokens_per_seq or words < 1:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: positions [T] and tree_mask [T, words] with a bit for every node")
     if not scale > 0 or (softcap is not None and softcap < 0) or (window is not None and window < 0):
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: the scale must be positive, softcap and window not negative")
-    keys = max_keys if not window else min(max_keys, window + max_tokens_per_seq)
-    group = n_q // n_kv
-    if tree_attention_tc_supported(q, out, k_cache, v_cache, group):
-        tile_rows = 128 // group * group
-        units = num_seqs * n_kv * -(-max_tokens_per_seq * group // (2 * tile_rows))
-        blocks = max(1, min(sm_count(q.device), units * (-(-keys // 128) + 1)))
-        rows = min(-(-max_tokens_per_seq * group // 32) * 32, -(-2 * tile_rows // 32) * 32)
-        scratch = torch.empty(2 * blocks * rows * (head_dim + 2), dtype=torch.float32, device=q.device)
-        f = _fn("tree_attention_tc", "photon_tree_attention_tc",
-                [c_void_p, c_long, c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int,
-                 c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_float, c_int, c_void_p, c_long, c_void_p, c_void_p])
-        _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[1],
-                 _ptr(cu_tokens), _ptr(context_lens), _ptr(positions), _ptr(tree_mask), tree_mask.shape[1], int(num_seqs), T,
-                 int(max_tokens_per_seq), n_q, n_kv, head_dim, k_cache.shape[2], k_cache.shape[0], int(window or 0), float(scale), _ptr(sink),
-                 float(softcap or 0.0), blocks, _ptr(scratch), scratch.numel(), _ptr(err), _stream()), "tree_attention")
-        _count_launches(1)
-        return
-    splits = _tree_splits(num_seqs, n_kv, max_tokens_per_seq * group, keys, sm_count(q.device))
-    part = torch.empty(T * n_q * splits * (head_dim + 2), dtype=torch.float32, device=q.device) if splits > 1 else None
-    f = _fn("tree_attention", "photon_tree_attention",
-            [c_void_p, c_long, c_void_p, c_long, c_int, c_void_p, c_void_p, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int,
-             c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_float, c_int, c_void_p, c_void_p, c_void_p, c_void_p])
-    _check(f(_ptr(q), q.stride(0), _ptr(out), out.stride(0), _dtype_code(q), _ptr(k_cache), _ptr(v_cache), _ptr(block_table), block_table.shape[1],
-             _ptr(cu_tokens), _ptr(context_lens), _ptr(positions), _ptr(tree_mask), tree_mask.shape[1], int(num_seqs), T,
-             int(max_tokens_per_seq), n_q, n_kv, head_dim, k_cache.shape[2], k_cache.shape[0], int(window or 0), float(scale), _ptr(sink),
-             float(softcap or 0.0), splits, _ptr(part), _ptr(part[T * n_q * splits * head_dim:] if splits > 1 else None), _ptr(err),
-             _stream()), "tree_attention")
-    if splits > 1:
-        _count_launches(1)
+    pages, _, page_size, _ = cache
+    group, device = n_q // n_kv, q.device
+    keys = min(max_keys, window + max_tokens_per_seq) if window else max_keys
+    pointers = [t.data_ptr() for t in (q, out, k_cache, v_cache)]
+    aligned = q_stride % 8 == 0 and out_stride % 8 == 0 and not any(p % 16 for p in pointers)
+    name, parts = _tree_route(dtype, head_dim, group, page_size, pages * n_kv * page_size, aligned, num_seqs, n_kv, max_tokens_per_seq * group, keys,
+                              sm_count(device))
+    floats = 0
+    if name == "tree_attention_tc":
+        floats = 2 * parts * (-(-min(max_tokens_per_seq * group, 2 * (128 // group * group)) // 32) * 32) * (head_dim + 2)
+    elif name == "tree_attention" and parts > 1:
+        floats = T * n_q * parts * (head_dim + 2)
+    scratch = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
+    call = _TREE_CALL.pack(*pointers, block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), positions.data_ptr(),
+                           tree_mask.data_ptr(), sink.data_ptr() if sink is not None else 0, scratch.data_ptr() if floats else 0,
+                           err.data_ptr() if err is not None else 0, q_stride, out_stride, floats, _dtype_code(q), block_table.shape[1], words,
+                           num_seqs, T, max_tokens_per_seq, n_q, n_kv, head_dim, page_size, pages, min(window or 0, 0x7fffffff), parts, scale, softcap or 0.0)
+    _check(_plain_fn(name, "photon_" + name, _CALL_ARGS)(call, _stream()), "tree_attention")
+    if floats:
+        _count_launches(1)                      # the second kernel, which joins partial results
 
 
 def _count_launches(n: int) -> None:
@@ -2600,20 +2611,21 @@ def _count_launches(n: int) -> None:
     _launch_count += n
 
 
-def tree_attention_tc_supported(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, group: int) -> bool:
-    """Whether the tcgen05 kernel takes the call: bfloat16, heads of 64 or 128, up to 128 of them per key/value head, pages of 8, 16, 32 or a
-    multiple of 64 tokens, rows and caches that TMA can read."""
-    pages, n_kv, page_size, d = k_cache.shape
-    return (q.dtype == torch.bfloat16 and d in (64, 128) and group <= 128
-            and page_size % 8 == 0 and (64 % page_size == 0 or page_size % 64 == 0)
-            and q.stride(0) % 8 == 0 and out.stride(0) % 8 == 0 and pages * n_kv * page_size <= 0x7fffff00
-            and all(t.data_ptr() % 16 == 0 for t in (q, out, k_cache, v_cache)))
-
-
-def _tree_splits(num_seqs: int, n_kv: int, rows: int, keys: int, sms: int) -> int:
-    """Shares of a request's keys for the general kernel: about four blocks an SM, none with less than two tiles of 32 keys."""
+def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, cache_rows: int, aligned: bool, num_seqs: int, n_kv: int, rows: int,
+                keys: int, sms: int):
+    """(kernel, parts) for a step whose requests have at most ``rows`` rows (nodes x query heads) per key/value head and ``keys`` visible keys."""
+    if dtype == torch.bfloat16 and head_dim in (64, 128) and aligned:
+        if rows <= 64:
+            parts = 8
+            while parts > 1 and (num_seqs * n_kv * parts > 2 * sms or parts > 2 * -(-keys // 64)):
+                parts //= 2
+            return "tree_attention_few", parts
+        if group <= 128 and page_size % 8 == 0 and (64 % page_size == 0 or page_size % 64 == 0) and cache_rows <= 0x7fffff00:
+            units = num_seqs * n_kv * -(-rows // (2 * (128 // group * group)))
+            return "tree_attention_tc", max(1, min(sms, units * (-(-keys // 128) + 1)))
+    # the general kernel: about four blocks an SM, none with less than two tiles of 32 keys
     blocks = max(1, num_seqs * n_kv * -(-rows // 32))
-    return max(1, min(4 * sms // blocks, keys // 64, 64))
+    return "tree_attention", max(1, min(4 * sms // blocks, keys // 64, 64))
 
 
 def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Tensor, num_seqs: int,

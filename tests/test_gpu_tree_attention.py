@@ -251,6 +251,21 @@ def test_what_a_row_does_not_see_does_not_reach_it(dtype, d, bad):
 
 
 @BOTH
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nodes,context", [([9, 4], [30, 200]), ([48, 9], [150, 700])])
+def test_a_query_that_is_not_finite_stays_in_its_row(dtype, d, nodes, context):
+    step = Step(nodes, context, 8, 2, d, 16, dtype, seed=12)
+    clean, _ = step.run()
+    step.q[3, 2 * d:3 * d] = float("nan")
+    got, _ = step.run()
+    view = lambda t: t.view(step.T, 8, d)
+    assert bool(torch.isnan(view(got)[3, 2].float()).all())
+    rest = torch.ones((step.T, 8), dtype=torch.bool, device=DEV)
+    rest[3, 2] = False
+    assert torch.equal(view(got)[rest], view(clean)[rest])
+
+
+@BOTH
 def test_strides_streams_and_order(dtype):
     """Queries as a view with a row stride, outputs with another; a stream of the caller's; a chain is ordinary causal attention."""
     from photon_infer_b200.kernels import ops
