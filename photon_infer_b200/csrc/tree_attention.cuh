@@ -54,8 +54,9 @@ __device__ __forceinline__ uint32_t tree_visible32(const TreeParams& P, const Tr
       m = __funnelshift_r(a, b, sh);
       if (r.n - i0 < 32) m &= (1u << (r.n - i0)) - 1u;
     }
-    if (P.window > 0) {
-      const int pos = P.positions[t];
+    // Nodes stand at base or behind, so a window that begins before base cuts none of them.
+    const int pos = P.window > 0 ? P.positions[t] : 0;
+    if (P.window > 0 && pos - P.window >= r.base) {
       for (uint32_t left = m; left != 0; left &= left - 1) {
         const int u = __ffs(left) - 1;
         if (P.positions[r.tok0 + i0 + u] <= pos - P.window) m &= ~(1u << u);

@@ -2592,7 +2592,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
                               sm_count(device))
     floats = 0
     if name == "tree_attention_tc":
-        floats = 2 * parts * (-(-min(max_tokens_per_seq * group, 2 * (128 // group * group)) // 32) * 32) * (head_dim + 2)
+        floats = 8 * parts + 2 * parts * (-(-min(max_tokens_per_seq * group, 128 // group * group) // 32) * 32) * (head_dim + 2)
     elif name == "tree_attention" and parts > 1:
         floats = T * n_q * parts * (head_dim + 2)
     scratch = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
@@ -2621,8 +2621,8 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
                 parts //= 2
             return "tree_attention_few", parts
         if group <= 128 and page_size % 8 == 0 and (64 % page_size == 0 or page_size % 64 == 0) and cache_rows <= 0x7fffff00:
-            units = num_seqs * n_kv * -(-rows // (2 * (128 // group * group)))
-            return "tree_attention_tc", max(1, min(sms, units * (-(-keys // 128) + 1)))
+            units = num_seqs * n_kv * -(-rows // (128 // group * group))
+            return "tree_attention_tc", max(1, min(2 * sms, 320, units * (-(-keys // 64) + 1)))
     # the general kernel: about four blocks an SM, none with less than two tiles of 32 keys
     blocks = max(1, num_seqs * n_kv * -(-rows // 32))
     return "tree_attention", max(1, min(4 * sms // blocks, keys // 64, 64))

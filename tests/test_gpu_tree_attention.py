@@ -184,6 +184,27 @@ def test_many_keys_shared_out(dtype, nodes, context, n_q, n_kv, d):
 
 
 @BOTH
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nodes,context,n_q,n_kv", [([40] * 40, [1600] * 40, 8, 2), ([12, 90, 33], [3000, 20000, 900], 8, 4), ([100] * 3, [700] * 3, 32, 2)])
+def test_maxima_that_keep_growing(dtype, d, nodes, context, n_q, n_kv):
+    """Scores that get larger along the keys: the running maximum moves in every tile and what was added up is scaled again, in requests whose keys one block
+    walks alone and in requests that several share; the same bits every time. """
+    step = Step(nodes, context, n_q, n_kv, d, 16, dtype, seed=13)
+    for s in range(step.S):
+        length = context[s] + nodes[s]
+        for i in range(-(-length // 16)):
+            step.k[int(step.table[s, i])] *= 1 + 9.0 * i * 16 / length
+    first, err = step.run()
+    assert err[0] == 0 and bool(torch.isfinite(first).all())
+    for _ in range(20):
+        assert torch.equal(step.run()[0], first)
+    if step.T <= 400:
+        want, largest = step.want()
+        # scores of up to some 200, summed up in 32 bits in either type, are off by 2e-5 of themselves at most: weights by 4e-3, and their sum as well
+        assert float((first.double().cpu() - want).abs().max()) <= (8e-3 + TOL[dtype]) * largest
+
+
+@BOTH
 def test_many_requests(dtype):
     """More requests than a block has threads in a warp, some without context, one without nodes."""
     nodes = [1 + (7 * i) % 19 for i in range(75)]
