@@ -596,17 +596,26 @@ PHOTON_EXPORT int photon_tree_attention_few(const photon_tree_call* call, cudaSt
 /* ------------------------------------------------------------------ tree_accept.cu */
 /* From node 0 of each request on: the token that the node's logits (float [T, V], row stride ld) give, greedily or with temperature[s] > 0 by
  * uniforms[t] as photon_sample does, then the first child (parents [T]: indices into the request's nodes, below the node's own; -1 for node 0) with that
- * token.  path, sampled [S, D]: the nodes gone through and the tokens they gave, -1 behind the last; counts [S].  Stops after D nodes. */
-PHOTON_EXPORT int photon_tree_accept(const float* logits, long ld, const int* tokens, const int* parents, const int* cu_tokens, int S, int T,
-                       int max_tokens_per_seq, int V, const float* temperature, const float* uniforms, int* path, int* counts,
-                       int* sampled, int D, cudaStream_t stream);
+ * token.  path, sampled [S, D]: the nodes gone through and the tokens they gave, -1 behind the last; counts [S].  Stops after D nodes.
+ * given (int [T]): where there is one, the logits of all nodes are read at once and the trees walked by a second kernel; where it is null, a
+ * cluster of blocks walks each tree and reads the logits on its path alone. */
+typedef struct {
+  const float* logits; const int* tokens; const int* parents; const int* cu_tokens;
+  const float* temperature; const float* uniforms;          /* null: greedy */
+  int* path; int* counts; int* sampled; int* given; int* err;
+  long ld;
+  int S, T, V, D, max_tokens_per_seq;
+} photon_accept_call;
+PHOTON_EXPORT int photon_tree_accept(const photon_accept_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ cache_rows.cu */
 /* kv [planes][num_pages][n_kv][page_size][d].  Key base + path[s][j] of request s goes to key base + j for 0 < j < counts[s], base = context_lens[s]
  * minus the request's nodes; paths ascend. */
-PHOTON_EXPORT int photon_cache_keep(void* kv, int dtype, int planes, int num_pages, int n_kv, int page_size, int d, const int* block_table,
-                      int max_pages, const int* cu_tokens, const int* context_lens, const int* path, const int* counts, int S,
-                      int D, int* err, cudaStream_t stream);
+typedef struct {
+  void* kv; const int* block_table; const int* cu_tokens; const int* context_lens; const int* path; const int* counts; int* err;
+  int dtype, planes, num_pages, n_kv, page_size, d, max_pages, S, D;
+} photon_keep_call;
+PHOTON_EXPORT int photon_cache_keep(const photon_keep_call* call, cudaStream_t stream);
 /* kv [planes][num_pages][page_elems]: page pairs[i][0] onto page pairs[i][1] in every plane.  No page is written twice, or both read and written. */
 PHOTON_EXPORT int photon_cache_copy_pages(void* kv, int dtype, int planes, int num_pages, long page_elems, const int* pairs, int count, int* err,
                             cudaStream_t stream);

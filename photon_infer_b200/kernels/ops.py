@@ -2651,11 +2651,23 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     if temperature is not None and (uniforms is None or any(t.dtype != torch.float32 or not t.is_contiguous() for t in (temperature, uniforms))
                                     or temperature.numel() < num_seqs or uniforms.numel() < T):
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_accept: temperature [requests] and uniforms [T] must be contiguous float32")
-    f = _fn("tree_accept", "photon_tree_accept",
-            [c_void_p, c_long, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_int,
-             c_void_p])
-    _check(f(_ptr(logits), logits.stride(0), _ptr(tokens), _ptr(parents), _ptr(cu_tokens), int(num_seqs), T, int(max_tokens_per_seq), V,
-             _ptr(temperature), _ptr(uniforms), _ptr(path), _ptr(counts), _ptr(sampled), path.shape[1], _stream()), "tree_accept")
+    # few logits: all nodes' at once, and a second kernel for the walk; many: a walk that reads those on the paths alone
+    given = torch.empty(T, dtype=torch.int32, device=logits.device) if num_seqs * max_tokens_per_seq * V <= ACCEPT_AT_ONCE else None
+    call = _ACCEPT_CALL.pack(logits.data_ptr(), tokens.data_ptr(), parents.data_ptr(), cu_tokens.data_ptr(),
+                             temperature.data_ptr() if temperature is not None else 0, uniforms.data_ptr() if temperature is not None else 0,
+                             path.data_ptr(), counts.data_ptr(), sampled.data_ptr(), given.data_ptr() if given is not None else 0,
+                             err.data_ptr() if err is not None else 0, logits.stride(0),
+                             num_seqs, T, V, path.shape[1], max_tokens_per_seq)
+    _check(_plain_fn("tree_accept", "photon_tree_accept", _CALL_ARGS)(call, _stream()), "tree_accept")
+    if given is not None:
+        _count_launches(1)
+
+
+#: photon_accept_call
+_ACCEPT_CALL = struct.Struct("12q5i4x")
+#: Logits up to which those of all nodes are read at once.  Walk and all at once, us, vocabulary of 128,256: 1 request of 16 nodes 10 and 7 (sampled 13 and 10), 1 of
+#: 64 10 and 12 (24 and 18), 4 of 16 16 and 12 (40 and 16), 4 of 64 12 and 39 (30 and 51), 32 of 8 28 and 39 (52 and 51), 32 of 64 27 and 268.
+ACCEPT_AT_ONCE = 12 << 20
 
 
 def _check_pool(what: str, kv: torch.Tensor) -> int:
@@ -2676,10 +2688,15 @@ def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Ten
     _int32(counts, "counts")
     if path.dim() != 2 or path.shape[0] < num_seqs or counts.numel() < num_seqs:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_keep: path must be [requests, depth], counts [requests]")
-    f = _fn("cache_rows", "photon_cache_keep",
-            [c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, c_void_p, c_void_p])
-    _check(f(_ptr(kv), _dtype_code(kv), planes, kv.shape[2], kv.shape[3], kv.shape[4], kv.shape[5], _ptr(block_table), block_table.shape[1],
-             _ptr(cu_tokens), _ptr(context_lens), _ptr(path), _ptr(counts), int(num_seqs), path.shape[1], _ptr(err), _stream()), "cache_keep")
+    _, _, pages, n_kv, page_size, d = kv.shape
+    call = _KEEP_CALL.pack(kv.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), path.data_ptr(), counts.data_ptr(),
+                           err.data_ptr() if err is not None else 0, _dtype_code(kv), planes, pages, n_kv, page_size, d, block_table.shape[1], num_seqs,
+                           path.shape[1])
+    _check(_plain_fn("cache_rows", "photon_cache_keep", _CALL_ARGS)(call, _stream()), "cache_keep")
+
+
+#: photon_keep_call
+_KEEP_CALL = struct.Struct("7q9i4x")
 
 
 def cache_copy_pages(kv: torch.Tensor, pairs: torch.Tensor, err: Optional[torch.Tensor]) -> None:
@@ -2690,9 +2707,10 @@ def cache_copy_pages(kv: torch.Tensor, pairs: torch.Tensor, err: Optional[torch.
     _int32(pairs, "pairs")
     if pairs.dim() != 2 or pairs.shape[1] != 2:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_copy_pages: pairs must be [pages, 2]")
-    f = _fn("cache_rows", "photon_cache_copy_pages", [c_void_p, c_int, c_int, c_int, c_long, c_void_p, c_int, c_void_p, c_void_p])
-    _check(f(_ptr(kv), _dtype_code(kv), planes, kv.shape[2], kv.shape[3] * kv.shape[4] * kv.shape[5], _ptr(pairs), pairs.shape[0], _ptr(err),
-             _stream()), "cache_copy_pages")
+    _, _, pages, n_kv, page_size, d = kv.shape
+    f = _plain_fn("cache_rows", "photon_cache_copy_pages", [c_void_p, c_int, c_int, c_int, c_long, c_void_p, c_int, c_void_p, c_void_p])
+    _check(f(kv.data_ptr(), _dtype_code(kv), planes, pages, n_kv * page_size * d, pairs.data_ptr(), pairs.shape[0],
+             err.data_ptr() if err is not None else 0, _stream()), "cache_copy_pages")
 
 
 # ----------------------------------------------------------------------------- sampling
