@@ -3,7 +3,7 @@
 // The rows of a unit are (node, query head) pairs of one request that share a key/value head, up to 128 (whole nodes).  A unit's keys are walked in tiles of 64.  All units'
 // tiles, one behind the other, are cut into equal ranges, one for each block of a grid that fills the chip once, so that requests of any
 // lengths keep every SM busy to the end; a block walks the pieces of units in its range ("segments").  Units that ranges cut through are joined by a second
-// kernel, in the blocks' order.
+// kernel, in the blocks' order.  Where whole units keep the chip as busy they are dealt out whole, the longest first, and there is nothing to join.
 //
 // Two blocks share an SM, so that one's loads and products run while the other begins or ends a segment.  In a block
 //   * warp 4 brings Q, key and value tiles by TMA along the block table into shared memory (128-byte swizzle); keys and values share one ring;
@@ -44,6 +44,7 @@ template <int D> struct Tt {
 
 struct TtParams {
   TreeParams t;
+  int whole, sorted, blocks_sm;                    // whole units in any case: one kernel; the longest of them first; blocks that the chip holds
   int tile_rows, tile_nodes, box_rows, total_rows, page_shift;
   int q_slots, q_slot_bytes, q_half_bytes, q_nodes;          // Q tiles in shared memory, bytes between them and between a tile's halves, nodes of a copy
   float scale_log2, cap_in;
@@ -51,10 +52,10 @@ struct TtParams {
   float* part_o; float* part_ml; int part_rows;    // partial results: [2 * blocks][D / 4][part_rows] of four, [2 * blocks][part_rows] of (maximum, sum)
 };
 
-// Keys and values share one ring, in the order in which they are wanted: K0 K1 V0 K2 V1 K3 V2 ..  The place in it of a block's key tile k and of its values, of
-// `tiles` in all; stage and parity follow from the place.
+// Keys and values share one ring, in the order in which they are wanted: K0 K1 V0 K2 V1 K3 V2 ..  The place in it of a block's key tile k and of its values; stage and
+// parity follow from the place.  (Behind the last keys one place stays free.)
 __device__ __forceinline__ int tt_place_k(int k) { return k == 0 ? 0 : 2 * k - 1; }
-__device__ __forceinline__ int tt_place_v(int k, int tiles) { return k == tiles - 1 ? 2 * tiles - 1 : 2 * k + 2; }
+__device__ __forceinline__ int tt_place_v(int k) { return 2 * k + 2; }
 
 // What a request asks for: its units and the tiles of each.
 struct TtLoad { TreeRequest r; int tile_lo, tiles, blocks, units; };     // blocks: row tiles
@@ -68,13 +69,14 @@ __device__ __forceinline__ TtLoad tt_load(const TtParams& P, int s) {
   q.units = q.blocks * P.t.n_kv;
   return q;
 }
-// Warp-wide: the tiles of all units together, or (at >= 0) the request that holds tile `at` of them and the tiles before it.
+// Warp-wide: the tiles of all units together and in `seq` those of the longest unit, or (at >= 0) the request that holds tile `at` of them and the tiles before it.
 __device__ __forceinline__ long long tt_scan(const TtParams& P, long long at, int& seq) {
   const int lane = threadIdx.x & 31;
   long long before = 0;
+  int longest = 0;
   for (int s0 = 0; s0 < P.t.S; s0 += 32) {
     int n = 0;
-    if (s0 + lane < P.t.S) { const TtLoad q = tt_load(P, s0 + lane); n = q.units * q.tiles; }
+    if (s0 + lane < P.t.S) { const TtLoad q = tt_load(P, s0 + lane); n = q.units * q.tiles; longest = max(longest, q.units > 0 ? q.tiles : 0); }
     int upto = n;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
@@ -91,57 +93,100 @@ __device__ __forceinline__ long long tt_scan(const TtParams& P, long long at, in
     }
     before += __shfl_sync(0xffffffffu, upto, 31);
   }
+  seq = __reduce_max_sync(0xffffffffu, longest);
   return before;
+}
+// Whole units are dealt out with the longest first: the units before each request, for up to TT_SORTED of them; more come as they are.
+#define TT_SORTED 64
+struct TtOrder { int tiles[TT_SORTED]; unsigned short front[TT_SORTED], units[TT_SORTED]; };
+// By the whole block, with a barrier inside.
+__device__ __forceinline__ void tt_sort(const TtParams& P, TtOrder& o) {
+  const int t = threadIdx.x;
+  int tiles = 0, units = 0, front = 0;
+  if (t < P.t.S) {
+    const TtLoad q = tt_load(P, t);
+    tiles = q.tiles; units = q.units;
+    o.tiles[t] = tiles; o.units[t] = (unsigned short)units;
+  }
+  __syncthreads();
+  if (t < P.t.S) {
+    for (int x = 0; x < P.t.S; ++x) if (o.tiles[x] > tiles || (o.tiles[x] == tiles && x < t)) front += o.units[x];
+    o.front[t] = (unsigned short)front;
+  }
+  __syncthreads();
+}
+// Warp-wide: the request that holds unit `at` of the whole units, and the units before it; false: there is no such unit.
+__device__ __forceinline__ bool tt_unit(const TtParams& P, const TtOrder& o, int at, int& seq, int& before) {
+  const int lane = threadIdx.x & 31;
+  if (P.sorted) {
+#pragma unroll
+    for (int s0 = 0; s0 < TT_SORTED; s0 += 32) {
+      const int s = s0 + lane;
+      const bool mine = s < P.t.S && at >= o.front[s] && at < o.front[s] + o.units[s];
+      const unsigned hit = __ballot_sync(0xffffffffu, mine);
+      if (hit != 0) {
+        seq = s0 + __ffs(hit) - 1;
+        before = o.front[seq];
+        return true;
+      }
+    }
+    return false;
+  }
+  int total = 0;
+  for (int s0 = 0; s0 < P.t.S; s0 += 32) {
+    int n = 0;
+    if (s0 + lane < P.t.S) n = tt_load(P, s0 + lane).units;
+    int upto = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, upto, d);
+      if (lane >= d) upto += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, total + upto > at);
+    if (hit != 0) {
+      const int l = __ffs(hit) - 1;
+      seq = s0 + l;
+      before = total + __shfl_sync(0xffffffffu, upto - n, l);
+      return true;
+    }
+    total += __shfl_sync(0xffffffffu, upto, 31);
+  }
+  return false;
 }
 // Blocks that have a range: every one of them has a tile at least.  The first tile of a block's range, and the block that has a tile.
 __device__ __forceinline__ int tt_blocks(long long total, int blocks) { return (int)min((long long)blocks, total); }
 __device__ __forceinline__ long long tt_first(long long total, int block, int blocks) { return total * block / blocks; }
 __device__ __forceinline__ int tt_owner(long long total, long long tile, int blocks) { return (int)(((tile + 1) * blocks - 1) / total); }
 
-// The segments of a block, in order.
+// The segments of a block, in order: the pieces of units in its range, or whole units.
 struct TtSegments {
-  int seq, unit, tile, left, serial;               // where the next one begins; tiles left in the block's range
+  int seq, unit, tile, left, serial, round;        // where the next one begins; tiles left in the block's range; whole units so far
+  const TtOrder* order;
+  bool units_whole;
   TtLoad q;
   // the segment
   int g, row0, rows, tile0, ntiles, bit;
   bool whole;
-  __device__ __forceinline__ void start(const TtParams& P, long long& total, long long& first) {
-    left = 0; serial = 0; seq = 0; unit = 0; tile = 0;
-    long long before;
-    if (P.t.S <= 32) {
-      // one look at the requests is enough
-      const int lane = threadIdx.x & 31;
-      int n = 0;
-      if (lane < P.t.S) { const TtLoad x = tt_load(P, lane); n = x.units * x.tiles; }
-      int upto = n;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int v = __shfl_up_sync(0xffffffffu, upto, o);
-        if (lane >= o) upto += v;
-      }
-      total = __shfl_sync(0xffffffffu, upto, 31);
-      if (!range(total, first)) return;
-      const int l = __ffs(__ballot_sync(0xffffffffu, upto > first)) - 1;
-      seq = l;
-      before = __shfl_sync(0xffffffffu, upto - n, l);
-    } else {
-      int dummy = 0;
-      total = tt_scan(P, -1, dummy);
-      if (!range(total, first)) return;
-      before = tt_scan(P, first, seq);
-    }
+  __device__ __forceinline__ void start(const TtParams& P, const TtOrder* o, bool w, long long total) {
+    order = o; units_whole = w;
+    left = 0; serial = 0; seq = 0; unit = 0; tile = 0; round = 0;
+    const int blocks = tt_blocks(total, gridDim.x);
+    if (w || (int)blockIdx.x >= blocks) return;
+    const long long first = tt_first(total, blockIdx.x, blocks);
+    left = (int)(tt_first(total, blockIdx.x + 1, blocks) - first);
+    const int off = (int)(first - tt_scan(P, first, seq));
     q = tt_load(P, seq);
-    const int off = (int)(first - before);
     unit = off / q.tiles; tile = off - unit * q.tiles;
   }
-  __device__ __forceinline__ bool range(long long total, long long& a) {
-    const int blocks = tt_blocks(total, gridDim.x);
-    if ((int)blockIdx.x >= blocks) return false;
-    a = tt_first(total, blockIdx.x, blocks);
-    left = (int)(tt_first(total, blockIdx.x + 1, blocks) - a);
-    return true;
-  }
-  __device__ __forceinline__ bool next(const TtParams& P) {
+  __device__ __forceinline__ bool next(const TtParams& P) {       // by whole warps
+    if (units_whole) {
+      // the longest units first, to and fro over the blocks
+      const int u = (round & 1) ? (round + 1) * (int)gridDim.x - 1 - (int)blockIdx.x : round * (int)gridDim.x + (int)blockIdx.x;
+      ++round;
+      int front;
+      if (!tt_unit(P, *order, u, seq, front)) return false;
+      q = tt_load(P, seq); unit = u - front; tile = 0; left = q.tiles;
+    }
     if (left <= 0) return false;
     while (unit >= q.units) {
       if (++seq >= P.t.S) return false;
@@ -184,6 +229,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   int* poison = reinterpret_cast<int*>(gone_s + 16);// the last segment whose values were not all finite
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(poison + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  TtOrder* order = reinterpret_cast<TtOrder*>(tmem_slot + 2);
 
   const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
@@ -206,19 +252,31 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   // the tiles' swizzle counts from 1024-byte boundaries
   const bool aligned = (tc_smem(tt_dyn) & 1023) == 0;
   if (!aligned && threadIdx.x == 0) *abort_flag = 1;
+  // Ranges or whole units?  In times of a tile on an SM with two blocks (0.5 to 0.65 us): whole units take as long as the longest takes its block, or their share of the chip;
+  // ranges a quarter more than their share, for what they put down and join, and the second kernel.  Measured with 32/8 heads of 128 and 128 rows a unit, ranges and whole units,
+  // us: 16 requests of 2,500 keys 58 and 45, of 5,000 83 and 79; 64 of up to 2,500 106 and 69; 4 of 2,500 31 and 43; 1 of 2,500 18 and 43.
+  int longest = 0;
+  long long total = 0;
+  bool whole = P.whole;
+  if (!whole) {
+    total = tt_scan(P, -1, longest);
+    const float part = (float)total / (P.blocks_sm * 0.5f);
+    whole = fmaxf(1.45f * longest, 1.05f * part) <= 1.25f * part + 15.f;
+  }
+  if (whole && P.sorted) tt_sort(P, *order);
   TtSegments s;
-  long long total = 0, range0 = 0;
-  if (aligned) s.start(P, total, range0); else s.left = 0;
-  const int all = s.left;
+  s.start(P, order, whole, total);
 
-  if (warp == 4) {
+  if (!aligned) {
+    if (threadIdx.x == 0 && !P.whole) P.meta[2 * blockIdx.x] = make_int4(0, 0, 0, 0);       // nothing can be run
+  } else if (warp == 4) {
     // ---------------- producer
     const bool elected = tc_elect();
     const int boxes = TT_KT / P.box_rows;           // parts of a tile that may lie in different pages
     int kn = 0, vn = 0, qn = 0;                     // key, value and Q tiles so far
     bool ok = true;
     // The ring's next stage for keys and for values (tt_place_k, tt_place_v step by step), and the parity that says it is free.
-    int kst = 0, kph = 1, vst = all == 1 ? 1 : 2, vph = 1;
+    int kst = 0, kph = 1, vst = 2, vph = 1;
     auto step = [&](int& st, int& ph, int by) {
       st += by;
       if (st >= C::NS) { st -= C::NS; ph ^= 1; }
@@ -290,7 +348,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             default: issue(std::integral_constant<int, 8>(), map, st, rows, from); break;
           }
           if (keys) { step(kst, kph, kn == 0 ? 1 : 2); ++kn; }
-          else { ++vn; step(vst, vph, vn + 1 == all ? 1 : 2); }
+          else { step(vst, vph, 2); ++vn; }
         }
         rowv = rowc; fromv = j * boxes;             // values lie as keys do
       }
@@ -300,7 +358,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       for (int j = (qn > P.q_slots ? qn - P.q_slots : 0); j < qn; ++j)
         for (uint32_t w = 0; w < TC_WAIT_LIMIT && !tc_mbar_try(&q_full[j & (P.q_slots - 1)], (j >> (P.q_slots - 1)) & 1); ++w) {}
       for (int j = (kn > C::NS ? kn - C::NS : 0); j < kn + 1; ++j) {
-        const int a = tt_place_k(j), b = tt_place_v(j, all);
+        const int a = tt_place_k(j), b = tt_place_v(j);
         for (uint32_t w = 0; j < kn && w < TC_WAIT_LIMIT && !tc_mbar_try(&full[a % C::NS], (a / C::NS) & 1); ++w) {}
         for (uint32_t w = 0; j < vn && w < TC_WAIT_LIMIT && !tc_mbar_try(&full[b % C::NS], (b / C::NS) & 1); ++w) {}
       }
@@ -340,7 +398,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     };
     int vn = 0;
     auto products = [&](uint32_t f) -> bool {
-      const int pb = f >> 2, place = tt_place_v(vn++, all), vs = place % C::NS;
+      const int pb = f >> 2, place = tt_place_v(vn++), vs = place % C::NS;
       if (!tc_wait(&full[vs], (place / C::NS) & 1, abort_flag)) return false;
       if (!tc_wait(&p_full[pb], f & 1, abort_flag)) return false;
       tc_fence_after();
@@ -375,8 +433,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     int n = 0;                                      // tiles so far
     bool ok = true;
     auto landed = [&](int k) { return tc_wait_warp(&o_full[k % C::NB], (k / C::NB) & 1, abort_flag); };      // the products of tile k
-    if (r < 2 && s.left == 0) P.meta[2 * blockIdx.x + r] = make_int4(0, 0, 0, 0);
-    bool said = s.left == 0;                        // what the second kernel is to do for this block
+    bool said = false;                        // what the second kernel is to do for this block
     while (ok && s.next(P)) {
       const bool valid = r < s.rows, busy = __any_sync(0xffffffffu, valid);
       const int t = s.q.r.tok0 + (valid ? (s.row0 + r) / P.t.group : 0);
@@ -393,7 +450,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const bool edge = key_base + TT_KT > base || key_base <= cut_lo || gone != 0;
         if (edge) {
           // values that are not finite, of nodes and before a row's window: zeros, before this tile's P says that they may be read
-          const int place = tt_place_v(n, all), st = place % C::NS;
+          const int place = tt_place_v(n), st = place % C::NS;
           if (!tc_wait_warp(&full[st], (place / C::NS) & 1, abort_flag)) { ok = false; break; }
           unsigned char* vst = kv_s + st * C::TILE;
           const int upto = min(max(cut_lo - key_base + 1, 0), TT_KT), from = max(min(max(base - key_base, 0), TT_KT), upto);
@@ -563,7 +620,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       }
       tc_fence_before();                            // O is read: the next segment's P may be handed over
     }
-    if (r == 0 && !said) P.meta[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (r == 0 && !said && !P.whole) P.meta[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
   }
   // ---------------- teardown
   tc_fence_before();
@@ -591,21 +648,32 @@ tree_join_tc_kernel(const TtParams P, int chunks) {
   const int rr = valid ? r0 + lane : rows - 1, cc = blockIdx.y * 8 + warp;
   const int t = tok0 + (a0.y + rr) / P.t.group, head = a0.w * P.t.group + (a0.y + rr) % P.t.group;
   auto slot = [&](int i) { return (size_t)2 * (c0 + i) + (i == 0 ? 1 : 0); };
-  auto ml = [&](int i) { return *reinterpret_cast<const float2*>(P.part_ml + (slot(i) * P.part_rows + rr) * 2); };
-  const float sink = P.t.sinks ? P.t.sinks[head] * TT_LOG2E : -INFINITY;
-  float top = sink;
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) top = fmaxf(top, ml(i).x);
-  const float sub = top == -INFINITY ? 0.f : top;
-  float sum = P.t.sinks ? at_exp2(sink - sub) : 0.f;
+  // the maximum and sum so far, the sink first; eight pieces are on their way at a time
+  float top = P.t.sinks ? P.t.sinks[head] * TT_LOG2E : -INFINITY, sum = P.t.sinks ? 1.f : 0.f;
   float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) {
-    const float2 x = ml(i);
-    const float4 y = *(reinterpret_cast<const float4*>(P.part_o) + (slot(i) * (D / 4) + cc) * P.part_rows + rr);
-    const float w = at_exp2(x.x - sub);
-    sum += x.y * w;
-    if (w != 0.f) { a.x = fmaf(w, y.x, a.x); a.y = fmaf(w, y.y, a.y); a.z = fmaf(w, y.z, a.z); a.w = fmaf(w, y.w, a.w); }
+  if (top == -INFINITY) sum = 0.f;
+  for (int i0 = 0; i0 < parts; i0 += 8) {
+    float2 ml[8];
+    float4 y[8];
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      const int i = min(i0 + k, parts - 1);
+      ml[k] = *reinterpret_cast<const float2*>(P.part_ml + (slot(i) * P.part_rows + rr) * 2);
+      y[k] = *(reinterpret_cast<const float4*>(P.part_o) + (slot(i) * (D / 4) + cc) * P.part_rows + rr);
+    }
+    float most = top;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) most = fmaxf(most, ml[k].x);
+    const float sub = most == -INFINITY ? 0.f : most, old = at_exp2(top - sub);
+    sum *= old; a.x *= old; a.y *= old; a.z *= old; a.w *= old;
+    top = most;
+#pragma unroll
+    for (int k = 0; k < 8; ++k) {
+      if (i0 + k >= parts) continue;
+      const float w = at_exp2(ml[k].x - sub);
+      sum += ml[k].y * w;
+      if (w != 0.f) { a.x = fmaf(w, y[k].x, a.x); a.y = fmaf(w, y[k].y, a.y); a.z = fmaf(w, y[k].z, a.z); a.w = fmaf(w, y[k].w, a.w); }
+    }
   }
   if (valid) {
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
@@ -621,7 +689,7 @@ static int tt_launch(TtParams& P, const CUtensorMap& mq, const CUtensorMap& mk, 
   int st = tree_smem_limit((const void*)tree_attention_tc_kernel<D>, Tt<D>::SMEM, ready);
   if (st != 0) return st;
   st = launch_pdl(tree_attention_tc_kernel<D>, dim3(blocks), dim3(TT_THREADS), (size_t)Tt<D>::SMEM, stream, mq, mk, mv, P);
-  if (st != 0) return st;
+  if (st != 0 || P.whole) return st;
   const int chunks = (P.part_rows + 31) / 32;
   return launch_pdl(tree_join_tc_kernel<D>, dim3((unsigned)(blocks * chunks), D / 32), dim3(256), 0, stream, P, chunks);
 }
@@ -649,8 +717,11 @@ PHOTON_API int photon_tree_attention_tc(const photon_tree_call* call, cudaStream
     return PHOTON_ERR_UNSUPPORTED;
   const long total_rows = (long)t.num_pages * t.n_kv * page_size;
   if (total_rows > 0x7fffff00L) return PHOTON_ERR_UNSUPPORTED;
-  if (call->parts > TT_MAX_BLOCKS) return PHOTON_ERR_ARGUMENT;
-  if (call->scratch == nullptr || call->scratch_floats < photon_tree_attention_tc_scratch(t.max_tokens, t.n_q, t.n_kv, d, call->parts)) return PHOTON_ERR_ARGUMENT;
+  P.whole = call->scratch == nullptr;
+  P.blocks_sm = 2 * photon_sm_count();
+  P.sorted = t.S <= TT_SORTED && (long)t.S * t.n_kv * ((t.max_tokens + 128 / G - 1) / (128 / G)) <= 65535;
+  if (!P.whole && call->parts > TT_MAX_BLOCKS) return PHOTON_ERR_ARGUMENT;
+  if (!P.whole && call->scratch_floats < photon_tree_attention_tc_scratch(t.max_tokens, t.n_q, t.n_kv, d, call->parts)) return PHOTON_ERR_ARGUMENT;
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return PHOTON_ERR_UNSUPPORTED;
   P.tile_nodes = 128 / G; P.tile_rows = P.tile_nodes * G;

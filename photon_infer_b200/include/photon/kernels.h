@@ -585,7 +585,8 @@ PHOTON_EXPORT int photon_tree_attention(const photon_tree_call* call, cudaStream
 
 /* ------------------------------------------------------------------ tree_attention_tc.cu: the same on tcgen05, bfloat16, d 64 or 128 */
 /* At most 128 query heads per key/value head, pages of 8, 16, 32 or a multiple of 64 tokens, 16-byte aligned rows.  parts: the grid, at most as many blocks
- * as the chip holds at once; scratch: as many floats as the first function says. */
+ * as the chip holds at once.  scratch: as many floats as the first function says, and the lengths on the device decide whether a request's keys are shared out
+ * over blocks; or null: they are not, in one kernel. */
 PHOTON_EXPORT long photon_tree_attention_tc_scratch(int max_tokens_per_seq, int n_q, int n_kv, int d, int blocks);
 PHOTON_EXPORT int photon_tree_attention_tc(const photon_tree_call* call, cudaStream_t stream);
 

@@ -2591,7 +2591,9 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     name, parts = _tree_route(dtype, head_dim, group, page_size, pages * n_kv * page_size, aligned, num_seqs, n_kv, max_tokens_per_seq * group, keys,
                               sm_count(device))
     floats = 0
-    if name == "tree_attention_tc":
+    if name == "tree_attention_tc" and parts < 0:
+        parts = -parts                              # whole units: no scratch
+    elif name == "tree_attention_tc":
         floats = 8 * parts + 2 * parts * (-(-min(max_tokens_per_seq * group, 128 // group * group) // 32) * 32) * (head_dim + 2)
     elif name == "tree_attention" and parts > 1:
         floats = T * n_q * parts * (head_dim + 2)
@@ -2611,18 +2613,30 @@ def _count_launches(n: int) -> None:
     _launch_count += n
 
 
+#: Tiles of 64 keys that a block of the kernel for few rows may walk one behind the other (waves counted), by head size.
+TREE_FEW_STEPS = {64: 12, 128: 5}
+
+
 def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, cache_rows: int, aligned: bool, num_seqs: int, n_kv: int, rows: int,
                 keys: int, sms: int):
-    """(kernel, parts) for a step whose requests have at most ``rows`` rows (nodes x query heads) per key/value head and ``keys`` visible keys."""
+    """(kernel, parts; below zero: blocks that take whole units) for a step whose requests have at most ``rows`` rows (nodes x query heads) per key/value head and ``keys`` visible keys."""
     if dtype == torch.bfloat16 and head_dim in (64, 128) and aligned:
+        tiles, units = -(-keys // 64), num_seqs * n_kv
+        tma = group <= 128 and page_size % 8 == 0 and (64 % page_size == 0 or page_size % 64 == 0) and cache_rows <= 0x7fffff00
         if rows <= 64:
             parts = 8
-            while parts > 1 and (num_seqs * n_kv * parts > 2 * sms or parts > 2 * -(-keys // 64)):
+            while parts > 1 and (units * parts > 2 * sms or parts > 2 * tiles):
                 parts //= 2
-            return "tree_attention_few", parts
-        if group <= 128 and page_size % 8 == 0 and (64 % page_size == 0 or page_size % 64 == 0) and cache_rows <= 0x7fffff00:
-            units = num_seqs * n_kv * -(-rows // (128 // group * group))
-            return "tree_attention_tc", max(1, min(2 * sms, 320, units * (-(-keys // 64) + 1)))
+            steps = -(-tiles // parts) * -(-units * parts // ((3 if head_dim == 64 else 2) * sms))
+            if not tma or steps <= TREE_FEW_STEPS[head_dim]:
+                return "tree_attention_few", parts
+        if tma:
+            units *= -(-rows // (128 // group * group))
+            # Few keys: whole units, one kernel.  More: the kernel decides by the lengths, which the host does not know, and a second kernel follows
+            # it; a block has four tiles at least.
+            if tiles <= 10 or (tiles <= 32 and 4 * units >= 3 * sms):
+                return "tree_attention_tc", -min(2 * sms, 320, units)
+            return "tree_attention_tc", min(2 * sms, 320, max(units, -(-units * (tiles + 1) // 4)))
     # the general kernel: about four blocks an SM, none with less than two tiles of 32 keys
     blocks = max(1, num_seqs * n_kv * -(-rows // 32))
     return "tree_attention", max(1, min(4 * sms // blocks, keys // 64, 64))
