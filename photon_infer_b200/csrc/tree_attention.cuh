@@ -67,6 +67,12 @@ __device__ __forceinline__ uint32_t tree_visible32(const TreeParams& P, const Tr
   return bits;
 }
 
+// tanh(y) for |y| <= 1/2 by its series up to y^11: off by less than 21844 / 6081075 y^13 < 5e-7.  Scores far below their bound need no exponential and no division.
+__device__ __forceinline__ float tree_tanh_half(float y) {
+  const float z = y * y;
+  return y * fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1382.f / 155925.f, 62.f / 2835.f), -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
+}
+
 // The cache row (of d numbers) of a key, or -1 where its page is missing, which is recorded.
 __device__ __forceinline__ long long tree_row(const TreeParams& P, const int* table, int g, int key, int tok0) {
   const int pidx = key / P.page_size;

@@ -209,11 +209,23 @@ tree_attention_few_kernel(const TfParams P) {
       }
     }
     if (t.softcap > 0.f) {
+      bool small = true;
 #pragma unroll
       for (int j = 0; j < C::NT; ++j)
 #pragma unroll
-        for (int u = 0; u < 4; ++u)                // tanh(x) = 1 - 2 / (2^(2 x log2 e) + 1)
-          s[j][u] = t.softcap - __fdividef(2.0f * t.softcap, tf_exp2(s[j][u] * P.cap_in * 2.8853900817779268f) + 1.0f);
+        for (int u = 0; u < 4; ++u) small = small && fabsf(s[j][u]) * P.cap_in <= 0.5f;
+      if (__all_sync(0xffffffffu, small)) {
+#pragma unroll
+        for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[j][u] = t.softcap * tree_tanh_half(s[j][u] * P.cap_in);
+      } else {
+#pragma unroll
+        for (int j = 0; j < C::NT; ++j)
+#pragma unroll
+          for (int u = 0; u < 4; ++u)              // tanh(x) = 1 - 2 / (2^(2 x log2 e) + 1)
+            s[j][u] = t.softcap - __fdividef(2.0f * t.softcap, tf_exp2(s[j][u] * P.cap_in * 2.8853900817779268f) + 1.0f);
+      }
     }
     if (edge) {
 #pragma unroll

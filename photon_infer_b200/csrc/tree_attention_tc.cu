@@ -208,6 +208,16 @@ struct TtSegments {
   }
 };
 
+// softcap tanh(x / softcap) = scale x' q(y^2) of two raw scores x' at a time, y = cap_in x': tree_tanh_half's series on pairs (sm_100 has one instruction for both).
+__device__ __forceinline__ uint64_t tt_both(float c) { return (uint64_t)__float_as_uint(c) << 32 | __float_as_uint(c); }
+__device__ __forceinline__ void tt_cap_pair(uint32_t& a, uint32_t& b, float cap_in, float scale) {
+  asm("{\n.reg .b64 x, y, z, p;\nmov.b64 x, {%0, %1};\nmul.rn.f32x2 y, x, %2;\nmul.rn.f32x2 z, y, y;\nfma.rn.f32x2 p, z, %4, %5;\nfma.rn.f32x2 p, p, z, %6;\n"
+      "fma.rn.f32x2 p, p, z, %7;\nfma.rn.f32x2 p, p, z, %8;\nfma.rn.f32x2 p, p, z, %9;\nmul.rn.f32x2 x, x, %3;\nmul.rn.f32x2 x, x, p;\nmov.b64 {%0, %1}, x;\n}"
+      : "+r"(a), "+r"(b)
+      : "l"(tt_both(cap_in)), "l"(tt_both(scale)), "l"(tt_both(-1382.f / 155925.f)), "l"(tt_both(62.f / 2835.f)), "l"(tt_both(-17.f / 315.f)), "l"(tt_both(2.f / 15.f)),
+        "l"(tt_both(-1.f / 3.f)), "l"(tt_both(1.f)));
+}
+
 template <int D>
 __global__ void __launch_bounds__(TT_THREADS, 2)
 tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
@@ -482,10 +492,18 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           tc_ld32_issue(s_addr + 32, sv + 32);
           tc_ld_wait();
           if (cap > 0.f) {
+            float most = 0.f;
 #pragma unroll
-            for (int u = 0; u < TT_KT; ++u) {
-              const float x = at_exp2(__uint_as_float(sv[u]) * cap_in);
-              sv[u] = __float_as_uint(cap - __fdividef(2.0f * cap, x + 1.0f));
+            for (int u = 0; u < TT_KT; u += 2) most = at_max3(most, fabsf(__uint_as_float(sv[u])), fabsf(__uint_as_float(sv[u + 1])));
+            if (__all_sync(0xffffffffu, most * P.cap_in <= 0.5f)) {                                // a NaN stays one either way
+#pragma unroll
+              for (int u = 0; u < TT_KT; u += 2) tt_cap_pair(sv[u], sv[u + 1], P.cap_in, P.t.scale);
+            } else {
+#pragma unroll
+              for (int u = 0; u < TT_KT; ++u) {
+                const float x = at_exp2(__uint_as_float(sv[u]) * cap_in);
+                sv[u] = __float_as_uint(cap - __fdividef(2.0f * cap, x + 1.0f));
+              }
             }
           }
           if (edge) {

@@ -2634,7 +2634,7 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
             units *= -(-rows // (128 // group * group))
             # Few keys: whole units, one kernel.  More: the kernel decides by the lengths, which the host does not know, and a second kernel follows
             # it; a block has four tiles at least.
-            if tiles <= 10 or (tiles <= 32 and 4 * units >= 3 * sms):
+            if tiles <= 12 or (tiles <= 32 and 4 * units >= 3 * sms):
                 return "tree_attention_tc", -min(2 * sms, 320, units)
             return "tree_attention_tc", min(2 * sms, 320, max(units, -(-units * (tiles + 1) // 4)))
     # the general kernel: about four blocks an SM, none with less than two tiles of 32 keys
