@@ -1,7 +1,8 @@
 """A cache group: the pages of all run-list entries whose mixers need the same thing
 per token (same key/value heads and head size, same window).  Each group has its own
 pool and its own block table per request, so a group that keeps a window gives its
-pages back without disturbing a group that keeps everything.
+pages back without disturbing a group that keeps everything.  A request that forks shares its full pages with the
+fork; a page is written only while it has one holder.
 
 The reference has one implicit group: a K and a V tensor ``[num_blocks, n_kv_heads,
 block_size, head_size]`` per layer and one table per sequence (src/runtime/
@@ -12,7 +13,7 @@ the K plane alone).
 """
 from __future__ import annotations
 
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Tuple
 
 import torch
 
@@ -101,6 +102,58 @@ class CacheGroup:
                 table[i] = NO_PAGE
                 n += 1
         return n
+
+    def pages_to_fork(self, length: int) -> int:
+        """Pages that a fork of a request of ``length`` tokens takes: its own copy of a partly filled last page."""
+        return 1 if length % self.page_size else 0
+
+    def fork(self, rid, new_rid, length: int) -> List[Tuple[int, int]]:
+        """A table for ``new_rid`` over the first ``length`` tokens of ``rid``: full pages, which nobody writes again, are shared, a partly
+        filled last one is to be copied.  Returns the copies (old page, new page)."""
+        self.add_request(new_rid)
+        table, copies = self.tables[new_rid], []
+        for i, page in enumerate(self.tables[rid][:-(-length // self.page_size)]):
+            if page == NO_PAGE:
+                table.append(NO_PAGE)
+            elif (i + 1) * self.page_size <= length:
+                table.append(self.pool.share(page))
+            else:
+                table.append(self.pool.allocate())
+                copies.append((page, table[-1]))
+        return copies
+
+    def release_behind(self, rid, length: int) -> int:
+        """Give back the pages behind the first ``length`` tokens.  Returns how many."""
+        table = self.tables[rid]
+        n = 0
+        while len(table) > -(-length // self.page_size):
+            page = table.pop()
+            if page != NO_PAGE:
+                self.pool.free(page)
+                n += 1
+        return n
+
+    def pack(self) -> List[Tuple[int, int]]:
+        """The pages that are held become the lowest ids of the pool; returns the copies (old page, new page) that this takes."""
+        moves = self.pool.pack()
+        for table in self.tables.values():
+            table[:] = [moves.get(page, page) for page in table]
+        return list(moves.items())
+
+    def copy_pages(self, copies: List[Tuple[int, int]]) -> None:
+        """Copies page contents in every entry of the group (nothing without device memory)."""
+        if not copies or self.kv is None:
+            return
+        from ..kernels import ops
+        pairs = torch.tensor(copies, dtype=torch.int32).to(self.kv.device, non_blocking=True)
+        for pools in self.pools():
+            ops.cache_copy_pages(pools, pairs, None)
+
+    def pools(self) -> List[torch.Tensor]:
+        """The group's tensors as ``[entries, planes, pages, n_kv, page_size, width]``."""
+        if self.kv is None:
+            return []
+        return [self.kv] if self.v_only is None else [self.kv, self.v_only.unsqueeze(1)]
 
     def free_request(self, rid) -> int:
         table = self.tables.pop(rid)

@@ -13,6 +13,7 @@ All methods are host-side and cheap; with ``device=None`` no device memory is to
 """
 from __future__ import annotations
 
+import collections
 import dataclasses
 from typing import Dict, List, Optional, Sequence, Tuple
 
@@ -144,6 +145,52 @@ class CacheManager:
         for g in self.groups:
             g.release_behind_window(rid, r.length)
 
+    def commit_kept(self, rid, kept: int) -> None:
+        """The step that wrote the nodes of a tree behind the request's tokens, and the moves that brought the ``kept`` accepted ones
+        to the front, are enqueued: advance the length by those and give back the pages behind them."""
+        r = self._requests[rid]
+        r.length += kept
+        for g in self.groups:
+            g.release_behind(rid, r.length)
+            g.release_behind_window(rid, r.length)
+
+    def fork(self, rid, new_rids: Sequence[object]) -> None:
+        """New requests with the tokens that ``rid`` has cached.  Full pages are shared, every fork gets its own copy of a partly filled
+        last page and of the state slot; all of them or none.  The copies run on the current stream."""
+        if rid not in self._requests:
+            raise PhotonError(ErrorCode.INVALID_STATE, f"request {rid!r} is not live")
+        new_rids = list(new_rids)
+        for i, new in enumerate(new_rids):
+            if new in self._requests or new in new_rids[:i]:
+                raise PhotonError(ErrorCode.INVALID_STATE, f"request {new!r} is already live")
+        length = self._requests[rid].length
+        if len(new_rids) > self.states.num_free:
+            raise PhotonError(ErrorCode.OUT_OF_MEMORY, f"{len(new_rids)} request slots wanted, {self.states.num_free} free")
+        for gi, g in enumerate(self.groups):
+            need = g.pages_to_fork(length) * len(new_rids)
+            if need > g.pool.num_free:
+                raise PhotonError(ErrorCode.OUT_OF_MEMORY, f"{len(new_rids)} forks of request {rid!r} need {need} more cache pages in group {gi}, "
+                                  f"{g.pool.num_free} of {g.num_pages} are free")
+        copies: List[List[Tuple[int, int]]] = [[] for _ in self.groups]
+        for new in new_rids:
+            self.states.allocate(new)
+            self.states.copy(rid, new)
+            for c, g in zip(copies, self.groups):
+                c.extend(g.fork(rid, new, length))
+            self._requests[new] = _Request(length)
+        for c, g in zip(copies, self.groups):
+            g.copy_pages(c)
+
+    def pack(self) -> int:
+        """Moves the contents of held pages so that they are the lowest ids of their pools (what lies behind them is unused
+        then).  Returns how many pages moved; the copies run on the current stream."""
+        moved = 0
+        for g in self.groups:
+            copies = g.pack()
+            g.copy_pages(copies)
+            moved += len(copies)
+        return moved
+
     def free_request(self, rid) -> None:
         if rid not in self._requests:
             raise PhotonError(ErrorCode.DOUBLE_FREE, f"request {rid!r} is not live")
@@ -220,14 +267,14 @@ class CacheManager:
         return total
 
     def check_consistency(self) -> None:
-        """No page lost, held twice or free while held (used by tests)."""
+        """No page lost, in more or fewer tables than it has holders, or free while held (used by tests)."""
         for gi, g in enumerate(self.groups):
-            held = [p for t in g.tables.values() for p in t if p != NO_PAGE]
-            if len(held) != len(set(held)):
-                raise PhotonError(ErrorCode.INVALID_STATE, f"group {gi}: a page is held twice")
+            held = collections.Counter(p for t in g.tables.values() for p in t if p != NO_PAGE)
+            for p, n in held.items():
+                if not g.pool.is_allocated(p):
+                    raise PhotonError(ErrorCode.INVALID_STATE, f"group {gi}: page {p} is in a table but free")
+                if n != g.pool.holders(p):
+                    raise PhotonError(ErrorCode.INVALID_STATE, f"group {gi}: page {p} is in {n} tables but has {g.pool.holders(p)} holders")
             if len(held) != g.pool.num_allocated:
                 raise PhotonError(ErrorCode.INVALID_STATE,
                                   f"group {gi}: {g.pool.num_allocated} pages are out but {len(held)} are in tables")
-            for p in held:
-                if not g.pool.is_allocated(p):
-                    raise PhotonError(ErrorCode.INVALID_STATE, f"group {gi}: page {p} is in a table but free")

@@ -41,6 +41,11 @@ class StateSlotPool:
             t[slot].zero_()
         return slot
 
+    def copy(self, rid, new_rid) -> None:
+        """The state of ``rid`` into the slot of ``new_rid``."""
+        for t in self.tensors.values():
+            t[self._owner[new_rid]].copy_(t[self._owner[rid]])
+
     def slot_of(self, rid) -> int:
         return self._owner[rid]
 
