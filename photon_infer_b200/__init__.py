@@ -16,6 +16,9 @@ def __getattr__(name):
     if name in ("ContinuousBatchEngine", "generate"):
         from .engine import engine as _e
         return getattr(_e, name)
+    if name in ("DraftingGenerator", "generate_drafted"):
+        from .engine import drafting as _d
+        return getattr(_d, name)
     if name == "write_random_model":
         from .weights import write_random_model
         return write_random_model

@@ -41,6 +41,10 @@ def main(argv=None) -> int:
     ap.add_argument("--chunk-size", type=int, default=256, help="longest prompt portion of a request in one step")
     ap.add_argument("--max-batched-tokens", type=int, default=2048, help="token budget of one step")
     ap.add_argument("--max-model-len", type=int, default=None)
+    ap.add_argument("--draft-nodes", type=int, default=0, metavar="N",
+                    help="decode with trees of up to N tokens drafted from the request's own text (0: one token a step)")
+    ap.add_argument("--draft-depth", type=int, default=6, help="longest draft")
+    ap.add_argument("--samples", type=int, default=1, help="answers to each prompt, with --draft-nodes; they share the prompt's cache pages")
     ap.add_argument("--random-weights", metavar="CONFIG_JSON",
                     help="write a model folder with random weights from this config.json into checkpoint_path first")
     ap.add_argument("--init-std", type=float, default=0.02)
@@ -76,6 +80,22 @@ def main(argv=None) -> int:
                                 chunk_size=args.chunk_size, max_num_batched_tokens=args.max_batched_tokens,
                                 max_model_len=args.max_model_len, seed=args.seed, device=device)
         print("PhotonInfer B200 - LLaMA Inference", file=sys.stderr)
+        if args.samples > 1 and args.draft_nodes < 1:
+            print("llama_infer: --samples needs --draft-nodes", file=sys.stderr)
+            return 1
+        if args.draft_nodes > 0:
+            from .drafting import DraftingGenerator
+            from .loading import build_runner
+            generator = DraftingGenerator(build_runner(args.checkpoint_path, options), options, args.draft_nodes, args.draft_depth)
+            t0 = time.perf_counter()
+            answers = generator.generate(prompts, args.max_new_tokens, args.temperature, args.seed, args.ignore_eos, args.samples)
+            dt = time.perf_counter() - t0
+            for i, tokens in enumerate(answers):
+                print(f"request {i}: " + " ".join(str(t) for t in tokens))
+            st = generator.stats
+            print(f"Generated {st.generated} tokens in {dt:.3f} s ({st.generated / dt:.1f} tokens/s), {st.steps} steps of trees, "
+                  f"{st.nodes} nodes", file=sys.stderr)
+            return 0
         engine = ContinuousBatchEngine(args.checkpoint_path, options)
         ids = [engine.add_request(p, args.max_new_tokens, args.temperature, args.seed, args.ignore_eos) for p in prompts]
         t0 = time.perf_counter()

@@ -19,7 +19,7 @@ import torch
 from ..cache.manager import CacheManager
 from ..errors import ErrorCode, PhotonError
 from ..models.model import CausalLM
-from ..parts.base import GroupView, StepContext
+from ..parts.base import GroupView, StepContext, TreeView
 
 
 @dataclasses.dataclass
@@ -37,6 +37,37 @@ class StepResult:
 
 
 @dataclasses.dataclass
+class TreeEntry:
+    """A request's drafted tree: ``tokens[0]`` is its last token, which is not cached yet, the others are drafts; ``parents[i]`` is the place
+    of an earlier token that ``tokens[i]`` would follow (-1 for the first)."""
+    request_id: object
+    tokens: Sequence[int]
+    parents: Sequence[int]
+
+
+@dataclasses.dataclass
+class TreeStepResult:
+    tokens: List[List[int]]             # per entry: the tokens it has generated, one for every node it went through
+    paths: List[List[int]]              # per entry: those nodes, in order; their keys and values are cached now
+    logits: torch.Tensor                # float32 [T, vocab] on the device
+
+
+def tree_layout(parents: Sequence[int], words: int):
+    """(depths, mask words int32 [n, words]) of a tree's nodes: a node sees itself and what it descends from."""
+    n = len(parents)
+    depth = np.zeros(n, dtype=np.int32)
+    seen = np.zeros((n, words * 32), dtype=bool)
+    for i, p in enumerate(parents):
+        if (p != -1) if i == 0 else not 0 <= p < i:
+            raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"node {i} of a tree follows node {p}: the first follows none (-1), the others an earlier one")
+        if i:
+            depth[i] = depth[p] + 1
+            seen[i] = seen[p]
+        seen[i, i] = True
+    return depth, np.packbits(seen, axis=1, bitorder="little").view("<i4")
+
+
+@dataclasses.dataclass
 class _DecodeGraph:
     graph: "torch.cuda.CUDAGraph"
     static_input: torch.Tensor
@@ -50,6 +81,10 @@ class _DecodeGraph:
 #: computes and stores exactly what the original does, and its logits are dropped), so that a batch that
 #: shrinks by one request replays a graph it already has instead of capturing a new one.
 GRAPH_BATCH_SIZES = (1, 2, 3, 4, 6, 8, 12, 16, 24, 32, 48, 64, 96, 128, 192, 256, 384, 512)
+
+
+#: What a step of drafted trees launches beside the model's own modules.
+TREE_MODULES = ("tree_attention", "tree_attention_tc", "tree_attention_few", "tree_accept", "cache_rows")
 
 
 def graph_batch_size(n: int) -> int:
@@ -161,6 +196,74 @@ class ModelRunner:
         self.tokens += sum(len(e.tokens) for e in entries)
         return StepResult(logits, rows, tokens)
 
+    # ------------------------------------------------------------------ steps of drafted trees
+    def tree_step(self, entries: Sequence[TreeEntry], depth: Optional[int] = None, sampling: Optional[tuple] = None) -> TreeStepResult:
+        """Runs the trees' tokens as one batch, keeps of each request the path on which the drafts are what the model generates, and
+        returns the tokens it has generated: one more than drafts were accepted, so at least one.  The last of them is not cached yet; it is
+        the next tree's first token.  ``depth``: nodes that a path may have at most (default: as the deepest tree).  ``sampling``: (temperatures, one per
+        entry; uniform numbers, one per node in order); greedy without.  Waits for the result."""
+        from ..csrc.build import ensure_built
+        from ..kernels import ops
+        cache = self.cache
+        entries = list(entries)
+        if not entries:
+            return TreeStepResult([], [], torch.empty((0, self.model.spec.vocab_size), dtype=torch.float32, device=self.device))
+        if not all(getattr(self.model.blocks[e.layer].mixer(), "supports_trees", False) for e in self.model.spec.run):
+            raise PhotonError(ErrorCode.UNSUPPORTED_MODEL, "a mixer of this model cannot run drafted trees")
+        seen = set()
+        for e in entries:
+            if e.request_id in seen:
+                raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"request {e.request_id!r} appears twice in one step")
+            seen.add(e.request_id)
+            if not cache.has_request(e.request_id):
+                raise PhotonError(ErrorCode.INVALID_STATE, f"request {e.request_id!r} is not registered with the cache")
+            if len(e.tokens) != len(e.parents) or not e.tokens:
+                raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"the tree of request {e.request_id!r} needs a token and a parent per node")
+            if cache.length(e.request_id) + len(e.tokens) > self.max_model_len:
+                raise PhotonError(ErrorCode.INVALID_ARGUMENT,
+                                  f"request {e.request_id!r} would exceed the longest request of {self.max_model_len} tokens")
+        T = sum(len(e.tokens) for e in entries)
+        if sampling is not None and (len(sampling[0]) != len(entries) or len(sampling[1]) != T):
+            raise PhotonError(ErrorCode.INVALID_ARGUMENT, "sampling needs a temperature per entry and a uniform number per node")
+        most = max(len(e.tokens) for e in entries)
+        layouts = [tree_layout(e.parents, -(-most // 32)) for e in entries]
+        need = [0] * len(cache.groups)
+        for e in entries:
+            for g, n in enumerate(cache.pages_needed(e.request_id, len(e.tokens))):
+                need[g] += n
+        for g, n in enumerate(need):
+            if n > cache.groups[g].pool.num_free:
+                raise PhotonError(ErrorCode.OUT_OF_MEMORY,
+                                  f"the step needs {n} more cache pages in group {g}, "
+                                  f"{cache.groups[g].pool.num_free} of {cache.groups[g].num_pages} are free")
+        ensure_built(TREE_MODULES)
+        for e in entries:
+            cache.extend(e.request_id, len(e.tokens))
+        steps = [StepEntry(e.request_id, e.tokens, range(len(e.tokens))) for e in entries]
+        ctx, logit_rows, _ = self._build_context(steps, trees=(entries, layouts, sampling))
+        logits = self.model.forward(ctx, self._layer_caches, logit_rows)
+        D = min(depth or T, int(max(d.max() for d, _ in layouts)) + 1)
+        S = len(entries)
+        answer = torch.empty(S * (2 * D + 1) + 4, dtype=torch.int32, device=self.device)
+        path, sampled, counts = answer[:S * D].view(S, D), answer[S * D: 2 * S * D].view(S, D), answer[2 * S * D: S * (2 * D + 1)]
+        ops.tree_accept(logits, ctx.token_ids, ctx.tree.parents, ctx.cu_tokens, S, most, path, counts, sampled,
+                        self._temps if sampling is not None else None, self._uniforms if sampling is not None else None, self.error_flag)
+        for g, view in zip(cache.groups, ctx.groups):
+            for pools in g.pools():
+                ops.cache_keep(pools, view.block_table, ctx.cu_tokens, ctx.context_lens, path, counts, S, self.error_flag)
+        answer[S * (2 * D + 1):].copy_(self.error_flag)
+        host = answer.tolist()
+        self.raise_device_error(host[-4:])
+        result = TreeStepResult([], [], logits)
+        for s, e in enumerate(entries):
+            kept = host[2 * S * D + s]
+            result.paths.append(host[s * D: s * D + kept])
+            result.tokens.append(host[(S + s) * D: (S + s) * D + kept])
+            cache.commit_kept(e.request_id, kept)
+        self.steps += 1
+        self.tokens += T
+        return result
+
     def _sample(self, logits: torch.Tensor) -> torch.Tensor:
         """Samples every row of ``logits`` with the temperatures and uniform numbers of the last built step."""
         from ..kernels import ops
@@ -171,11 +274,12 @@ class ModelRunner:
 
     def _build_context(self, entries: Sequence[StepEntry], widths: Optional[List[int]] = None,
                        static_input: Optional[torch.Tensor] = None, bound_context: Optional[int] = None,
-                       sampling: Optional[tuple] = None, stateless_from: Optional[int] = None):
+                       sampling: Optional[tuple] = None, stateless_from: Optional[int] = None, trees: Optional[tuple] = None):
         """Builds every index array of the step in one pinned buffer and copies it to the device once.
         ``widths``: block-table widths to use (default: what the requests need).  ``static_input``: a
         device buffer of the same layout to copy into (for a captured graph).  ``bound_context``: the
-        context length that kernels may assume as an upper bound when they size their grids."""
+        context length that kernels may assume as an upper bound when they size their grids.  ``trees``: (tree entries, their
+        layouts, sampling) of a step of drafted trees."""
         cache = self.cache
         S = len(entries)
         q_lens = [len(e.tokens) for e in entries]
@@ -189,6 +293,10 @@ class ModelRunner:
         # layout of the one staging buffer (int32 counts)
         n_samp = n_want if sampling is not None else 0
         sizes = [T, T, T, S + 1, S, S, n_want] + [T] * G + [S * w for w in widths] + [n_samp, n_samp]
+        if trees is not None:
+            words = trees[1][0][1].shape[1]
+            sizes[-2:] = [S, T] if trees[2] is not None else [0, 0]
+            sizes += [T, T * words]
         offs = np.concatenate([[0], np.cumsum([(s + 3) // 4 * 4 for s in sizes])]).astype(np.int64)
         total = int(offs[-1])
         self._last_total = total
@@ -199,7 +307,7 @@ class ModelRunner:
         seg = lambda i: host[offs[i]: offs[i] + sizes[i]]
         tok, pos, tseq, cu, ctxl, slots, lrows = (seg(i) for i in range(7))
         rows: List[tuple] = []
-        if T == S:
+        if T == S and trees is None:
             # every request brings one token (a decode step): whole arrays at once
             tok[:] = [e.tokens[0] for e in entries]
             pos[:] = starts
@@ -248,6 +356,15 @@ class ModelRunner:
                     cache.fill_slot_mapping(g, e.request_id, starts[s], q_lens[s], sm[t:t + q_lens[s]])
                     t += q_lens[s]
                 cache.fill_block_table(g, rids, seg(7 + G + g).reshape(S, widths[g]))
+        if trees is not None:
+            tree_entries, layouts, sampling = trees
+            seg(9 + 2 * G)[:] = [p for e in tree_entries for p in e.parents]
+            mask, t = seg(10 + 2 * G).reshape(T, words), 0
+            for n, start, (depth, bits) in zip(q_lens, starts, layouts):
+                pos[t:t + n] = start + depth
+                mask[t:t + n] = bits
+                t += n
+            n_samp = 0 if sampling is None else T
         if sampling is not None and n_samp:
             seg(7 + 2 * G).view(np.float32)[:] = sampling[0]
             seg(8 + 2 * G).view(np.float32)[:] = sampling[1]
@@ -268,6 +385,8 @@ class ModelRunner:
             host_query_lens=q_lens, host_context_lens=[a + b for a, b in zip(starts, q_lens)],
             host_start_positions=starts, host_state_slots=[int(x) for x in slots[:S]], max_query_len=max(q_lens),
             max_context_len=bound_context or max(a + b for a, b in zip(starts, q_lens)), error_flag=self.error_flag)
+        if trees is not None:
+            ctx.tree = TreeView(parents=dseg(9 + 2 * G), mask=dseg(10 + 2 * G).view(T, words))
         if sampling is not None:
             self._temps = dseg(7 + 2 * G).view(torch.float32)
             self._uniforms = dseg(8 + 2 * G).view(torch.float32)

@@ -106,6 +106,10 @@ class PagedAttention(Mixer):
         self.attend(q, attn, ctx, cache)
         return project(attn, self.w_o), residual
 
+    @property
+    def supports_trees(self) -> bool:
+        return self.head_dim <= 256
+
     # -- one step
     def forward(self, h: torch.Tensor, ctx: StepContext, cache: LayerCache) -> torch.Tensor:
         T = h.shape[0]
@@ -149,7 +153,11 @@ class PagedAttention(Mixer):
 
     def attend(self, q: torch.Tensor, out: torch.Tensor, ctx: StepContext, cache: LayerCache) -> None:
         """bfloat16 with a head size the tensor-core kernel is compiled for: that kernel.  float32 and
-        other sizes: the general kernel, whose sums depend only on a token's position."""
+        other sizes: the general kernel, whose sums depend only on a token's position.  A step of drafted trees: the kernels
+        whose masks follow the trees."""
+        if getattr(ctx, "tree", None) is not None:
+            attend_tree(self, q, out, ctx, cache)
+            return
         if ops.flash_attention_supported(q.dtype, self.head_dim):
             attend_tensor_cores(self, q, out, ctx, cache)
             return
@@ -160,6 +168,14 @@ class PagedAttention(Mixer):
             return
         ops.paged_attention(q, out, cache.k, cache.v, group.block_table, ctx.token_seq, ctx.positions,
                             self.n_q, self.n_kv, self.head_dim, self.window, self.scale, ctx.error_flag)
+
+
+def attend_tree(mixer, q: torch.Tensor, out: torch.Tensor, ctx: StepContext, cache: LayerCache, sink: Optional[torch.Tensor] = None,
+                softcap: Optional[float] = None) -> None:
+    """A step of drafted trees for ``mixer`` (``n_q``, ``n_kv``, ``head_dim``, ``window``, ``scale``; values as wide as keys)."""
+    ops.tree_attention(q, out, cache.k, cache.v, ctx.groups[cache.group].block_table, ctx.cu_tokens, ctx.context_lens, ctx.positions,
+                       ctx.tree.mask, ctx.num_seqs, ctx.max_query_len, ctx.max_context_len, mixer.n_q, mixer.n_kv, mixer.head_dim,
+                       mixer.window, mixer.scale, ctx.error_flag, sink=sink, softcap=softcap)
 
 
 def rows_together(ctx: StepContext, q: torch.Tensor, out: torch.Tensor, cache: LayerCache, n_q: int, n_kv: int, head_dim: int) -> bool:

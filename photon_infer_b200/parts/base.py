@@ -113,6 +113,14 @@ class LayerCache:
 
 
 @dataclasses.dataclass
+class TreeView:
+    """The drafted trees of a step: the tokens of a request are the nodes of its tree, node 0 its last token.  ``positions`` of the step are places
+    on the nodes' paths, their rows of the cache lie one behind the other."""
+    parents: torch.Tensor           # int32 [T]; index among the request's nodes, -1 for node 0
+    mask: torch.Tensor              # int32 [T, words]; bit i: the node sees node i of its request
+
+
+@dataclasses.dataclass
 class StepContext:
     """Everything a part may read about the current step.
 
@@ -138,6 +146,7 @@ class StepContext:
     error_flag: Optional[torch.Tensor] = None   # int32 [4] written by kernels on bad indices
     scratch: Optional[object] = None            # engine.workspace.Workspace
     host_state_slots: Sequence[int] = ()        # host copy of state_slots
+    tree: Optional[TreeView] = None             # set: the step's tokens are drafted trees (mixers with ``supports_trees``)
 
 
 # ----------------------------------------------------------------------------- parts
@@ -290,6 +299,8 @@ class Mixer(Part):
     #: True when the mixer treats a negative state slot as "start from a zero state and store nothing"; decode
     #: steps of a model whose stateful mixers all do are replayed as CUDA graphs.
     state_skips_negative_slots = False
+    #: True when the mixer runs steps whose tokens are the nodes of drafted trees (``StepContext.tree``).
+    supports_trees = False
 
     def cache_spec(self) -> Optional[PagedCacheSpec]:
         return None

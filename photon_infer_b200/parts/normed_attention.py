@@ -22,7 +22,7 @@ from typing import Dict, List, Optional
 import torch
 
 from ..kernels import ops
-from .attention import attend_tensor_cores, rows_together
+from .attention import attend_tensor_cores, attend_tree, rows_together
 from .base import LayerCache, Mixer, PagedCacheSpec, StepContext, TensorSpec
 from .linear import project
 from .registry import register_mixer
@@ -133,6 +133,10 @@ class NormedAttention(Mixer):
     def cache_spec(self) -> Optional[PagedCacheSpec]:
         return PagedCacheSpec(self.n_kv, self.head_dim, self.window, value_dim=self.value_dim, keep_first=self.keep_first)
 
+    @property
+    def supports_trees(self) -> bool:
+        return self.value_dim == self.head_dim <= 256 and not self.keep_first
+
     # -- one step
     def forward(self, h: torch.Tensor, ctx: StepContext, cache: LayerCache) -> torch.Tensor:
         T = h.shape[0]
@@ -160,7 +164,12 @@ class NormedAttention(Mixer):
         """bfloat16 with heads and values the tensor-core kernels are compiled for (multiples of 16 up to 128): those
         kernels, tcgen05 for prompt portions and the split-key kernel for decoded tokens.  float32 and other sizes:
         the general kernel, whose sums depend on a token's position alone; its bfloat16 decode steps share a
-        token's keys out over blocks."""
+        token's keys out over blocks.  A step of drafted trees: the kernels whose masks follow the trees."""
+        if getattr(ctx, "tree", None) is not None:
+            attend_tree(self, q, out, ctx, cache, self.sinks, self.softcap)
+            if gate is not None:
+                ops.gate_mul(out, gate)
+            return
         if self._flash_ok(q.dtype):
             attend_tensor_cores(self, q, out, ctx, cache, keep_first=self.keep_first, sink=self.sinks, softcap=self.softcap,
                                 gate=gate)
