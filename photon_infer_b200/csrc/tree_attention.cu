@@ -5,10 +5,16 @@
 // (bounded scores: x_j = softcap tanh(scale q . k_j / softcap); m the largest of the scores and the sink) over the keys that node t sees
 // (tree_attention.cuh); a row that sees nothing is zero.  Scores, weights, sums and outputs are held in 32 bits.
 //
-// A block takes 32 rows, (node, query head) pairs that share a key/value head, and a share of the request's keys, in tiles of 32.  A thread holds the scores
-// of four rows with two keys, then the outputs of those rows for D / 16 numbers; its rows' other scores lie with the 15 threads beside it, so
-// maxima and sums are butterflies inside half a warp and the weights pass through shared memory between the lanes of one warp.
-// Shares are joined in their order by a second kernel.
+// A block takes 32 rows, (node, query head) pairs that share a key/value head, and a share of the request's keys, in tiles of 64; a warp has 16 of the rows and half a
+// tile's keys.  A thread holds the scores of four rows with four keys, then those rows' outputs for D / 8 numbers, and a lane's neighbours read the same operands, so
+// that a product costs a quarter of a word of shared memory; products go in pairs (fma.rn.f32x2).  Each warp has its own maxima and sums; the
+// weights pass through shared memory inside the warp.  The warps' results, and those of a cluster of up to eight blocks that share a row tile's keys, are joined in
+// shared memory in their order; where more blocks share them, by a second kernel.
+//
+// What bounds it: 32-bit products.  4 requests of 13 nodes behind up to 700 keys (32/8 heads of 64): 25 us, 1 us of it for the bytes; 8 of 32 behind up to 2,000:
+// 104 us = 15 TFLOP/s of products that are needed.  A tile ahead in shared memory left two blocks an SM and was slower (32 and 25 us, 132 and 108);
+// tiles of 32 keys 23 and 118; four warps for a row's keys 23 and 116; the sums of products in one number after the other, 32 keys a tile,
+// 36 and 334.
 //
 // A key that a row does not see has weight 0, and 0 times a value that is not finite would not be: in tiles where masks cut, products with a weight of 0
 // are left out, and rows behind the last key or of a missing page are zeros.
@@ -16,27 +22,83 @@
 #include <math.h>
 
 #define TG_ROWS 32
-#define TG_KEYS 32
-#define TG_THREADS 128
-#define TG_PS (TG_KEYS + 4)
+#define TG_KEYS 64
+#define TG_SHARES 2                                // warps that share a row's keys
+#define TG_THREADS (64 * TG_SHARES)
+#define TG_MINE (TG_KEYS / TG_SHARES)              // a warp's keys
+#define TG_PS (TG_MINE + 4)                        // row stride of a warp's weights, [16][TG_MINE]
 
 struct TreeShares {
   float* part_o;                                   // [T * n_q, splits, d]
   float* part_ml;                                  // [T * n_q, splits, 2]: maximum and sum of a share
-  int splits, row_tiles;
+  int splits, cluster, row_tiles;                  // cluster: the shares of a row tile are a cluster's blocks, which join them; else 1
 };
+
+// Four neighbouring numbers of a row in shared memory, in 32 bits.
+__device__ __forceinline__ float4 tg_four(const float* p) { return *(const float4*)p; }
+__device__ __forceinline__ float4 tg_four(const bf16* p) {
+  const uint2 u = *(const uint2*)p;
+  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16), __uint_as_float(u.y & 0xffff0000u));
+}
+
+// 16 bytes into shared memory, without waiting; zeros where nothing is to be read.
+__device__ __forceinline__ void tg_copy16(void* dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" :: "r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src), "r"(there ? 16 : 0) : "memory");
+}
+
+// Keys and values of a tile into shared memory; rows that are not there and the columns behind d are zeros.
+template <typename T, int D, int KS>
+__device__ __forceinline__ void tg_load_tile(const TreeParams& P, const long long* krow, T* ks, T* vs, bool wide, int tid) {
+  const T* kc = (const T*)P.k_cache;
+  const T* vc = (const T*)P.v_cache;
+  constexpr int E = 16 / (int)sizeof(T), PIECES = D / E;
+  if (wide) {
+#pragma unroll
+    for (int e = tid; e < TG_KEYS * PIECES; e += TG_THREADS) {
+      const int r = e / PIECES, j = e % PIECES * E;
+      const long long at = krow[r];
+      const bool there = at >= 0 && j < P.d;
+      const size_t from = there ? (size_t)at * P.d + j : 0;
+      tg_copy16(ks + r * KS + j, kc + from, there);
+      tg_copy16(vs + r * D + j, vc + from, there);
+    }
+  } else {                                         // rows that do not begin at 16 bytes
+    for (int e = tid; e < TG_KEYS * D; e += TG_THREADS) {
+      const int r = e / D, j = e % D;
+      const long long at = krow[r];
+      const bool there = at >= 0 && j < P.d;
+      ks[r * KS + j] = there ? kc[at * P.d + j] : from_f32<T>(0.f);
+      vs[r * D + j] = there ? vc[at * P.d + j] : from_f32<T>(0.f);
+    }
+  }
+  asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
+}
+
+template <typename T, int D>
+constexpr size_t tg_smem_bytes() {
+  const size_t tile = TG_KEYS * (D + 16 / sizeof(T) + D) * sizeof(T), results = TG_SHARES * TG_ROWS * (D + 4) * sizeof(float);
+  return (size_t)(TG_ROWS * (D + 4) + 2 * TG_SHARES * 16 * TG_PS) * sizeof(float) + (tile > results ? tile : results);
+}
+
+// Two products and sums at once, each rounded like fmaf.
+__device__ __forceinline__ void tg_fma2(float2& acc, const float2 a, const float2 b) {
+  asm("{\n\t.reg .b64 x, y, z;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%0, %1};\n\tfma.rn.f32x2 z, x, y, z;\n\t"
+      "mov.b64 {%0, %1}, z;\n\t}" : "+f"(acc.x), "+f"(acc.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+}
 
 template <typename T, int D>
 __global__ void __launch_bounds__(TG_THREADS)
 tree_attention_kernel(const TreeParams P, const TreeShares H) {
-  constexpr int S = D + 4, C4 = D / 64;            // row stride in shared memory; groups of four output numbers a thread has
+  constexpr int S = D + 4, C = D / 32, U = TG_MINE / 8;             // row stride of the queries; groups of four output numbers a thread has
+  constexpr int KS = D + 16 / (int)sizeof(T);         // row stride of the keys
   extern __shared__ __align__(16) float tg_smem[];
   float* qs = tg_smem;                             // [TG_ROWS][S]
-  float* ks = qs + TG_ROWS * S;                    // [TG_KEYS][S]
-  float* vs = ks + TG_KEYS * S;                    // [TG_KEYS][D]
-  float* ps = vs + TG_KEYS * D;                    // [TG_ROWS][TG_PS]
+  float* ps = qs + TG_ROWS * S;                    // per warp [16][TG_PS]
+  T* ks = (T*)(ps + 2 * TG_SHARES * 16 * TG_PS);               // [TG_KEYS][KS]
+  T* vs = ks + TG_KEYS * KS;                       // [TG_KEYS][D]
   __shared__ long long krow[TG_KEYS];
-  __shared__ uint32_t seen[TG_ROWS];
+  __shared__ float ml_s[2][TG_SHARES][TG_ROWS], factor[TG_ROWS][8 * TG_SHARES];
+  __shared__ uint32_t seen[2][2][TG_ROWS];   // a warp may be at work on the tile before when the next one's are found
   pdl_wait();
   int b = blockIdx.x;
   const int split = b % H.splits; b /= H.splits;
@@ -47,7 +109,8 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
   if (row0 >= rows) return;
   const int nrows = min(TG_ROWS, rows - row0);
   const int* table = P.block_table + (size_t)seq * P.max_pages;
-  const int tid = threadIdx.x, tr = tid >> 4, tc = tid & 15;     // rows tr + 8 i; keys tc, tc + 16; columns 4 tc + 64 j
+  const int tid = threadIdx.x, lane = tid & 31, rw = (tid >> 5) & 1, kw = tid >> 6;
+  const int lr = lane >> 3, lc = lane & 7;         // rows 16 rw + lr + 4 i; keys TG_MINE kw + lc + 8 u; columns 4 lc + 32 c
 
   // the first cached key that any of the rows sees
   int key_lo = 0;
@@ -59,120 +122,142 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
   }
   const int key_end = R.base + R.n;
   const int tile0 = key_lo / TG_KEYS, tiles = (key_end + TG_KEYS - 1) / TG_KEYS - tile0;
-  const int per = (tiles + H.splits - 1) / H.splits;
-  const int begin = tile0 + split * per, end = min(tile0 + tiles, begin + per);
+  const int begin = tile0 + (int)((long long)tiles * split / H.splits), end = tile0 + (int)((long long)tiles * (split + 1) / H.splits);
+  // what threads r and r + 32 know of row r; rows that are none see every key, so that they cut no tile
+  const int my_t = tid < TG_KEYS && lane < nrows ? R.tok0 + (row0 + lane) / G : -1;
+  const int my_lo = my_t >= 0 && P.window > 0 ? max(0, P.positions[my_t] - P.window + 1) : 0;
+  // Table entries are read a tile before the rows they lead to.
+  auto entry = [&](int tile) {
+    const int key = tile * TG_KEYS + tid, at = key / P.page_size;
+    return tid < TG_KEYS && tile < end && key >= key_lo && key < key_end && at < P.max_pages ? table[at] : -1;
+  };
+  auto find = [&](int tile, int page) {            // a tile's rows, and which of them are seen
+    if (tid < TG_KEYS) {
+      const int key = tile * TG_KEYS + tid;
+      long long at = -1;
+      if (key >= key_lo && key < key_end) {
+        if (page >= 0 && page < P.num_pages) at = ((long long)page * P.n_kv + g) * P.page_size + key % P.page_size;
+        else report_error(P.err, PHOTON_DEV_BAD_PAGE, R.tok0, key, page);
+      }
+      krow[tid] = at;
+      const unsigned there = __ballot_sync(0xffffffffu, at >= 0);
+      seen[tile & 1][tid >> 5][lane] = my_t >= 0 ? tree_visible32(P, R, my_t, key - lane, my_lo) & there : there;
+    }
+  };
+  int page = entry(begin);
 
   const T* q = (const T*)P.q;
+#pragma unroll 8
   for (int e = tid; e < TG_ROWS * D; e += TG_THREADS) {
     const int r = e / D, j = e % D, row = row0 + r;
     qs[r * S + j] = r < nrows && j < d ? to_f32(q[(size_t)(R.tok0 + row / G) * P.q_stride + (size_t)(g * G + row % G) * d + j]) : 0.f;
   }
-  // what thread r < 32 knows of row r
-  const int my_t = tid < nrows ? R.tok0 + (row0 + tid) / G : -1;
-  const int my_lo = my_t >= 0 && P.window > 0 ? max(0, P.positions[my_t] - P.window + 1) : 0;
 
-  float m[4], l[4], o[4][C4 * 4];
+  float m[4], l[4];                                // l: of this thread's keys
+  float2 o[4][C * 2];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     m[i] = -INFINITY; l[i] = 0.f;
 #pragma unroll
-    for (int j = 0; j < C4 * 4; ++j) o[i][j] = 0.f;
+    for (int j = 0; j < C * 2; ++j) o[i][j] = make_float2(0.f, 0.f);
   }
-  const T* kc = (const T*)P.k_cache;
-  const T* vc = (const T*)P.v_cache;
+  const float* my_q = qs + (16 * rw + lr) * S;
+  const T* my_k = ks + (TG_MINE * kw + lc) * KS;
+  const T* my_v = vs + TG_MINE * kw * D + lc * 4;
+  float* my_p = ps + (tid >> 5) * 16 * TG_PS;
+  const bool wide = (size_t)d * sizeof(T) % 16 == 0 && ((((uintptr_t)P.k_cache | (uintptr_t)P.v_cache) & 15) == 0);
   for (int tile = begin; tile < end; ++tile) {
-    const int key0 = tile * TG_KEYS;
-    __syncthreads();                               // the tile before is read
-    if (tid < TG_KEYS) {
-      const int key = key0 + tid;
-      const long long at = key < key_end && key >= key_lo ? tree_row(P, table, g, key, R.tok0) : -1;
-      krow[tid] = at;
-      const unsigned there = __ballot_sync(0xffffffffu, at >= 0);
-      seen[tid] = my_t >= 0 ? tree_visible32(P, R, my_t, key0, my_lo) & there : 0u;
-    }
+    find(tile, page);
+    page = entry(tile + 1);
+    __syncthreads();                               // the rows are known; the tile before is read
+    tg_load_tile<T, D, KS>(P, krow, ks, vs, wide, tid);
     __syncthreads();
-    for (int e = tid; e < TG_KEYS * D; e += TG_THREADS) {
-      const int r = e / D, j = e % D;
-      const long long at = krow[r];
-      const bool ok = at >= 0 && j < d;
-      ks[r * S + j] = ok ? to_f32(kc[at * d + j]) : 0.f;
-      vs[r * D + j] = ok ? to_f32(vc[at * d + j]) : 0.f;
-    }
-    __syncthreads();
-    float s[4][2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) s[i][0] = s[i][1] = 0.f;
-#pragma unroll 4
-    for (int j = 0; j < D; j += 4) {
-      const float4 k0 = *(const float4*)(ks + tc * S + j), k1 = *(const float4*)(ks + (tc + 16) * S + j);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const float4 a = *(const float4*)(qs + (tr + 8 * i) * S + j);
-        s[i][0] = fmaf(a.x, k0.x, s[i][0]); s[i][0] = fmaf(a.y, k0.y, s[i][0]);
-        s[i][0] = fmaf(a.z, k0.z, s[i][0]); s[i][0] = fmaf(a.w, k0.w, s[i][0]);
-        s[i][1] = fmaf(a.x, k1.x, s[i][1]); s[i][1] = fmaf(a.y, k1.y, s[i][1]);
-        s[i][1] = fmaf(a.z, k1.z, s[i][1]); s[i][1] = fmaf(a.w, k1.w, s[i][1]);
-      }
-    }
-    bool cut = false;
+    constexpr uint32_t MINE = TG_MINE < 32 ? (1u << (TG_MINE & 31)) - 1u : 0xffffffffu;
+    uint32_t see[4], all = 0xffffffffu, any = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      const uint32_t see = seen[tr + 8 * i];
-      cut |= see != 0xffffffffu;
+      see[i] = seen[tile & 1][TG_MINE * kw >> 5][16 * rw + lr + 4 * i] >> (TG_MINE * kw & 31);
+      all &= see[i] | ~MINE;
+      any |= see[i] & MINE;
+    }
+    if (16 * rw >= nrows || !__any_sync(0xffffffffu, any != 0)) continue;            // none of the warp's rows sees one of its keys
+    float2 s[4][U];
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        float x = s[i][u] * P.scale;
-        if (P.softcap > 0.f) x = P.softcap * tanhf(x / P.softcap);
-        s[i][u] = (see >> (tc + 16 * u)) & 1u ? x : -INFINITY;
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int u = 0; u < U; ++u) s[i][u] = make_float2(0.f, 0.f);
+#pragma unroll 4
+    for (int j = 0; j < D; j += 4) {
+      float4 k[U];
+#pragma unroll
+      for (int u = 0; u < U; ++u) k[u] = tg_four(my_k + u * 8 * KS + j);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const float4 a = *(const float4*)(my_q + i * 4 * S + j);
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+          tg_fma2(s[i][u], make_float2(a.x, a.y), make_float2(k[u].x, k[u].y));
+          tg_fma2(s[i][u], make_float2(a.z, a.w), make_float2(k[u].z, k[u].w));
+        }
       }
-      float mx = fmaxf(s[i][0], s[i][1]);
+    }
 #pragma unroll
-      for (int w = 8; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
+    for (int i = 0; i < 4; ++i) {
+      float x[U], mx = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < U; ++u) {
+        x[u] = (s[i][u].x + s[i][u].y) * P.scale;
+        if (P.softcap > 0.f) x[u] = P.softcap * tanhf(x[u] / P.softcap);
+        x[u] = (see[i] >> (lc + 8 * u)) & 1u ? x[u] : -INFINITY;
+        mx = fmaxf(mx, x[u]);
+      }
+#pragma unroll
+      for (int w = 4; w > 0; w >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, w));
       const float mn = fmaxf(m[i], mx), sub = mn == -INFINITY ? 0.f : mn;
       const float keep = expf(m[i] - sub);         // e^-inf = 0 before the first key
-      const float p0 = expf(s[i][0] - sub), p1 = expf(s[i][1] - sub);
-      float sum = p0 + p1;
-#pragma unroll
-      for (int w = 8; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
       m[i] = mn;
-      l[i] = l[i] * keep + sum;
+      l[i] *= keep;
 #pragma unroll
-      for (int j = 0; j < C4 * 4; ++j) o[i][j] *= keep;
-      ps[(tr + 8 * i) * TG_PS + tc] = p0;
-      ps[(tr + 8 * i) * TG_PS + tc + 16] = p1;
+      for (int u = 0; u < U; ++u) {
+        const float p = expf(x[u] - sub);
+        l[i] += p;
+        my_p[(lr + 4 * i) * TG_PS + lc + 8 * u] = p;
+      }
+#pragma unroll
+      for (int j = 0; j < C * 2; ++j) { o[i][j].x *= keep; o[i][j].y *= keep; }
     }
-    __syncwarp();                                  // a row's weights come from the lanes of this warp
-    if (cut) {
-      for (int k = 0; k < TG_KEYS; ++k) {
+    __syncwarp();
+    if (__any_sync(0xffffffffu, all != 0xffffffffu)) {
+      for (int k = 0; k < TG_MINE; ++k) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = ps[(tr + 8 * i) * TG_PS + k];
+          const float p = my_p[(lr + 4 * i) * TG_PS + k];
           if (p != 0.f) {                          // a NaN is not 0
 #pragma unroll
-            for (int c = 0; c < C4; ++c) {
-              const float4 v = *(const float4*)(vs + k * D + c * 64 + tc * 4);
-              o[i][c * 4] = fmaf(p, v.x, o[i][c * 4]); o[i][c * 4 + 1] = fmaf(p, v.y, o[i][c * 4 + 1]);
-              o[i][c * 4 + 2] = fmaf(p, v.z, o[i][c * 4 + 2]); o[i][c * 4 + 3] = fmaf(p, v.w, o[i][c * 4 + 3]);
+            for (int c = 0; c < C; ++c) {
+              const float4 v = tg_four(my_v + k * D + c * 32);
+              tg_fma2(o[i][2 * c], make_float2(p, p), make_float2(v.x, v.y));
+              tg_fma2(o[i][2 * c + 1], make_float2(p, p), make_float2(v.z, v.w));
             }
           }
         }
       }
     } else {
 #pragma unroll 2
-      for (int k = 0; k < TG_KEYS; k += 4) {
+      for (int k = 0; k < TG_MINE; k += 4) {
         float4 p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = *(const float4*)(ps + (tr + 8 * i) * TG_PS + k);
+        for (int i = 0; i < 4; ++i) p[i] = *(const float4*)(my_p + (lr + 4 * i) * TG_PS + k);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
 #pragma unroll
-          for (int c = 0; c < C4; ++c) {
-            const float4 v = *(const float4*)(vs + (k + u) * D + c * 64 + tc * 4);
+          for (int c = 0; c < C; ++c) {
+            const float4 v = tg_four(my_v + (k + u) * D + c * 32);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
               const float w = u == 0 ? p[i].x : u == 1 ? p[i].y : u == 2 ? p[i].z : p[i].w;
-              o[i][c * 4] = fmaf(w, v.x, o[i][c * 4]); o[i][c * 4 + 1] = fmaf(w, v.y, o[i][c * 4 + 1]);
-              o[i][c * 4 + 2] = fmaf(w, v.z, o[i][c * 4 + 2]); o[i][c * 4 + 3] = fmaf(w, v.w, o[i][c * 4 + 3]);
+              tg_fma2(o[i][2 * c], make_float2(w, w), make_float2(v.x, v.y));
+              tg_fma2(o[i][2 * c + 1], make_float2(w, w), make_float2(v.z, v.w));
             }
           }
         }
@@ -182,34 +267,83 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
   }
   pdl_launch_dependents();
 #pragma unroll
+  for (int i = 0; i < 4; ++i)
+#pragma unroll
+    for (int w = 4; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
+
+  // The warps of a row's keys, and the blocks of a cluster, leave their results where the tiles were.
+  float* po = (float*)ks;                          // [TG_SHARES][TG_ROWS][S]
+  __syncthreads();
+#pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const int r = tr + 8 * i, row = row0 + r;
-    if (r >= nrows) continue;
-    const int t = R.tok0 + row / G, head = g * G + row % G;
-    if (H.splits == 1) {
-      float total = l[i], scale = 1.f;
-      if (P.sinks) {                               // relative to the larger of the two maxima
-        const float top = fmaxf(m[i], P.sinks[head]), sub = top == -INFINITY ? 0.f : top;
-        scale = expf(m[i] - sub);
-        total = l[i] * scale + expf(P.sinks[head] - sub);
-      }
-      const float inv = total != 0.f ? scale / total : 0.f;
-      T* dst = (T*)P.out + (size_t)t * P.out_stride + (size_t)head * d;
+    const int r = 16 * rw + lr + 4 * i;
 #pragma unroll
-      for (int c = 0; c < C4 * 4; ++c) {
-        const int j = (c >> 2) * 64 + tc * 4 + (c & 3);
-        if (j < d) dst[j] = from_f32<T>(l[i] != 0.f ? o[i][c] * inv : 0.f);
-      }
-    } else {
-      const size_t slot = ((size_t)t * P.n_q + head) * H.splits + split;
+    for (int c = 0; c < C; ++c)
+      *(float4*)(po + (kw * TG_ROWS + r) * S + c * 32 + lc * 4) = make_float4(o[i][2 * c].x, o[i][2 * c].y, o[i][2 * c + 1].x, o[i][2 * c + 1].y);
+    if (lc == 0) { ml_s[0][kw][r] = m[i]; ml_s[1][kw][r] = l[i]; }
+  }
+  const int rank = H.cluster > 1 ? split : 0;
+  if (H.cluster > 1) tree_cluster_sync();
+  else __syncthreads();
+  const bool last = H.cluster == H.splits;         // else: a share of several
+  // Each result's factor: 2 TG_SHARES threads a row, four results each.
+  {
+    constexpr int W = 2 * TG_SHARES;
+    const int r = tid / W, n = TG_SHARES * H.cluster;
+    float mx[4], top = -INFINITY, sum = 0.f;
 #pragma unroll
-      for (int c = 0; c < C4 * 4; ++c) {
-        const int j = (c >> 2) * 64 + tc * 4 + (c & 3);
-        if (j < d) H.part_o[slot * d + j] = o[i][c];
-      }
-      if (tc == 0) { H.part_ml[slot * 2] = m[i]; H.part_ml[slot * 2 + 1] = l[i]; }
+    for (int u = 0; u < 4; ++u) {
+      const int w = tid % W + W * u;
+      mx[u] = w < n ? tree_peer(&ml_s[0][w % TG_SHARES][r], w / TG_SHARES) : -INFINITY;
+      top = fmaxf(top, mx[u]);
+    }
+#pragma unroll
+    for (int w = W / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    const float sink = last && P.sinks && r < nrows ? P.sinks[g * G + (row0 + r) % G] : -INFINITY;
+    const float most = fmaxf(top, sink), sub = most == -INFINITY ? 0.f : most;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int w = tid % W + W * u;
+      mx[u] = expf(mx[u] - sub);                   // 0 for what is not there
+      if (w < n) sum += tree_peer(&ml_s[1][w % TG_SHARES][r], w / TG_SHARES) * mx[u];
+    }
+#pragma unroll
+    for (int w = W / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    const float total = sum + (sink == -INFINITY ? 0.f : expf(sink - sub)), inv = !last ? 1.f : sum != 0.f ? 1.f / total : 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (tid % W + W * u < n) factor[r][tid % W + W * u] = mx[u] * inv;
+    if (!last && tid % W == 0 && r < nrows) {
+      const size_t slot = ((size_t)(R.tok0 + (row0 + r) / G) * P.n_q + g * G + (row0 + r) % G) * H.splits + split;
+      H.part_ml[slot * 2] = sub; H.part_ml[slot * 2 + 1] = sum;
     }
   }
+  __syncthreads();
+  const int fours = nrows * (D / 4), stop = fours * (rank + 1) / H.cluster;
+  for (int e = fours * rank / H.cluster + tid; e < stop; e += TG_THREADS) {
+    const int r = e / (D / 4), j = e % (D / 4) * 4, row = row0 + r, t = R.tok0 + row / G, head = g * G + row % G;
+    if (j >= d) continue;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < H.cluster; ++c) {
+#pragma unroll
+      for (int k = 0; k < TG_SHARES; ++k) {
+        const float w = factor[r][TG_SHARES * c + k];
+        const float4 x = tree_peer4(po + (k * TG_ROWS + r) * S + j, c);
+        if (w != 0.f) { a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w); }
+      }
+    }
+    const float v[4] = {a.x, a.y, a.z, a.w};
+    if (last) {
+      T* dst = (T*)P.out + (size_t)t * P.out_stride + (size_t)head * d + j;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) if (j + u < d) dst[u] = from_f32<T>(v[u]);
+    } else {
+      float* dst = H.part_o + (((size_t)t * P.n_q + head) * H.splits + split) * d + j;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) if (j + u < d) dst[u] = v[u];
+    }
+  }
+  if (H.cluster > 1) tree_cluster_sync();          // the others have read this block's results
 }
 
 // Joins the shares of a row in their order: a warp a row.
@@ -244,11 +378,12 @@ tree_join_kernel(const TreeParams P, const TreeShares H) {
 
 template <typename T, int D>
 static int tree_launch(const TreeParams& P, const TreeShares& H, long blocks, cudaStream_t stream) {
-  const size_t smem = (size_t)(TG_ROWS * (D + 4) + TG_KEYS * (D + 4) + TG_KEYS * D + TG_ROWS * TG_PS) * sizeof(float);
+  const size_t smem = tg_smem_bytes<T, D>();
   static bool ready[64] = {};                      // the limit is set once a device
   const int set = tree_smem_limit((const void*)tree_attention_kernel<T, D>, (int)smem, ready);
   if (set != 0) return set;
-  int st = launch_pdl(tree_attention_kernel<T, D>, dim3((unsigned)blocks), dim3(TG_THREADS), smem, stream, P, H);
+  if (H.cluster > 1) return tree_launch_clusters(tree_attention_kernel<T, D>, blocks, H.cluster, TG_THREADS, smem, stream, P, H);
+  const int st = launch_pdl(tree_attention_kernel<T, D>, dim3((unsigned)blocks), dim3(TG_THREADS), smem, stream, P, H);
   if (st != 0 || H.splits == 1) return st;
   return launch_pdl(tree_join_kernel<T>, dim3((unsigned)(((long)P.T * P.n_q + 3) / 4)), dim3(128), 0, stream, P, H);
 }
@@ -259,9 +394,10 @@ PHOTON_API int photon_tree_attention(const photon_tree_call* call, cudaStream_t 
   const int st = tree_params(call, P);
   if (st != 0) return st;
   const long rows = (long)P.T * P.n_q * call->parts;
-  if (call->parts > 1 && (call->scratch == nullptr || call->scratch_floats < rows * (P.d + 2))) return PHOTON_ERR_ARGUMENT;
+  const bool clusters = call->parts == 2 || call->parts == 4 || call->parts == 8;
+  if (call->parts > 1 && !clusters && (call->scratch == nullptr || call->scratch_floats < rows * (P.d + 2))) return PHOTON_ERR_ARGUMENT;
   TreeShares H;
-  H.part_o = call->scratch; H.part_ml = call->scratch + rows * P.d; H.splits = call->parts;
+  H.part_o = call->scratch; H.part_ml = call->scratch + rows * P.d; H.splits = call->parts; H.cluster = clusters ? call->parts : 1;
   H.row_tiles = (int)(((long)P.max_tokens * P.group + TG_ROWS - 1) / TG_ROWS);
   const long blocks = (long)P.S * H.row_tiles * P.n_kv * H.splits;
   if (blocks > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;

@@ -45,23 +45,6 @@ __device__ __forceinline__ uint32_t tf_pack(float lo, float hi) {
   __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
   return *reinterpret_cast<uint32_t*>(&v);
 }
-__device__ __forceinline__ void tf_cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
-}
-__device__ __forceinline__ float tf_peer(const float* p, int rank) {        // the float at the same place in another block of the cluster
-  uint32_t a;
-  float v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tf_smem(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(a) : "memory");
-  return v;
-}
-__device__ __forceinline__ float4 tf_peer4(const float* p, int rank) {
-  uint32_t a;
-  float4 v;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(tf_smem(p)), "r"(rank));
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(a) : "memory");
-  return v;
-}
 
 template <int D, int MT> struct Tf {
   static constexpr int KG = 4 / MT;                // warps that share a row tile, each with a part of every key tile
@@ -316,7 +299,7 @@ tree_attention_few_kernel(const TfParams P) {
 #pragma unroll
     for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(po + (warp * 16 + r) * C::LO + n * 8 + c2) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
   }
-  tf_cluster_sync();
+  tree_cluster_sync();
   // ---- every block joins its share of the rows' numbers: over the blocks in their order, over a block's warps in theirs
   for (int r = tid; r < rows; r += TF_THREADS) {
     const int w0 = r / 16 * C::KG, rr = r & 15, head = g * G + r % G;
@@ -324,12 +307,12 @@ tree_attention_few_kernel(const TfParams P) {
     float top = -INFINITY;
     for (int b = 0; b < P.cluster; ++b)
 #pragma unroll
-      for (int k = 0; k < C::KG; ++k) top = fmaxf(top, tf_peer(&ml_s[0][w0 + k][rr], b));
+      for (int k = 0; k < C::KG; ++k) top = fmaxf(top, tree_peer(&ml_s[0][w0 + k][rr], b));
     const float sub = fmaxf(top, sink) == -INFINITY ? 0.f : fmaxf(top, sink);
     float keys = 0.f;
     for (int b = 0; b < P.cluster; ++b)
 #pragma unroll
-      for (int k = 0; k < C::KG; ++k) keys += tf_peer(&ml_s[1][w0 + k][rr], b) * tf_exp2(tf_peer(&ml_s[0][w0 + k][rr], b) - sub);
+      for (int k = 0; k < C::KG; ++k) keys += tree_peer(&ml_s[1][w0 + k][rr], b) * tf_exp2(tree_peer(&ml_s[0][w0 + k][rr], b) - sub);
     const float sum = keys + (t.sinks ? tf_exp2(sink - sub) : 0.f);
     scale_s[r][0] = sub;
     scale_s[r][1] = sum != 0.f ? 1.f / sum : 0.f;
@@ -343,15 +326,15 @@ tree_attention_few_kernel(const TfParams P) {
     for (int b = 0; b < P.cluster; ++b)
 #pragma unroll
       for (int k = 0; k < C::KG; ++k) {
-        const float w = tf_exp2(tf_peer(&ml_s[0][w0 + k][rr], b) - sub);
-        const float4 x = tf_peer4(po + ((w0 + k) * 16 + rr) * C::LO + j, b);
+        const float w = tf_exp2(tree_peer(&ml_s[0][w0 + k][rr], b) - sub);
+        const float4 x = tree_peer4(po + ((w0 + k) * 16 + rr) * C::LO + j, b);
         if (w != 0.f) { a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w); }
       }
     uint2 v;
     v.x = tf_pack(a.x * inv, a.y * inv); v.y = tf_pack(a.z * inv, a.w * inv);
     *reinterpret_cast<uint2*>((bf16*)t.out + (size_t)(R.tok0 + r / G) * t.out_stride + (size_t)(g * G + r % G) * D + j) = v;
   }
-  tf_cluster_sync();                               // the others have read this block's results
+  tree_cluster_sync();                               // the others have read this block's results
 }
 
 template <int D, int MT>
@@ -359,18 +342,7 @@ static int tf_launch(const TfParams& P, cudaStream_t stream) {
   static bool ready[64] = {};
   int st = tree_smem_limit((const void*)tree_attention_few_kernel<D, MT>, Tf<D, MT>::SMEM, ready);
   if (st != 0) return st;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)((long)P.t.S * P.t.n_kv * P.cluster)); cfg.blockDim = dim3(TF_THREADS);
-  cfg.dynamicSmemBytes = Tf<D, MT>::SMEM; cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = P.cluster; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
-  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  attr[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = photon_pdl_enabled() ? 2 : 1;
-  const cudaError_t e = cudaLaunchKernelEx(&cfg, tree_attention_few_kernel<D, MT>, P);
-  return e != cudaSuccess ? (int)e : (int)cudaGetLastError();
+  return tree_launch_clusters(tree_attention_few_kernel<D, MT>, (long)P.t.S * P.t.n_kv * P.cluster, P.cluster, TF_THREADS, Tf<D, MT>::SMEM, stream, P);
 }
 
 PHOTON_API int photon_tree_attention_few(const photon_tree_call* call, cudaStream_t stream) {

@@ -580,7 +580,7 @@ typedef struct {
   int parts;                            /* tree_attention.cu: shares of a request's keys; tree_attention_tc.cu: blocks of the grid */
   float scale, softcap;                 /* softcap 0: off */
 } photon_tree_call;
-/* Either type, d <= 256.  parts > 1: scratch of T * n_q * parts * (d + 2) floats. */
+/* Either type, d <= 256.  parts other than 1, 2, 4 and 8: scratch of T * n_q * parts * (d + 2) floats. */
 PHOTON_EXPORT int photon_tree_attention(const photon_tree_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ tree_attention_tc.cu: the same on tcgen05, bfloat16, d 64 or 128 */

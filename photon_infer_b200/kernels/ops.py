@@ -2595,7 +2595,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         parts = -parts                              # whole units: no scratch
     elif name == "tree_attention_tc":
         floats = 8 * parts + 2 * parts * (-(-min(max_tokens_per_seq * group, 128 // group * group) // 32) * 32) * (head_dim + 2)
-    elif name == "tree_attention" and parts > 1:
+    elif name == "tree_attention" and parts not in (1, 2, 4, 8):
         floats = T * n_q * parts * (head_dim + 2)
     scratch = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
     call = _TREE_CALL.pack(*pointers, block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), positions.data_ptr(),
@@ -2637,9 +2637,21 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
             if tiles <= 12 or (tiles <= 32 and 4 * units >= 3 * sms):
                 return "tree_attention_tc", -min(2 * sms, 320, units)
             return "tree_attention_tc", min(2 * sms, 320, max(units, -(-units * (tiles + 1) // 4)))
-    # the general kernel: about four blocks an SM, none with less than two tiles of 32 keys
-    blocks = max(1, num_seqs * n_kv * -(-rows // 32))
-    return "tree_attention", max(1, min(4 * sms // blocks, keys // 64, 64))
+    # The general kernel: 32 rows a block, 3, 2 or 1 blocks an SM (registers, shared memory).  A row tile's keys go to a cluster of up to eight blocks, as many as
+    # take the fewest steps, a step being a tile of 64 keys or a third of what a block costs beside its tiles; very long requests that leave most of the chip
+    # idle go to more, which a second kernel joins.  32-bit, 8 key/value heads of 64, 8 nodes x 4 heads, parts and us: 2,000 keys 4: 39, 8: 25, 16: 23, 32: 23; 4,000 keys
+    # 8: 39, 16: 30, 32: 28; 16,000 keys 8: 145, 52: 62; 4 requests of 13 x 4 behind up to 700 keys 1: 53, 2: 33, 4: 25, 8: 23, 16: 31; 8 of 32 x 4
+    # behind up to 2,000: 1: 156, 2: 109, 4: 104, 8: 107.
+    blocks, tiles = max(1, num_seqs * n_kv * -(-rows // 32)), -(-keys // 64)
+    slots = (3 if head_dim <= 64 else 2 if head_dim <= 128 else 1) * sms
+    if tiles >= 48 and 16 * blocks <= slots:
+        return "tree_attention", min(slots // blocks, tiles // 2, 64)
+    parts, least = 1, 0.0
+    for p in (1, 2, 4, 8):
+        cost = -(-blocks * p // slots) * (tiles / p + 3)
+        if p == 1 or (cost < least and p <= tiles):
+            parts, least = p, cost
+    return "tree_attention", parts
 
 
 def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Tensor, num_seqs: int,
