@@ -2532,17 +2532,19 @@ def moe_gemv(x: torch.Tensor, x_div: int, ids: torch.Tensor, weight: torch.Tenso
 
 # ----------------------------------------------------------------------------- trees of drafted tokens
 
-def _check_step(what: str, num_seqs: int, cu_tokens: torch.Tensor, context_lens: Optional[torch.Tensor], block_table: Optional[torch.Tensor]) -> None:
-    _int32(cu_tokens, "cu_tokens")
-    covered = 0 <= num_seqs < cu_tokens.numel()
-    if context_lens is not None:
-        _int32(context_lens, "context_lens")
-        covered = covered and context_lens.numel() >= num_seqs
-    if block_table is not None:
-        _int32(block_table, "block_table")
-        covered = covered and block_table.dim() == 2 and block_table.shape[0] >= num_seqs and block_table.numel() > 0
-    if not covered:
+def _check_step(what: str, num_seqs: int, cu_tokens: torch.Tensor, context_lens: torch.Tensor, block_table: torch.Tensor) -> int:
+    """The step's tables cover its requests; returns the table's width."""
+    _int32s(("cu_tokens", "context_lens", "block_table"), (cu_tokens, context_lens, block_table))
+    table = block_table.shape
+    if not 0 <= num_seqs < cu_tokens.numel() or context_lens.numel() < num_seqs or len(table) != 2 or table[0] < num_seqs or table[0] * table[1] < 1:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: cu_tokens, context_lens and block_table must cover every request")
+    return table[1]
+
+
+def _int32s(names, tensors) -> None:
+    for t in tensors:
+        if t.dtype is not torch.int32 or not t.is_contiguous():
+            _int32(t, names[[x is t for x in tensors].index(True)])
 
 
 #: photon_tree_call: pointers, strides and the scratch's size, sizes, scale and bound
@@ -2565,21 +2567,21 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         _check_sink(sink, n_q)
     if n_kv <= 0 or n_q <= 0 or n_q % n_kv or not 1 <= head_dim <= 256:
         raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, f"tree_attention: {n_q}/{n_kv} heads of {head_dim} are not supported (up to 256 numbers)")
-    dtype, cache = q.dtype, k_cache.shape
-    if q.dim() != 2 or out.shape != q.shape or q.shape[1] != n_q * head_dim:
+    dtype, cache, shape = q.dtype, k_cache.shape, q.shape
+    if len(shape) != 2 or out.shape != shape or shape[1] != n_q * head_dim:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: q and out must be [T, n_q * head_dim]")
-    T, (q_stride, q_inner), (out_stride, out_inner) = q.shape[0], q.stride(), out.stride()
+    T, (q_stride, q_inner), (out_stride, out_inner) = shape[0], q.stride(), out.stride()
     if (q_inner != 1 or out_inner != 1) and T:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: rows of q and out must be contiguous")
     if out.dtype != dtype or k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: q, out and the caches must share one dtype")
     if len(cache) != 4 or v_cache.shape != cache or cache[1] != n_kv or cache[3] != head_dim or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: the caches must be contiguous [pages, n_kv, page_size, head_dim]")
-    _check_step("tree_attention", num_seqs, cu_tokens, context_lens, block_table)
-    _int32(positions, "positions")
-    _int32(tree_mask, "tree_mask")
-    words = tree_mask.shape[1] if tree_mask.dim() == 2 else 0
-    if positions.numel() < T or tree_mask.numel() < T * words or words * 32 < max_tokens_per_seq or words < 1:
+    width = _check_step("tree_attention", num_seqs, cu_tokens, context_lens, block_table)
+    _int32s(("positions", "tree_mask"), (positions, tree_mask))
+    mask = tree_mask.shape
+    words = mask[1] if len(mask) == 2 else 0
+    if positions.numel() < T or mask[0] < T or words * 32 < max_tokens_per_seq or words < 1:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: positions [T] and tree_mask [T, words] with a bit for every node")
     if not scale > 0 or (softcap is not None and softcap < 0) or (window is not None and window < 0):
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: the scale must be positive, softcap and window not negative")
@@ -2600,7 +2602,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     scratch = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
     call = _TREE_CALL.pack(*pointers, block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), positions.data_ptr(),
                            tree_mask.data_ptr(), sink.data_ptr() if sink is not None else 0, scratch.data_ptr() if floats else 0,
-                           err.data_ptr() if err is not None else 0, q_stride, out_stride, floats, _dtype_code(q), block_table.shape[1], words,
+                           err.data_ptr() if err is not None else 0, q_stride, out_stride, floats, _dtype_code(q), width, words,
                            num_seqs, T, max_tokens_per_seq, n_q, n_kv, head_dim, page_size, pages, min(window or 0, 0x7fffffff), parts, scale, softcap or 0.0)
     _check(_plain_fn(name, "photon_" + name, _CALL_ARGS)(call, _stream()), "tree_attention")
     if floats:
@@ -2664,15 +2666,16 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     node 0.  ``path``, ``sampled`` (int32 ``[S, D]``): the nodes gone through and the tokens they gave, -1 behind the last of ``counts [S]``; the walk
     ends after ``D`` nodes."""
     _cuda(logits, tokens, parents, cu_tokens, path, counts, sampled, temperature, uniforms, err)
-    if logits.dim() != 2 or logits.dtype != torch.float32 or logits.stride(1) != 1 or logits.shape[1] < 1:
+    shape, place = logits.shape, path.shape
+    if len(shape) != 2 or logits.dtype is not torch.float32 or logits.stride(1) != 1 or shape[1] < 1:
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_accept: logits must be float32 [T, V] with unit inner stride")
-    T, V = logits.shape
-    for name, t in (("tokens", tokens), ("parents", parents), ("path", path), ("counts", counts), ("sampled", sampled)):
-        _int32(t, name)
-    _check_step("tree_accept", num_seqs, cu_tokens, None, None)
+    T, V = shape
+    _int32s(("tokens", "parents", "cu_tokens", "path", "counts", "sampled"), (tokens, parents, cu_tokens, path, counts, sampled))
+    if not 0 <= num_seqs < cu_tokens.numel():
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_accept: cu_tokens must cover every request")
     if tokens.numel() < T or parents.numel() < T:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_accept: tokens and parents must have one entry per row of logits")
-    if path.dim() != 2 or path.shape[0] < num_seqs or path.shape[1] < 1 or sampled.shape != path.shape or counts.numel() < num_seqs:
+    if len(place) != 2 or place[0] < num_seqs or place[1] < 1 or sampled.shape != place or counts.numel() < num_seqs:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_accept: path and sampled must be [requests, depth], counts [requests]")
     if temperature is not None and (uniforms is None or any(t.dtype != torch.float32 or not t.is_contiguous() for t in (temperature, uniforms))
                                     or temperature.numel() < num_seqs or uniforms.numel() < T):
@@ -2683,7 +2686,7 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
                              temperature.data_ptr() if temperature is not None else 0, uniforms.data_ptr() if temperature is not None else 0,
                              path.data_ptr(), counts.data_ptr(), sampled.data_ptr(), given.data_ptr() if given is not None else 0,
                              err.data_ptr() if err is not None else 0, logits.stride(0),
-                             num_seqs, T, V, path.shape[1], max_tokens_per_seq)
+                             num_seqs, T, V, place[1], max_tokens_per_seq)
     _check(_plain_fn("tree_accept", "photon_tree_accept", _CALL_ARGS)(call, _stream()), "tree_accept")
     if given is not None:
         _count_launches(1)
@@ -2696,10 +2699,13 @@ _ACCEPT_CALL = struct.Struct("12q5i4x")
 ACCEPT_AT_ONCE = 12 << 20
 
 
-def _check_pool(what: str, kv: torch.Tensor) -> int:
-    if kv.dim() != 6 or not kv.is_contiguous() or kv.numel() == 0:
+def _check_pool(what: str, kv: torch.Tensor):
+    """(planes of all entries, pages, n_kv, page_size, d) of a cache group's pools."""
+    shape = kv.shape
+    if len(shape) != 6 or not kv.is_contiguous() or kv.numel() == 0:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: the pools must be contiguous [entries, planes, pages, n_kv, page_size, d]")
-    return kv.shape[0] * kv.shape[1]
+    entries, planes, pages, n_kv, page_size, d = shape
+    return entries * planes, pages, n_kv, page_size, d
 
 
 def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Tensor, context_lens: torch.Tensor, path: torch.Tensor,
@@ -2708,16 +2714,14 @@ def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Ten
     planes, pages, n_kv, page_size, d]``: key ``base + path[s, j]`` of request ``s`` goes to key ``base + j`` for ``0 < j < counts[s]``, with ``base =
     context_lens[s]`` minus the request's nodes of the step.  ``path`` and ``counts`` as ``tree_accept`` leaves them (paths ascend)."""
     _cuda(kv, block_table, cu_tokens, context_lens, path, counts, err)
-    planes = _check_pool("cache_keep", kv)
-    _check_step("cache_keep", num_seqs, cu_tokens, context_lens, block_table)
-    _int32(path, "path")
-    _int32(counts, "counts")
-    if path.dim() != 2 or path.shape[0] < num_seqs or counts.numel() < num_seqs:
+    pool = _check_pool("cache_keep", kv)
+    width = _check_step("cache_keep", num_seqs, cu_tokens, context_lens, block_table)
+    _int32s(("path", "counts"), (path, counts))
+    place = path.shape
+    if len(place) != 2 or place[0] < num_seqs or counts.numel() < num_seqs:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_keep: path must be [requests, depth], counts [requests]")
-    _, _, pages, n_kv, page_size, d = kv.shape
     call = _KEEP_CALL.pack(kv.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), path.data_ptr(), counts.data_ptr(),
-                           err.data_ptr() if err is not None else 0, _dtype_code(kv), planes, pages, n_kv, page_size, d, block_table.shape[1], num_seqs,
-                           path.shape[1])
+                           err.data_ptr() if err is not None else 0, _dtype_code(kv), *pool, width, num_seqs, place[1])
     _check(_plain_fn("cache_rows", "photon_cache_keep", _CALL_ARGS)(call, _stream()), "cache_keep")
 
 
@@ -2725,17 +2729,20 @@ def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Ten
 _KEEP_CALL = struct.Struct("7q9i4x")
 
 
+_COPY_ARGS = [c_void_p, c_int, c_int, c_int, c_long, c_void_p, c_int, c_void_p, c_void_p]
+
+
 def cache_copy_pages(kv: torch.Tensor, pairs: torch.Tensor, err: Optional[torch.Tensor]) -> None:
     """Page ``pairs[i, 0]`` onto page ``pairs[i, 1]`` (int32 ``[N, 2]``) in every entry and plane of a cache group's pools ``kv [entries, planes,
     pages, n_kv, page_size, d]``.  No page may be written twice, or be both read and written.  A page outside the pool is left out and recorded in ``err``."""
     _cuda(kv, pairs, err)
-    planes = _check_pool("cache_copy_pages", kv)
+    planes, pages, n_kv, page_size, d = _check_pool("cache_copy_pages", kv)
     _int32(pairs, "pairs")
-    if pairs.dim() != 2 or pairs.shape[1] != 2:
+    shape = pairs.shape
+    if len(shape) != 2 or shape[1] != 2:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_copy_pages: pairs must be [pages, 2]")
-    _, _, pages, n_kv, page_size, d = kv.shape
-    f = _plain_fn("cache_rows", "photon_cache_copy_pages", [c_void_p, c_int, c_int, c_int, c_long, c_void_p, c_int, c_void_p, c_void_p])
-    _check(f(kv.data_ptr(), _dtype_code(kv), planes, pages, n_kv * page_size * d, pairs.data_ptr(), pairs.shape[0],
+    f = _plain_fn("cache_rows", "photon_cache_copy_pages", _COPY_ARGS)
+    _check(f(kv.data_ptr(), _dtype_code(kv), planes, pages, n_kv * page_size * d, pairs.data_ptr(), shape[0],
              err.data_ptr() if err is not None else 0, _stream()), "cache_copy_pages")
 
 
