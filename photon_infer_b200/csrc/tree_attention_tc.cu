@@ -650,54 +650,73 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   if (threadIdx.x == 0 && *abort_flag) report_error(P.t.err, PHOTON_DEV_WAIT_TIMEOUT, blockIdx.x, 0, 0);
 }
 
-// Joins the pieces of the unit that block `blockIdx.x / chunks` of the first kernel began and left to the blocks behind it, in their order: 32 rows and 32
-// columns a block.
+// Joins the pieces of the units that blocks of the first kernel shared, in their order.  A unit's record stands at the block that began it; each block here finds
+// the records and takes its share of the work, 32 rows and 32 columns at a time.
 template <int D>
 __global__ void __launch_bounds__(256)
-tree_join_tc_kernel(const TtParams P, int chunks) {
-  pdl_wait();
+tree_join_tc_kernel(const TtParams P, int blocks, int chunks) {
+  __shared__ short first_s[TT_MAX_BLOCKS];         // the blocks that began a shared unit
+  __shared__ int count_s[TT_MAX_BLOCKS / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c0 = blockIdx.x / chunks, r0 = (blockIdx.x % chunks) * 32;
-  const int4 a0 = P.meta[2 * c0];
-  const int parts = a0.x, rows = a0.z;
-  if (parts < 2 || parts > TT_MAX_BLOCKS || r0 >= rows) return;
-  const int tok0 = P.meta[2 * c0 + 1].x;
-  const bool valid = r0 + lane < rows;
-  const int rr = valid ? r0 + lane : rows - 1, cc = blockIdx.y * 8 + warp;
-  const int t = tok0 + (a0.y + rr) / P.t.group, head = a0.w * P.t.group + (a0.y + rr) % P.t.group;
-  auto slot = [&](int i) { return (size_t)2 * (c0 + i) + (i == 0 ? 1 : 0); };
-  // the maximum and sum so far, the sink first; eight pieces are on their way at a time
-  float top = P.t.sinks ? P.t.sinks[head] * TT_LOG2E : -INFINITY, sum = P.t.sinks ? 1.f : 0.f;
-  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (top == -INFINITY) sum = 0.f;
-  for (int i0 = 0; i0 < parts; i0 += 8) {
-    float2 ml[8];
-    float4 y[8];
+  pdl_wait();
+  unsigned mine[(TT_MAX_BLOCKS + 255) / 256];      // this warp's 32 blocks at a time: those that began one
 #pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      const int i = min(i0 + k, parts - 1);
-      ml[k] = *reinterpret_cast<const float2*>(P.part_ml + (slot(i) * P.part_rows + rr) * 2);
-      y[k] = *(reinterpret_cast<const float4*>(P.part_o) + (slot(i) * (D / 4) + cc) * P.part_rows + rr);
-    }
-    float most = top;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) most = fmaxf(most, ml[k].x);
-    const float sub = most == -INFINITY ? 0.f : most, old = at_exp2(top - sub);
-    sum *= old; a.x *= old; a.y *= old; a.z *= old; a.w *= old;
-    top = most;
-#pragma unroll
-    for (int k = 0; k < 8; ++k) {
-      if (i0 + k >= parts) continue;
-      const float w = at_exp2(ml[k].x - sub);
-      sum += ml[k].y * w;
-      if (w != 0.f) { a.x = fmaf(w, y[k].x, a.x); a.y = fmaf(w, y[k].y, a.y); a.z = fmaf(w, y[k].z, a.z); a.w = fmaf(w, y[k].w, a.w); }
-    }
+  for (int k = 0; k < (TT_MAX_BLOCKS + 255) / 256; ++k) {
+    const int c = k * 256 + threadIdx.x, parts = c < blocks ? P.meta[2 * c].x : 0;
+    mine[k] = __ballot_sync(0xffffffffu, parts >= 2 && parts <= TT_MAX_BLOCKS);
+    if (lane == 0 && c < TT_MAX_BLOCKS) count_s[c >> 5] = __popc(mine[k]);
   }
-  if (valid) {
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
-    uint2 v2;
-    v2.x = at_pack(a.x * inv, a.y * inv); v2.y = at_pack(a.z * inv, a.w * inv);
-    *reinterpret_cast<uint2*>((bf16*)P.t.out + (size_t)t * P.t.out_stride + (size_t)head * D + cc * 4) = v2;
+  __syncthreads();
+  int units = 0;
+#pragma unroll
+  for (int w = 0; w < TT_MAX_BLOCKS / 32; ++w) {
+    if (w % 8 == warp && (mine[w / 8] >> lane & 1u)) first_s[units + __popc(mine[w / 8] & ((1u << lane) - 1u))] = (short)(w * 32 + lane);
+    units += count_s[w];
+  }
+  __syncthreads();
+  for (int item = blockIdx.x; item < units * chunks * (D / 32); item += gridDim.x) {
+    const int c0 = first_s[item / (chunks * (D / 32))], r0 = item / (D / 32) % chunks * 32, cc = item % (D / 32) * 8 + warp;
+    const int4 a0 = P.meta[2 * c0];
+    const int parts = a0.x, rows = a0.z;
+    if (r0 >= rows) continue;
+    const int tok0 = P.meta[2 * c0 + 1].x;
+    const bool valid = r0 + lane < rows;
+    const int rr = valid ? r0 + lane : rows - 1;
+    const int t = tok0 + (a0.y + rr) / P.t.group, head = a0.w * P.t.group + (a0.y + rr) % P.t.group;
+    auto slot = [&](int i) { return (size_t)2 * (c0 + i) + (i == 0 ? 1 : 0); };
+    // the maximum and sum so far, the sink first; eight pieces are on their way at a time
+    float top = P.t.sinks ? P.t.sinks[head] * TT_LOG2E : -INFINITY, sum = P.t.sinks ? 1.f : 0.f;
+    float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (top == -INFINITY) sum = 0.f;
+    for (int i0 = 0; i0 < parts; i0 += 8) {
+      float2 ml[8];
+      float4 y[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        const int i = min(i0 + k, parts - 1);
+        ml[k] = *reinterpret_cast<const float2*>(P.part_ml + (slot(i) * P.part_rows + rr) * 2);
+        y[k] = *(reinterpret_cast<const float4*>(P.part_o) + (slot(i) * (D / 4) + cc) * P.part_rows + rr);
+      }
+      float most = top;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) most = fmaxf(most, ml[k].x);
+      const float sub = most == -INFINITY ? 0.f : most, old = at_exp2(top - sub);
+      sum *= old; a.x *= old; a.y *= old; a.z *= old; a.w *= old;
+      top = most;
+#pragma unroll
+      for (int k = 0; k < 8; ++k) {
+        if (i0 + k >= parts) continue;
+        const float w = at_exp2(ml[k].x - sub);
+        sum += ml[k].y * w;
+        if (w != 0.f) { a.x = fmaf(w, y[k].x, a.x); a.y = fmaf(w, y[k].y, a.y); a.z = fmaf(w, y[k].z, a.z); a.w = fmaf(w, y[k].w, a.w); }
+      }
+    }
+    if (valid) {
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      uint2 v2;
+      v2.x = at_pack(a.x * inv, a.y * inv); v2.y = at_pack(a.z * inv, a.w * inv);
+      *reinterpret_cast<uint2*>((bf16*)P.t.out + (size_t)t * P.t.out_stride + (size_t)head * D + cc * 4) = v2;
+    }
   }
 }
 
@@ -709,7 +728,8 @@ static int tt_launch(TtParams& P, const CUtensorMap& mq, const CUtensorMap& mk, 
   st = launch_pdl(tree_attention_tc_kernel<D>, dim3(blocks), dim3(TT_THREADS), (size_t)Tt<D>::SMEM, stream, mq, mk, mv, P);
   if (st != 0 || P.whole) return st;
   const int chunks = (P.part_rows + 31) / 32;
-  return launch_pdl(tree_join_tc_kernel<D>, dim3((unsigned)(blocks * chunks), D / 32), dim3(256), 0, stream, P, chunks);
+  const int items = blocks * chunks * (D / 32), grid = 2 * P.blocks_sm;     // four blocks an SM
+  return launch_pdl(tree_join_tc_kernel<D>, dim3((unsigned)(items < grid ? items : grid)), dim3(256), 0, stream, P, blocks, chunks);
 }
 
 // Rows of a unit that a partial result has room for.
