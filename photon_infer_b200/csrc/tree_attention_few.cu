@@ -6,6 +6,11 @@
 // At the end the warps' partial results lie in shared memory, and the blocks of the cluster join them there, each for its share of the outputs: one
 // launch, no scratch, the same order of sums in every run.
 //
+// What bounds it: latency.  5 nodes behind 640 keys (32/8 heads of 64): 7.7 us, where the bytes take 0.2; 1 node behind 100: 5.9; 2 requests of 8 behind 1,000 (32/8
+// heads of 128): 12.6 (bytes: 1.3).  A launch, the request's range and its pages, the first keys, two tiles of work and the join follow one another; in the
+// kernel's wait counters memory, barriers and instructions that are not there yet have like parts.  A second kernel for the join took 15.8 us for the first of
+// these; each row's factors worked out for every four of its outputs 8.4; short tables read behind the request's range 7.9.
+//
 // Which keys a row sees: tree_attention.cuh.  In tiles where some row's mask cuts, values that are not finite are set to zero in shared memory before the
 // products (0 times them would not be 0), and rows that see them get them back at the end from the cache.
 #include "tree_attention.cuh"
@@ -69,27 +74,36 @@ tree_attention_few_kernel(const TfParams P) {
   __shared__ int table_s[TF_TABLE];
   __shared__ uint64_t gone_s[C::STAGES];           // keys of a stage whose page is missing
   __shared__ int poison;                           // 1: some value of a tile where a mask cuts was not finite
-  __shared__ float ml_s[2][4][16];                 // [maximum, sum][warp][row], then the block's [ROWS] of each
-  __shared__ float scale_s[C::ROWS][2];            // the maximum of a row that its partial results are taken relative to; 1 / sum
+  __shared__ float ml_s[2][4][16];                 // [maximum, sum][warp][row]
+  __shared__ float factor_s[C::ROWS][32 / MT];     // of each partial result of a row
   const TreeParams& t = P.t;
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x % P.cluster, unit = blockIdx.x / P.cluster, g = unit % t.n_kv, seq = unit / t.n_kv;
   if (tid == 0) poison = 0;
   if (tid < C::STAGES) gone_s[tid] = 0;
   pdl_wait();
+  // The request's pages: a short table is read whole, beside the request's range; of a long one the entries of the block's keys, once they are known.
+  const int* table = t.block_table + (size_t)seq * t.max_pages;
+  const bool whole = t.max_pages <= TF_TABLE;
+  int entry[TF_TABLE / TF_THREADS];
+#pragma unroll
+  for (int k = 0; k < TF_TABLE / TF_THREADS; ++k) entry[k] = whole && k * TF_THREADS + tid < t.max_pages ? table[k * TF_THREADS + tid] : -1;
   const TreeRequest R = tree_request(t, seq);
   const int G = t.group, rows = min(R.n * G, C::ROWS);
   const int key_end = R.base + R.n, key_lo = t.window > 0 ? max(0, R.base - t.window + 1) : 0;
   const int cut_lo = t.window > 0 ? key_end - t.window : -1;      // no row's window begins behind this key
   const int tile_lo = key_lo / TF_KT, all = rows > 0 ? (key_end + TF_KT - 1) / TF_KT - tile_lo : 0;
   const int tile0 = tile_lo + all * rank / P.cluster, ntiles = tile_lo + all * (rank + 1) / P.cluster - tile0;
-  const int* table = t.block_table + (size_t)seq * t.max_pages;
   auto page_of = [&](int key) { return P.page_shift >= 0 ? key >> P.page_shift : key / t.page_size; };
-  // the pages of the block's keys
-  const int page0 = page_of(tile0 * TF_KT), pages = ntiles > 0 ? page_of(min(key_end, (tile0 + ntiles) * TF_KT) - 1) - page0 + 1 : 0;
-  const bool kept = pages <= TF_TABLE;
-  if (kept)
+  const int from = page_of(tile0 * TF_KT), pages = ntiles > 0 ? page_of(min(key_end, (tile0 + ntiles) * TF_KT) - 1) - from + 1 : 0;
+  const int page0 = whole ? 0 : from;
+  const bool kept = whole || pages <= TF_TABLE;
+  if (whole) {
+#pragma unroll
+    for (int k = 0; k < TF_TABLE / TF_THREADS; ++k) table_s[k * TF_THREADS + tid] = entry[k];
+  } else if (kept) {
     for (int i = tid; i < pages; i += TF_THREADS) table_s[i] = page0 + i < t.max_pages ? table[page0 + i] : -1;
+  }
   // Q, zeros behind the rows
   {
     const bf16* q = (const bf16*)t.q;
@@ -114,7 +128,7 @@ tree_attention_few_kernel(const TfParams P) {
       size_t row = 0;
       if (there) {
         const int pidx = page_of(key);
-        const int page = kept ? table_s[pidx - page0] : pidx < t.max_pages ? table[pidx] : -1;
+        const int page = pidx >= t.max_pages ? -1 : kept ? table_s[pidx - page0] : table[pidx];
         if (page < 0 || page >= t.num_pages) {
           there = false;
           if (j == 0) { atomicOr((unsigned long long*)&gone_s[st], 1ull << r); report_error(t.err, PHOTON_DEV_BAD_PAGE, R.tok0, key, page); }
@@ -301,37 +315,48 @@ tree_attention_few_kernel(const TfParams P) {
   }
   tree_cluster_sync();
   // ---- every block joins its share of the rows' numbers: over the blocks in their order, over a block's warps in theirs
-  for (int r = tid; r < rows; r += TF_THREADS) {
-    const int w0 = r / 16 * C::KG, rr = r & 15, head = g * G + r % G;
-    const float sink = t.sinks ? t.sinks[head] * TF_LOG2E : -INFINITY;
-    float top = -INFINITY;
-    for (int b = 0; b < P.cluster; ++b)
+  {
+    constexpr int W = TF_THREADS / (16 * MT);      // threads a row, four of its results each
+    const int r = tid / W, n = P.cluster * C::KG, w0 = r / 16 * C::KG, rr = r & 15;
+    const float sink = t.sinks && r < rows ? t.sinks[g * G + r % G] * TF_LOG2E : -INFINITY;
+    float f[4], s[4], top = sink, sum = 0.f;
 #pragma unroll
-      for (int k = 0; k < C::KG; ++k) top = fmaxf(top, tree_peer(&ml_s[0][w0 + k][rr], b));
-    const float sub = fmaxf(top, sink) == -INFINITY ? 0.f : fmaxf(top, sink);
-    float keys = 0.f;
-    for (int b = 0; b < P.cluster; ++b)
+    for (int u = 0; u < 4; ++u) {
+      const int w = tid % W + W * u;
+      f[u] = w < n ? tree_peer(&ml_s[0][w0 + w % C::KG][rr], w / C::KG) : -INFINITY;
+      s[u] = w < n ? tree_peer(&ml_s[1][w0 + w % C::KG][rr], w / C::KG) : 0.f;
+      top = fmaxf(top, f[u]);
+    }
 #pragma unroll
-      for (int k = 0; k < C::KG; ++k) keys += tree_peer(&ml_s[1][w0 + k][rr], b) * tf_exp2(tree_peer(&ml_s[0][w0 + k][rr], b) - sub);
-    const float sum = keys + (t.sinks ? tf_exp2(sink - sub) : 0.f);
-    scale_s[r][0] = sub;
-    scale_s[r][1] = sum != 0.f ? 1.f / sum : 0.f;
+    for (int w = W / 2; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+    const float sub = top == -INFINITY ? 0.f : top;
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      f[u] = tf_exp2(f[u] - sub);                  // 0 for what is not there
+      sum += s[u] * f[u];
+    }
+#pragma unroll
+    for (int w = W / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
+    sum += tf_exp2(sink - sub);
+    const float inv = sum != 0.f ? 1.f / sum : 0.f;
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (tid % W + W * u < n) factor_s[r][tid % W + W * u] = f[u] * inv;
   }
   __syncthreads();
   const int pieces = rows * (D / 4), first = pieces * rank / P.cluster, last = pieces * (rank + 1) / P.cluster;
   for (int e = first + tid; e < last; e += TF_THREADS) {
     const int r = e / (D / 4), j = e % (D / 4) * 4, w0 = r / 16 * C::KG, rr = r & 15;
-    const float sub = scale_s[r][0], inv = scale_s[r][1];
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int b = 0; b < P.cluster; ++b)
 #pragma unroll
       for (int k = 0; k < C::KG; ++k) {
-        const float w = tf_exp2(tree_peer(&ml_s[0][w0 + k][rr], b) - sub);
+        const float w = factor_s[r][b * C::KG + k];
         const float4 x = tree_peer4(po + ((w0 + k) * 16 + rr) * C::LO + j, b);
         if (w != 0.f) { a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w); }
       }
     uint2 v;
-    v.x = tf_pack(a.x * inv, a.y * inv); v.y = tf_pack(a.z * inv, a.w * inv);
+    v.x = tf_pack(a.x, a.y); v.y = tf_pack(a.z, a.w);
     *reinterpret_cast<uint2*>((bf16*)t.out + (size_t)(R.tok0 + r / G) * t.out_stride + (size_t)(g * G + r % G) * D + j) = v;
   }
   tree_cluster_sync();                               // the others have read this block's results
