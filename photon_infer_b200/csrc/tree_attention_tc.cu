@@ -3,7 +3,8 @@
 // The rows of a unit are (node, query head) pairs of one request that share a key/value head, up to 128 (whole nodes).  A unit's keys are walked in tiles of 64.  All units'
 // tiles, one behind the other, are cut into equal ranges, one for each block of a grid that fills the chip once, so that requests of any
 // lengths keep every SM busy to the end; a block walks the pieces of units in its range ("segments").  Units that ranges cut through are joined by a second
-// kernel, in the blocks' order.  Where whole units keep the chip as busy they are dealt out whole, the longest first, and there is nothing to join.
+// kernel, in the blocks' order.  Where whole units keep the chip as busy they are dealt out whole, the longest first, and there is nothing to join.  Where there are
+// few units, each is a cluster's: its blocks have equal runs of its tiles and join their results in each other's shared memory, once their rings are empty.
 //
 // Two blocks share an SM, so that one's loads and products run while the other begins or ends a segment.  In a block
 //   * warp 4 brings Q, key and value tiles by TMA along the block table into shared memory (128-byte swizzle); keys and values share one ring;
@@ -26,6 +27,7 @@
 #define TT_KT 64                                   // keys per tile
 #define TT_THREADS 192
 #define TT_MAX_BLOCKS 320                          // of the first kernel's grid
+#define TT_CLUSTER 8                               // blocks that may share a unit
 #define TT_LOG2E 1.4426950408889634f
 #define TT_RESCALE_STEP 8.0f                       // log2 units that a maximum in use may lag behind
 
@@ -44,7 +46,7 @@ template <int D> struct Tt {
 
 struct TtParams {
   TreeParams t;
-  int whole, sorted, blocks_sm;                    // whole units in any case: one kernel; the longest of them first; blocks that the chip holds
+  int whole, sorted, blocks_sm, cluster;                   // whole units in any case: one kernel; the longest of them first; blocks that the chip holds; blocks that share a unit
   int tile_rows, tile_nodes, box_rows, total_rows, page_shift;
   int q_slots, q_slot_bytes, q_half_bytes, q_nodes;          // Q tiles in shared memory, bytes between them and between a tile's halves, nodes of a copy
   float scale_log2, cap_in;
@@ -169,7 +171,7 @@ struct TtSegments {
   bool whole;
   __device__ __forceinline__ void start(const TtParams& P, const TtOrder* o, bool w, long long total) {
     order = o; units_whole = w;
-    left = 0; serial = 0; seq = 0; unit = 0; tile = 0; round = 0;
+    left = 0; serial = 0; seq = 0; unit = 0; tile = 0; round = 0; rows = 0;
     const int blocks = tt_blocks(total, gridDim.x);
     if (w || (int)blockIdx.x >= blocks) return;
     const long long first = tt_first(total, blockIdx.x, blocks);
@@ -178,7 +180,28 @@ struct TtSegments {
     q = tt_load(P, seq);
     unit = off / q.tiles; tile = off - unit * q.tiles;
   }
+  __device__ __forceinline__ void place(const TtParams& P) {      // the unit's head and rows
+    // Row tiles of a head side by side: they read the same keys.  Requests begin with different heads: blocks that are as far in different requests
+    // otherwise read the same part of every page at a time, and some of the memory's channels wait for others (148 requests of 12,288 keys: 6 %).
+    const int rb = unit % q.blocks, h = unit / q.blocks + seq % P.t.n_kv;
+    g = h < P.t.n_kv ? h : h - P.t.n_kv;
+    row0 = rb * P.tile_rows;
+    rows = min(q.r.n * P.t.group - row0, P.tile_rows);
+  }
   __device__ __forceinline__ bool next(const TtParams& P) {       // by whole warps
+    if (P.cluster > 1) {
+      // one unit for the cluster, and this block's part of its tiles; a short unit leaves some blocks without
+      if (round++ > 0) return false;
+      int front;
+      rows = 0;
+      if (!tt_unit(P, *order, blockIdx.x / P.cluster, seq, front)) return false;
+      q = tt_load(P, seq); unit = blockIdx.x / P.cluster - front;
+      place(P);
+      const int rank = blockIdx.x % P.cluster, first = q.tiles * rank / P.cluster;
+      ntiles = q.tiles * (rank + 1) / P.cluster - first;
+      tile0 = q.tile_lo + first; whole = false; bit = 0; serial = 1;
+      return ntiles > 0;
+    }
     if (units_whole) {
       // the longest units first, to and fro over the blocks
       const int u = (round & 1) ? (round + 1) * (int)gridDim.x - 1 - (int)blockIdx.x : round * (int)gridDim.x + (int)blockIdx.x;
@@ -192,12 +215,7 @@ struct TtSegments {
       if (++seq >= P.t.S) return false;
       q = tt_load(P, seq); unit = 0; tile = 0;
     }
-    // Row tiles of a head side by side: they read the same keys.  Requests begin with different heads: blocks that are as far in different requests
-    // otherwise read the same part of every page at a time, and some of the memory's channels wait for others (148 requests of 12,288 keys: 6 %).
-    const int rb = unit % q.blocks, h = unit / q.blocks + seq % P.t.n_kv;
-    g = h < P.t.n_kv ? h : h - P.t.n_kv;
-    row0 = rb * P.tile_rows;
-    rows = min(q.r.n * P.t.group - row0, P.tile_rows);
+    place(P);
     ntiles = min(left, q.tiles - tile);
     tile0 = q.tile_lo + tile;
     whole = ntiles == q.tiles;
@@ -276,6 +294,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   if (whole && P.sorted) tt_sort(P, *order);
   TtSegments s;
   s.start(P, order, whole, total);
+  float row_m = -INFINITY, row_l = 0.f;             // of a row whose unit a cluster shares
 
   if (!aligned) {
     if (threadIdx.x == 0 && !P.whole) P.meta[2 * blockIdx.x] = make_int4(0, 0, 0, 0);       // nothing can be run
@@ -576,6 +595,8 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         float sum = l;
         if (P.t.sinks && l != 0.f) sum += exp2f(fmaf(P.t.sinks[head], TT_LOG2E, -m_used));         // the sink's weight, relative to the maximum in use
         inv = sum != 0.f ? 1.f / sum : 0.f;
+      } else if (P.cluster > 1) {
+        row_m = m_used; row_l = l;
       } else {
         if (valid) *reinterpret_cast<float2*>(P.part_ml + (slot * P.part_rows + r) * 2) = make_float2(m_used, l);
         if (r == 0 && s.bit) {
@@ -618,7 +639,12 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
               }
             }
           }
-          if (valid) {
+          if (P.cluster > 1) {
+            // the ring has served: nothing comes behind a cluster's one unit
+            float4* dst = reinterpret_cast<float4*>(kv_s) + cc / 4 * 128 + r;
+#pragma unroll
+            for (int u = 0; u < 8; ++u) dst[u * 128] = make_float4(x[4 * u], x[4 * u + 1], x[4 * u + 2], x[4 * u + 3]);
+          } else if (valid) {
             if (s.whole) {
               bf16* dst = (bf16*)P.t.out + (size_t)t * P.t.out_stride + (size_t)head * D + cc;
 #pragma unroll
@@ -639,6 +665,54 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       tc_fence_before();                            // O is read: the next segment's P may be handed over
     }
     if (r == 0 && !said && !P.whole) P.meta[2 * blockIdx.x] = make_int4(0, 0, 0, 0);
+  }
+  if (P.cluster > 1) {
+    // ---------------- the blocks of a cluster join their unit in their order, each for its share of the columns
+    float2* ml = reinterpret_cast<float2*>(kv_s + D / 4 * 128 * 16);        // [128]
+    if (warp < 4) ml[threadIdx.x] = make_float2(row_m, row_l);
+    tree_cluster_sync();
+    const int r = threadIdx.x;
+    if (warp < 4 && r < s.rows && !*abort_flag) {
+      const int rank = blockIdx.x % P.cluster, t = s.q.r.tok0 + (s.row0 + r) / P.t.group, head = s.g * P.t.group + (s.row0 + r) % P.t.group;
+      float w[TT_CLUSTER], sum = 0.f, top = P.t.sinks ? P.t.sinks[head] * TT_LOG2E : -INFINITY;
+      const float sink = top;
+#pragma unroll
+      for (int k = 0; k < TT_CLUSTER; ++k) {
+        w[k] = k < P.cluster ? tree_peer(&ml[r].x, k) : -INFINITY;
+        top = fmaxf(top, w[k]);
+      }
+      const float sub = top == -INFINITY ? 0.f : top;
+#pragma unroll
+      for (int k = 0; k < TT_CLUSTER; ++k) {
+        w[k] = at_exp2(w[k] - sub);                 // 0 for what is not there
+        if (k < P.cluster) sum += tree_peer(&ml[r].y, k) * w[k];
+      }
+      sum += at_exp2(sink - sub);
+      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      bf16* dst = (bf16*)P.t.out + (size_t)t * P.t.out_stride + (size_t)head * D;
+#pragma unroll 1
+      for (int c4 = D / 4 * rank / P.cluster; c4 < D / 4 * (rank + 1) / P.cluster; c4 += 2) {
+        float4 y[TT_CLUSTER][2], a[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+#pragma unroll
+        for (int k = 0; k < TT_CLUSTER; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (k < P.cluster) y[k][u] = tree_peer4(reinterpret_cast<const float*>(kv_s) + ((c4 + u) * 128 + r) * 4, k);
+#pragma unroll
+        for (int k = 0; k < TT_CLUSTER; ++k)
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (k < P.cluster && w[k] != 0.f) {
+              a[u].x = fmaf(w[k], y[k][u].x, a[u].x); a[u].y = fmaf(w[k], y[k][u].y, a[u].y);
+              a[u].z = fmaf(w[k], y[k][u].z, a[u].z); a[u].w = fmaf(w[k], y[k][u].w, a[u].w);
+            }
+        uint4 v4;
+        v4.x = at_pack(a[0].x * inv, a[0].y * inv); v4.y = at_pack(a[0].z * inv, a[0].w * inv);
+        v4.z = at_pack(a[1].x * inv, a[1].y * inv); v4.w = at_pack(a[1].z * inv, a[1].w * inv);
+        *reinterpret_cast<uint4*>(dst + c4 * 4) = v4;
+      }
+    }
+    tree_cluster_sync();                            // the others have read this block's results
   }
   // ---------------- teardown
   tc_fence_before();
@@ -725,6 +799,8 @@ static int tt_launch(TtParams& P, const CUtensorMap& mq, const CUtensorMap& mk, 
   static bool ready[64] = {};                      // the limit is set once a device
   int st = tree_smem_limit((const void*)tree_attention_tc_kernel<D>, Tt<D>::SMEM, ready);
   if (st != 0) return st;
+  if (P.cluster > 1)
+    return tree_launch_clusters(tree_attention_tc_kernel<D>, (long)blocks, P.cluster, TT_THREADS, (size_t)Tt<D>::SMEM, stream, mq, mk, mv, P);
   st = launch_pdl(tree_attention_tc_kernel<D>, dim3(blocks), dim3(TT_THREADS), (size_t)Tt<D>::SMEM, stream, mq, mk, mv, P);
   if (st != 0 || P.whole) return st;
   const int chunks = (P.part_rows + 31) / 32;
@@ -757,7 +833,9 @@ PHOTON_API int photon_tree_attention_tc(const photon_tree_call* call, cudaStream
   if (total_rows > 0x7fffff00L) return PHOTON_ERR_UNSUPPORTED;
   P.whole = call->scratch == nullptr;
   P.blocks_sm = 2 * photon_sm_count();
-  P.sorted = t.S <= TT_SORTED && (long)t.S * t.n_kv * ((t.max_tokens + 128 / G - 1) / (128 / G)) <= 65535;
+  P.cluster = call->cluster;
+  if (P.cluster < 1 || P.cluster > TT_CLUSTER || (P.cluster & (P.cluster - 1)) || (P.cluster > 1 && (!P.whole || call->parts % P.cluster))) return PHOTON_ERR_ARGUMENT;
+  P.sorted = P.cluster == 1 && t.S <= TT_SORTED && (long)t.S * t.n_kv * ((t.max_tokens + 128 / G - 1) / (128 / G)) <= 65535;
   if (!P.whole && call->parts > TT_MAX_BLOCKS) return PHOTON_ERR_ARGUMENT;
   if (!P.whole && call->scratch_floats < photon_tree_attention_tc_scratch(t.max_tokens, t.n_q, t.n_kv, d, call->parts)) return PHOTON_ERR_ARGUMENT;
   EncodeTiledFn fn = encode_fn();

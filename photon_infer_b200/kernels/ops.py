@@ -2548,7 +2548,7 @@ def _int32s(names, tensors) -> None:
 
 
 #: photon_tree_call: pointers, strides and the scratch's size, sizes, scale and bound
-_TREE_CALL = struct.Struct("15q13i2f4x")
+_TREE_CALL = struct.Struct("15q13i2fi")
 _CALL_ARGS = [c_char_p, c_void_p]
 
 
@@ -2590,11 +2590,11 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     keys = min(max_keys, window + max_tokens_per_seq) if window else max_keys
     pointers = [t.data_ptr() for t in (q, out, k_cache, v_cache)]
     aligned = q_stride % 8 == 0 and out_stride % 8 == 0 and not any(p % 16 for p in pointers)
-    name, parts = _tree_route(dtype, head_dim, group, page_size, pages * n_kv * page_size, aligned, num_seqs, n_kv, max_tokens_per_seq * group, keys,
+    name, parts, cluster = _tree_route(dtype, head_dim, group, page_size, pages * n_kv * page_size, aligned, num_seqs, n_kv, max_tokens_per_seq * group, keys,
                               sm_count(device))
     floats = 0
-    if name == "tree_attention_tc" and parts < 0:
-        parts = -parts                              # whole units: no scratch
+    if name == "tree_attention_tc" and (parts < 0 or cluster > 1):
+        parts = abs(parts)                          # whole units: no scratch
     elif name == "tree_attention_tc":
         floats = 8 * parts + 2 * parts * (-(-min(max_tokens_per_seq * group, 128 // group * group) // 32) * 32) * (head_dim + 2)
     elif name == "tree_attention" and parts not in (1, 2, 4, 8):
@@ -2603,7 +2603,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     call = _TREE_CALL.pack(*pointers, block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), positions.data_ptr(),
                            tree_mask.data_ptr(), sink.data_ptr() if sink is not None else 0, scratch.data_ptr() if floats else 0,
                            err.data_ptr() if err is not None else 0, q_stride, out_stride, floats, _dtype_code(q), width, words,
-                           num_seqs, T, max_tokens_per_seq, n_q, n_kv, head_dim, page_size, pages, min(window or 0, 0x7fffffff), parts, scale, softcap or 0.0)
+                           num_seqs, T, max_tokens_per_seq, n_q, n_kv, head_dim, page_size, pages, min(window or 0, 0x7fffffff), parts, scale, softcap or 0.0, cluster)
     _check(_plain_fn(name, "photon_" + name, _CALL_ARGS)(call, _stream()), "tree_attention")
     if floats:
         _count_launches(1)                      # the second kernel, which joins partial results
@@ -2615,13 +2615,18 @@ def _count_launches(n: int) -> None:
     _launch_count += n
 
 
-#: Tiles of 64 keys that a block of the kernel for few rows may walk one behind the other (waves counted), by head size.
-TREE_FEW_STEPS = {64: 12, 128: 5}
+#: Tiles of 64 keys that a block of the kernel for few rows may walk one behind the other (waves counted), by head size, for up to 16, 32 and 64 rows.  That
+#: kernel and tcgen05, us, 4, 8 and 14 nodes: 32/8 heads of 64, 1 request of 1,000 keys (2 tiles) 8.6 and 10.2, 8.6 and 10.2, 9.2 and 10.6; 4 of 2,000 (4) 13.1 and
+#: 13.7, 13.5 and 13.9, 15.6 and 14.5; 16 of up to 1,000 (8) 14.5 and 17.6, 18.0 and 17.6, 20.9 and 17.6; 4 of 6,000 (12) 23.8 and 20.9, 26.2 and 21.1, 31.3 and
+#: 21.7; heads of 128, 4 of 600 (2) 13.5 and 13.9, 13.7 and 14.1, 15.8 and 14.5; 16 of up to 300 (3) 13.5 and 15.2, 15.4 and 16.4, 18.0 and 16.6; 4 of 2,000 (4) 17.8 and
+#: 15.6, 18.6 and 16.2, 20.9 and 17.2.
+TREE_FEW_STEPS = {64: (10, 8, 4), 128: (3, 3, 1)}
 
 
 def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, cache_rows: int, aligned: bool, num_seqs: int, n_kv: int, rows: int,
                 keys: int, sms: int):
-    """(kernel, parts; below zero: blocks that take whole units) for a step whose requests have at most ``rows`` rows (nodes x query heads) per key/value head and ``keys`` visible keys."""
+    """(kernel, parts; below zero: blocks that take whole units, blocks that share a unit) for a step whose requests have at most ``rows`` rows (nodes x query
+    heads) per key/value head and ``keys`` visible keys."""
     if dtype == torch.bfloat16 and head_dim in (64, 128) and aligned:
         tiles, units = -(-keys // 64), num_seqs * n_kv
         tma = group <= 128 and page_size % 8 == 0 and (64 % page_size == 0 or page_size % 64 == 0) and cache_rows <= 0x7fffff00
@@ -2630,15 +2635,25 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
             while parts > 1 and (units * parts > 2 * sms or parts > 2 * tiles):
                 parts //= 2
             steps = -(-tiles // parts) * -(-units * parts // ((3 if head_dim == 64 else 2) * sms))
-            if not tma or steps <= TREE_FEW_STEPS[head_dim]:
-                return "tree_attention_few", parts
+            if not tma or steps <= TREE_FEW_STEPS[head_dim][(rows > 16) + (rows > 32)]:
+                return "tree_attention_few", parts, 1
         if tma:
             units *= -(-rows // (128 // group * group))
+            # Where the chip holds two blocks or more for each unit, a cluster of them shares it, with two tiles a block at least, and joins it in its own memory.  It
+            # costs what equal ranges would have shared out better: all of the chip over, and requests shorter than the longest.  Ranges with the second kernel, and
+            # clusters, us: 8 requests of 27 nodes behind up to 2,500 keys (32/8 heads of 64) 25.4 and 20.8, behind 4,000 34.0 and 28.0, up to 8,000 38.4 and 41.8, up to
+            # 16,000 47 and 68; 4 of 30 behind up to 4,000 (heads of 128) 30.2 and 25.1; 16 of 30 behind up to 4,000 55.1 and 48.8, up to 8,000 74 and 81;
+            # 1 of 32 behind 1,000 18.3 and 15.5, 4,000 18.6 and 18.8, 16,000 32 and 42; a window of 1,024 and bounded scores, 16 of 16, whole units 39 and clusters 30.
+            cluster = 1
+            while cluster < 8 and 2 * cluster * units <= 2 * sms and 4 * cluster <= tiles:
+                cluster *= 2
+            if cluster > 1 and tiles * (2 * sms - units * cluster) <= 16 * sms * cluster:
+                return "tree_attention_tc", units * cluster, cluster
             # Few keys: whole units, one kernel.  More: the kernel decides by the lengths, which the host does not know, and a second kernel follows
             # it; a block has four tiles at least.
             if tiles <= 12 or (tiles <= 32 and 4 * units >= 3 * sms):
-                return "tree_attention_tc", -min(2 * sms, 320, units)
-            return "tree_attention_tc", min(2 * sms, 320, max(units, -(-units * (tiles + 1) // 4)))
+                return "tree_attention_tc", -min(2 * sms, 320, units), 1
+            return "tree_attention_tc", min(2 * sms, 320, max(units, -(-units * (tiles + 1) // 4))), 1
     # The general kernel: 32 rows a block, 3, 2 or 1 blocks an SM (registers, shared memory).  A row tile's keys go to a cluster of up to eight blocks, as many as
     # take the fewest steps, a step being a tile of 64 keys or a third of what a block costs beside its tiles; very long requests that leave most of the chip
     # idle go to more, which a second kernel joins.  32-bit, 8 key/value heads of 64, 8 nodes x 4 heads, parts and us: 2,000 keys 4: 39, 8: 25, 16: 23, 32: 23; 4,000 keys
@@ -2647,13 +2662,13 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
     blocks, tiles = max(1, num_seqs * n_kv * -(-rows // 32)), -(-keys // 64)
     slots = (3 if head_dim <= 64 else 2 if head_dim <= 128 else 1) * sms
     if tiles >= 48 and 16 * blocks <= slots:
-        return "tree_attention", min(slots // blocks, tiles // 2, 64)
+        return "tree_attention", min(slots // blocks, tiles // 2, 64), 1
     parts, least = 1, 0.0
     for p in (1, 2, 4, 8):
         cost = -(-blocks * p // slots) * (tiles / p + 3)
         if p == 1 or (cost < least and p <= tiles):
             parts, least = p, cost
-    return "tree_attention", parts
+    return "tree_attention", parts, 1
 
 
 def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tensor, cu_tokens: torch.Tensor, num_seqs: int,
