@@ -2638,7 +2638,8 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
             if not tma or steps <= TREE_FEW_STEPS[head_dim][(rows > 16) + (rows > 32)]:
                 return "tree_attention_few", parts, 1
         if tma:
-            units *= -(-rows // (128 // group * group))
+            levels = -(-rows // (128 // group * group))
+            units *= levels
             # Where the chip holds two blocks or more for each unit, a cluster of them shares it, with two tiles a block at least, and joins it in its own memory.  It
             # costs what equal ranges would have shared out better: all of the chip over, and requests shorter than the longest.  Ranges with the second kernel, and
             # clusters, us: 8 requests of 27 nodes behind up to 2,500 keys (32/8 heads of 64) 25.4 and 20.8, behind 4,000 34.0 and 28.0, up to 8,000 38.4 and 41.8, up to
@@ -2653,7 +2654,9 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
             # it; a block has four tiles at least.
             if tiles <= 12 or (tiles <= 32 and 4 * units >= 3 * sms):
                 return "tree_attention_tc", -min(2 * sms, 320, units), 1
-            return "tree_attention_tc", min(2 * sms, 320, max(units, -(-units * (tiles + 1) // 4))), 1
+            # As many ranges for each of a request's row tiles, which then read the same keys at the same time.
+            parts = min(2 * sms, 320, max(units, -(-units * (tiles + 1) // 4)))
+            return "tree_attention_tc", max(parts - parts % levels, 1), 1
     # The general kernel: 32 rows a block, 3, 2 or 1 blocks an SM (registers, shared memory).  A row tile's keys go to a cluster of up to eight blocks, as many as
     # take the fewest steps, a step being a tile of 64 keys or a third of what a block costs beside its tiles; very long requests that leave most of the chip
     # idle go to more, which a second kernel joins.  32-bit, 8 key/value heads of 64, 8 nodes x 4 heads, parts and us: 2,000 keys 4: 39, 8: 25, 16: 23, 32: 23; 4,000 keys
