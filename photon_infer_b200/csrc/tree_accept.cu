@@ -7,10 +7,10 @@
 // A row of logits is a cluster of blocks' work: a block takes a run of the vocabulary, up to 32 numbers a thread in registers (longer runs are read again), and the blocks'
 // maxima and sums meet in each other's shared memory.  Sums are in 32 bits, added up in an order that the sizes alone give.
 //
-// Two ways.  Few logits in all: a cluster for every node at once, and a second kernel walks the trees.  Many: a cluster for every request walks its
-// tree, and reads the logits of the nodes on the path alone, one after the other.
+// Two ways.  A cluster for every request walks its tree, and reads the logits of the nodes on the path alone, one after the other.  Few logits in all that tokens are
+// drawn from: a cluster for every node at once, and a second kernel walks the trees.
 // A step of a walk is latency: 2.1 us greedily (a row from memory, the warps' and the blocks' maxima, one exchange), 5.6 us with a temperature (weights, sums, and
-// a second exchange, which tells all blocks what one of them has chosen).  128,256 tokens: one request of 8 nodes 4.6 us at once, 6.5 to 8 us as a walk; 32 requests of 64
+// a second exchange, which tells all blocks what one of them has chosen).  128,256 tokens: one request of 8 nodes 4.4 us greedily, sampled 13 as a walk and 7.5 at once; 32 requests of 64
 // nodes, half of them sampled, walk in 52 us (all 1.05 GB of logits would take 268 and more), the paths' 65 MB at the copy rate 10.
 #include "common.cuh"
 #include <math.h>

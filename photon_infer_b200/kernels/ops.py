@@ -2698,8 +2698,9 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     if temperature is not None and (uniforms is None or any(t.dtype != torch.float32 or not t.is_contiguous() for t in (temperature, uniforms))
                                     or temperature.numel() < num_seqs or uniforms.numel() < T):
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_accept: temperature [requests] and uniforms [T] must be contiguous float32")
-    # few logits: all nodes' at once, and a second kernel for the walk; many: a walk that reads those on the paths alone
-    given = torch.empty(T, dtype=torch.int32, device=logits.device) if num_seqs * max_tokens_per_seq * V <= ACCEPT_AT_ONCE else None
+    # a walk that reads the logits on the paths alone; few logits to draw from: all nodes' at once, and a second kernel for the walk
+    at_once = temperature is not None and num_seqs * max_tokens_per_seq * V <= ACCEPT_AT_ONCE
+    given = torch.empty(T, dtype=torch.int32, device=logits.device) if at_once else None
     call = _ACCEPT_CALL.pack(logits.data_ptr(), tokens.data_ptr(), parents.data_ptr(), cu_tokens.data_ptr(),
                              temperature.data_ptr() if temperature is not None else 0, uniforms.data_ptr() if temperature is not None else 0,
                              path.data_ptr(), counts.data_ptr(), sampled.data_ptr(), given.data_ptr() if given is not None else 0,
@@ -2712,8 +2713,9 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
 
 #: photon_accept_call
 _ACCEPT_CALL = struct.Struct("12q5i4x")
-#: Logits up to which those of all nodes are read at once.  Walk and all at once, us, vocabulary of 128,256: 1 request of 16 nodes 10 and 7 (sampled 13 and 10), 1 of
-#: 64 10 and 12 (24 and 18), 4 of 16 16 and 12 (40 and 16), 4 of 64 12 and 39 (30 and 51), 32 of 8 28 and 39 (52 and 51), 32 of 64 27 and 268.
+#: Logits up to which those of all nodes are read at once where tokens are drawn.  Walk and all at once, us on the device (and calls in a row: the second has another
+#: launch), vocabulary of 128,256: 1 request of 8 nodes greedily 4.4 and 4.8 (15 and 20), 1 of 64 10 and 14 (15 and 19), 8 of 12 12 and 18 (15 and 19); sampled 1 of 8 13
+#: and 7 (16 and 20), 1 of 16 29 and 10 (29 and 20), 2 of 32 35 and 17 (35 and 20), 8 of 8 24 and 18 (24 and 20), 4 of 64 30 and 51, 32 of 64 52 and 268.
 ACCEPT_AT_ONCE = 12 << 20
 
 
