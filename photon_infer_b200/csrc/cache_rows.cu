@@ -6,8 +6,9 @@
 // path[s][j], j < counts[s], goes to key base + j.  A path ascends from its root, so path[j] >= j: a row is never needed after a later one has been written.  A
 // thread owns one piece of the rows of one head and moves eight rows at a time: all eight are read before the first is written, and what a later eight read lies
 // behind all that an earlier eight wrote.  Threads share nothing, so there is nothing to wait for.
-// Bound by the latency of one round (path, table, rows, rows back) for few rows: 8 requests, 16 layers of 8 heads of 64: 3.0 us; 48 requests, 28 layers of 8 heads of
-// 128, 44 MB read and written: 12.8 us (3.4 TB/s, rows of 256 bytes in no order).
+// Bound by the latency of one round (path, table, rows, rows back) for few rows: 8 requests, 16 layers of 8 heads of 64: 2.9 us (3.2 with the path read behind the count);
+// 48 requests, 28 layers of 8 heads of 128, 44 MB read and written: 12.3 us (3.6 TB/s, rows of 256 bytes in no order; 13.0 with a block for every 256 pieces, two rounds
+// of blocks); 20 requests of as many layers in 32 bits 7.2 (8.7).
 //
 // cache_copy_pages: page pairs[i][0] onto page pairs[i][1]; a block copies a part of one page in one plane, 64 bytes a thread in flight.
 // 512 pages of 28 layers, 1.88 GB: 285 us, the copy rate; 8 pages of 16 layers 2.0 us.
@@ -15,6 +16,7 @@
 
 #define CR_THREADS 256
 #define CR_ROWS 8                                  // rows of a path that a thread moves at a time
+#define CR_BLOCKS 4                                // an SM, of a kernel that moves rows: a second round of blocks would go the way to the rows again
 #define CR_PIECES 4                                // pieces of a page that a thread copies at a time
 
 template <typename V>
@@ -25,16 +27,11 @@ cache_keep_kernel(V* __restrict__ kv, long units, int num_pages, int n_kv, int p
   __shared__ long long src_s[CR_THREADS], dst_s[CR_THREADS];      // rows (page, slot) of the moves that there are, a block's worth at a time
   pdl_wait();
   const int seq = blockIdx.y;
+  const int node = 1 + (int)threadIdx.x < D ? path[(size_t)seq * D + 1 + threadIdx.x] : 0;      // beside the count, not behind it
+  const int first = cu_tokens[seq], n = cu_tokens[seq + 1] - first, base = context_lens[seq] - n;
   const int count = min(counts[seq], D);
   if (count < 2) return;
-  const int n = cu_tokens[seq + 1] - cu_tokens[seq], base = context_lens[seq] - n;
   const int* table = block_table + (size_t)seq * max_pages;
-  const long unit = (long)blockIdx.x * CR_THREADS + threadIdx.x;              // (entry and plane, head, piece)
-  const int piece = (int)(unit % pieces);
-  const long head = unit / pieces;
-  const int g = (int)(head % n_kv);
-  const long plane = head / n_kv;
-  V* rows = kv + ((plane * num_pages) * n_kv + g) * (long)page_size * pieces + piece;
   const long page_step = (long)n_kv * page_size * pieces;                     // from a page's row to the same row of the next page
   auto place = [&](int key) -> long long {         // page and slot of a key, packed; -1: no page
     const int pidx = key / page_size;
@@ -49,7 +46,7 @@ cache_keep_kernel(V* __restrict__ kv, long units, int num_pages, int n_kv, int p
     const int here = min(CR_THREADS, count - j0), j = j0 + (int)threadIdx.x;
     __syncthreads();
     if (j < count) {
-      const int from = path[(size_t)seq * D + j];
+      const int from = j0 == 1 ? node : path[(size_t)seq * D + j];
       long long src = -1, dst = -1;
       if (from < j || from >= n) {
         if (blockIdx.x == 0) report_error(err, PHOTON_DEV_BAD_TOKEN, seq, from, n);
@@ -61,14 +58,17 @@ cache_keep_kernel(V* __restrict__ kv, long units, int num_pages, int n_kv, int p
       dst_s[threadIdx.x] = dst;
     }
     __syncthreads();
-    if (unit >= units) continue;
-    auto at = [&](long long p) { return rows + (p >> 32) * page_step + (long)(uint32_t)p * pieces; };
-    for (int k = 0; k < here; k += CR_ROWS) {
-      V x[CR_ROWS];
+    for (long unit = (long)blockIdx.x * CR_THREADS + threadIdx.x; unit < units; unit += (long)gridDim.x * CR_THREADS) {      // (entry and plane, head, piece)
+      const long head = unit / pieces, plane = head / n_kv;
+      V* rows = kv + (plane * num_pages * n_kv + (head - plane * n_kv)) * (long)page_size * pieces + (unit - head * pieces);
+      auto at = [&](long long p) { return rows + (p >> 32) * page_step + (long)(uint32_t)p * pieces; };
+      for (int k = 0; k < here; k += CR_ROWS) {
+        V x[CR_ROWS];
 #pragma unroll
-      for (int i = 0; i < CR_ROWS; ++i) if (k + i < here && src_s[k + i] >= 0) x[i] = *at(src_s[k + i]);
+        for (int i = 0; i < CR_ROWS; ++i) if (k + i < here && src_s[k + i] >= 0) x[i] = *at(src_s[k + i]);
 #pragma unroll
-      for (int i = 0; i < CR_ROWS; ++i) if (k + i < here && src_s[k + i] >= 0) *at(dst_s[k + i]) = x[i];
+        for (int i = 0; i < CR_ROWS; ++i) if (k + i < here && src_s[k + i] >= 0) *at(dst_s[k + i]) = x[i];
+      }
     }
   }
 }
@@ -110,7 +110,8 @@ PHOTON_API int photon_cache_keep(const photon_keep_call* c, cudaStream_t stream)
   const long row = (long)c->d * (c->dtype == PHOTON_F32 ? 4 : 2);
   const int b = piece_bytes(c->kv, row), pieces = (int)(row / b);
   const long units = (long)c->planes * c->n_kv * pieces;
-  const dim3 grid((unsigned)((units + CR_THREADS - 1) / CR_THREADS), (unsigned)c->S);
+  const long blocks = (units + CR_THREADS - 1) / CR_THREADS, most = (CR_BLOCKS * photon_sm_count() + c->S - 1) / c->S;
+  const dim3 grid((unsigned)(blocks < most ? blocks : most), (unsigned)c->S);
 #define KEEP(V) launch_pdl(cache_keep_kernel<V>, grid, dim3(CR_THREADS), 0, stream, (V*)c->kv, units, c->num_pages, c->n_kv, c->page_size, pieces, c->block_table, \
                            c->max_pages, c->cu_tokens, c->context_lens, c->path, c->counts, c->D, c->err)
   return b == 16 ? KEEP(uint4) : b == 8 ? KEEP(uint2) : b == 4 ? KEEP(uint32_t) : KEEP(uint16_t);
