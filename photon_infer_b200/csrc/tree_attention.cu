@@ -5,28 +5,31 @@
 // (bounded scores: x_j = softcap tanh(scale q . k_j / softcap); m the largest of the scores and the sink) over the keys that node t sees
 // (tree_attention.cuh); a row that sees nothing is zero.  Scores, weights, sums and outputs are held in 32 bits.
 //
-// A block takes 32 rows, (node, query head) pairs that share a key/value head, and a share of the request's keys, in tiles of 64; a warp has 16 of the rows and half a
-// tile's keys.  A thread holds the scores of four rows with four keys, then those rows' outputs for D / 8 numbers, and a lane's neighbours read the same operands, so
-// that a product costs a quarter of a word of shared memory; products go in pairs (fma.rn.f32x2).  Each warp has its own maxima and sums; the
-// weights pass through shared memory inside the warp.  The warps' results, and those of a cluster of up to eight blocks that share a row tile's keys, are joined in
-// shared memory in their order; where more blocks share them, by a second kernel.
+// A block takes up to 32 rows, (node, query head) pairs that share a key/value head, and a share of the request's keys, in tiles of 64; a warp has 16 of the rows and a half, a
+// quarter or an eighth of a tile's keys (tree_choose).  A thread holds the scores of four rows with up to four keys, then those rows' outputs for D / 8 numbers, and a
+// lane's neighbours read the same operands, so that a product costs a quarter of a word of shared memory; products go in pairs (fma.rn.f32x2).  Each warp has its own
+// maxima and sums; the weights pass through shared memory inside the warp.  The warps' results, and those of a cluster of up to eight blocks that share a row tile's
+// keys, are joined in shared memory in their order; where more blocks share them, by a second kernel.
 //
-// What bounds it: 32-bit products.  4 requests of 13 nodes behind up to 700 keys (32/8 heads of 64): 25 us, 1 us of it for the bytes; 8 of 32 behind up to 2,000:
-// 104 us = 15 TFLOP/s of products that are needed.  A tile ahead in shared memory left two blocks an SM and was slower (32 and 25 us, 132 and 108);
-// tiles of 32 keys 23 and 118; four warps for a row's keys 23 and 116; the sums of products in one number after the other, 32 keys a tile,
-// 36 and 334.
+// What bounds it: 32-bit products, and for small calls their latency.  4 requests of 13 nodes behind up to 700 keys (32/8 heads of 64): 25 us, 1 us of it for the bytes; 8 of
+// 32 behind up to 2,000: 104 us = 15 TFLOP/s of products that are needed; 1 of 8 behind 640: 16; 3 of 5 behind up to 36: 9.  A tile ahead in shared memory left two
+// blocks an SM and was slower (32 and 25 us, 132 and 108); tiles of 32 keys 23 and 118; the sums of products in one number after the other, 32 keys a
+// tile, 36 and 334.
 //
 // A key that a row does not see has weight 0, and 0 times a value that is not finite would not be: in tiles where masks cut, products with a weight of 0
 // are left out, and rows behind the last key or of a missing page are zeros.
 #include "tree_attention.cuh"
 #include <math.h>
+#include <type_traits>
 
-#define TG_ROWS 32
 #define TG_KEYS 64
-#define TG_SHARES 2                                // warps that share a row's keys
-#define TG_THREADS (64 * TG_SHARES)
-#define TG_MINE (TG_KEYS / TG_SHARES)              // a warp's keys
-#define TG_PS (TG_MINE + 4)                        // row stride of a warp's weights, [16][TG_MINE]
+
+// How a block's warps share a tile: GROUPS of 16 rows, SHARES of the keys.
+template <int GROUPS, int SHARES> struct Tg {
+  static constexpr int ROWS = 16 * GROUPS, THREADS = 32 * GROUPS * SHARES;
+  static constexpr int MINE = TG_KEYS / SHARES;    // a warp's keys
+  static constexpr int PS = MINE + 4;              // row stride of a warp's weights, [16][MINE]
+};
 
 struct TreeShares {
   float* part_o;                                   // [T * n_q, splits, d]
@@ -47,14 +50,14 @@ __device__ __forceinline__ void tg_copy16(void* dst, const void* src, bool there
 }
 
 // Keys and values of a tile into shared memory; rows that are not there and the columns behind d are zeros.
-template <typename T, int D, int KS>
+template <typename T, int D, int KS, int THREADS>
 __device__ __forceinline__ void tg_load_tile(const TreeParams& P, const long long* krow, T* ks, T* vs, bool wide, int tid) {
   const T* kc = (const T*)P.k_cache;
   const T* vc = (const T*)P.v_cache;
   constexpr int E = 16 / (int)sizeof(T), PIECES = D / E;
   if (wide) {
 #pragma unroll
-    for (int e = tid; e < TG_KEYS * PIECES; e += TG_THREADS) {
+    for (int e = tid; e < TG_KEYS * PIECES; e += THREADS) {
       const int r = e / PIECES, j = e % PIECES * E;
       const long long at = krow[r];
       const bool there = at >= 0 && j < P.d;
@@ -63,7 +66,7 @@ __device__ __forceinline__ void tg_load_tile(const TreeParams& P, const long lon
       tg_copy16(vs + r * D + j, vc + from, there);
     }
   } else {                                         // rows that do not begin at 16 bytes
-    for (int e = tid; e < TG_KEYS * D; e += TG_THREADS) {
+    for (int e = tid; e < TG_KEYS * D; e += THREADS) {
       const int r = e / D, j = e % D;
       const long long at = krow[r];
       const bool there = at >= 0 && j < P.d;
@@ -74,10 +77,11 @@ __device__ __forceinline__ void tg_load_tile(const TreeParams& P, const long lon
   asm volatile("cp.async.commit_group;\n\tcp.async.wait_group 0;" ::: "memory");
 }
 
-template <typename T, int D>
+template <typename T, int D, int GROUPS, int SHARES>
 constexpr size_t tg_smem_bytes() {
-  const size_t tile = TG_KEYS * (D + 16 / sizeof(T) + D) * sizeof(T), results = TG_SHARES * TG_ROWS * (D + 4) * sizeof(float);
-  return (size_t)(TG_ROWS * (D + 4) + 2 * TG_SHARES * 16 * TG_PS) * sizeof(float) + (tile > results ? tile : results);
+  using C = Tg<GROUPS, SHARES>;
+  const size_t tile = TG_KEYS * (D + 16 / sizeof(T) + D) * sizeof(T), results = SHARES * C::ROWS * (D + 4) * sizeof(float);
+  return (size_t)(C::ROWS * (D + 4) + GROUPS * SHARES * 16 * C::PS) * sizeof(float) + (tile > results ? tile : results);
 }
 
 // Two products and sums at once, each rounded like fmaf.
@@ -86,31 +90,33 @@ __device__ __forceinline__ void tg_fma2(float2& acc, const float2 a, const float
       "mov.b64 {%0, %1}, z;\n\t}" : "+f"(acc.x), "+f"(acc.y) : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
 }
 
-template <typename T, int D>
-__global__ void __launch_bounds__(TG_THREADS)
+template <typename T, int D, int GROUPS, int SHARES>
+__global__ void __launch_bounds__(32 * GROUPS * SHARES)
 tree_attention_kernel(const TreeParams P, const TreeShares H) {
-  constexpr int S = D + 4, C = D / 32, U = TG_MINE / 8;             // row stride of the queries; groups of four output numbers a thread has
+  using Y = Tg<GROUPS, SHARES>;
+  constexpr int ROWS = Y::ROWS, THREADS = Y::THREADS, MINE = Y::MINE, PS = Y::PS;
+  constexpr int S = D + 4, C = D / 32, U = MINE / 8;             // row stride of the queries; groups of four output numbers a thread has
   constexpr int KS = D + 16 / (int)sizeof(T);         // row stride of the keys
   extern __shared__ __align__(16) float tg_smem[];
-  float* qs = tg_smem;                             // [TG_ROWS][S]
-  float* ps = qs + TG_ROWS * S;                    // per warp [16][TG_PS]
-  T* ks = (T*)(ps + 2 * TG_SHARES * 16 * TG_PS);               // [TG_KEYS][KS]
+  float* qs = tg_smem;                             // [ROWS][S]
+  float* ps = qs + ROWS * S;                       // per warp [16][PS]
+  T* ks = (T*)(ps + GROUPS * SHARES * 16 * PS);               // [TG_KEYS][KS]
   T* vs = ks + TG_KEYS * KS;                       // [TG_KEYS][D]
   __shared__ long long krow[TG_KEYS];
-  __shared__ float ml_s[2][TG_SHARES][TG_ROWS], factor[TG_ROWS][8 * TG_SHARES];
-  __shared__ uint32_t seen[2][2][TG_ROWS];   // a warp may be at work on the tile before when the next one's are found
+  __shared__ float ml_s[2][SHARES][ROWS], factor[ROWS][8 * SHARES];
+  __shared__ uint32_t seen[2][2][32];   // a warp may be at work on the tile before when the next one's are found
   pdl_wait();
   int b = blockIdx.x;
   const int split = b % H.splits; b /= H.splits;
   const int g = b % P.n_kv; b /= P.n_kv;
   const int rt = b % H.row_tiles, seq = b / H.row_tiles;
   const TreeRequest R = tree_request(P, seq);
-  const int G = P.group, d = P.d, rows = R.n * G, row0 = rt * TG_ROWS;
+  const int G = P.group, d = P.d, rows = R.n * G, row0 = rt * ROWS;
   if (row0 >= rows) return;
-  const int nrows = min(TG_ROWS, rows - row0);
+  const int nrows = min(ROWS, rows - row0);
   const int* table = P.block_table + (size_t)seq * P.max_pages;
-  const int tid = threadIdx.x, lane = tid & 31, rw = (tid >> 5) & 1, kw = tid >> 6;
-  const int lr = lane >> 3, lc = lane & 7;         // rows 16 rw + lr + 4 i; keys TG_MINE kw + lc + 8 u; columns 4 lc + 32 c
+  const int tid = threadIdx.x, lane = tid & 31, rw = (tid >> 5) % GROUPS, kw = (tid >> 5) / GROUPS;
+  const int lr = lane >> 3, lc = lane & 7;         // rows 16 rw + lr + 4 i; keys MINE kw + lc + 8 u; columns 4 lc + 32 c
 
   // the first cached key that any of the rows sees
   int key_lo = 0;
@@ -148,7 +154,7 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
 
   const T* q = (const T*)P.q;
 #pragma unroll 8
-  for (int e = tid; e < TG_ROWS * D; e += TG_THREADS) {
+  for (int e = tid; e < ROWS * D; e += THREADS) {
     const int r = e / D, j = e % D, row = row0 + r;
     qs[r * S + j] = r < nrows && j < d ? to_f32(q[(size_t)(R.tok0 + row / G) * P.q_stride + (size_t)(g * G + row % G) * d + j]) : 0.f;
   }
@@ -162,23 +168,23 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
     for (int j = 0; j < C * 2; ++j) o[i][j] = make_float2(0.f, 0.f);
   }
   const float* my_q = qs + (16 * rw + lr) * S;
-  const T* my_k = ks + (TG_MINE * kw + lc) * KS;
-  const T* my_v = vs + TG_MINE * kw * D + lc * 4;
-  float* my_p = ps + (tid >> 5) * 16 * TG_PS;
+  const T* my_k = ks + (MINE * kw + lc) * KS;
+  const T* my_v = vs + MINE * kw * D + lc * 4;
+  float* my_p = ps + (tid >> 5) * 16 * PS;
   const bool wide = (size_t)d * sizeof(T) % 16 == 0 && ((((uintptr_t)P.k_cache | (uintptr_t)P.v_cache) & 15) == 0);
   for (int tile = begin; tile < end; ++tile) {
     find(tile, page);
     page = entry(tile + 1);
     __syncthreads();                               // the rows are known; the tile before is read
-    tg_load_tile<T, D, KS>(P, krow, ks, vs, wide, tid);
+    tg_load_tile<T, D, KS, THREADS>(P, krow, ks, vs, wide, tid);
     __syncthreads();
-    constexpr uint32_t MINE = TG_MINE < 32 ? (1u << (TG_MINE & 31)) - 1u : 0xffffffffu;
+    constexpr uint32_t KEYS = MINE < 32 ? (1u << (MINE & 31)) - 1u : 0xffffffffu;
     uint32_t see[4], all = 0xffffffffu, any = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      see[i] = seen[tile & 1][TG_MINE * kw >> 5][16 * rw + lr + 4 * i] >> (TG_MINE * kw & 31);
-      all &= see[i] | ~MINE;
-      any |= see[i] & MINE;
+      see[i] = seen[tile & 1][MINE * kw >> 5][16 * rw + lr + 4 * i] >> (MINE * kw & 31);
+      all &= see[i] | ~KEYS;
+      any |= see[i] & KEYS;
     }
     if (16 * rw >= nrows || !__any_sync(0xffffffffu, any != 0)) continue;            // none of the warp's rows sees one of its keys
     float2 s[4][U];
@@ -221,17 +227,17 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
       for (int u = 0; u < U; ++u) {
         const float p = expf(x[u] - sub);
         l[i] += p;
-        my_p[(lr + 4 * i) * TG_PS + lc + 8 * u] = p;
+        my_p[(lr + 4 * i) * PS + lc + 8 * u] = p;
       }
 #pragma unroll
       for (int j = 0; j < C * 2; ++j) { o[i][j].x *= keep; o[i][j].y *= keep; }
     }
     __syncwarp();
     if (__any_sync(0xffffffffu, all != 0xffffffffu)) {
-      for (int k = 0; k < TG_MINE; ++k) {
+      for (int k = 0; k < MINE; ++k) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float p = my_p[(lr + 4 * i) * TG_PS + k];
+          const float p = my_p[(lr + 4 * i) * PS + k];
           if (p != 0.f) {                          // a NaN is not 0
 #pragma unroll
             for (int c = 0; c < C; ++c) {
@@ -244,10 +250,10 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
       }
     } else {
 #pragma unroll 2
-      for (int k = 0; k < TG_MINE; k += 4) {
+      for (int k = 0; k < MINE; k += 4) {
         float4 p[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) p[i] = *(const float4*)(my_p + (lr + 4 * i) * TG_PS + k);
+        for (int i = 0; i < 4; ++i) p[i] = *(const float4*)(my_p + (lr + 4 * i) * PS + k);
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
 #pragma unroll
@@ -272,29 +278,29 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
     for (int w = 4; w > 0; w >>= 1) l[i] += __shfl_xor_sync(0xffffffffu, l[i], w);
 
   // The warps of a row's keys, and the blocks of a cluster, leave their results where the tiles were.
-  float* po = (float*)ks;                          // [TG_SHARES][TG_ROWS][S]
+  float* po = (float*)ks;                          // [SHARES][ROWS][S]
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int r = 16 * rw + lr + 4 * i;
 #pragma unroll
     for (int c = 0; c < C; ++c)
-      *(float4*)(po + (kw * TG_ROWS + r) * S + c * 32 + lc * 4) = make_float4(o[i][2 * c].x, o[i][2 * c].y, o[i][2 * c + 1].x, o[i][2 * c + 1].y);
+      *(float4*)(po + (kw * ROWS + r) * S + c * 32 + lc * 4) = make_float4(o[i][2 * c].x, o[i][2 * c].y, o[i][2 * c + 1].x, o[i][2 * c + 1].y);
     if (lc == 0) { ml_s[0][kw][r] = m[i]; ml_s[1][kw][r] = l[i]; }
   }
   const int rank = H.cluster > 1 ? split : 0;
   if (H.cluster > 1) tree_cluster_sync();
   else __syncthreads();
   const bool last = H.cluster == H.splits;         // else: a share of several
-  // Each result's factor: 2 TG_SHARES threads a row, four results each.
+  // Each result's factor: 2 SHARES threads a row, four results each.
   {
-    constexpr int W = 2 * TG_SHARES;
-    const int r = tid / W, n = TG_SHARES * H.cluster;
+    constexpr int W = 2 * SHARES;
+    const int r = tid / W, n = SHARES * H.cluster;
     float mx[4], top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int w = tid % W + W * u;
-      mx[u] = w < n ? tree_peer(&ml_s[0][w % TG_SHARES][r], w / TG_SHARES) : -INFINITY;
+      mx[u] = w < n ? tree_peer(&ml_s[0][w % SHARES][r], w / SHARES) : -INFINITY;
       top = fmaxf(top, mx[u]);
     }
 #pragma unroll
@@ -305,7 +311,7 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
     for (int u = 0; u < 4; ++u) {
       const int w = tid % W + W * u;
       mx[u] = expf(mx[u] - sub);                   // 0 for what is not there
-      if (w < n) sum += tree_peer(&ml_s[1][w % TG_SHARES][r], w / TG_SHARES) * mx[u];
+      if (w < n) sum += tree_peer(&ml_s[1][w % SHARES][r], w / SHARES) * mx[u];
     }
 #pragma unroll
     for (int w = W / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
@@ -320,15 +326,15 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
   }
   __syncthreads();
   const int fours = nrows * (D / 4), stop = fours * (rank + 1) / H.cluster;
-  for (int e = fours * rank / H.cluster + tid; e < stop; e += TG_THREADS) {
+  for (int e = fours * rank / H.cluster + tid; e < stop; e += THREADS) {
     const int r = e / (D / 4), j = e % (D / 4) * 4, row = row0 + r, t = R.tok0 + row / G, head = g * G + row % G;
     if (j >= d) continue;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int c = 0; c < H.cluster; ++c) {
 #pragma unroll
-      for (int k = 0; k < TG_SHARES; ++k) {
-        const float w = factor[r][TG_SHARES * c + k];
-        const float4 x = tree_peer4(po + (k * TG_ROWS + r) * S + j, c);
+      for (int k = 0; k < SHARES; ++k) {
+        const float w = factor[r][SHARES * c + k];
+        const float4 x = tree_peer4(po + (k * ROWS + r) * S + j, c);
         if (w != 0.f) { a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w); }
       }
     }
@@ -376,16 +382,36 @@ tree_join_kernel(const TreeParams P, const TreeShares H) {
   }
 }
 
-template <typename T, int D>
+template <typename T, int D, int GROUPS, int SHARES>
 static int tree_launch(const TreeParams& P, const TreeShares& H, long blocks, cudaStream_t stream) {
-  const size_t smem = tg_smem_bytes<T, D>();
+  constexpr int THREADS = Tg<GROUPS, SHARES>::THREADS;
+  const size_t smem = tg_smem_bytes<T, D, GROUPS, SHARES>();
   static bool ready[64] = {};                      // the limit is set once a device
-  const int set = tree_smem_limit((const void*)tree_attention_kernel<T, D>, (int)smem, ready);
+  const int set = tree_smem_limit((const void*)tree_attention_kernel<T, D, GROUPS, SHARES>, (int)smem, ready);
   if (set != 0) return set;
-  if (H.cluster > 1) return tree_launch_clusters(tree_attention_kernel<T, D>, blocks, H.cluster, TG_THREADS, smem, stream, P, H);
-  const int st = launch_pdl(tree_attention_kernel<T, D>, dim3((unsigned)blocks), dim3(TG_THREADS), smem, stream, P, H);
+  if (H.cluster > 1) return tree_launch_clusters(tree_attention_kernel<T, D, GROUPS, SHARES>, blocks, H.cluster, THREADS, smem, stream, P, H);
+  const int st = launch_pdl(tree_attention_kernel<T, D, GROUPS, SHARES>, dim3((unsigned)blocks), dim3(THREADS), smem, stream, P, H);
   if (st != 0 || H.splits == 1) return st;
   return launch_pdl(tree_join_kernel<T>, dim3((unsigned)(((long)P.T * P.n_q + 3) / 4)), dim3(128), 0, stream, P, H);
+}
+
+template <typename T>
+static int tree_choose(const TreeParams& P, TreeShares& H, cudaStream_t stream) {
+  const long rows = (long)P.max_tokens * P.group;
+  H.row_tiles = (int)((rows + 31) / 32);
+  const long blocks = (long)P.S * H.row_tiles * P.n_kv * H.splits;
+  if (blocks > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
+  // Four warps a block, so that several blocks share an SM; eight where every block has an SM to itself (32-bit, four and eight warps, us: 1 request of 8 x 4 rows behind
+  // 640 keys 17.2 and 16.0; 8 of 32 x 4 behind up to 2,000: 104 and 116).  Up to 16 rows: no warps for others (3 of 4 x 4 behind up to 187, heads of 128: 25.4
+  // with half of four warps idle, 17.6 with eight at work; 8 of 4 x 4 behind up to 2,000: 67 and, with four at work, 58).
+  const bool alone = blocks <= photon_sm_count();
+  auto launch = [&](auto head) {
+    constexpr int D = decltype(head)::value;
+    if (rows <= 16) return alone ? tree_launch<T, D, 1, 8>(P, H, blocks, stream) : tree_launch<T, D, 1, 4>(P, H, blocks, stream);
+    return alone ? tree_launch<T, D, 2, 4>(P, H, blocks, stream) : tree_launch<T, D, 2, 2>(P, H, blocks, stream);
+  };
+  return P.d <= 64 ? launch(std::integral_constant<int, 64>()) : P.d <= 128 ? launch(std::integral_constant<int, 128>())
+                                                                           : tree_launch<T, 256, 2, 2>(P, H, blocks, stream);
 }
 
 PHOTON_API int photon_tree_attention(const photon_tree_call* call, cudaStream_t stream) {
@@ -398,12 +424,5 @@ PHOTON_API int photon_tree_attention(const photon_tree_call* call, cudaStream_t 
   if (call->parts > 1 && !clusters && (call->scratch == nullptr || call->scratch_floats < rows * (P.d + 2))) return PHOTON_ERR_ARGUMENT;
   TreeShares H;
   H.part_o = call->scratch; H.part_ml = call->scratch + rows * P.d; H.splits = call->parts; H.cluster = clusters ? call->parts : 1;
-  H.row_tiles = (int)(((long)P.max_tokens * P.group + TG_ROWS - 1) / TG_ROWS);
-  const long blocks = (long)P.S * H.row_tiles * P.n_kv * H.splits;
-  if (blocks > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
-  if (call->dtype == PHOTON_F32)
-    return P.d <= 64 ? tree_launch<float, 64>(P, H, blocks, stream) : P.d <= 128 ? tree_launch<float, 128>(P, H, blocks, stream)
-                                                                                : tree_launch<float, 256>(P, H, blocks, stream);
-  return P.d <= 64 ? tree_launch<bf16, 64>(P, H, blocks, stream) : P.d <= 128 ? tree_launch<bf16, 128>(P, H, blocks, stream)
-                                                                              : tree_launch<bf16, 256>(P, H, blocks, stream);
+  return call->dtype == PHOTON_F32 ? tree_choose<float>(P, H, stream) : tree_choose<bf16>(P, H, stream);
 }

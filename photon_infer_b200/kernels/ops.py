@@ -2657,19 +2657,19 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
             # As many ranges for each of a request's row tiles, which then read the same keys at the same time.
             parts = min(2 * sms, 320, max(units, -(-units * (tiles + 1) // 4)))
             return "tree_attention_tc", max(parts - parts % levels, 1), 1
-    # The general kernel: 32 rows a block, 3, 2 or 1 blocks an SM (registers, shared memory).  A row tile's keys go to a cluster of up to eight blocks, as many as
-    # take the fewest steps, a step being a tile of 64 keys or a third of what a block costs beside its tiles; very long requests that leave most of the chip
-    # idle go to more, which a second kernel joins.  32-bit, 8 key/value heads of 64, 8 nodes x 4 heads, parts and us: 2,000 keys 4: 39, 8: 25, 16: 23, 32: 23; 4,000 keys
-    # 8: 39, 16: 30, 32: 28; 16,000 keys 8: 145, 52: 62; 4 requests of 13 x 4 behind up to 700 keys 1: 53, 2: 33, 4: 25, 8: 23, 16: 31; 8 of 32 x 4
-    # behind up to 2,000: 1: 156, 2: 109, 4: 104, 8: 107.
+    # The general kernel: up to 32 rows a block, so many blocks an SM as registers and shared memory allow.  A row tile's keys go to a cluster of up to eight blocks, as many
+    # as take the fewest steps, a step being a tile of 64 keys or a third of what a block costs beside its tiles; very long requests that leave most of the chip
+    # idle go to more, which a second kernel joins.  32-bit, 8 key/value heads of 64, parts and us: 8 nodes x 4 heads behind 2,000 keys 4: 39, 8: 25, 16: 23, 32: 23; 4,000
+    # keys 8: 39, 16: 30, 32: 28; 16,000 keys 8: 145, 52: 62; 4 requests of 13 x 4 behind up to 700 1: 49, 2: 30, 4: 25, 8: 24, 16: 32; 8 of 32 x 4 behind up to
+    # 2,000 1: 157, 2: 111, 4: 104, 8: 131; 8 of 4 x 4 1: 107, 2: 58, 4: 44, 8: 32, 16: 40; 2 of 5 x 4 behind up to 163 1: 16, 2: 13, 4: 10, 8: 13.
     blocks, tiles = max(1, num_seqs * n_kv * -(-rows // 32)), -(-keys // 64)
-    slots = (3 if head_dim <= 64 else 2 if head_dim <= 128 else 1) * sms
+    slots = (4 if rows <= 16 and head_dim <= 64 else 3 if head_dim <= 64 else 2 if head_dim <= 128 else 1) * sms
     if tiles >= 48 and 16 * blocks <= slots:
         return "tree_attention", min(slots // blocks, tiles // 2, 64), 1
-    parts, least = 1, 0.0
+    parts, least = 1, 0
     for p in (1, 2, 4, 8):
-        cost = -(-blocks * p // slots) * (tiles / p + 3)
-        if p == 1 or (cost < least and p <= tiles):
+        cost = -(-blocks * p // slots) * (-(-tiles // p) + 3)
+        if p == 1 or (cost < least and p < 2 * tiles):
             parts, least = p, cost
     return "tree_attention", parts, 1
 

@@ -109,6 +109,14 @@ def test_missing_pages_in_every_way(route, dtype, kernel, parts, cluster):
     assert float((got.double().cpu() - want).abs().max()) <= TOL[dtype] * largest
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.float32, 128), (torch.float32, 200), (torch.bfloat16, 40), (torch.bfloat16, 96)])
+@pytest.mark.parametrize("most", [3, 20])
+def test_many_small_requests(dtype, d, most):
+    """More row tiles than the chip has SMs, of up to 16 rows and of more."""
+    nodes = [1 + i % most for i in range(60)]
+    Step(nodes, [(29 * i) % 150 for i in range(60)], 4, 4, d, 16, dtype, seed=29).check()
+
+
 def test_ways_that_the_entry_points_refuse(route):
     from photon_infer_b200.errors import ErrorCode, PhotonError
     from photon_infer_b200.kernels import ops
