@@ -420,7 +420,7 @@ PHOTON_API int photon_tree_attention(const photon_tree_call* call, cudaStream_t 
   const int st = tree_params(call, P);
   if (st != 0) return st;
   const long rows = (long)P.T * P.n_q * call->parts;
-  const bool clusters = call->parts == 2 || call->parts == 4 || call->parts == 8;
+  const bool clusters = call->parts > 1 && call->parts <= 8;
   if (call->parts > 1 && !clusters && (call->scratch == nullptr || call->scratch_floats < rows * (P.d + 2))) return PHOTON_ERR_ARGUMENT;
   TreeShares H;
   H.part_o = call->scratch; H.part_ml = call->scratch + rows * P.d; H.splits = call->parts; H.cluster = clusters ? call->parts : 1;

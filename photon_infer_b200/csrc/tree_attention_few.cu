@@ -381,7 +381,7 @@ PHOTON_API int photon_tree_attention_few(const photon_tree_call* call, cudaStrea
   if (((uintptr_t)t.q & 15) || (t.q_stride & 7) || ((uintptr_t)t.k_cache & 15) || ((uintptr_t)t.v_cache & 15) || ((uintptr_t)t.out & 7) || (t.out_stride & 3))
     return PHOTON_ERR_UNSUPPORTED;
   P.cluster = call->parts;
-  if (P.cluster != 1 && P.cluster != 2 && P.cluster != 4 && P.cluster != 8) return PHOTON_ERR_ARGUMENT;
+  if (P.cluster < 1 || P.cluster > 8) return PHOTON_ERR_ARGUMENT;
   if ((long)t.S * t.n_kv * P.cluster > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
   P.page_shift = -1;
   for (int sh = 0; sh < 20; ++sh) if ((1 << sh) == t.page_size) P.page_shift = sh;

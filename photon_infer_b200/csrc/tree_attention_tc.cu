@@ -721,7 +721,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       const float inv = sum != 0.f ? 1.f / sum : 0.f;
       bf16* dst = (bf16*)P.t.out + (size_t)t * P.t.out_stride + (size_t)head * D;
 #pragma unroll 1
-      for (int c4 = D / 4 * rank / P.cluster; c4 < D / 4 * (rank + 1) / P.cluster; c4 += 2) {
+      for (int c4 = D / 8 * rank / P.cluster * 2; c4 < D / 8 * (rank + 1) / P.cluster * 2; c4 += 2) {
         float4 y[TT_CLUSTER][2], a[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
 #pragma unroll
         for (int k = 0; k < TT_CLUSTER; ++k)
@@ -864,7 +864,7 @@ PHOTON_API int photon_tree_attention_tc(const photon_tree_call* call, cudaStream
   P.whole = call->scratch == nullptr;
   P.blocks_sm = 2 * photon_sm_count();
   P.cluster = call->cluster;
-  if (P.cluster < 1 || P.cluster > TT_CLUSTER || (P.cluster & (P.cluster - 1)) || (P.cluster > 1 && (!P.whole || call->parts % P.cluster))) return PHOTON_ERR_ARGUMENT;
+  if (P.cluster < 1 || P.cluster > TT_CLUSTER || (P.cluster > 1 && (!P.whole || call->parts % P.cluster))) return PHOTON_ERR_ARGUMENT;
   P.sorted = P.cluster == 1 && t.S <= TT_SORTED && (long)t.S * t.n_kv * ((t.max_tokens + 128 / G - 1) / (128 / G)) <= 65535;
   if (!P.whole && call->parts > TT_MAX_BLOCKS) return PHOTON_ERR_ARGUMENT;
   if (!P.whole && call->scratch_floats < photon_tree_attention_tc_scratch(t.max_tokens, t.n_q, t.n_kv, d, call->parts)) return PHOTON_ERR_ARGUMENT;

@@ -579,21 +579,21 @@ typedef struct {
   int dtype, max_pages, mask_words, S, T, max_tokens_per_seq, n_q, n_kv, d, page_size, num_pages, window;
   int parts;                            /* tree_attention.cu: shares of a request's keys; tree_attention_tc.cu: blocks of the grid */
   float scale, softcap;                 /* softcap 0: off */
-  int cluster;                          /* tree_attention_tc.cu: blocks that share a unit, 1, 2, 4 or 8 */
+  int cluster;                          /* tree_attention_tc.cu: blocks that share a unit, 1 to 8 */
 } photon_tree_call;
-/* Either type, d <= 256.  parts other than 1, 2, 4 and 8: scratch of T * n_q * parts * (d + 2) floats. */
+/* Either type, d <= 256.  parts > 8: scratch of T * n_q * parts * (d + 2) floats. */
 PHOTON_EXPORT int photon_tree_attention(const photon_tree_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ tree_attention_tc.cu: the same on tcgen05, bfloat16, d 64 or 128 */
 /* At most 128 query heads per key/value head, pages of 8, 16, 32 or a multiple of 64 tokens, 16-byte aligned rows.  parts: the grid, at most as many blocks
  * as the chip holds at once.  scratch: as many floats as the first function says, and the lengths on the device decide whether a request's keys are shared out
- * over blocks; or null: they are not, in one kernel.  cluster 2, 4 or 8: that many blocks share a unit (128 rows of a request and head) and parts is units * cluster;
+ * over blocks; or null: they are not, in one kernel.  cluster 2 to 8: that many blocks share a unit (128 rows of a request and head) and parts is units * cluster;
  * no scratch. */
 PHOTON_EXPORT long photon_tree_attention_tc_scratch(int max_tokens_per_seq, int n_q, int n_kv, int d, int blocks);
 PHOTON_EXPORT int photon_tree_attention_tc(const photon_tree_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ tree_attention_few.cu: the same for few rows, bfloat16, d 64 or 128 */
-/* max_tokens_per_seq * n_q / n_kv <= 64; 16-byte aligned rows and caches.  parts: blocks of a cluster that share a request's keys, 1, 2, 4 or 8; no scratch. */
+/* max_tokens_per_seq * n_q / n_kv <= 64; 16-byte aligned rows and caches.  parts: blocks of a cluster that share a request's keys, 1 to 8; no scratch. */
 PHOTON_EXPORT int photon_tree_attention_few(const photon_tree_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ tree_accept.cu */

@@ -2597,7 +2597,7 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         parts = abs(parts)                          # whole units: no scratch
     elif name == "tree_attention_tc":
         floats = 8 * parts + 2 * parts * (-(-min(max_tokens_per_seq * group, 128 // group * group) // 32) * 32) * (head_dim + 2)
-    elif name == "tree_attention" and parts not in (1, 2, 4, 8):
+    elif name == "tree_attention" and parts > 8:
         floats = T * n_q * parts * (head_dim + 2)
     scratch = torch.empty(floats, dtype=torch.float32, device=device) if floats else None
     call = _TREE_CALL.pack(*pointers, block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), positions.data_ptr(),
@@ -2627,27 +2627,27 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
                 keys: int, sms: int):
     """(kernel, parts; below zero: blocks that take whole units, blocks that share a unit) for a step whose requests have at most ``rows`` rows (nodes x query
     heads) per key/value head and ``keys`` visible keys."""
+    rows = max(rows, 1)
     if dtype == torch.bfloat16 and head_dim in (64, 128) and aligned:
-        tiles, units = -(-keys // 64), num_seqs * n_kv
+        tiles, units = -(-keys // 64), max(1, num_seqs) * n_kv
         tma = group <= 128 and page_size % 8 == 0 and (64 % page_size == 0 or page_size % 64 == 0) and cache_rows <= 0x7fffff00
         if rows <= 64:
-            parts = 8
-            while parts > 1 and (units * parts > 2 * sms or parts > 2 * tiles):
-                parts //= 2
-            steps = -(-tiles // parts) * -(-units * parts // ((3 if head_dim == 64 else 2) * sms))
+            slots = (3 if head_dim == 64 else 2) * sms
+            parts = max(1, min(8, slots * 7 // 8 // units, 2 * tiles))
+            steps = -(-tiles // parts) * -(-units * parts // slots)
             if not tma or steps <= TREE_FEW_STEPS[head_dim][(rows > 16) + (rows > 32)]:
                 return "tree_attention_few", parts, 1
         if tma:
             levels = -(-rows // (128 // group * group))
             units *= levels
-            # Where the chip holds two blocks or more for each unit, a cluster of them shares it, with two tiles a block at least, and joins it in its own memory.  It
-            # costs what equal ranges would have shared out better: all of the chip over, and requests shorter than the longest.  Ranges with the second kernel, and
-            # clusters, us: 8 requests of 27 nodes behind up to 2,500 keys (32/8 heads of 64) 25.4 and 20.8, behind 4,000 34.0 and 28.0, up to 8,000 38.4 and 41.8, up to
-            # 16,000 47 and 68; 4 of 30 behind up to 4,000 (heads of 128) 30.2 and 25.1; 16 of 30 behind up to 4,000 55.1 and 48.8, up to 8,000 74 and 81;
-            # 1 of 32 behind 1,000 18.3 and 15.5, 4,000 18.6 and 18.8, 16,000 32 and 42; a window of 1,024 and bounded scores, 16 of 16, whole units 39 and clusters 30.
-            cluster = 1
-            while cluster < 8 and 2 * cluster * units <= 2 * sms and 4 * cluster <= tiles:
-                cluster *= 2
+            # Where the chip holds two blocks or more for each unit, a cluster of them shares it, with two tiles a block at least, and joins it in its own memory.
+            # Clusters leave places free, so seven eighths are counted (5 requests of 30 nodes behind 4,000 keys, 32/8 heads of 128, clusters of 4, 5, 6 and 7: 33, 30,
+            # 28 and 46 us).  What they cost is what equal ranges would have shared out better: all of the chip over, and requests shorter than the longest.  Ranges
+            # with the second kernel, and clusters, us: 8 requests of 27 nodes behind up to 2,500 keys (32/8 heads of 64) 25.4 and 20.8, behind 4,000 34.0 and 28.0, up to
+            # 8,000 38.4 and 41.8, up to 16,000 47 and 68; 4 of 30 behind up to 4,000 (heads of 128) 30.2 and 25.1; 16 of 30 behind up to 4,000 55.1 and 48.8,
+            # up to 8,000 74 and 81; 1 of 32 behind 1,000 18.3 and 15.5, 4,000 18.6 and 18.8, 16,000 32 and 42; a window of 1,024 and bounded scores, 16 of 16,
+            # whole units 39 and clusters 30.
+            cluster = min(8, 2 * sms * 7 // 8 // units, tiles // 2)
             if cluster > 1 and tiles * (2 * sms - units * cluster) <= 16 * sms * cluster:
                 return "tree_attention_tc", units * cluster, cluster
             # Few keys: whole units, one kernel.  More: the kernel decides by the lengths, which the host does not know, and a second kernel follows
@@ -2657,19 +2657,20 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
             # As many ranges for each of a request's row tiles, which then read the same keys at the same time.
             parts = min(2 * sms, 320, max(units, -(-units * (tiles + 1) // 4)))
             return "tree_attention_tc", max(parts - parts % levels, 1), 1
-    # The general kernel: up to 32 rows a block, so many blocks an SM as registers and shared memory allow.  A row tile's keys go to a cluster of up to eight blocks, as many
-    # as take the fewest steps, a step being a tile of 64 keys or a third of what a block costs beside its tiles; very long requests that leave most of the chip
-    # idle go to more, which a second kernel joins.  32-bit, 8 key/value heads of 64, parts and us: 8 nodes x 4 heads behind 2,000 keys 4: 39, 8: 25, 16: 23, 32: 23; 4,000
-    # keys 8: 39, 16: 30, 32: 28; 16,000 keys 8: 145, 52: 62; 4 requests of 13 x 4 behind up to 700 1: 49, 2: 30, 4: 25, 8: 24, 16: 32; 8 of 32 x 4 behind up to
-    # 2,000 1: 157, 2: 111, 4: 104, 8: 131; 8 of 4 x 4 1: 107, 2: 58, 4: 44, 8: 32, 16: 40; 2 of 5 x 4 behind up to 163 1: 16, 2: 13, 4: 10, 8: 13.
+    # The general kernel: up to 32 rows a block, so many blocks an SM as registers and shared memory allow (seven eighths of them, as above).  A row tile's keys go to a
+    # cluster of up to eight blocks, as many as take the fewest steps, a step being a tile of 64 keys or a third of what a block costs beside its tiles; in several waves
+    # clusters of 3, 5, 6 or 7 fare worse.  Very long requests that leave most of the chip idle go to more blocks, which a second kernel joins.  32-bit, 8
+    # key/value heads of 64, parts and us: 8 nodes x 4 heads behind 2,000 keys 4: 39, 8: 25, 16: 23, 32: 23; 4,000 keys 8: 39, 16: 30, 32: 28; 16,000 keys 8: 145, 52: 62;
+    # 4 requests of 13 x 4 behind up to 700 1: 49, 2: 30, 4: 25, 6: 23, 8: 23, 16: 32; 8 of 32 x 4 behind up to 2,000 1: 153, 2: 112, 3: 116, 4: 103, 8: 131; 8 of 4 x 4 1: 107,
+    # 2: 58, 4: 44, 8: 32, 16: 40; 2 of 5 x 4 behind up to 163 1: 16, 2: 13, 3: 10, 8: 13.
     blocks, tiles = max(1, num_seqs * n_kv * -(-rows // 32)), -(-keys // 64)
-    slots = (4 if rows <= 16 and head_dim <= 64 else 3 if head_dim <= 64 else 2 if head_dim <= 128 else 1) * sms
+    slots = (4 if rows <= 16 and head_dim <= 64 else 3 if head_dim <= 64 else 2 if head_dim <= 128 else 1) * sms * 7 // 8
     if tiles >= 48 and 16 * blocks <= slots:
         return "tree_attention", min(slots // blocks, tiles // 2, 64), 1
     parts, least = 1, 0
-    for p in (1, 2, 4, 8):
+    for p in range(1, min(8, tiles) + 1):
         cost = -(-blocks * p // slots) * (-(-tiles // p) + 3)
-        if p == 1 or (cost < least and p < 2 * tiles):
+        if p == 1 or (cost <= least and (blocks * p <= slots or p in (2, 4, 8))):
             parts, least = p, cost
     return "tree_attention", parts, 1
 

@@ -26,10 +26,9 @@ def route(monkeypatch):
     return use
 
 
-TC = [("tree_attention_tc", "whole", 1), ("tree_attention_tc", 7, 1), ("tree_attention_tc", 290, 1), ("tree_attention_tc", 0, 2),
-      ("tree_attention_tc", 0, 4), ("tree_attention_tc", 0, 8)]
-FEW = [("tree_attention_few", n, 1) for n in (1, 2, 4, 8)]
-GENERAL = [("tree_attention", n, 1) for n in (1, 2, 3, 4, 8, 13)]
+TC = [("tree_attention_tc", "whole", 1), ("tree_attention_tc", 7, 1), ("tree_attention_tc", 290, 1)] + [("tree_attention_tc", 0, n) for n in range(2, 9)]
+FEW = [("tree_attention_few", n, 1) for n in range(1, 9)]
+GENERAL = [("tree_attention", n, 1) for n in (1, 2, 3, 5, 8, 13)]
 WAYS = [(torch.bfloat16, *w) for w in TC + FEW + GENERAL] + [(torch.float32, *w) for w in GENERAL]
 ALL = pytest.mark.parametrize("dtype,kernel,parts,cluster", WAYS, ids=["-".join(str(x).split(".")[-1] for x in w) for w in WAYS])
 
@@ -117,6 +116,22 @@ def test_many_small_requests(dtype, d, most):
     Step(nodes, [(29 * i) % 150 for i in range(60)], 4, 4, d, 16, dtype, seed=29).check()
 
 
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 40)])
+@pytest.mark.parametrize("most,keys", [(0, 0), (16, 0), (40, 1000)])
+def test_no_requests(dtype, d, most, keys):
+    """A step of no requests, or of no nodes, leaves the output as it is."""
+    step = Step([16, 9], [900, 20], 8, 2, d, 16, dtype, seed=30)
+    a = step.arguments()
+    bound = dict(max_tokens_per_seq=most, max_keys=keys, tree_mask=torch.zeros((step.T, 2), dtype=torch.int32, device="cuda:0"))
+    got, err = step.run(num_seqs=0, **bound)
+    assert bool((got == 7.0).all()) and err[0] == 0
+    zero = torch.zeros(3, dtype=torch.int32, device="cuda:0")
+    got, err = step.run(cu_tokens=zero, context_lens=zero[:2], **bound)
+    assert bool((got == 7.0).all()) and err[0] == 0
+    out = torch.empty((0, 8 * d), dtype=dtype, device="cuda:0")
+    step.run(q=a["q"][:0], out=out, cu_tokens=zero, context_lens=zero[:2], **bound)
+
+
 def test_ways_that_the_entry_points_refuse(route):
     from photon_infer_b200.errors import ErrorCode, PhotonError
     from photon_infer_b200.kernels import ops
@@ -128,9 +143,8 @@ def test_ways_that_the_entry_points_refuse(route):
             step.run()
         assert e.value.code == code
     route("tree_attention", 1, 1)                       # put back at the end
-    refused(("tree_attention_tc", 12, 3), ErrorCode.INVALID_ARGUMENT)
     refused(("tree_attention_tc", 13, 2), ErrorCode.INVALID_ARGUMENT)
     refused(("tree_attention_tc", 64, 16), ErrorCode.INVALID_ARGUMENT)
     refused(("tree_attention_tc", 400, 1), ErrorCode.INVALID_ARGUMENT)
-    refused(("tree_attention_few", 3, 1), ErrorCode.INVALID_ARGUMENT)
+    refused(("tree_attention_few", 9, 1), ErrorCode.INVALID_ARGUMENT)
     refused(("tree_attention", 0, 1), ErrorCode.INVALID_ARGUMENT)
