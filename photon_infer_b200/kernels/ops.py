@@ -2533,18 +2533,19 @@ def moe_gemv(x: torch.Tensor, x_div: int, ids: torch.Tensor, weight: torch.Tenso
 # ----------------------------------------------------------------------------- trees of drafted tokens
 
 def _check_step(what: str, num_seqs: int, cu_tokens: torch.Tensor, context_lens: torch.Tensor, block_table: torch.Tensor) -> int:
-    """The step's tables cover its requests; returns the table's width."""
-    _int32s(("cu_tokens", "context_lens", "block_table"), (cu_tokens, context_lens, block_table))
+    """The step's tables cover its requests; returns the table's width.  Their type: ``_int32s``."""
     table = block_table.shape
-    if not 0 <= num_seqs < cu_tokens.numel() or context_lens.numel() < num_seqs or len(table) != 2 or table[0] < num_seqs or table[0] * table[1] < 1:
+    if len(table) != 2 or not 0 <= num_seqs < cu_tokens.numel() or context_lens.numel() < num_seqs or table[0] < num_seqs or table[0] * table[1] < 1:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: cu_tokens, context_lens and block_table must cover every request")
     return table[1]
 
 
-def _int32s(names, tensors) -> None:
+def _int32s(names: str, *tensors: torch.Tensor) -> None:
+    """``_int32`` of several; ``names``: theirs, with spaces between them."""
+    int32 = torch.int32
     for t in tensors:
-        if t.dtype is not torch.int32 or not t.is_contiguous():
-            _int32(t, names[[x is t for x in tensors].index(True)])
+        if t.dtype is not int32 or not t.is_contiguous():
+            _int32(t, names.split()[[x is t for x in tensors].index(True)])
 
 
 #: photon_tree_call: pointers, strides and the scratch's size, sizes, scale and bound
@@ -2577,8 +2578,8 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: q, out and the caches must share one dtype")
     if len(cache) != 4 or v_cache.shape != cache or cache[1] != n_kv or cache[3] != head_dim or not k_cache.is_contiguous() or not v_cache.is_contiguous():
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: the caches must be contiguous [pages, n_kv, page_size, head_dim]")
+    _int32s("cu_tokens context_lens block_table positions tree_mask", cu_tokens, context_lens, block_table, positions, tree_mask)
     width = _check_step("tree_attention", num_seqs, cu_tokens, context_lens, block_table)
-    _int32s(("positions", "tree_mask"), (positions, tree_mask))
     mask = tree_mask.shape
     words = mask[1] if len(mask) == 2 else 0
     if positions.numel() < T or mask[0] < T or words * 32 < max_tokens_per_seq or words < 1:
@@ -2667,11 +2668,13 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
     slots = (4 if rows <= 16 and head_dim <= 64 else 3 if head_dim <= 64 else 2 if head_dim <= 128 else 1) * sms * 7 // 8
     if tiles >= 48 and 16 * blocks <= slots:
         return "tree_attention", min(slots // blocks, tiles // 2, 64), 1
-    parts, least = 1, 0
-    for p in range(1, min(8, tiles) + 1):
-        cost = -(-blocks * p // slots) * (-(-tiles // p) + 3)
-        if p == 1 or (cost <= least and (blocks * p <= slots or p in (2, 4, 8))):
-            parts, least = p, cost
+    parts = max(1, min(8, tiles, slots // blocks))              # the most that one wave has room for
+    least = -(-blocks * parts // slots) * (-(-tiles // parts) + 3)
+    if parts < 8:
+        for p in (2, 4, 8):
+            cost = -(-blocks * p // slots) * (-(-tiles // p) + 3)
+            if parts < p <= tiles and cost <= least:
+                parts, least = p, cost
     return "tree_attention", parts, 1
 
 
@@ -2689,7 +2692,7 @@ def tree_accept(logits: torch.Tensor, tokens: torch.Tensor, parents: torch.Tenso
     if len(shape) != 2 or logits.dtype is not torch.float32 or logits.stride(1) != 1 or shape[1] < 1:
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_accept: logits must be float32 [T, V] with unit inner stride")
     T, V = shape
-    _int32s(("tokens", "parents", "cu_tokens", "path", "counts", "sampled"), (tokens, parents, cu_tokens, path, counts, sampled))
+    _int32s("tokens parents cu_tokens path counts sampled", tokens, parents, cu_tokens, path, counts, sampled)
     if not 0 <= num_seqs < cu_tokens.numel():
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_accept: cu_tokens must cover every request")
     if tokens.numel() < T or parents.numel() < T:
@@ -2736,8 +2739,8 @@ def cache_keep(kv: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Ten
     context_lens[s]`` minus the request's nodes of the step.  ``path`` and ``counts`` as ``tree_accept`` leaves them (paths ascend)."""
     _cuda(kv, block_table, cu_tokens, context_lens, path, counts, err)
     pool = _check_pool("cache_keep", kv)
+    _int32s("cu_tokens context_lens block_table path counts", cu_tokens, context_lens, block_table, path, counts)
     width = _check_step("cache_keep", num_seqs, cu_tokens, context_lens, block_table)
-    _int32s(("path", "counts"), (path, counts))
     place = path.shape
     if len(place) != 2 or place[0] < num_seqs or counts.numel() < num_seqs:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_keep: path must be [requests, depth], counts [requests]")
