@@ -215,12 +215,15 @@ struct TtSegments {
     if (P.cluster > 1) {
       // one unit for the cluster, and this block's part of its tiles; a short unit leaves some blocks without
       if (round++ > 0) return false;
-      int front;
       rows = 0;
-      if (!tt_unit(P, *order, blockIdx.x / P.cluster, seq, front)) return false;
-      q = tt_load(P, seq); unit = blockIdx.x / P.cluster - front;
-      place(P, unit % q.blocks, unit / q.blocks);             // row tiles of a head side by side
-      const int rank = blockIdx.x % P.cluster, first = q.tiles * rank / P.cluster;
+      const int u = blockIdx.x / P.cluster, rank = blockIdx.x - u * P.cluster, per = P.t.n_kv * P.levels;
+      seq = u / per;
+      if (seq >= P.t.S) return false;
+      q = tt_load(P, seq);
+      const int h = (u - seq * per) / P.levels, rb = u - seq * per - h * P.levels;       // row tiles of a head side by side
+      if (rb >= q.blocks) return false;
+      place(P, rb, h);
+      const int first = q.tiles * rank / P.cluster;
       ntiles = q.tiles * (rank + 1) / P.cluster - first;
       tile0 = q.tile_lo + first; whole = false; bit = 0; serial = 1;
       return ntiles > 0;
@@ -704,43 +707,55 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     const int r = threadIdx.x;
     if (warp < 4 && r < s.rows && !*abort_flag) {
       const int rank = blockIdx.x % P.cluster, t = s.q.r.tok0 + (s.row0 + r) / P.t.group, head = s.g * P.t.group + (s.row0 + r) % P.t.group;
-      float w[TT_CLUSTER], sum = 0.f, top = P.t.sinks ? P.t.sinks[head] * TT_LOG2E : -INFINITY;
-      const float sink = top;
-#pragma unroll
-      for (int k = 0; k < TT_CLUSTER; ++k) {
-        w[k] = k < P.cluster ? tree_peer(&ml[r].x, k) : -INFINITY;
-        top = fmaxf(top, w[k]);
-      }
-      const float sub = top == -INFINITY ? 0.f : top;
-#pragma unroll
-      for (int k = 0; k < TT_CLUSTER; ++k) {
-        w[k] = at_exp2(w[k] - sub);                 // 0 for what is not there
-        if (k < P.cluster) sum += tree_peer(&ml[r].y, k) * w[k];
-      }
-      sum += at_exp2(sink - sub);
-      const float inv = sum != 0.f ? 1.f / sum : 0.f;
+      const float sink = P.t.sinks ? P.t.sinks[head] * TT_LOG2E : -INFINITY;
       bf16* dst = (bf16*)P.t.out + (size_t)t * P.t.out_stride + (size_t)head * D;
+      // K: room for the blocks of the cluster; U: pieces of four columns at a time, so that eight loads are on their way
+      auto join = [&](auto blocks, auto pieces) {
+        constexpr int K = decltype(blocks)::value, U = decltype(pieces)::value;
+        float w[K], l[K], sum = 0.f, top = sink;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          w[k] = k < P.cluster ? tree_peer(&ml[r].x, k) : -INFINITY;
+          l[k] = k < P.cluster ? tree_peer(&ml[r].y, k) : 0.f;
+        }
+#pragma unroll
+        for (int k = 0; k < K; ++k) top = fmaxf(top, w[k]);
+        const float sub = top == -INFINITY ? 0.f : top;
+#pragma unroll
+        for (int k = 0; k < K; ++k) {
+          w[k] = at_exp2(w[k] - sub);               // 0 for what is not there
+          sum += l[k] * w[k];
+        }
+        sum += at_exp2(sink - sub);
+        const float inv = sum != 0.f ? 1.f / sum : 0.f;
+        const int end = D / 8 * (rank + 1) / P.cluster * 2;
 #pragma unroll 1
-      for (int c4 = D / 8 * rank / P.cluster * 2; c4 < D / 8 * (rank + 1) / P.cluster * 2; c4 += 2) {
-        float4 y[TT_CLUSTER][2], a[2] = {make_float4(0.f, 0.f, 0.f, 0.f), make_float4(0.f, 0.f, 0.f, 0.f)};
+        for (int c4 = D / 8 * rank / P.cluster * 2; c4 < end; c4 += U) {
+          float4 y[K][U];
 #pragma unroll
-        for (int k = 0; k < TT_CLUSTER; ++k)
+          for (int k = 0; k < K; ++k)
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (k < P.cluster) y[k][u] = tree_peer4(reinterpret_cast<const float*>(kv_s) + ((c4 + u) * 128 + r) * 4, k);
+            for (int u = 0; u < U; ++u)
+              if (k < P.cluster) y[k][u] = tree_peer4(reinterpret_cast<const float*>(kv_s) + (min(c4 + u, D / 4 - 1) * 128 + r) * 4, k);
 #pragma unroll
-        for (int k = 0; k < TT_CLUSTER; ++k)
+          for (int u = 0; u < U; ++u) {
+            float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-          for (int u = 0; u < 2; ++u)
-            if (k < P.cluster && w[k] != 0.f) {
-              a[u].x = fmaf(w[k], y[k][u].x, a[u].x); a[u].y = fmaf(w[k], y[k][u].y, a[u].y);
-              a[u].z = fmaf(w[k], y[k][u].z, a[u].z); a[u].w = fmaf(w[k], y[k][u].w, a[u].w);
+            for (int k = 0; k < K; ++k)
+              if (k < P.cluster && w[k] != 0.f) {
+                a.x = fmaf(w[k], y[k][u].x, a.x); a.y = fmaf(w[k], y[k][u].y, a.y); a.z = fmaf(w[k], y[k][u].z, a.z); a.w = fmaf(w[k], y[k][u].w, a.w);
+              }
+            if (c4 + u < end) {
+              uint2 v;
+              v.x = at_pack(a.x * inv, a.y * inv); v.y = at_pack(a.z * inv, a.w * inv);
+              *reinterpret_cast<uint2*>(dst + (c4 + u) * 4) = v;
             }
-        uint4 v4;
-        v4.x = at_pack(a[0].x * inv, a[0].y * inv); v4.y = at_pack(a[0].z * inv, a[0].w * inv);
-        v4.z = at_pack(a[1].x * inv, a[1].y * inv); v4.w = at_pack(a[1].z * inv, a[1].w * inv);
-        *reinterpret_cast<uint4*>(dst + c4 * 4) = v4;
-      }
+          }
+        }
+      };
+      if (P.cluster == 2) join(std::integral_constant<int, 2>(), std::integral_constant<int, 4>());
+      else if (P.cluster <= 4) join(std::integral_constant<int, 4>(), std::integral_constant<int, 2>());
+      else join(std::integral_constant<int, 8>(), std::integral_constant<int, 1>());
     }
     tree_cluster_sync();                            // the others have read this block's results
   }
