@@ -11,13 +11,13 @@
 // maxima and sums; the weights pass through shared memory inside the warp.  The warps' results, and those of a cluster of up to eight blocks that share a row tile's
 // keys, are joined in shared memory in their order; where more blocks share them, by a second kernel.
 //
-// What bounds it: 32-bit products, and for small calls their latency.  4 requests of 13 nodes behind up to 700 keys (32/8 heads of 64): 25 us, 1 us of it for the bytes; 8 of
-// 32 behind up to 2,000: 104 us = 15 TFLOP/s of products that are needed; 1 of 8 behind 640: 16; 3 of 5 behind up to 36: 9.  A tile ahead in shared memory left two
+// What bounds it: 32-bit products, and for small calls their latency.  4 requests of 13 nodes behind up to 700 keys (32/8 heads of 64): 19 us, 1 us of it for the bytes; 8 of
+// 32 behind up to 2,000: 89 us = 17 TFLOP/s of products that are needed; 1 of 8 behind 640: 14; 3 of 5 behind up to 36: 7.5.  A tile ahead in shared memory left two
 // blocks an SM and was slower (32 and 25 us, 132 and 108); tiles of 32 keys 23 and 118; the sums of products in one number after the other, 32 keys a
 // tile, 36 and 334.
 //
-// A key that a row does not see has weight 0, and 0 times a value that is not finite would not be: in tiles where masks cut, products with a weight of 0
-// are left out, and rows behind the last key or of a missing page are zeros.
+// A key that a row does not see has weight 0, and 0 times a value that is not finite would not be: in tiles where masks cut and such values lie, products with a
+// weight of 0 are left out; rows behind the last key or of a missing page are zeros.
 #include "tree_attention.cuh"
 #include <math.h>
 #include <type_traits>
@@ -102,7 +102,7 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
   float* ps = qs + ROWS * S;                       // per warp [16][PS]
   T* ks = (T*)(ps + GROUPS * SHARES * 16 * PS);               // [TG_KEYS][KS]
   T* vs = ks + TG_KEYS * KS;                       // [TG_KEYS][D]
-  __shared__ long long krow[TG_KEYS];
+  __shared__ long long krow[TG_KEYS], qrow[32];
   __shared__ float ml_s[2][SHARES][ROWS], factor[ROWS][8 * SHARES];
   __shared__ uint32_t seen[2][2][32];   // a warp may be at work on the tile before when the next one's are found
   pdl_wait();
@@ -133,16 +133,19 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
   const int my_t = tid < TG_KEYS && lane < nrows ? R.tok0 + (row0 + lane) / G : -1;
   const int my_lo = my_t >= 0 && P.window > 0 ? max(0, P.positions[my_t] - P.window + 1) : 0;
   // Table entries are read a tile before the rows they lead to.
+  int pidx = 0;                                    // of this thread's key in the next tile
   auto entry = [&](int tile) {
-    const int key = tile * TG_KEYS + tid, at = key / P.page_size;
-    return tid < TG_KEYS && tile < end && key >= key_lo && key < key_end && at < P.max_pages ? table[at] : -1;
+    const int key = tile * TG_KEYS + tid;
+    if (tid >= TG_KEYS || tile >= end || key < key_lo || key >= key_end) return -1;
+    pidx = key / P.page_size;
+    return pidx < P.max_pages ? table[pidx] : -1;
   };
   auto find = [&](int tile, int page) {            // a tile's rows, and which of them are seen
     if (tid < TG_KEYS) {
       const int key = tile * TG_KEYS + tid;
       long long at = -1;
       if (key >= key_lo && key < key_end) {
-        if (page >= 0 && page < P.num_pages) at = ((long long)page * P.n_kv + g) * P.page_size + key % P.page_size;
+        if (page >= 0 && page < P.num_pages) at = ((long long)page * P.n_kv + g) * P.page_size + (key - pidx * P.page_size);
         else report_error(P.err, PHOTON_DEV_BAD_PAGE, R.tok0, key, page);
       }
       krow[tid] = at;
@@ -151,12 +154,23 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
     }
   };
   int page = entry(begin);
-
+  if (tid < 32) qrow[tid] = tid < nrows ? (long long)my_t * P.q_stride + (long long)(g * G + row0 + tid - (my_t - R.tok0) * G) * d : -1;
+  __syncthreads();
   const T* q = (const T*)P.q;
+  if (d % 4 == 0 && P.q_stride % 4 == 0 && (uintptr_t)q % (4 * sizeof(T)) == 0) {
 #pragma unroll 8
-  for (int e = tid; e < ROWS * D; e += THREADS) {
-    const int r = e / D, j = e % D, row = row0 + r;
-    qs[r * S + j] = r < nrows && j < d ? to_f32(q[(size_t)(R.tok0 + row / G) * P.q_stride + (size_t)(g * G + row % G) * d + j]) : 0.f;
+    for (int e = tid; e < ROWS * (D / 4); e += THREADS) {
+      const int r = e / (D / 4), j = e % (D / 4) * 4;
+      const long long at = qrow[r];
+      *(float4*)(qs + r * S + j) = at >= 0 && j < d ? tg_four(q + at + j) : make_float4(0.f, 0.f, 0.f, 0.f);
+    }
+  } else {
+#pragma unroll 8
+    for (int e = tid; e < ROWS * D; e += THREADS) {
+      const int r = e / D, j = e % D;
+      const long long at = qrow[r];
+      qs[r * S + j] = at >= 0 && j < d ? to_f32(q[at + j]) : 0.f;
+    }
   }
 
   float m[4], l[4];                                // l: of this thread's keys
@@ -233,7 +247,15 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
       for (int j = 0; j < C * 2; ++j) { o[i][j].x *= keep; o[i][j].y *= keep; }
     }
     __syncwarp();
+    // A mask cuts: is there a value that a weight of 0 must not meet?
+    bool odd = false;
     if (__any_sync(0xffffffffu, all != 0xffffffffu)) {
+      for (int e = lane; e < MINE * (D / 4); e += 32) {
+        const float4 v = tg_four(vs + MINE * kw * D + e * 4);
+        odd |= !(isfinite(v.x) && isfinite(v.y) && isfinite(v.z) && isfinite(v.w));
+      }
+    }
+    if (__any_sync(0xffffffffu, odd)) {
       for (int k = 0; k < MINE; ++k) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
