@@ -128,7 +128,9 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
   }
   const int key_end = R.base + R.n;
   const int tile0 = key_lo / TG_KEYS, tiles = (key_end + TG_KEYS - 1) / TG_KEYS - tile0;
-  const int begin = tile0 + (int)((long long)tiles * split / H.splits), end = tile0 + (int)((long long)tiles * (split + 1) / H.splits);
+  // the last share, whose tiles masks cut, is no longer than the others
+  const int begin = tile0 + (int)(((long long)tiles * split + H.splits - 1) / H.splits);
+  const int end = tile0 + (int)(((long long)tiles * (split + 1) + H.splits - 1) / H.splits);
   // what threads r and r + 32 know of row r; rows that are none see every key, so that they cut no tile
   const int my_t = tid < TG_KEYS && lane < nrows ? R.tok0 + (row0 + lane) / G : -1;
   const int my_lo = my_t >= 0 && P.window > 0 ? max(0, P.positions[my_t] - P.window + 1) : 0;

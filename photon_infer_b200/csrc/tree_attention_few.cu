@@ -6,7 +6,7 @@
 // At the end the warps' partial results lie in shared memory, and the blocks of the cluster join them there, each for its share of the outputs: one
 // launch, no scratch, the same order of sums in every run.
 //
-// What bounds it: latency.  5 nodes behind 640 keys (32/8 heads of 64): 7.7 us, where the bytes take 0.2; 1 node behind 100: 5.9; 2 requests of 8 behind 1,000 (32/8
+// What bounds it: latency.  5 nodes behind 640 keys (32/8 heads of 64): 7.2 us, where the bytes take 0.2; 1 node behind 100: 5.8; 2 requests of 8 behind 1,000 (32/8
 // heads of 128): 12.6 (bytes: 1.3).  A launch, the request's range and its pages, the first keys, two tiles of work and the join follow one another; in the
 // kernel's wait counters memory, barriers and instructions that are not there yet have like parts.  A second kernel for the join took 15.8 us for the first of
 // these; each row's factors worked out for every four of its outputs 8.4; short tables read behind the request's range 7.9.
@@ -93,7 +93,8 @@ tree_attention_few_kernel(const TfParams P) {
   const int key_end = R.base + R.n, key_lo = t.window > 0 ? max(0, R.base - t.window + 1) : 0;
   const int cut_lo = t.window > 0 ? key_end - t.window : -1;      // no row's window begins behind this key
   const int tile_lo = key_lo / TF_KT, all = rows > 0 ? (key_end + TF_KT - 1) / TF_KT - tile_lo : 0;
-  const int tile0 = tile_lo + all * rank / P.cluster, ntiles = tile_lo + all * (rank + 1) / P.cluster - tile0;
+  // the last block, whose tiles masks cut, has one that is no longer than the others'
+  const int first = (all * rank + P.cluster - 1) / P.cluster, ntiles = (all * (rank + 1) + P.cluster - 1) / P.cluster - first, tile0 = tile_lo + first;
   auto page_of = [&](int key) { return P.page_shift >= 0 ? key >> P.page_shift : key / t.page_size; };
   const int from = page_of(tile0 * TF_KT), pages = ntiles > 0 ? page_of(min(key_end, (tile0 + ntiles) * TF_KT) - 1) - from + 1 : 0;
   const int page0 = whole ? 0 : from;
@@ -344,17 +345,29 @@ tree_attention_few_kernel(const TfParams P) {
       if (tid % W + W * u < n) factor_s[r][tid % W + W * u] = f[u] * inv;
   }
   __syncthreads();
-  const int pieces = rows * (D / 4), first = pieces * rank / P.cluster, last = pieces * (rank + 1) / P.cluster;
-  for (int e = first + tid; e < last; e += TF_THREADS) {
+  const int pieces = rows * (D / 4), last = pieces * (rank + 1) / P.cluster;
+  for (int e = pieces * rank / P.cluster + tid; e < last; e += TF_THREADS) {
     const int r = e / (D / 4), j = e % (D / 4) * 4, w0 = r / 16 * C::KG, rr = r & 15;
     float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int b = 0; b < P.cluster; ++b)
+    constexpr int B = 8 / C::KG;                   // blocks whose results are on their way at a time
+    for (int b0 = 0; b0 < P.cluster; b0 += B) {
+      float4 x[B][C::KG];
+      float w[B][C::KG];
 #pragma unroll
-      for (int k = 0; k < C::KG; ++k) {
-        const float w = factor_s[r][b * C::KG + k];
-        const float4 x = tree_peer4(po + ((w0 + k) * 16 + rr) * C::LO + j, b);
-        if (w != 0.f) { a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w); }
-      }
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int k = 0; k < C::KG; ++k) {
+          w[b][k] = b0 + b < P.cluster ? factor_s[r][(b0 + b) * C::KG + k] : 0.f;
+          x[b][k] = tree_peer4(po + ((w0 + k) * 16 + rr) * C::LO + j, min(b0 + b, P.cluster - 1));
+        }
+#pragma unroll
+      for (int b = 0; b < B; ++b)
+#pragma unroll
+        for (int k = 0; k < C::KG; ++k)
+          if (w[b][k] != 0.f) {
+            a.x = fmaf(w[b][k], x[b][k].x, a.x); a.y = fmaf(w[b][k], x[b][k].y, a.y); a.z = fmaf(w[b][k], x[b][k].z, a.z); a.w = fmaf(w[b][k], x[b][k].w, a.w);
+          }
+    }
     uint2 v;
     v.x = tf_pack(a.x, a.y); v.y = tf_pack(a.z, a.w);
     *reinterpret_cast<uint2*>((bf16*)t.out + (size_t)(R.tok0 + r / G) * t.out_stride + (size_t)(g * G + r % G) * D + j) = v;

@@ -223,8 +223,9 @@ struct TtSegments {
       const int h = (u - seq * per) / P.levels, rb = u - seq * per - h * P.levels;       // row tiles of a head side by side
       if (rb >= q.blocks) return false;
       place(P, rb, h);
-      const int first = q.tiles * rank / P.cluster;
-      ntiles = q.tiles * (rank + 1) / P.cluster - first;
+      // the last block, whose tiles masks cut, has a run that is no longer than the others'
+      const int first = (q.tiles * rank + P.cluster - 1) / P.cluster;
+      ntiles = (q.tiles * (rank + 1) + P.cluster - 1) / P.cluster - first;
       tile0 = q.tile_lo + first; whole = false; bit = 0; serial = 1;
       return ntiles > 0;
     }
