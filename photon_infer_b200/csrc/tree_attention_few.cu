@@ -6,10 +6,11 @@
 // At the end the warps' partial results lie in shared memory, and the blocks of the cluster join them there, each for its share of the outputs: one
 // launch, no scratch, the same order of sums in every run.
 //
-// What bounds it: latency.  5 nodes behind 640 keys (32/8 heads of 64): 7.2 us, where the bytes take 0.2; 1 node behind 100: 5.8; 2 requests of 8 behind 1,000 (32/8
-// heads of 128): 12.6 (bytes: 1.3).  A launch, the request's range and its pages, the first keys, two tiles of work and the join follow one another; in the
+// What bounds it: latency.  5 nodes behind 640 keys (32/8 heads of 64): 6.5 us, where the bytes take 0.2; 1 node behind 100: 5.5; 2 requests of 8 behind 1,000 (32/8
+// heads of 128): 11.1 (bytes: 1.3).  A launch, the request's range and its pages, the first keys, two tiles of work and the join follow one another; in the
 // kernel's wait counters memory, barriers and instructions that are not there yet have like parts.  A second kernel for the join took 15.8 us for the first of
-// these; each row's factors worked out for every four of its outputs 8.4; short tables read behind the request's range 7.9.
+// these.  Each step below half a microsecond: a row's factors once for all its outputs, short tables read beside the request's range, the shorter run for the block
+// whose tiles masks cut, a key's row in the cache found once for all its pieces.
 //
 // Which keys a row sees: tree_attention.cuh.  In tiles where some row's mask cuts, values that are not finite are set to zero in shared memory before the
 // products (0 times them would not be 0), and rows that see them get them back at the end from the cache.
@@ -72,7 +73,9 @@ tree_attention_few_kernel(const TfParams P) {
   bf16* qs = reinterpret_cast<bf16*>(tf_dyn);
   bf16* ring = qs + C::ROWS * C::LD;
   __shared__ int table_s[TF_TABLE];
-  __shared__ uint64_t gone_s[C::STAGES];           // keys of a stage whose page is missing
+  constexpr int SLOTS = C::STAGES + 1;
+  __shared__ long long row_s[SLOTS][TF_KT];        // the cache rows of a tile's keys, found a tile before they are asked for; -1: none
+  __shared__ uint32_t gone_s[SLOTS][2];            // its keys whose page is missing
   __shared__ int poison;                           // 1: some value of a tile where a mask cuts was not finite
   __shared__ float ml_s[2][4][16];                 // [maximum, sum][warp][row]
   __shared__ float factor_s[C::ROWS][32 / MT];     // of each partial result of a row
@@ -80,7 +83,6 @@ tree_attention_few_kernel(const TfParams P) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int rank = blockIdx.x % P.cluster, unit = blockIdx.x / P.cluster, g = unit % t.n_kv, seq = unit / t.n_kv;
   if (tid == 0) poison = 0;
-  if (tid < C::STAGES) gone_s[tid] = 0;
   pdl_wait();
   // The request's pages: a short table is read whole, beside the request's range; of a long one the entries of the block's keys, once they are known.
   const int* table = t.block_table + (size_t)seq * t.max_pages;
@@ -116,31 +118,35 @@ tree_attention_few_kernel(const TfParams P) {
     }
   }
   __syncthreads();
+  auto find = [&](int i, int x) {                  // key x of tile i of the block; by whole warps
+    const int key = (tile0 + i) * TF_KT + x;
+    long long row = -1;
+    bool bad = false;
+    if (i < ntiles && key >= key_lo && key < key_end) {
+      const int pidx = page_of(key), page = pidx >= t.max_pages ? -1 : kept ? table_s[pidx - page0] : table[pidx];
+      bad = page < 0 || page >= t.num_pages;
+      if (bad) report_error(t.err, PHOTON_DEV_BAD_PAGE, R.tok0, key, page);
+      else row = ((long long)page * t.n_kv + g) * t.page_size + (key - pidx * t.page_size);
+    }
+    const uint32_t gone = __ballot_sync(0xffffffffu, bad);
+    row_s[i % SLOTS][x] = row;
+    if (lane == 0) gone_s[i % SLOTS][x >> 5] = gone;
+  };
   auto load = [&](int i) {                         // tile i of the block into its stage
-    const int st = i % C::STAGES, key0 = (tile0 + i) * TF_KT;
-    bf16* ks = ring + st * C::STAGE;
+    bf16* ks = ring + i % C::STAGES * C::STAGE;
     bf16* vs = ks + TF_KT * C::LD;
     constexpr int CPR = D / 8, STEP = TF_THREADS / CPR;           // 16-byte pieces of a row; rows that the block copies at a time
     const int j = tid % CPR * 8;
-#pragma unroll 4
+#pragma unroll
     for (int r = tid / CPR; r < TF_KT; r += STEP) {
-      const int key = key0 + r;
-      bool there = key >= key_lo && key < key_end;
-      size_t row = 0;
-      if (there) {
-        const int pidx = page_of(key);
-        const int page = pidx >= t.max_pages ? -1 : kept ? table_s[pidx - page0] : table[pidx];
-        if (page < 0 || page >= t.num_pages) {
-          there = false;
-          if (j == 0) { atomicOr((unsigned long long*)&gone_s[st], 1ull << r); report_error(t.err, PHOTON_DEV_BAD_PAGE, R.tok0, key, page); }
-        } else {
-          row = ((size_t)page * t.n_kv + g) * t.page_size + (key - pidx * t.page_size);
-        }
-      }
-      tf_copy16(ks + r * C::LD + j, (const bf16*)t.k_cache + row * D + j, there);
-      tf_copy16(vs + r * C::LD + j, (const bf16*)t.v_cache + row * D + j, there);
+      const long long row = row_s[i % SLOTS][r];
+      const size_t at = row >= 0 ? (size_t)row * D + j : 0;
+      tf_copy16(ks + r * C::LD + j, (const bf16*)t.k_cache + at, row >= 0);
+      tf_copy16(vs + r * C::LD + j, (const bf16*)t.v_cache + at, row >= 0);
     }
   };
+  for (int i = tid / TF_KT; i < min(C::STAGES, ntiles); i += TF_THREADS / TF_KT) find(i, tid % TF_KT);
+  __syncthreads();
 #pragma unroll
   for (int i = 0; i < C::STAGES - 1; ++i) {
     if (i < ntiles) load(i);
@@ -173,7 +179,8 @@ tree_attention_few_kernel(const TfParams P) {
 #pragma unroll
       for (int kd = 0; kd < D / 16; ++kd) tf_ld4(qa[kd], qs + (rt * 16 + (lane & 15)) * C::LD + kd * 16 + ((lane >> 4) << 3));
     }
-    const uint64_t gone = gone_s[st];
+    const uint64_t gone = (uint64_t)gone_s[i % SLOTS][1] << 32 | gone_s[i % SLOTS][0];
+    if (tid < TF_KT && i + C::STAGES < ntiles) find(i + C::STAGES, tid);
     const bool edge = key_base + TF_KT > R.base || key_base <= cut_lo || gone != 0;
     if (edge) {
       bool found = false;
@@ -191,7 +198,6 @@ tree_attention_few_kernel(const TfParams P) {
       }
       if (found) poison = 1;
       __syncthreads();
-      if (tid == 0) gone_s[st] = 0;                // read by all; the stage's next tile is asked for behind the next barrier
     }
     float s[C::NT][4];
 #pragma unroll
