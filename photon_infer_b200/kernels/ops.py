@@ -2617,11 +2617,11 @@ def _count_launches(n: int) -> None:
 
 
 #: Tiles of 64 keys that a block of the kernel for few rows may walk one behind the other (waves counted), by head size, for up to 16, 32 and 64 rows.  That
-#: kernel and tcgen05, us, 4, 8 and 14 nodes: 32/8 heads of 64, 1 request of 1,000 keys (2 tiles) 8.6 and 10.2, 8.6 and 10.2, 9.2 and 10.6; 4 of 2,000 (4) 13.1 and
-#: 13.7, 13.5 and 13.9, 15.6 and 14.5; 16 of up to 1,000 (8) 14.5 and 17.6, 18.0 and 17.6, 20.9 and 17.6; 4 of 6,000 (12) 23.8 and 20.9, 26.2 and 21.1, 31.3 and
-#: 21.7; heads of 128, 4 of 600 (2) 13.5 and 13.9, 13.7 and 14.1, 15.8 and 14.5; 16 of up to 300 (3) 13.5 and 15.2, 15.4 and 16.4, 18.0 and 16.6; 4 of 2,000 (4) 17.8 and
-#: 15.6, 18.6 and 16.2, 20.9 and 17.2.
-TREE_FEW_STEPS = {64: (10, 8, 4), 128: (3, 3, 1)}
+#: kernel and tcgen05, us, 4, 8 and 14 nodes: 32/8 heads of 64, 4 requests of 2,000 keys (4 tiles) 12.1 and 13.1, 12.7 and 13.5, 14.5 and 14.1; 16 of up to 1,000 (6) 12.1 and
+#: 17.0, 13.3 and 16.6, 17.6 and 16.8; 4 of 4,000 (8) 15.2 and 15.6, 16.6 and 16.0, 20.1 and 16.6; 48 of up to 1,000 (16) 21.5 and 25.6, 25.4 and 29.9, 31.7 and 25.8;
+#: heads of 128, 4 of 600 (2) 11.3 and 13.1, 11.5 and 13.5, 12.9 and 14.3; 16 of up to 300 (3) 9.8 and 13.1, 12.5 and 14.1, 16.6 and 14.1; 4 of 2,000 (4) 15.0 and 15.4, 15.8 and
+#: 16.0, 17.8 and 16.6; 16 of up to 1,000 (8) 17.2 and 18.0, 20.7 and 18.2, 27.8 and 18.4; 48 of up to 600 (20) 33 and 26, 37 and 26, 52 and 27.
+TREE_FEW_STEPS = {64: (16, 16, 5), 128: (8, 5, 2)}
 
 
 def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, cache_rows: int, aligned: bool, num_seqs: int, n_kv: int, rows: int,
