@@ -19,7 +19,7 @@
 //
 // What bounds it.  Full batches: memory.  64 requests of 32 nodes behind up to 6,000 keys (24/8 heads of 128): 170 us, 0.85 of the copy rate.  Many rows: the softmax between two products;
 // 2 requests of 64 nodes behind 32,768 keys (32/8 heads of 128): 90 us, 770 TFLOP/s, tensor pipe and exponentials each below half.  Few units: begin, end and join.  8 of 27
-// behind up to 2,500 (32/8 heads of 64): 20.5 us for 32 MB.  Measured slower there: tiles of 128 keys, a segment's end behind the next one's first scores, two threads a row,
+// behind up to 2,500 (32/8 heads of 64): 20 us for 32 MB.  Measured slower there: tiles of 128 keys, a segment's end behind the next one's first scores, two threads a row,
 // copies of a row with a part of a tile's keys each, weights by the old maximum before the tile's own is known.
 //
 // Every wait on an mbarrier is bounded: when one runs out the block raises a flag that all roles poll, records PHOTON_DEV_WAIT_TIMEOUT, waits (bounded) for

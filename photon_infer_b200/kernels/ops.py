@@ -2636,7 +2636,10 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
             slots = (3 if head_dim == 64 else 2) * sms
             parts = max(1, min(8, slots * 7 // 8 // units, 2 * tiles))
             steps = -(-tiles // parts) * -(-units * parts // slots)
-            if not tma or steps <= TREE_FEW_STEPS[head_dim][(rows > 16) + (rows > 32)]:
+            # Heads of 64 and up to 32 rows: longer ones too where its blocks fill the chip twice, since tcgen05's tiles are 128 rows whatever is in them.  Few rows and
+            # tcgen05, us, 4 nodes: 48 requests of 6,000 keys (32/8 heads) 100 and 180, of up to 6,000 88 and 95; 8 of 8,000 30 and 37; 20 of 3 behind 10,723 (16/16
+            # heads) 163 and 300; 8 nodes: 48 of 6,000 118 and 180, of up to 6,000 108 and 96; where they do not: 30 of 4 behind 10,000 175 and 150.
+            if not tma or steps <= TREE_FEW_STEPS[head_dim][(rows > 16) + (rows > 32)] or (head_dim == 64 and rows <= 32 and units * parts >= 2 * sms):
                 return "tree_attention_few", parts, 1
         if tma:
             levels = -(-rows // (128 // group * group))
