@@ -288,8 +288,10 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
   // tiles before have landed, and one barrier's parity could not tell the tiles between apart.
   uint64_t* o_full = p_full + C::NB;
   uint32_t* gone_s = reinterpret_cast<uint32_t*>(o_full + C::NB);             // [16]: parts of a key tile (by its number) whose page is missing, one bit a part
-  int* poison = reinterpret_cast<int*>(gone_s + 16);// the last segment whose values were not all finite
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(poison + 1);
+  // The last segments of odd and of even number whose values were not all finite.  A warp may be in the segment behind the one whose word another warp still has to read;
+  // it is never two behind, since a segment's products want all four warps' weights.
+  int* poison = reinterpret_cast<int*>(gone_s + 16);                          // [2]
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(poison + 2);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   TtOrder* order = reinterpret_cast<TtOrder*>(tmem_slot + 2);
 
@@ -298,7 +300,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
     for (int b = 0; b < 2; ++b) { tc_mbar_init(&q_full[b], 1); tc_mbar_init(&q_empty[b], 1); }
     for (int s = 0; s < C::NS; ++s) { tc_mbar_init(&full[s], 1); tc_mbar_init(&empty[s], 1); }
     for (int b = 0; b < C::NB; ++b) { tc_mbar_init(&s_full[b], 1); tc_mbar_init(&p_full[b], 4); tc_mbar_init(&o_full[b], 1); }
-    *poison = 0;
+    poison[0] = poison[1] = 0;
     *abort_flag = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
@@ -536,7 +538,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
           };
           clean(0, upto);
           clean(from, TT_KT);
-          if (found) *(volatile int*)poison = s.serial;
+          if (found) *(volatile int*)&poison[s.serial & 1] = s.serial;
           asm volatile("fence.proxy.async.shared::cta;" ::: "memory");       // generic writes -> the tensor core's reads
         }
         if (busy) {
@@ -621,7 +623,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
       // ---- the segment's end
       if (!landed(n - 1)) break;
       tc_fence_after();
-      const bool fix = *(volatile int*)poison == s.serial;
+      const bool fix = *(volatile int*)&poison[s.serial & 1] == s.serial;
       const int head = s.g * P.t.group + (valid ? (s.row0 + r) % P.t.group : 0);
       const size_t slot = (size_t)blockIdx.x * 2 + s.bit;
       float inv = 1.f;
