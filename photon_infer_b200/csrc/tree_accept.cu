@@ -32,7 +32,8 @@ struct TaParams {
 struct TaShared {
   float4 x[2][TA_MAX_CLUSTER];                     // what the cluster's blocks have found, (value, index, sum, -), twice in turn
   uint64_t bar[2];                                 // all of them are there
-  uint32_t key[TA_THREADS / 32]; int at[TA_THREADS / 32];      // of each warp: its largest number's key and place, and the sum of its weights
+  // of each warp: its largest number's key and place, twice in turn (greedily nothing holds a warp back until all have read them), and the sum of its weights
+  uint32_t key[2][TA_THREADS / 32]; int at[2][TA_THREADS / 32];
   float wsum[TA_THREADS / 32];
   int chosen;
 };
@@ -143,12 +144,13 @@ __device__ int ta_token(const TaParams& P, TaShared& sh, const float* row, int r
     }
   }
   at = __reduce_min_sync(ALL, (unsigned)at);
-  if (lane == 0) { sh.key[warp] = key; sh.at[warp] = at; }
+  const int half = turn.count & 1;
+  if (lane == 0) { sh.key[half][warp] = key; sh.at[half][warp] = at; }
   __syncthreads();
   // every warp: the block's
   {
-    const uint32_t k = lane < WARPS ? sh.key[lane] : 0u, top = __reduce_max_sync(ALL, k);
-    at = (int)__reduce_min_sync(ALL, lane < WARPS && k == top ? (unsigned)sh.at[lane] : 0x7fffffffu);
+    const uint32_t k = lane < WARPS ? sh.key[half][lane] : 0u, top = __reduce_max_sync(ALL, k);
+    at = (int)__reduce_min_sync(ALL, lane < WARPS && k == top ? (unsigned)sh.at[half][lane] : 0x7fffffffu);
     best = __uint_as_float(top ^ ((top >> 31) ? 0x80000000u : 0xffffffffu));
   }
   // With a temperature the warps' sums of weights relative to the block's largest number go along.

@@ -1,8 +1,10 @@
-"""Tree attention over scores and values where a way of sharing out the work could lose something: values that are not finite in one segment behind the other."""
+"""Tree attention and acceptance where a way of sharing out the work could lose something: values that are not finite in one segment behind the other; walks of many
+steps."""
 import pytest
 import torch
 
 from test_gpu_tree_attention import Step
+from test_gpu_tree_cache import _run_accept
 from test_gpu_tree_routes import route                      # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -36,3 +38,20 @@ def test_segments_with_such_values_in_turn(route, d, parts, every):     # noqa: 
         assert err[0] == 0
         assert bool(torch.isnan(_rows(step, got)[hit][..., 3]).all())
         assert torch.equal(_rows(step, got)[~hit], _rows(step, clean)[~hit]) and torch.equal(_rows(step, got)[..., others], _rows(step, clean)[..., others])
+
+
+@pytest.mark.parametrize("V", [5, 5000, 40000, 128256, 151936])
+def test_long_greedy_walks(V):
+    """Chains whose every step has another token, found by another warp of another block: a step's maxima are read by all before they are written again."""
+    n = 150
+    g = torch.Generator().manual_seed(V)
+    logits = torch.rand((2 * n, V), generator=g)
+    best = torch.randint(0, V, (2 * n,), generator=g)
+    logits[torch.arange(2 * n), best] = 2.0
+    best = best.tolist()
+    tokens = [0] + best[:n - 1] + [0] + best[n:2 * n - 1]
+    parents = (list(range(-1, n - 1))) * 2
+    want = ([list(range(n))] * 2, [n] * 2, [best[:n], best[n:]])
+    logits = logits.to("cuda:0")
+    for _ in range(5):
+        assert _run_accept(logits, tokens, parents, [n, n], n) == want
