@@ -33,7 +33,7 @@ template <int GROUPS, int SHARES> struct Tg {
 
 struct TreeShares {
   float* part_o;                                   // [T * n_q, splits, d]
-  float* part_ml;                                  // [T * n_q, splits, 2]: maximum and sum of a share
+  float* part_ml;                                  // [T * n_q, splits, 2]: maximum (-inf: nothing is seen) and sum of a share
   int splits, cluster, row_tiles;                  // cluster: the shares of a row tile are a cluster's blocks, which join them; else 1
 };
 
@@ -345,7 +345,7 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
       if (tid % W + W * u < n) factor[r][tid % W + W * u] = mx[u] * inv;
     if (!last && tid % W == 0 && r < nrows) {
       const size_t slot = ((size_t)(R.tok0 + (row0 + r) / G) * P.n_q + g * G + (row0 + r) % G) * H.splits + split;
-      H.part_ml[slot * 2] = sub; H.part_ml[slot * 2 + 1] = sum;
+      H.part_ml[slot * 2] = top; H.part_ml[slot * 2 + 1] = sum;         // -inf: a share that the row sees nothing of
     }
   }
   __syncthreads();

@@ -1,11 +1,11 @@
-"""Tree attention and acceptance where a way of sharing out the work could lose something: values that are not finite in one segment behind the other; walks of many
-steps."""
+"""Tree attention and acceptance where a way of sharing out the work could lose something: values that are not finite in one segment behind the other, scores far
+below 0; walks of many steps."""
 import pytest
 import torch
 
-from test_gpu_tree_attention import Step
+from test_gpu_tree_attention import TOL, Step
 from test_gpu_tree_cache import _run_accept
-from test_gpu_tree_routes import route                      # noqa: F401  (a fixture)
+from test_gpu_tree_routes import ALL, CONTEXT, NODES, route                      # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -38,6 +38,42 @@ def test_segments_with_such_values_in_turn(route, d, parts, every):     # noqa: 
         assert err[0] == 0
         assert bool(torch.isnan(_rows(step, got)[hit][..., 3]).all())
         assert torch.equal(_rows(step, got)[~hit], _rows(step, clean)[~hit]) and torch.equal(_rows(step, got)[..., others], _rows(step, clean)[..., others])
+
+
+def _below(step, level):
+    """All scores of a step lie around ``-level``: one number of every query is 64, and the same one of every key what ``-level`` wants."""
+    step.q.view(step.T, step.n_q, step.d)[..., 0] = 64.0
+    there = ~step.k[..., 0].isnan()
+    step.k[..., 0][there] = -float(round(level * step.d ** 0.5 / 64))
+
+
+@ALL
+@pytest.mark.parametrize("level", [95, 150, 300])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("with_sink", [False, True])
+def test_scores_far_below_zero_in_every_way(route, dtype, kernel, parts, cluster, level, d, with_sink):     # noqa: F811
+    """Requests from one key to 5,116: most shares of the short ones are empty, and an empty share has no maximum.  A score is a sum of d products of
+    at most 1.2 level + 20 together, each addition off by 2^-23 of that at most (tensor cores cut off); weights and their sum by as much, beside the operator's tolerance."""
+    route(kernel, parts, cluster)
+    step = Step(NODES, CONTEXT, 8, 2, d, 16, dtype, seed=41)
+    _below(step, level)
+    sink = torch.randn(8, generator=torch.Generator().manual_seed(5)) * 2 - level if with_sink else None
+    got, err = step.run(sink=sink)
+    want, largest = step.want(sink=sink)
+    off = 2 * (d + 4) * 2.0 ** -23 * (1.2 * level + 20)
+    assert err[0] == 0 and float((got.double().cpu() - want).abs().max()) <= (TOL[dtype] + off) * largest
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.float32, 64), (torch.bfloat16, 80)], ids=["f32", "bf16"])
+@pytest.mark.parametrize("level", [95, 150])
+def test_scores_far_below_zero_beside_a_long_request(dtype, d, level):
+    """The rule's own choice: two requests of 8 nodes, one behind 16,000 keys and one behind 100."""
+    step = Step([8, 8], [16000, 100], 32, 8, d, 16, dtype, seed=42)
+    _below(step, level)
+    got, err = step.run()
+    want, largest = step.want()
+    off = 2 * (d + 4) * 2.0 ** -23 * (1.2 * level + 20)
+    assert err[0] == 0 and float((got.double().cpu() - want).abs().max()) <= (TOL[dtype] + off) * largest
 
 
 @pytest.mark.parametrize("V", [5, 5000, 40000, 128256, 151936])
