@@ -285,25 +285,27 @@ tree_attention_few_kernel(const TfParams P) {
   asm volatile("cp.async.wait_group 0;" ::: "memory");
   pdl_launch_dependents();
   __syncthreads();                                 // the ring is read; poison is known
-  if (poison && kg == 0) {
-    // what was not finite, for the rows that see it
+  if (poison) {
+    // what was not finite, for the rows that see it: each warp the keys of its own part, whose weights its sum has
     for (int i = 0; i < ntiles; ++i) {
       const int key_base = (tile0 + i) * TF_KT;
       if (!(key_base + TF_KT > R.base || key_base <= cut_lo)) continue;
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
-        for (int w = 0; w < 2 && tok[h] >= 0; ++w) {
-          for (uint32_t bits = tree_visible32(t, R, tok[h], key_base + 32 * w, lo[h]); bits != 0; bits &= bits - 1) {
-            const int key = key_base + 32 * w + __ffs(bits) - 1, pidx = page_of(key);
-            const int page = pidx < t.max_pages ? table[pidx] : -1;
-            if (page < 0 || page >= t.num_pages) continue;
-            const bf16* vr = (const bf16*)t.v_cache + (((size_t)page * t.n_kv + g) * t.page_size + (key - pidx * t.page_size)) * D + c2;
+        uint64_t bits = 0;
+        if (tok[h] >= 0)
+          bits = (uint64_t)tree_visible32(t, R, tok[h], key_base, lo[h]) | (uint64_t)tree_visible32(t, R, tok[h], key_base + 32, lo[h]) << 32;
+        if (C::KG > 1) bits &= ((1ull << (TF_KT / C::KG & 63)) - 1ull) << krow;
+        for (; bits != 0; bits &= bits - 1) {
+          const int key = key_base + __ffsll(bits) - 1, pidx = page_of(key);
+          const int page = pidx < t.max_pages ? table[pidx] : -1;
+          if (page < 0 || page >= t.num_pages) continue;
+          const bf16* vr = (const bf16*)t.v_cache + (((size_t)page * t.n_kv + g) * t.page_size + (key - pidx * t.page_size)) * D + c2;
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) {
-              const float y0 = to_f32(vr[n * 8]), y1 = to_f32(vr[n * 8 + 1]);
-              if (!isfinite(y0)) o[n][2 * h] += y0;
-              if (!isfinite(y1)) o[n][2 * h + 1] += y1;
-            }
+          for (int n = 0; n < D / 8; ++n) {
+            const float y0 = to_f32(vr[n * 8]), y1 = to_f32(vr[n * 8 + 1]);
+            if (!isfinite(y0)) o[n][2 * h] += y0;
+            if (!isfinite(y1)) o[n][2 * h + 1] += y1;
           }
         }
       }

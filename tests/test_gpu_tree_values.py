@@ -5,7 +5,7 @@ import torch
 
 from test_gpu_tree_attention import TOL, Step
 from test_gpu_tree_cache import _run_accept
-from test_gpu_tree_routes import ALL, CONTEXT, NODES, route                      # noqa: F401  (a fixture)
+from test_gpu_tree_routes import ALL, CONTEXT, NODES, WAYS, route                      # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
 
@@ -38,6 +38,33 @@ def test_segments_with_such_values_in_turn(route, d, parts, every):     # noqa: 
         assert err[0] == 0
         assert bool(torch.isnan(_rows(step, got)[hit][..., 3]).all())
         assert torch.equal(_rows(step, got)[~hit], _rows(step, clean)[~hit]) and torch.equal(_rows(step, got)[..., others], _rows(step, clean)[..., others])
+
+
+FEW_ROWS = [w for w in WAYS if w[1] != "tree_attention_tc" and w[2] != 13]
+
+
+@pytest.mark.parametrize("dtype,kernel,parts,cluster", FEW_ROWS, ids=["-".join(str(x).split(".")[-1] for x in w) for w in FEW_ROWS])
+@pytest.mark.parametrize("nodes", [[3], [7]])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [float("nan"), -float("inf")])
+def test_a_seen_value_where_part_of_a_tile_is_hidden(route, dtype, kernel, parts, cluster, nodes, d, bad):      # noqa: F811
+    """Up to 16 and up to 32 rows, whose warps have a part of every tile's keys each: the first keys of the first tile lie before the window, and a block may have that
+    tile alone.  One value at a time, in each part of the first and the last tile: the rows that see it have it, and no other number changes."""
+    route(kernel, parts, cluster)
+    base, window = 855, 256                             # the first tile any row sees begins at 576, the first row's window at 600
+    build = lambda: Step(nodes, [base], 4 * 2, 2, d, 16, dtype, seed=43, fan=2)
+    clean, _ = build().run(window=window)
+    for key in (577, 598, 610, 630, 639, 840, 852, base, base + 2):
+        step = build()
+        page, slot = step.slot(0, key)
+        step.v[page, :, slot, 5] = bad
+        got, err = step.run(window=window)
+        where = key if key < base else base + int(step.depth[0][key - base])
+        sees = torch.tensor([(key < base or bool(step.seen[0][i, key - base])) and where > base + int(step.depth[0][i]) - window for i in range(nodes[0])])
+        assert err[0] == 0 and not bool(torch.isfinite(_rows(step, got)[sees][..., 5].float()).any()), key
+        assert torch.equal(_rows(step, got)[~sees], _rows(step, clean)[~sees])
+        others = [j for j in range(d) if j != 5]
+        assert torch.equal(_rows(step, got)[..., others], _rows(step, clean)[..., others])
 
 
 def _below(step, level):
