@@ -181,8 +181,8 @@ tree_attention_few_kernel(const TfParams P) {
     }
     const uint64_t gone = (uint64_t)gone_s[i % SLOTS][1] << 32 | gone_s[i % SLOTS][0];
     if (tid < TF_KT && i + C::STAGES < ntiles) find(i + C::STAGES, tid);
-    const bool edge = key_base + TF_KT > R.base || key_base <= cut_lo || gone != 0;
-    if (edge) {
+    const bool cut = key_base + TF_KT > R.base || key_base <= cut_lo;           // some row's mask cuts; rows of a missing page are zeros
+    if (cut) {
       bool found = false;
       for (int c = tid; c < TF_KT * (D / 8); c += TF_THREADS) {
         uint4* at = reinterpret_cast<uint4*>(vs + c / (D / 8) * C::LD + c % (D / 8) * 8);
@@ -231,7 +231,7 @@ tree_attention_few_kernel(const TfParams P) {
             s[j][u] = t.softcap - __fdividef(2.0f * t.softcap, tf_exp2(s[j][u] * P.cap_in * 2.8853900817779268f) + 1.0f);
       }
     }
-    if (edge) {
+    if (cut || gone != 0) {
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         uint64_t bits = 0;

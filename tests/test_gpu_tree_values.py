@@ -67,6 +67,23 @@ def test_a_seen_value_where_part_of_a_tile_is_hidden(route, dtype, kernel, parts
         assert torch.equal(_rows(step, got)[..., others], _rows(step, clean)[..., others])
 
 
+@ALL
+@pytest.mark.parametrize("d", [64, 128])
+def test_a_seen_value_beside_a_missing_page(route, dtype, kernel, parts, cluster, d):      # noqa: F811
+    """A tile that no mask cuts, of a page that is missing and one with a value that is not finite: the missing keys are left out, the value is not."""
+    route(kernel, parts, cluster)
+    step = Step([7, 9], [500, 60], 8, 2, d, 16, dtype, seed=44)
+    step.table[0, 9] = -1                               # keys 144 .. 159
+    clean, err = step.run()
+    assert err[0] == 3 and bool(torch.isfinite(clean).all())
+    page, slot = step.slot(0, 170)
+    step.v[page, :, slot, 5] = float("nan")
+    got, err = step.run()
+    assert err[0] == 3 and bool(torch.isnan(_rows(step, got)[:7][..., 5].float()).all())
+    others = [j for j in range(d) if j != 5]
+    assert torch.equal(_rows(step, got)[..., others], _rows(step, clean)[..., others]) and torch.equal(_rows(step, got)[7:], _rows(step, clean)[7:])
+
+
 def _below(step, level):
     """All scores of a step lie around ``-level``: one number of every query is 64, and the same one of every key what ``-level`` wants."""
     step.q.view(step.T, step.n_q, step.d)[..., 0] = 64.0
