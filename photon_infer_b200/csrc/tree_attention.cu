@@ -16,8 +16,8 @@
 // blocks an SM and was slower (32 and 25 us, 132 and 108); tiles of 32 keys 23 and 118; the sums of products in one number after the other, 32 keys a
 // tile, 36 and 334.
 //
-// A key that a row does not see has weight 0, and 0 times a value that is not finite would not be: in tiles where masks cut and such values lie, products with a
-// weight of 0 are left out; rows behind the last key or of a missing page are zeros.
+// A key that a row does not see has weight 0, and 0 times a value that is not finite would not be: in tiles where masks cut and such values lie, products with keys that
+// a row does not see are left out, and so are shares of which it sees nothing; rows behind the last key or of a missing page are zeros.
 #include "tree_attention.cuh"
 #include <math.h>
 #include <type_traits>
@@ -262,7 +262,7 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const float p = my_p[(lr + 4 * i) * PS + k];
-          if (p != 0.f) {                          // a NaN is not 0
+          if ((see[i] >> k) & 1u) {
 #pragma unroll
             for (int c = 0; c < C; ++c) {
               const float4 v = tg_four(my_v + k * D + c * 32);
@@ -320,11 +320,12 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
   {
     constexpr int W = 2 * SHARES;
     const int r = tid / W, n = SHARES * H.cluster;
-    float mx[4], top = -INFINITY, sum = 0.f;
+    float mx[4], l4[4], top = -INFINITY, sum = 0.f;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const int w = tid % W + W * u;
       mx[u] = w < n ? tree_peer(&ml_s[0][w % SHARES][r], w / SHARES) : -INFINITY;
+      l4[u] = w < n ? tree_peer(&ml_s[1][w % SHARES][r], w / SHARES) : 0.f;
       top = fmaxf(top, mx[u]);
     }
 #pragma unroll
@@ -333,16 +334,17 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
     const float most = fmaxf(top, sink), sub = most == -INFINITY ? 0.f : most;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
-      const int w = tid % W + W * u;
+      const bool none = tree_nothing(mx[u], l4[u]);
       mx[u] = expf(mx[u] - sub);                   // 0 for what is not there
-      if (w < n) sum += tree_peer(&ml_s[1][w % SHARES][r], w / SHARES) * mx[u];
+      sum += l4[u] * mx[u];
+      l4[u] = none ? TREE_NOTHING : 0.f;
     }
 #pragma unroll
     for (int w = W / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
     const float total = sum + (sink == -INFINITY ? 0.f : expf(sink - sub)), inv = !last ? 1.f : sum != 0.f ? 1.f / total : 0.f;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (tid % W + W * u < n) factor[r][tid % W + W * u] = mx[u] * inv;
+      if (tid % W + W * u < n) factor[r][tid % W + W * u] = l4[u] == TREE_NOTHING ? TREE_NOTHING : mx[u] * inv;
     if (!last && tid % W == 0 && r < nrows) {
       const size_t slot = ((size_t)(R.tok0 + (row0 + r) / G) * P.n_q + g * G + (row0 + r) % G) * H.splits + split;
       H.part_ml[slot * 2] = top; H.part_ml[slot * 2 + 1] = sum;         // -inf: a share that the row sees nothing of
@@ -359,7 +361,7 @@ tree_attention_kernel(const TreeParams P, const TreeShares H) {
       for (int k = 0; k < SHARES; ++k) {
         const float w = factor[r][SHARES * c + k];
         const float4 x = tree_peer4(po + (k * ROWS + r) * S + j, c);
-        if (w != 0.f) { a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w); }
+        if (!(w < 0.f)) { a.x = fmaf(w, x.x, a.x); a.y = fmaf(w, x.y, a.y); a.z = fmaf(w, x.z, a.z); a.w = fmaf(w, x.w, a.w); }
       }
     }
     const float v[4] = {a.x, a.y, a.z, a.w};
@@ -392,7 +394,6 @@ tree_join_kernel(const TreeParams P, const TreeShares H) {
   const float sub = top == -INFINITY ? 0.f : top;
   float total = 0.f;
   for (int s = 0; s < H.splits; ++s) total += ml[2 * s + 1] * expf(ml[2 * s] - sub);
-  const float keys = total;
   if (P.sinks) total += expf(sink - sub);
   const float inv = total != 0.f ? 1.f / total : 0.f;
   T* dst = (T*)P.out + (size_t)(row / P.n_q) * P.out_stride + (size_t)head * P.d;
@@ -400,9 +401,9 @@ tree_join_kernel(const TreeParams P, const TreeShares H) {
     float a = 0.f;
     for (int s = 0; s < H.splits; ++s) {
       const float w = expf(ml[2 * s] - sub);
-      if (w != 0.f) a = fmaf(w, po[(size_t)s * P.d + j], a);
+      if (!tree_nothing(ml[2 * s], ml[2 * s + 1])) a = fmaf(w, po[(size_t)s * P.d + j], a);
     }
-    dst[j] = from_f32<T>(keys != 0.f ? a * inv : 0.f);
+    dst[j] = from_f32<T>(a * inv);
   }
 }
 

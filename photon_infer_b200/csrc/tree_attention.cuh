@@ -73,6 +73,11 @@ __device__ __forceinline__ float tree_tanh_half(float y) {
   return y * fmaf(z, fmaf(z, fmaf(z, fmaf(z, fmaf(z, -1382.f / 155925.f, 62.f / 2835.f), -17.f / 315.f), 2.f / 15.f), -1.f / 3.f), 1.f);
 }
 
+// A partial result of a row that sees none of its keys: it has no part in the row, whatever lies in its place.  One whose weights are merely too small beside the
+// others' has, so that a value that is not finite shows wherever the keys are cut.  In a list of factors it is marked.
+__device__ __forceinline__ bool tree_nothing(float maximum, float sum) { return maximum == -INFINITY && sum == 0.f; }       // the sum of scores that are NaN is one
+#define TREE_NOTHING (-1.f)
+
 // The cache row (of d numbers) of a key, or -1 where its page is missing, which is recorded.
 __device__ __forceinline__ long long tree_row(const TreeParams& P, const int* table, int g, int key, int tok0) {
   const int pidx = key / P.page_size;

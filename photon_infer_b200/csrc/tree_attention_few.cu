@@ -341,8 +341,10 @@ tree_attention_few_kernel(const TfParams P) {
     const float sub = top == -INFINITY ? 0.f : top;
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
+      const bool none = tree_nothing(f[u], s[u]);
       f[u] = tf_exp2(f[u] - sub);                  // 0 for what is not there
       sum += s[u] * f[u];
+      s[u] = none ? TREE_NOTHING : 0.f;
     }
 #pragma unroll
     for (int w = W / 2; w > 0; w >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, w);
@@ -350,7 +352,7 @@ tree_attention_few_kernel(const TfParams P) {
     const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
     for (int u = 0; u < 4; ++u)
-      if (tid % W + W * u < n) factor_s[r][tid % W + W * u] = f[u] * inv;
+      if (tid % W + W * u < n) factor_s[r][tid % W + W * u] = s[u] == TREE_NOTHING ? TREE_NOTHING : f[u] * inv;
   }
   __syncthreads();
   const int pieces = rows * (D / 4), last = pieces * (rank + 1) / P.cluster;
@@ -365,14 +367,14 @@ tree_attention_few_kernel(const TfParams P) {
       for (int b = 0; b < B; ++b)
 #pragma unroll
         for (int k = 0; k < C::KG; ++k) {
-          w[b][k] = b0 + b < P.cluster ? factor_s[r][(b0 + b) * C::KG + k] : 0.f;
+          w[b][k] = b0 + b < P.cluster ? factor_s[r][(b0 + b) * C::KG + k] : TREE_NOTHING;
           x[b][k] = tree_peer4(po + ((w0 + k) * 16 + rr) * C::LO + j, min(b0 + b, P.cluster - 1));
         }
 #pragma unroll
       for (int b = 0; b < B; ++b)
 #pragma unroll
         for (int k = 0; k < C::KG; ++k)
-          if (w[b][k] != 0.f) {
+          if (!(w[b][k] < 0.f)) {
             a.x = fmaf(w[b][k], x[b][k].x, a.x); a.y = fmaf(w[b][k], x[b][k].y, a.y); a.z = fmaf(w[b][k], x[b][k].z, a.z); a.w = fmaf(w[b][k], x[b][k].w, a.w);
           }
     }

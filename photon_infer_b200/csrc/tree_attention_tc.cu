@@ -726,8 +726,10 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
         const float sub = top == -INFINITY ? 0.f : top;
 #pragma unroll
         for (int k = 0; k < K; ++k) {
+          const bool none = tree_nothing(w[k], l[k]);
           w[k] = at_exp2(w[k] - sub);               // 0 for what is not there
           sum += l[k] * w[k];
+          if (none) w[k] = TREE_NOTHING;
         }
         sum += at_exp2(sink - sub);
         const float inv = sum != 0.f ? 1.f / sum : 0.f;
@@ -745,7 +747,7 @@ tree_attention_tc_kernel(const __grid_constant__ CUtensorMap map_q, const __grid
             float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
             for (int k = 0; k < K; ++k)
-              if (k < P.cluster && w[k] != 0.f) {
+              if (k < P.cluster && !(w[k] < 0.f)) {
                 a.x = fmaf(w[k], y[k][u].x, a.x); a.y = fmaf(w[k], y[k][u].y, a.y); a.z = fmaf(w[k], y[k][u].z, a.z); a.w = fmaf(w[k], y[k][u].w, a.w);
               }
             if (c4 + u < end) {
@@ -830,7 +832,7 @@ tree_join_tc_kernel(const TtParams P, int blocks, int chunks) {
         if (i0 + k >= parts) continue;
         const float w = at_exp2(ml[k].x - sub);
         sum += ml[k].y * w;
-        if (w != 0.f) { a.x = fmaf(w, y[k].x, a.x); a.y = fmaf(w, y[k].y, a.y); a.z = fmaf(w, y[k].z, a.z); a.w = fmaf(w, y[k].w, a.w); }
+        if (!tree_nothing(ml[k].x, ml[k].y)) { a.x = fmaf(w, y[k].x, a.x); a.y = fmaf(w, y[k].y, a.y); a.z = fmaf(w, y[k].z, a.z); a.w = fmaf(w, y[k].w, a.w); }
       }
     }
     if (valid) {

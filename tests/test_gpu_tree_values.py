@@ -84,6 +84,62 @@ def test_a_seen_value_beside_a_missing_page(route, dtype, kernel, parts, cluster
     assert torch.equal(_rows(step, got)[..., others], _rows(step, clean)[..., others]) and torch.equal(_rows(step, got)[7:], _rows(step, clean)[7:])
 
 
+@ALL
+@pytest.mark.parametrize("d", [64, 128])
+def test_seen_values_of_no_weight(route, dtype, kernel, parts, cluster, d):      # noqa: F811
+    """A value that is not finite shows in the rows that see it although its score lies 300 below the others', so that its weight, or that of the whole share that has
+    this key alone, is 0 in 32 bits: 0 times it is not 0.  In tiles that masks cut and in tiles that they do not; rows that do not see it keep their bits."""
+    route(kernel, parts, cluster)
+    build = lambda: Step([9, 16], [700, 2300], 8, 2, d, 16, dtype, seed=45)
+    step = build()
+    step.q.view(step.T, 8, d)[..., 0] = 64.0
+    there = ~step.k[..., 0].isnan()
+    step.k[..., 0][there] = 0.0
+    keys = [(0, 100), (0, 650), (1, 5), (1, 2299), (1, 2301)]
+    for s, key in keys:
+        page, slot = step.slot(s, key)
+        step.k[page, :, slot, 0] = -float(round(300 * d ** 0.5 / 64))
+    clean, _ = step.run()
+    for s, key in keys:
+        page, slot = step.slot(s, key)
+        good = step.v[page, :, slot, 3].clone()
+        step.v[page, :, slot, 3] = float("inf")
+        got, err = step.run()
+        step.v[page, :, slot, 3] = good
+        sees = torch.zeros(step.T, dtype=torch.bool)
+        first, base = (0, 700) if s == 0 else (9, 2300)
+        sees[first:first + step.nodes[s]] = True if key < base else step.seen[s][:, key - base]
+        assert err[0] == 0 and not bool(torch.isfinite(_rows(step, got)[sees][..., 3].float()).any()), (s, key)
+        assert torch.equal(_rows(step, got)[~sees], _rows(step, clean)[~sees])
+        others = [j for j in range(d) if j != 3]
+        assert torch.equal(_rows(step, got)[..., others], _rows(step, clean)[..., others])
+
+
+@ALL
+@pytest.mark.parametrize("d", [64, 128])
+def test_seen_values_in_shares_of_no_weight(route, dtype, kernel, parts, cluster, d):      # noqa: F811
+    """The same where a run of keys has such scores, so that some blocks have no others."""
+    route(kernel, parts, cluster)
+    step = Step([9, 16], [700, 2300], 8, 2, d, 16, dtype, seed=46)
+    step.q.view(step.T, 8, d)[..., 0] = 64.0
+    there = ~step.k[..., 0].isnan()
+    step.k[..., 0][there] = 0.0
+    for key in range(64, 1100):
+        page, slot = step.slot(1, key)
+        step.k[page, :, slot, 0] = -float(round(300 * d ** 0.5 / 64))
+    clean, _ = step.run()
+    for key in (64, 500, 700, 900, 1099):
+        page, slot = step.slot(1, key)
+        good = step.v[page, :, slot, 3].clone()
+        step.v[page, :, slot, 3] = float("inf")
+        got, err = step.run()
+        step.v[page, :, slot, 3] = good
+        assert err[0] == 0 and not bool(torch.isfinite(_rows(step, got)[9:][..., 3].float()).any()), key
+        assert torch.equal(_rows(step, got)[:9], _rows(step, clean)[:9])
+        others = [j for j in range(d) if j != 3]
+        assert torch.equal(_rows(step, got)[..., others], _rows(step, clean)[..., others])
+
+
 def _below(step, level):
     """All scores of a step lie around ``-level``: one number of every query is 64, and the same one of every key what ``-level`` wants."""
     step.q.view(step.T, step.n_q, step.d)[..., 0] = 64.0
