@@ -191,7 +191,9 @@ __device__ int ta_token(const TaParams& P, TaShared& sh, const float* row, int r
   if (rank == owner) {
     // what is left of the target, relative to this block's largest number; in the block the warp, in the warp the run, in the run the lane, in the lane the number: the first
     // of any weight whose sum reaches the target, or else the last of any weight
-    float want = hit != 0 ? (target - before) * ta_exp2((top - own) * scale) : INFINITY;
+    // (a block some 90 temperatures below the row's largest number has a share of so few bits that its weights' factor is infinite: the target's part of the share then)
+    const float factor = ta_exp2((top - own) * scale), left = target - before;
+    float want = hit == 0 ? INFINITY : isfinite(factor) ? left * factor : left / __shfl_sync(ALL, share, owner) * sum;
     const unsigned with = __ballot_sync(ALL, part > 0.f), reach = __ballot_sync(ALL, part > 0.f && upto >= want);
     const int w = reach != 0 ? __ffs(reach) - 1 : 31 - __clz(with);
     if (warp == w) {

@@ -191,3 +191,19 @@ def test_long_greedy_walks(V):
     logits = logits.to("cuda:0")
     for _ in range(5):
         assert _run_accept(logits, tokens, parents, [n, n], n) == want
+
+
+@pytest.mark.parametrize("V", [4096, 32768, 128256, 151936, 262144])
+@pytest.mark.parametrize("walk", [False, True])
+@pytest.mark.parametrize("below", [0.0, 60.0, 80.0, 86.0, 90.0, 95.0, 100.0])
+def test_the_first_of_any_probability(monkeypatch, V, walk, below):
+    """u = 0 takes the first token of any probability, in whichever block of a row's cluster it lies: here token 5 with several behind it, ``below`` temperatures under the largest logit,
+    which lies at the row's end.  All nodes' logits at once, and as a walk."""
+    from photon_infer_b200.kernels import ops
+    if walk:
+        monkeypatch.setattr(ops, "ACCEPT_AT_ONCE", 0)
+    logits = torch.full((3, V), -float("inf"))
+    logits[:, [5, 6, 700, 1500]] = 3.0 - below
+    logits[:, V - 2] = 3.0
+    got = _run_accept(logits.to("cuda:0"), [9, 5, V - 2], [-1, 0, 0], [3], 3, [1.0], [0.0, 0.5 if below > 0 else 0.9, 0.25])
+    assert got == ([[0, 1, -1]], [2], [[5, V - 2, -1]])
