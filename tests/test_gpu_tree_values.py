@@ -4,7 +4,7 @@ import pytest
 import torch
 
 from test_gpu_tree_attention import TOL, Step
-from test_gpu_tree_cache import _run_accept
+from test_gpu_tree_cache import _accept, _case, _run_accept
 from test_gpu_tree_routes import ALL, CONTEXT, NODES, WAYS, route                      # noqa: F401  (a fixture)
 
 pytestmark = pytest.mark.gpu
@@ -207,3 +207,20 @@ def test_the_first_of_any_probability(monkeypatch, V, walk, below):
     logits[:, V - 2] = 3.0
     got = _run_accept(logits.to("cuda:0"), [9, 5, V - 2], [-1, 0, 0], [3], 3, [1.0], [0.0, 0.5 if below > 0 else 0.9, 0.25])
     assert got == ([[0, 1, -1]], [2], [[5, V - 2, -1]])
+
+
+@pytest.mark.parametrize("V", [131073, 151936, 262144, 500009])
+@pytest.mark.parametrize("temperature", [0.0, 0.7])
+@pytest.mark.parametrize("walk", [False, True])
+def test_vocabularies_that_threads_read_again(monkeypatch, V, temperature, walk):
+    """More than 131,072 tokens: a thread has more numbers than it keeps.  Rows on and off 16-byte boundaries, all nodes at once and as a walk."""
+    from photon_infer_b200.kernels import ops
+    monkeypatch.setattr(ops, "ACCEPT_AT_ONCE", 0 if walk else 1 << 40)
+    nodes = [7, 1, 5]
+    logits, tokens, parents, uniforms = _case(nodes, V, seed=V, temperature=temperature)
+    temps = [temperature, 0.0, temperature]
+    want = _accept(logits, tokens, parents, nodes, 6, temps, uniforms)
+    for width, at in ((V, 0), (V + 5, 0), (V + 8 - V % 4, 1)):
+        rows = torch.zeros((13, width), device="cuda:0")[:, at:at + V].copy_(logits)
+        assert _run_accept(rows, tokens, parents, nodes, 6, temps, uniforms) == want
+    assert max(want[1]) > 1
