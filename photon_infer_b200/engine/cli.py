@@ -90,8 +90,8 @@ def main(argv=None) -> int:
             t0 = time.perf_counter()
             answers = generator.generate(prompts, args.max_new_tokens, args.temperature, args.seed, args.ignore_eos, args.samples)
             dt = time.perf_counter() - t0
-            for i, tokens in enumerate(answers):
-                print(f"request {i}: " + " ".join(str(t) for t in tokens))
+            for i, (tokens, reason) in enumerate(zip(answers, generator.finish_reasons)):
+                print(f"request {i} ({reason}): " + " ".join(str(t) for t in tokens))
             st = generator.stats
             print(f"Generated {st.generated} tokens in {dt:.3f} s ({st.generated / dt:.1f} tokens/s), {st.steps} steps of trees, "
                   f"{st.nodes} nodes", file=sys.stderr)

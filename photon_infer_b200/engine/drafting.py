@@ -6,13 +6,15 @@ draft (``lookup_tree``).  Several drafts share their beginnings, so they form a 
 uniform numbers that an ordinary step would use, so the drafts change how many steps it takes and not what comes out (but for
 the last bits of logits, which another batch gives).
 
-Several samples of one prompt share its pages: the prompt runs once and the request forks (``CacheManager.fork``).  The reference
+Several samples of one prompt share its pages: the prompt runs once and the request forks (``CacheManager.fork``).  Where pages run out the
+request that came last waits, as in the scheduler: its pages are freed and its tokens are computed again later.  The reference
 generates one token a step (demo/llama_infer.cpp:160-200).
 """
 from __future__ import annotations
 
+import collections
 import dataclasses
-from typing import Callable, List, Optional, Sequence, Tuple
+from typing import Callable, Deque, List, Optional, Sequence, Tuple
 
 from ..config.engine_options import EngineOptions
 from ..errors import ErrorCode, PhotonError
@@ -54,6 +56,13 @@ class _Sample:
     generated: List[int] = dataclasses.field(default_factory=list)
     finish_reason: Optional[str] = None
 
+    def tokens(self) -> List[int]:
+        return self.prompt + self.generated
+
+
+#: Samples of one prompt that run it once and fork; one that had to wait is a group of its own.
+_Group = List[_Sample]
+
 
 @dataclasses.dataclass
 class DraftStats:
@@ -72,10 +81,12 @@ class DraftingGenerator:
         self.runner, self.options, self.drafter = runner, options, drafter
         self.max_nodes, self.max_depth = max_nodes, max_depth
         self.stats = DraftStats()
+        self.finish_reasons: List[str] = []     # of the last call's answers: "eos", "length", "model_len" or "out_of_memory"
 
     def generate(self, prompts: Sequence[Sequence[int]], max_new_tokens: int = 16, temperature: float = 0.0, seed: int = 0,
                  ignore_eos: bool = False, samples: int = 1) -> List[List[int]]:
-        """``samples`` answers to each prompt, one behind the other.  Answer ``i`` of all is sampled as request ``i`` of an engine is."""
+        """``samples`` answers to each prompt, one behind the other.  Answer ``i`` of all is sampled as request ``i`` of an engine is.  An answer that
+        does not fit the cache although nothing else runs ends there, as in an engine (``finish_reasons``)."""
         vocab = self.runner.model.spec.vocab_size
         for p in prompts:
             if not p or any(not 0 <= int(t) < vocab for t in p):
@@ -84,62 +95,114 @@ class DraftingGenerator:
                 raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"a prompt of {len(p)} tokens leaves no room in {self.runner.max_model_len}")
         if max_new_tokens < 1 or samples < 1:
             raise PhotonError(ErrorCode.INVALID_ARGUMENT, "at least one new token and one sample are wanted")
-        out: List[List[int]] = []
-        room = max(1, min(self.options.max_batch_size, self.options.max_sequences) // samples)
-        for first in range(0, len(prompts), room):
-            group = [[_Sample((first + i) * samples + j, seed, [int(t) for t in p]) for j in range(samples)]
-                     for i, p in enumerate(prompts[first:first + room])]
-            try:
-                self._prefill(group)
-                self._decode([s for g in group for s in g], max_new_tokens, temperature, ignore_eos)
-            finally:
-                for s in (s for g in group for s in g):
-                    if self.runner.cache.has_request(s.rid):
-                        self.runner.cache.free_request(s.rid)
-            out.extend(s.generated for g in group for s in g)
-        return out
+        groups: List[_Group] = [[_Sample(i * samples + j, seed, [int(t) for t in p]) for j in range(samples)] for i, p in enumerate(prompts)]
+        answers = [s for g in groups for s in g]
+        waiting: Deque[_Group] = collections.deque(groups)
+        try:
+            while waiting:
+                self._decode(self._prefill(waiting), waiting, max_new_tokens, temperature, ignore_eos)
+        finally:
+            for s in answers:
+                if self.runner.cache.has_request(s.rid):
+                    self.runner.cache.free_request(s.rid)
+        self.finish_reasons = [s.finish_reason for s in answers]
+        return [s.generated for s in answers]
 
-    def _prefill(self, group: List[List[_Sample]]) -> None:
-        """Every prompt but its last token, once, in portions; then the prompt's samples fork from the first."""
-        cache, budget = self.runner.cache, self.options.max_num_batched_tokens
-        waiting = [(g[0], 0) for g in group]
-        for s, _ in waiting:
-            cache.add_request(s.rid)
-        while waiting:
-            entries, left, rest = [], budget, []
-            for s, done in waiting:
-                n = min(len(s.prompt) - 1 - done, self.options.chunk_size, left)
+    def _prefill(self, waiting: Deque[_Group]) -> List[_Sample]:
+        """As many groups as may run together: every group's tokens but the last, once, in portions; then its samples fork from the first.  Returns
+        those that run.  What finds no pages goes back to ``waiting``, the last group first."""
+        cache, limit = self.runner.cache, min(self.options.max_batch_size, self.options.max_sequences)
+        batch: List[_Group] = []
+        while waiting and (not batch or sum(len(g) for g in batch) + len(waiting[0]) <= limit):
+            batch.append(waiting.popleft())
+            cache.add_request(batch[-1][0].rid)
+
+        def last_waits() -> None:
+            g = batch.pop()
+            cache.free_request(g[0].rid)
+            waiting.appendleft(g)
+
+        todo = [(g, 0) for g in batch]
+        while todo:
+            entries, left, rest = [], self.options.max_num_batched_tokens, []
+            taken = [0] * len(cache.groups)         # pages of the step's entries
+            for g, done in todo:
+                if not any(g is b for b in batch):
+                    continue                        # it waits
+                s, tokens = g[0], g[0].tokens()[:-1]
+                n = min(len(tokens) - done, self.options.chunk_size, left)
                 if n > 0:
-                    entries.append(StepEntry(s.rid, s.prompt[done:done + n]))
+                    need = [a + b for a, b in zip(taken, cache.pages_needed(s.rid, n))]
+                    while not self._free(need) and batch[-1] is not g:
+                        last_waits()
+                    if not self._free(need):
+                        last_waits()
+                        if not batch:               # alone and still too large for the pool
+                            for s in waiting.popleft():
+                                s.finish_reason = "out_of_memory"
+                        continue
+                    entries.append(StepEntry(s.rid, tokens[done:done + n]))
+                    taken = need
                 left -= n
-                if done + n < len(s.prompt) - 1:
-                    rest.append((s, done + n))
+                if done + n < len(tokens):
+                    rest.append((g, done + n))
             if entries:
                 self.runner.step(entries)
-            waiting = rest
-        for g in group:
-            if len(g) > 1:
-                cache.fork(g[0].rid, [s.rid for s in g[1:]])
+            todo = rest
+        live: List[_Sample] = []
+        at = 0
+        while at < len(batch):
+            g = batch[at]
+            at += 1
+            while self._forks(g[0].rid, len(g) - 1, limit - len(live) - 1) < len(g) - 1 and at < len(batch):
+                last_waits()
+            n = self._forks(g[0].rid, len(g) - 1, limit - len(live) - 1)
+            if n > 0:
+                cache.fork(g[0].rid, [s.rid for s in g[1:n + 1]])
+            live += g[:n + 1]
+            if n + 1 < len(g):
+                waiting.appendleft(g[n + 1:])
+        return live
 
-    def _fits(self, sizes: List[Tuple[int, int]]) -> bool:
-        """Whether trees of (request, nodes) find their pages."""
+    def _forks(self, rid, wanted: int, room: int) -> int:
+        """How many forks of a request find their pages and slots, up to ``wanted`` and ``room``."""
         cache = self.runner.cache
-        need = [sum(n) for n in zip(*(cache.pages_needed(rid, n) for rid, n in sizes))]
-        return all(n <= free for n, free in zip(need, cache.free_pages()))
+        n = min(wanted, max(0, room), cache.states.num_free)
+        for g, free in zip(cache.groups, cache.free_pages()):
+            each = g.pages_to_fork(cache.length(rid))
+            n = min(n, free // each if each else n)
+        return n
 
-    def _decode(self, live: List[_Sample], max_new_tokens: int, temperature: float, ignore_eos: bool) -> None:
-        eos = self.runner.model.spec.eos_token_ids
+    def _free(self, need: List[int]) -> bool:
+        """Whether as many pages are free in every cache group."""
+        return all(n <= free for n, free in zip(need, self.runner.cache.free_pages()))
+
+    def _decode(self, live: List[_Sample], waiting: Deque[_Group], max_new_tokens: int, temperature: float, ignore_eos: bool) -> None:
+        eos, cache = self.runner.model.spec.eos_token_ids, self.runner.cache
         while live:
+            ones = [cache.pages_needed(s.rid, 1) for s in live]
+            while not self._free([sum(n) for n in zip(*ones)]):
+                s = live.pop()
+                ones.pop()
+                cache.free_request(s.rid)
+                if not live:                        # alone and still too large for the pool
+                    s.finish_reason = "out_of_memory"
+                    return
+                waiting.appendleft([s])
+            taken = [sum(n) for n in zip(*ones)]    # pages of the step: one node each, and the drafts so far
             # one node each whatever the budget, drafts as far as it goes
             spare = max(0, self.options.max_num_batched_tokens - len(live)) // len(live)
             entries, temps, us = [], [], []
-            for s in live:
-                tokens = s.prompt + s.generated
+            for s, one in zip(live, ones):
+                tokens = s.tokens()
                 room = min(max_new_tokens - len(s.generated), self.runner.max_model_len - len(tokens) + 1)
                 nodes = max(1, min(self.max_nodes, 1 + spare, self.runner.max_model_len - len(tokens) + 1))
                 drafted, parents = self.drafter(tokens, nodes, min(self.max_depth, max(0, room - 1)))
-                others = [(e.request_id, len(e.tokens)) for e in entries] + [(o.rid, 1) for o in live[len(entries) + 1:]]
-                while len(drafted) > 1 and not self._fits(others + [(s.rid, len(drafted))]):
+                while len(drafted) > 1:
+                    need = [t - a + b for t, a, b in zip(taken, one, cache.pages_needed(s.rid, len(drafted)))]
+                    if self._free(need):
+                        taken = need
+                        break
                     drafted, parents = drafted[:len(drafted) // 2], parents[:len(drafted) // 2]     # few pages are left
                 entries.append(TreeEntry(s.rid, drafted, parents))
                 depth: List[int] = []
@@ -163,7 +226,7 @@ class DraftingGenerator:
                     if s.finish_reason is not None:
                         break
                 if s.finish_reason is not None:
-                    self.runner.cache.free_request(s.rid)
+                    cache.free_request(s.rid)
             live = [s for s in live if s.finish_reason is None]
 
 
