@@ -198,6 +198,8 @@ class DraftingGenerator:
                 room = min(max_new_tokens - len(s.generated), self.runner.max_model_len - len(tokens) + 1)
                 nodes = max(1, min(self.max_nodes, 1 + spare, self.runner.max_model_len - len(tokens) + 1))
                 drafted, parents = self.drafter(tokens, nodes, min(self.max_depth, max(0, room - 1)))
+                if not drafted or drafted[0] != tokens[-1]:
+                    raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"the drafter's tree for request {s.rid} begins with {list(drafted[:1])}, not with its last token, {tokens[-1]}")
                 while len(drafted) > 1:
                     need = [t - a + b for t, a, b in zip(taken, one, cache.pages_needed(s.rid, len(drafted)))]
                     if self._free(need):

@@ -154,3 +154,13 @@ def test_more_samples_than_slots():
     generator = DraftingGenerator(runner, EngineOptions(max_batch_size=3, max_sequences=4), 6, 3, _knowing)
     got = generator.generate(_prompts([9, 6]), 7, 0.9, seed=2, ignore_eos=True, samples=10)
     assert got == [_want(p, 7, 10 * i + j, 0.9, 2, True) for i, p in enumerate(_prompts([9, 6])) for j in range(10)] and runner.most <= 3
+
+
+@pytest.mark.parametrize("drafted", [([], []), ([8], [-1]), ([8, 9], [-1, 0])])
+def test_drafts_that_do_not_begin_with_the_last_token(drafted):
+    """A tree that would put another token, or none, in the place of the request's last one is refused; nothing stays taken."""
+    runner = _Runner(20)
+    generator = DraftingGenerator(runner, EngineOptions(), 6, 3, lambda text, n, d: drafted)
+    with pytest.raises(PhotonError) as e:
+        generator.generate([[1, 2, 7]], 4, ignore_eos=True)
+    assert e.value.code == ErrorCode.INVALID_ARGUMENT and runner.cache.live_requests() == [] and runner.cache.free_pages() == [20]
