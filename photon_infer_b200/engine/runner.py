@@ -223,6 +223,8 @@ class ModelRunner:
                 raise PhotonError(ErrorCode.INVALID_ARGUMENT,
                                   f"request {e.request_id!r} would exceed the longest request of {self.max_model_len} tokens")
         T = sum(len(e.tokens) for e in entries)
+        if depth is not None and depth < 1:
+            raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"a path has one node at least, depth is {depth}")
         if sampling is not None and (len(sampling[0]) != len(entries) or len(sampling[1]) != T):
             raise PhotonError(ErrorCode.INVALID_ARGUMENT, "sampling needs a temperature per entry and a uniform number per node")
         most = max(len(e.tokens) for e in entries)
@@ -242,7 +244,7 @@ class ModelRunner:
         steps = [StepEntry(e.request_id, e.tokens, range(len(e.tokens))) for e in entries]
         ctx, logit_rows, _ = self._build_context(steps, trees=(entries, layouts, sampling))
         logits = self.model.forward(ctx, self._layer_caches, logit_rows)
-        D = min(depth or T, int(max(d.max() for d, _ in layouts)) + 1)
+        D = min(depth if depth is not None else T, int(max(d.max() for d, _ in layouts)) + 1)
         S = len(entries)
         answer = torch.empty(S * (2 * D + 1) + 4, dtype=torch.int32, device=self.device)
         path, sampled, counts = answer[:S * D].view(S, D), answer[S * D: 2 * S * D].view(S, D), answer[2 * S * D: S * (2 * D + 1)]

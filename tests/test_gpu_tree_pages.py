@@ -34,3 +34,16 @@ def test_prompts_that_do_not_fit_together(folders, name, temperature):
         assert generator.finish_reasons == ["length"] * 10
         assert runner.cache.live_requests() == [] and runner.cache.free_pages() == [g.num_pages for g in runner.cache.groups]
     assert answers[1] == answers[0] and answers[3] == answers[0]
+
+
+@pytest.mark.parametrize("depth", [0, -1])
+def test_a_depth_below_one_is_refused(folders, depth):
+    from photon_infer_b200.engine.loading import build_runner
+    from photon_infer_b200.engine.runner import TreeEntry
+    from photon_infer_b200.errors import ErrorCode, PhotonError
+    runner = build_runner(folders["tiny_a"], _options("tiny_a", "float32"))
+    runner.cache.add_request("a")
+    free = runner.cache.free_pages()
+    with pytest.raises(PhotonError) as e:
+        runner.tree_step([TreeEntry("a", [1, 2], [-1, 0])], depth=depth)
+    assert e.value.code == ErrorCode.INVALID_ARGUMENT and runner.cache.free_pages() == free
