@@ -5,7 +5,7 @@
 // cache_keep: the rows of a tree's accepted nodes go to the places behind the request's cached tokens.  Node i of request s lies at key base + i;
 // path[s][j], j < counts[s], goes to key base + j.  A path ascends from its root, so path[j] >= j: a row is never needed after a later one has been written.  A
 // thread owns one piece of the rows of one head and moves eight rows at a time: all eight are read before the first is written, and what a later eight read lies
-// behind all that an earlier eight wrote.  Threads share nothing, so there is nothing to wait for.
+// behind all that an earlier eight wrote.  A block's threads share the list of moves, up to 256 at a time behind a barrier, and nothing of the rows.
 // Bound by the latency of one round (path, table, rows, rows back) for few rows: 8 requests, 16 layers of 8 heads of 64: 2.9 us (3.2 with the path read behind the count);
 // 48 requests, 28 layers of 8 heads of 128, 44 MB read and written: 12.3 us (3.6 TB/s, rows of 256 bytes in no order; 13.0 with a block for every 256 pieces, two rounds
 // of blocks); 20 requests of as many layers in 32 bits 7.2 (8.7).

@@ -57,7 +57,7 @@ template <int D, int MT> struct Tf {
   static constexpr int NT = TF_KT / KG / 8;        // a warp's n-tiles of keys
   static constexpr int LD = D + 8;                 // padded row: conflict-free ldmatrix
   static constexpr int ROWS = 16 * MT;
-  static constexpr int STAGES = D == 64 ? 3 : 2;   // three blocks an SM either way (heads of 128 and 64 rows: two)
+  static constexpr int STAGES = D == 64 ? 3 : 2;   // three blocks an SM with heads of 64, two with heads of 128
   static constexpr int STAGE = 2 * TF_KT * LD;     // elements: a K tile, then a V tile
   static constexpr int LO = D + 4;                 // row of the joined partial results (floats)
   static constexpr int RING = (ROWS * LD + STAGES * STAGE) * 2;

@@ -2638,7 +2638,8 @@ def _tree_route(dtype: torch.dtype, head_dim: int, group: int, page_size: int, c
             steps = -(-tiles // parts) * -(-units * parts // slots)
             # Heads of 64 and up to 32 rows: longer ones too where its blocks fill the chip twice, since tcgen05's tiles are 128 rows whatever is in them.  Few rows and
             # tcgen05, us, 4 nodes: 48 requests of 6,000 keys (32/8 heads) 100 and 180, of up to 6,000 88 and 95; 8 of 8,000 30 and 37; 20 of 3 behind 10,723 (16/16
-            # heads) 163 and 300; 8 nodes: 48 of 6,000 118 and 180, of up to 6,000 108 and 96; where they do not: 30 of 4 behind 10,000 175 and 150.
+            # heads) 163 and 300; 8 nodes: 48 of 6,000 118 and 180, of up to 6,000 104 and 96 (only the longest
+            # is known here: uneven requests pay 8 us for the 62 that even ones save); where they do not: 30 of 4 behind 10,000 175 and 150.
             if not tma or steps <= TREE_FEW_STEPS[head_dim][(rows > 16) + (rows > 32)] or (head_dim == 64 and rows <= 32 and units * parts >= 2 * sms):
                 return "tree_attention_few", parts, 1
         if tma:
