@@ -877,7 +877,8 @@ PHOTON_API int photon_tree_attention_tc(const photon_tree_call* call, cudaStream
   const int G = t.group, d = t.d, page_size = t.page_size;
   if (call->dtype != PHOTON_BF16 || (d != 64 && d != 128) || G > 128) return PHOTON_ERR_UNSUPPORTED;
   if (page_size < 8 || (page_size & 7) || !((64 % page_size) == 0 || (page_size % 64) == 0)) return PHOTON_ERR_UNSUPPORTED;
-  if (((uintptr_t)t.q & 15) || (t.q_stride & 7) || ((uintptr_t)t.k_cache & 15) || ((uintptr_t)t.v_cache & 15) || ((uintptr_t)t.out & 15) || (t.out_stride & 7))
+  if (((uintptr_t)t.q & 15) || (t.q_stride & 7) || ((uintptr_t)t.k_cache & 15) || ((uintptr_t)t.v_cache & 15) || ((uintptr_t)t.out & 15) || (t.out_stride & 7) ||
+      t.q_stride < (long)t.n_q * d)                // a tensor map's stride holds the dimensions before it
     return PHOTON_ERR_UNSUPPORTED;
   const long total_rows = (long)t.num_pages * t.n_kv * page_size;
   if (total_rows > 0x7fffff00L) return PHOTON_ERR_UNSUPPORTED;

@@ -585,7 +585,7 @@ typedef struct {
 PHOTON_EXPORT int photon_tree_attention(const photon_tree_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ tree_attention_tc.cu: the same on tcgen05, bfloat16, d 64 or 128 */
-/* At most 128 query heads per key/value head, pages of 8, 16, 32 or a multiple of 64 tokens, 16-byte aligned rows.  parts: the grid, at most as many blocks
+/* At most 128 query heads per key/value head, pages of 8, 16, 32 or a multiple of 64 tokens, 16-byte aligned rows, q_stride >= n_q * d.  parts: the grid, at most as many blocks
  * as the chip holds at once.  scratch: as many floats as the first function says, and the lengths on the device decide whether a request's keys are shared out
  * over blocks; or null: they are not, in one kernel.  cluster 2 to 8: that many blocks share a unit (128 rows of a request and head) and parts is units * cluster;
  * no scratch. */

@@ -2574,6 +2574,12 @@ def tree_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_
     T, (q_stride, q_inner), (out_stride, out_inner) = shape[0], q.stride(), out.stride()
     if (q_inner != 1 or out_inner != 1) and T:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: rows of q and out must be contiguous")
+    if q_stride < shape[1] or out_stride < shape[1]:
+        if T > 1 and out_stride < shape[1]:
+            raise PhotonError(ErrorCode.SHAPE_MISMATCH, "tree_attention: rows of out must not overlap")
+        if T > 1 and q_stride < shape[1]:
+            q = q.contiguous()                      # a broadcast query: the copies by tiles want rows apart
+        q_stride, out_stride = (max(s, shape[1]) for s in (q_stride, out_stride))     # of one row: any
     if out.dtype != dtype or k_cache.dtype != dtype or v_cache.dtype != dtype:
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, "tree_attention: q, out and the caches must share one dtype")
     if len(cache) != 4 or v_cache.shape != cache or cache[1] != n_kv or cache[3] != head_dim or not k_cache.is_contiguous() or not v_cache.is_contiguous():

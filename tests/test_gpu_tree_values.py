@@ -224,3 +224,25 @@ def test_vocabularies_that_threads_read_again(monkeypatch, V, temperature, walk)
         rows = torch.zeros((13, width), device="cuda:0")[:, at:at + V].copy_(logits)
         assert _run_accept(rows, tokens, parents, nodes, 6, temps, uniforms) == want
     assert max(want[1]) > 1
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("nodes,context", [([5, 3], [40, 300]), ([30, 17], [40, 900])])
+def test_one_query_for_all_nodes(dtype, d, nodes, context):
+    """A broadcast query, whose rows are no numbers apart, and a single row with any stride; outputs whose rows overlap are refused."""
+    from photon_infer_b200.errors import ErrorCode, PhotonError
+    step = Step(nodes, context, 8, 2, d, 16, dtype, seed=47)
+    step.q[:] = step.q[:1].clone()
+    want, _ = step.run()
+    one = step.q[:1].to(dtype).to("cuda:0")
+    got, err = step.run(q=one.expand(step.T, -1))
+    assert err[0] == 0 and torch.equal(got, want)
+    with pytest.raises(PhotonError) as e:
+        step.run(out=torch.zeros((1, 8 * d), dtype=dtype, device="cuda:0").expand(step.T, -1))
+    assert e.value.code == ErrorCode.SHAPE_MISMATCH
+    single = Step([1], [context[1]], 8, 2, d, 16, dtype, seed=48)
+    want, _ = single.run()
+    row = single.q.to(dtype).to("cuda:0")
+    for stride in (0, 1, 3 * 8 * d):
+        assert torch.equal(single.run(q=row.as_strided((1, 8 * d), (stride, 1)))[0], want)
