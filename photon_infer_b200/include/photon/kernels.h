@@ -623,6 +623,66 @@ PHOTON_EXPORT int photon_cache_keep(const photon_keep_call* call, cudaStream_t s
 PHOTON_EXPORT int photon_cache_copy_pages(void* kv, int dtype, int planes, int num_pages, long page_elems, const int* pairs, int count, int* err,
                             cudaStream_t stream);
 
+/* ------------------------------------------------------------------ kv4.cu: a paged cache with 4 bits a number */
+/* K and V of one layer: bytes [num_pages][n_kv][page_size * (d / 2 + d / 32)], 16-byte aligned; of each page and head first the rows' codes, d / 2 bytes each, then
+ * their scales, d / 32 bytes each (csrc/kv4.cuh has the format).  d: a multiple of 32 up to 256; page_size * d: a multiple of 512.
+ * Row t of k and v [T, n_kv * d] (rows k_stride and v_stride elements apart) goes to slot_mapping[t]; -1: nowhere. */
+typedef struct {
+  const void* k; const void* v; const int* slot_mapping; void* k_cache; void* v_cache; int* err;
+  long k_stride, v_stride;
+  int dtype, T, n_kv, d, page_size, num_pages;
+} photon_kv4_write_call;
+PHOTON_EXPORT int photon_kv4_write(const photon_kv4_write_call* call, cudaStream_t stream);
+/* Pages read back, k_out and v_out [S * per][n_kv][page_size][d], 16-byte aligned: page s * per + p is page table[s * stride + p]; one outside the pool is left out.  With cu_tokens
+ * (else null): of request s only the pages below context_lens[s], and only where it has more than min_rows rows (tokens x group), with zeros behind the last key; new_table
+ * [S * per] (may be null) gets each output page's own number, or -1, positions [T] (may be null) each token's place in its request;
+ * with flags [S * per * ceil(2 * n_kv * page_size * d / 2048)] (may be null) values that are not finite are laid out as zero and marked there for photon_kv4_spoil. */
+typedef struct {
+  const void* k_cache; const void* v_cache; const int* table; void* k_out; void* v_out; const int* cu_tokens; const int* context_lens; int* new_table; int* positions;
+  int* flags; int* err;
+  long stride;
+  int dtype, S, per, n_kv, d, page_size, num_pages, group, min_rows;
+} photon_kv4_unpack_call;
+PHOTON_EXPORT int photon_kv4_unpack(const photon_kv4_unpack_call* call, cudaStream_t stream);
+/* Behind an attention over what that call laid out: rows of out (bfloat16 [T, n_kv * group * d]) that see a marked value become NaN in its group's numbers. */
+PHOTON_EXPORT int photon_kv4_spoil(const photon_kv4_unpack_call* call, void* out, long out_stride, int window, cudaStream_t stream);
+
+/* ------------------------------------------------------------------ kv4_attention.cu */
+/* The tokens cu_tokens[s] .. cu_tokens[s + 1] - 1 of the step are the last of request s's context_lens[s] keys; the one at place p sees keys p - window + 1 .. p (window 0:
+ * 0 .. p).  A row that sees nothing is zero.  Requests with rows (tokens x n_q / n_kv) in (min_rows, max_rows] only.  lse (may be null): float [T, n_q], each row's logarithm of the
+ * sum of the exponentials of its scores, the sink's among them.  scratch: T * n_q * parts * (d + 2) floats for parts > 1. */
+typedef struct {
+  const void* q; void* out; const void* k_cache; const void* v_cache; const int* block_table; const int* cu_tokens; const int* context_lens;
+  const float* sinks; float* lse; float* scratch; int* err;
+  long q_stride, out_stride;
+  int dtype, max_pages, S, max_tokens_per_seq, n_q, n_kv, d, page_size, num_pages, window, parts, min_rows, max_rows;
+  float scale, softcap;
+} photon_kv4_attention_call;
+PHOTON_EXPORT int photon_kv4_attention(const photon_kv4_attention_call* call, cudaStream_t stream);
+
+/* ------------------------------------------------------------------ key_weights.cu */
+/* weights [num_pages][n_kv][page_size]: what the keys below context_lens[s] got of the softmax of request s's rows is added; keys from held[s] on (held null: the call's own tokens)
+ * are set.  k_cache: of dtype, [num_pages][n_kv][page_size][d], or with packed 4 bits a number.  Rows and masks as in photon_kv4_attention; lse as that leaves it, or null:
+ * then scratch has T * n_q * parts * 2 floats. */
+typedef struct {
+  const void* q; float* weights; const void* k_cache; const int* block_table; const int* cu_tokens; const int* context_lens; const int* held; const float* sinks;
+  const float* lse; float* scratch; int* err;
+  long q_stride;
+  int dtype, packed, max_pages, S, max_keys, n_q, n_kv, d, page_size, num_pages, window, parts, max_tokens_per_seq;
+  float scale, softcap;
+} photon_key_weights_call;
+PHOTON_EXPORT int photon_key_weights(const photon_key_weights_call* call, cudaStream_t stream);
+
+/* ------------------------------------------------------------------ cache_evict.cu */
+/* kv [entries][planes][num_pages][n_kv][page_size * (row_bytes + scale_bytes)], rows first, then scales; weights [entries][num_pages][n_kv][page_size].  Requests with more than
+ * `keep` keys keep that many: in every entry and head the first `first`, the last `last` and those with the largest weights (of equal ones the lower place), moved to the
+ * front in their order, the weights with them.  kept [entries][S][n_kv][keep]: their old places (of requests that lose keys).  new_lens [S] = min(context_lens, keep), another array than context_lens. */
+typedef struct {
+  void* kv; float* weights; const int* block_table; const int* context_lens; int* new_lens; int* kept; int* err;
+  int entries, planes, num_pages, n_kv, page_size, max_pages, S, keep, first, last, row_bytes, scale_bytes;
+} photon_evict_call;
+PHOTON_EXPORT int photon_cache_evict(const photon_evict_call* call, cudaStream_t stream);
+
 /* ------------------------------------------------------------------ sampling.cu */
 /* Per row: first maximum where temperature is null or <= 0, else the first index whose running sum of
  * softmax(logits / temperature) reaches u.  scratch: float [rows * 128] for V > 16384, else may be null. */

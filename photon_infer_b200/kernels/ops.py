@@ -2780,6 +2780,306 @@ def cache_copy_pages(kv: torch.Tensor, pairs: torch.Tensor, err: Optional[torch.
              err.data_ptr() if err is not None else 0, _stream()), "cache_copy_pages")
 
 
+# ----------------------------------------------------------------------------- caches that hold less
+
+#: Bytes that a page of one head takes in 4 bits, for every 32 numbers of a token: 16 of codes and a scale.
+_KV4_GROUP = 17
+
+
+def kv4_supported(page_size: int, head_dim: int) -> bool:
+    """Whether a paged cache in 4 bits can have these pages: heads of a multiple of 32 numbers up to 256, pieces of 16 bytes."""
+    return head_dim > 0 and head_dim % 32 == 0 and head_dim <= 256 and page_size > 0 and page_size * head_dim % 512 == 0
+
+
+def kv4_page_bytes(page_size: int, head_dim: int) -> int:
+    """Bytes of a page of one key/value head: a cache in 4 bits is uint8 ``[pages, n_kv, kv4_page_bytes(page_size, head_dim)]`` for the keys, and
+    as much for the values.  Rows of ``head_dim / 2`` bytes lie in front, then rows of ``head_dim / 32`` scales (``csrc/kv4.cuh`` has the format): numbers in groups of 32,
+    each a whole multiple (-7 to 7) of its group's scale, a number with 4 bits of mantissa."""
+    if not kv4_supported(page_size, head_dim):
+        raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, f"a cache in 4 bits: heads of {head_dim} in pages of {page_size} are not supported (multiples of 32 up to 256, "
+                          "page_size * head_dim a multiple of 512)")
+    return page_size * (head_dim // 32) * _KV4_GROUP
+
+
+def _on_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
+    """All on the current CUDA device, whose stream the kernels run on."""
+    index = None
+    for t in tensors:
+        if t is None:
+            continue
+        if not t.is_cuda:
+            _cuda(t)
+        if index is None:
+            index = torch._C._cuda_getDevice()
+        if t.get_device() != index:
+            raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"{what}: a tensor is on another device than the current one")
+
+
+def _kv4_cache(what: str, cache: torch.Tensor, n_kv: int, head_dim: int) -> int:
+    """Checks a cache in 4 bits; returns its page size."""
+    shape, row = cache.shape, head_dim // 32 * _KV4_GROUP
+    if head_dim <= 0 or head_dim % 32 or head_dim > 256:
+        raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, f"{what}: heads of {head_dim} are not supported (multiples of 32 up to 256)")
+    if cache.dtype is not torch.uint8 or len(shape) != 3 or shape[1] != n_kv or shape[2] == 0 or shape[2] % row or not cache.is_contiguous():
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: a cache in 4 bits must be contiguous uint8 [pages, n_kv, kv4_page_bytes(page_size, head_dim)]")
+    if cache.data_ptr() % 16:
+        raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"{what}: a cache in 4 bits must begin on a 16-byte boundary")
+    page_size = shape[2] // row
+    kv4_page_bytes(page_size, head_dim)
+    return page_size
+
+
+#: photon_kv4_write_call, photon_kv4_unpack_call, photon_kv4_attention_call, photon_key_weights_call, photon_evict_call
+_KV4_WRITE_CALL = struct.Struct("6q2q6i")
+_KV4_UNPACK_CALL = struct.Struct("11q1q9i4x")
+_KV4_ATTENTION_CALL = struct.Struct("11q2q13i2f4x")
+_KEY_WEIGHTS_CALL = struct.Struct("11q1q13i2f4x")
+_EVICT_CALL = struct.Struct("7q12i")
+
+
+def _data(t: Optional[torch.Tensor]) -> int:
+    return 0 if t is None else t.data_ptr()
+
+
+def kv4_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, n_kv: int, head_dim: int,
+              err: Optional[torch.Tensor]) -> None:
+    """Rows of ``k`` and ``v [T, n_kv * head_dim]`` (views with any row stride) are rounded to 4 bits and stored at ``slot_mapping [T]`` (page * page_size + place; -1: nowhere; no slot
+    twice) in a paged cache in 4 bits (``kv4_page_bytes``).  A group of 32 numbers gets the scale nearest to its largest magnitude / 7 and each number the nearest multiple of
+    it, halves the even one; magnitudes above 430,080 are held as that, a group with a number that is not finite reads as NaN."""
+    _on_device("kv4_write", k, v, slot_mapping, k_cache, v_cache, err)
+    page_size = _kv4_cache("kv4_write", k_cache, n_kv, head_dim)
+    T = slot_mapping.numel()
+    for name, t in (("k", k), ("v", v)):
+        if t.shape != (T, n_kv * head_dim) or (t.stride(1) != 1 and T) or t.dtype != k.dtype:
+            raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"kv4_write: {name} must be [T, {n_kv} * {head_dim}] with contiguous heads, of one type")
+    _int32(slot_mapping, "slot_mapping")
+    if v_cache.shape != k_cache.shape:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_write: the caches must have one shape")
+    _kv4_cache("kv4_write", v_cache, n_kv, head_dim)
+    call = _KV4_WRITE_CALL.pack(k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _data(err), k.stride(0), v.stride(0),
+                                _dtype_code(k), T, n_kv, head_dim, page_size, k_cache.shape[0])
+    _check(_plain_fn("kv4", "photon_kv4_write", _CALL_ARGS)(call, _stream()), "kv4_write")
+
+
+def kv4_unpack(k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor, k_out: torch.Tensor, v_out: torch.Tensor, err: Optional[torch.Tensor]) -> None:
+    """Pages ``pages [N]`` of a cache in 4 bits as numbers: ``k_out`` and ``v_out [N, n_kv, page_size, head_dim]`` in bfloat16 (which holds them exactly) or float32.
+    A page outside the pool is left out and recorded in ``err``."""
+    _on_device("kv4_unpack", k_cache, v_cache, pages, k_out, v_out, err)
+    _int32(pages, "pages")
+    shape = k_out.shape
+    if len(shape) != 4 or shape[0] != pages.numel() or v_out.shape != shape or v_out.dtype != k_out.dtype or not k_out.is_contiguous() or not v_out.is_contiguous():
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_unpack: the outputs must be contiguous [pages, n_kv, page_size, head_dim], of one type")
+    N, n_kv, page_size, head_dim = shape
+    if _kv4_cache("kv4_unpack", k_cache, n_kv, head_dim) != page_size or v_cache.shape != k_cache.shape:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_unpack: the outputs' pages must be those of the caches")
+    _kv4_cache("kv4_unpack", v_cache, n_kv, head_dim)
+    call = _KV4_UNPACK_CALL.pack(k_cache.data_ptr(), v_cache.data_ptr(), pages.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), 0, 0, 0, 0, 0, _data(err), N,
+                                 _dtype_code(k_out), 1, N, n_kv, head_dim, page_size, k_cache.shape[0], 1, 0)
+    _check(_plain_fn("kv4", "photon_kv4_unpack", _CALL_ARGS)(call, _stream()), "kv4_unpack")
+
+
+def _rows_view(what: str, q: torch.Tensor, n_q: int, head_dim: int) -> None:
+    if q.dim() != 2 or q.shape[1] != n_q * head_dim or (q.stride(1) != 1 and q.numel()):
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: the rows must be [T, n_q * head_dim], each contiguous")
+
+
+def _check_heads(what: str, n_q: int, n_kv: int, scale: float, softcap: Optional[float], window: Optional[int]) -> None:
+    if n_kv <= 0 or n_q <= 0 or n_q % n_kv:
+        raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, f"{what}: {n_q}/{n_kv} heads are not supported")
+    if not scale > 0 or (softcap is not None and not softcap >= 0) or (window is not None and window < 0):
+        raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"{what}: the scale must be positive, softcap and window not negative")
+
+
+def _check_lse(what: str, lse: Optional[torch.Tensor], T: int, n_q: int) -> None:
+    if lse is not None and (lse.dtype != torch.float32 or lse.shape != (T, n_q) or not lse.is_contiguous()):
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: lse must be contiguous float32 [T, n_q]")
+
+
+#: Rows (tokens x query heads per key/value head) up to which ``attention_tc`` leaves a request to other kernels.
+KV4_FEW_ROWS = 16
+#: Bytes of a prompt portion's keys and values in bfloat16 that are laid out at a time.
+KV4_PROMPT_BYTES = 2 << 30
+
+
+def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Tensor,
+                  context_lens: torch.Tensor, num_seqs: int, max_tokens_per_seq: int, max_keys: int, n_q: int, n_kv: int, head_dim: int, window: Optional[int],
+                  scale: float, err: Optional[torch.Tensor], sink: Optional[torch.Tensor] = None, softcap: Optional[float] = None,
+                  lse: Optional[torch.Tensor] = None) -> None:
+    """Causal attention over a paged cache in 4 bits (``kv4_page_bytes``).  The tokens ``cu_tokens[s] .. cu_tokens[s + 1]`` of the step (at most ``max_tokens_per_seq``) are the last
+    of request ``s``'s ``context_lens[s]`` keys (at most ``max_keys``); the token at place ``p`` sees keys ``max(0, p - window + 1) .. p``: places in the cache, which are a
+    token's position as long as none has left it.  A row that sees nothing is zero.  ``q`` and ``out [T, n_q * d]`` may be views with a row stride; ``sink``, ``softcap``: as in
+    ``paged_attention``.  ``lse`` (float32 ``[T, n_q]``): gets the logarithm of the sum of each row's exponentials (the sink's among them; -inf where there is nothing), which
+    ``key_weights`` takes.  A query that is not finite makes its row NaN."""
+    _on_device("kv4_attention", q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, sink, lse, err)
+    if sink is not None:
+        _check_sink(sink, n_q)
+    _check_heads("kv4_attention", n_q, n_kv, scale, softcap, window)
+    _rows_view("kv4_attention", q, n_q, head_dim)
+    _rows_view("kv4_attention", out, n_q, head_dim)
+    T, width = q.shape
+    if out.shape[0] != T or out.dtype != q.dtype:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_attention: q and out must have one shape and type")
+    if T > 1 and out.stride(0) < width:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_attention: rows of out must not overlap")
+    page_size = _kv4_cache("kv4_attention", k_cache, n_kv, head_dim)
+    if v_cache.shape != k_cache.shape:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_attention: the caches must have one shape")
+    _kv4_cache("kv4_attention", v_cache, n_kv, head_dim)
+    _int32s("cu_tokens context_lens block_table", cu_tokens, context_lens, block_table)
+    pages = _check_step("kv4_attention", num_seqs, cu_tokens, context_lens, block_table)
+    _check_lse("kv4_attention", lse, T, n_q)
+    if T == 0 or num_seqs == 0 or max_tokens_per_seq <= 0 or max_keys <= 0:
+        return
+    group, window = n_q // n_kv, min(window or 0, 0x7fffffff)
+    most = max_tokens_per_seq * group                   # rows of a request
+    if most > KV4_FEW_ROWS and lse is None and attention_tc_supported(q.dtype, head_dim, group, page_size):
+        _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, num_seqs, max_tokens_per_seq, max_keys, n_q, n_kv, head_dim, page_size, window,
+                    scale, err, sink, softcap)
+        most = KV4_FEW_ROWS
+    tokens = -(-most // group)
+    keys = min(max_keys, window + tokens) if window else max_keys
+    tiles, blocks = -(-keys // 128), num_seqs * n_kv * -(-tokens * group // 8)
+    parts = max(1, min(tiles, 4 * sm_count(q.device) // blocks, 64))
+    scratch = torch.empty(T * n_q * parts * (head_dim + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
+    call = _KV4_ATTENTION_CALL.pack(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(),
+                                    _data(sink), _data(lse), _data(scratch), _data(err), q.stride(0), out.stride(0), _dtype_code(q), pages, num_seqs, tokens, n_q, n_kv,
+                                    head_dim, page_size, k_cache.shape[0], window, parts, 0, most, scale, softcap or 0.0)
+    _check(_plain_fn("kv4_attention", "photon_kv4_attention", _CALL_ARGS)(call, _stream()), "kv4_attention")
+    if parts > 1:
+        _count_launches(1)
+
+
+_KV4_SPOIL_ARGS = [c_char_p, c_void_p, c_long, c_int, c_void_p]
+
+
+def _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, num_seqs, max_tokens, max_keys, n_q, n_kv, head_dim, page_size, window, scale, err,
+                sink, softcap) -> None:
+    """The requests with more than ``KV4_FEW_ROWS`` rows: their pages are laid out in bfloat16, which holds them exactly, and the tcgen05 kernel attends to them.  Their
+    products are many times the bytes: 2,048 tokens of 32/8 heads of 128 behind 4,096 keys are 86 GFLOP and 25 MB laid out."""
+    per = min(-(-max_keys // page_size), block_table.shape[1])
+    device, (T, width) = q.device, q.shape
+    if q.stride(0) < width or q.stride(0) % 8 or q.data_ptr() % 16:
+        q = q.contiguous()
+    into = out if out.is_contiguous() and out.data_ptr() % 16 == 0 else out.contiguous()
+    if into.data_ptr() % 16:
+        into = into.clone(memory_format=torch.contiguous_format)
+    one = per * n_kv * page_size * head_dim * 4
+    some = max(1, min(num_seqs, KV4_PROMPT_BYTES // one, 65535 // -(-max_tokens // (128 // (n_q // n_kv)))))
+    numbers = torch.empty((2, some * per, n_kv, page_size, head_dim), dtype=q.dtype, device=device)
+    parts = -(-2 * n_kv * page_size * head_dim // 2048)
+    where = torch.empty(some * per * (1 + parts) + T, dtype=torch.int32, device=device)
+    table, flags, positions = where[:some * per].view(some, per), where[some * per:some * per * (1 + parts)], where[some * per * (1 + parts):]
+    for s0 in range(0, num_seqs, some):
+        n = min(some, num_seqs - s0)
+        cu, lens = cu_tokens[s0:s0 + n + 1], context_lens[s0:s0 + n]
+        call = _KV4_UNPACK_CALL.pack(k_cache.data_ptr(), v_cache.data_ptr(), block_table[s0:].data_ptr(), numbers[0].data_ptr(), numbers[1].data_ptr(), cu.data_ptr(),
+                                     lens.data_ptr(), table.data_ptr(), positions.data_ptr(), flags.data_ptr(), _data(err), block_table.shape[1], _dtype_code(q), n, per, n_kv, head_dim,
+                                     page_size, k_cache.shape[0], n_q // n_kv, KV4_FEW_ROWS)
+        _check(_plain_fn("kv4", "photon_kv4_unpack", _CALL_ARGS)(call, _stream()), "kv4_attention")
+        attention_tc(q, into, numbers[0], numbers[1], table[:n], cu, positions, n, max_tokens, n_q, n_kv, head_dim, window, scale, err, sink=sink, softcap=softcap,
+                     keys=max_keys)
+        _check(_plain_fn("kv4", "photon_kv4_spoil", _KV4_SPOIL_ARGS)(call, into.data_ptr(), into.stride(0), window, _stream()), "kv4_attention")
+    if into is not out:
+        out.copy_(into)
+
+
+def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, block_table: torch.Tensor, cu_tokens: torch.Tensor, context_lens: torch.Tensor,
+                num_seqs: int, max_tokens_per_seq: int, max_keys: int, n_q: int, n_kv: int, head_dim: int, window: Optional[int], scale: float,
+                err: Optional[torch.Tensor], held: Optional[torch.Tensor] = None, sink: Optional[torch.Tensor] = None, softcap: Optional[float] = None,
+                lse: Optional[torch.Tensor] = None) -> None:
+    """What every cached key got of the softmax of the given queries, added to ``weights`` (float32 ``[pages, n_kv, page_size]``, beside the keys): key ``j`` of a request
+    gets, for its key/value head, the sum over the request's rows of ``exp(score - lse)``.  Tokens, keys, masks, ``sink`` and ``softcap`` as in ``kv4_attention``; the
+    queries may be a step's, or the last ones of a prompt (``cu_tokens`` then counts those).  Keys from ``held[s]`` (int32) on have no sum yet and get this one; without
+    ``held`` those are the given tokens' own keys.  ``k_cache``: a plain one of the type of ``q`` (``[pages, n_kv, page_size, d]``, ``d`` a multiple of 8 up to 256) or one in 4 bits.
+    ``lse``: as ``kv4_attention`` leaves it for the same queries; without it the keys are read twice."""
+    _on_device("key_weights", q, weights, k_cache, block_table, cu_tokens, context_lens, held, sink, lse, err)
+    if sink is not None:
+        _check_sink(sink, n_q)
+    _check_heads("key_weights", n_q, n_kv, scale, softcap, window)
+    _rows_view("key_weights", q, n_q, head_dim)
+    T, packed = q.shape[0], k_cache.dtype is torch.uint8
+    if packed:
+        page_size = _kv4_cache("key_weights", k_cache, n_kv, head_dim)
+    else:
+        if head_dim % 8 or not 0 < head_dim <= 256:
+            raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, f"key_weights: heads of {head_dim} are not supported (multiples of 8 up to 256)")
+        if k_cache.dim() != 4 or k_cache.shape[1] != n_kv or k_cache.shape[3] != head_dim or k_cache.dtype != q.dtype or not k_cache.is_contiguous() \
+                or k_cache.data_ptr() % 16:
+            raise PhotonError(ErrorCode.SHAPE_MISMATCH, "key_weights: the cache must be contiguous [pages, n_kv, page_size, head_dim] of the type of q, on a 16-byte boundary")
+        page_size = k_cache.shape[2]
+    if weights.dtype != torch.float32 or weights.shape != (k_cache.shape[0], n_kv, page_size) or not weights.is_contiguous():
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "key_weights: weights must be contiguous float32 [pages, n_kv, page_size]")
+    _int32s("cu_tokens context_lens block_table", cu_tokens, context_lens, block_table)
+    pages = _check_step("key_weights", num_seqs, cu_tokens, context_lens, block_table)
+    if held is not None:
+        _int32(held, "held")
+        if held.numel() < num_seqs:
+            raise PhotonError(ErrorCode.SHAPE_MISMATCH, "key_weights: held must cover every request")
+    _check_lse("key_weights", lse, T, n_q)
+    if num_seqs == 0 or max_keys <= 0:
+        return
+    tiles = -(-max_keys // 128)
+    parts = max(1, min(tiles, 8 * sm_count(q.device) // (num_seqs * n_kv)))
+    scratch = torch.empty(max(T, 1) * n_q * parts * 2, dtype=torch.float32, device=q.device) if lse is None else None
+    call = _KEY_WEIGHTS_CALL.pack(q.data_ptr(), weights.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), _data(held),
+                                  _data(sink), _data(lse), _data(scratch), _data(err), q.stride(0), _dtype_code(q), int(packed), pages, num_seqs, max_keys, n_q, n_kv, head_dim,
+                                  page_size, k_cache.shape[0], min(window or 0, 0x7fffffff), parts, max_tokens_per_seq, scale, softcap or 0.0)
+    _check(_plain_fn("key_weights", "photon_key_weights", _CALL_ARGS)(call, _stream()), "key_weights")
+    if lse is None:
+        _count_launches(1)
+
+
+def cache_evict(kv: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor, num_seqs: int,
+                max_keys: int, keep: int, keep_first: int, keep_last: int, err: Optional[torch.Tensor], kept: Optional[torch.Tensor] = None) -> None:
+    """Requests with more than ``keep`` of at most ``max_keys`` cached tokens fall back to ``keep``: in every entry and key/value head of a cache group's pools the first ``keep_first``
+    tokens stay, the last ``keep_last``, and of the others those with the largest ``weights`` (of equal ones the earlier; a NaN counts as the largest), and
+    move to the front of the request's pages in their order; where ``keep`` is too small for that, the first ones come before the last ones.  ``kv``: ``[entries, planes, pages, n_kv,
+    page_size, d]``, or uint8 ``[entries, planes, pages, n_kv, kv4_page_bytes]`` in 4 bits; ``weights`` (float32 ``[entries, pages, n_kv, page_size]``, as ``key_weights``
+    leaves them) move along.  ``new_lens [S]``: the tokens that are left; what lies behind them stays as it was.  ``kept`` (int32 ``[entries, S, n_kv, keep]``): gets the old places
+    of the rows of requests that lose some.  Heads keep different tokens, so a request's later tokens take their positions from its text and their slots from the cache."""
+    _on_device("cache_evict", kv, weights, block_table, context_lens, new_lens, kept, err)
+    shape, wanted = kv.shape, weights.shape
+    if weights.dtype != torch.float32 or len(wanted) != 4 or not weights.is_contiguous() or weights.numel() == 0:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_evict: weights must be contiguous float32 [entries, pages, n_kv, page_size]")
+    entries, pages, n_kv, page_size = wanted
+    packed = kv.dtype is torch.uint8
+    if len(shape) != (5 if packed else 6) or shape[0] != entries or tuple(shape[2:4]) != (pages, n_kv) or shape[1] < 1 or not kv.is_contiguous():
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_evict: kv must be contiguous [entries, planes, pages, n_kv, page_size, d], in 4 bits [entries, planes, pages, n_kv, "
+                          "kv4_page_bytes], beside weights [entries, pages, n_kv, page_size]")
+    if packed:
+        row = shape[4] // page_size
+        head_dim = row // _KV4_GROUP * 32
+        if not kv4_supported(page_size, head_dim) or shape[4] != kv4_page_bytes(page_size, head_dim):
+            raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"cache_evict: {shape[4]} bytes are no page of {page_size} tokens in 4 bits")
+        row_bytes, scale_bytes = head_dim // 2, head_dim // 32
+    else:
+        if shape[4] != page_size:
+            raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_evict: the pages of kv and weights differ")
+        _dtype_code(kv)
+        row_bytes, scale_bytes = shape[5] * kv.element_size(), 0
+    if row_bytes % 16 or row_bytes > 4096 or kv.data_ptr() % 16:
+        raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, "cache_evict: rows must be pieces of 16 bytes, up to 4,096")
+    _int32s("context_lens block_table new_lens", context_lens, block_table, new_lens)
+    table = block_table.shape
+    if len(table) != 2 or num_seqs < 0 or table[0] < num_seqs or context_lens.numel() < num_seqs or new_lens.numel() < num_seqs or table[0] * table[1] < 1:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_evict: block_table, context_lens and new_lens must cover every request")
+    if keep < 0 or keep_first < 0 or keep_last < 0:
+        raise PhotonError(ErrorCode.INVALID_ARGUMENT, "cache_evict: keep, keep_first and keep_last must not be negative")
+    if num_seqs and new_lens.data_ptr() < context_lens.data_ptr() + 4 * num_seqs and context_lens.data_ptr() < new_lens.data_ptr() + 4 * num_seqs:
+        raise PhotonError(ErrorCode.INVALID_ARGUMENT, "cache_evict: new_lens must be another tensor than context_lens, which is read while it is written")
+    if kept is None:
+        kept = torch.empty(entries * num_seqs * n_kv * keep, dtype=torch.int32, device=kv.device)
+    else:
+        _int32(kept, "kept")
+        if kept.shape != (entries, num_seqs, n_kv, keep):
+            raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_evict: kept must be [entries, requests, n_kv, keep]")
+    call = _EVICT_CALL.pack(kv.data_ptr(), weights.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), _data(err), entries,
+                            shape[1], pages, n_kv, page_size, table[1], num_seqs, keep, keep_first, keep_last, row_bytes, scale_bytes)
+    _check(_plain_fn("cache_evict", "photon_cache_evict", _CALL_ARGS)(call, _stream()), "cache_evict")
+    if keep:
+        _count_launches(1)
+
+
 # ----------------------------------------------------------------------------- sampling
 
 def sample(logits: torch.Tensor, temperature: Optional[torch.Tensor], u: Optional[torch.Tensor],
