@@ -1,0 +1,602 @@
+// Attention of decoded tokens over a paged cache in 4 bits (the format: kv4.cuh): bfloat16, heads of 64 or 128 numbers, few rows (tokens x query heads of a key/value
+// head) a request.
+//
+// The codes go to the tensor cores as they are: a code c under a mask is the 16-bit float c 2^-24 where its nibble is the lowest of its half, c 2^-20 where it is the
+// second (both below the normal numbers, and exact), so two shifts and ANDs make two numbers of an operand.  With K as the first operand (16 keys) and the queries as the
+// second (8 rows, each scaled by a power of two to 16-bit floats, the numbers beside the second nibbles by 1/16 more):
+//   score[key][row] = factor[row] sum over groups  scale[key][group] (sum over the group  c q  -  8 sum over the group  q),
+// the last sum being what the product's result begins with.  The weights, as 16-bit floats, are turned over in registers and multiplied by the values' scales:
+//   out[number][row] = sum over keys  c (p scale)[key][group(number)][row]  -  8 sum over keys (p scale)[key][group][row],
+// where the last sum of each group is one more product, with ones in one row of the first operand.  Weights are lifted by 2^15 and scales by a power of two for each group
+// that keeps the largest product below 65,504, so that small values beside few large weights keep their bits; sums and the softmax are in 32 bits.
+//
+// Every warp walks keys of its own, 32 at a time, straight from the cache into registers, the next keys' codes asked for as soon as these are in the operands.  All
+// blocks have equal runs of the requests' tiles of 128 keys; results of a unit (request, head, 8 or 16 rows) that lies in one block are written, others are joined by a
+// second kernel in ascending order.
+#include "kv4.cuh"
+#include <math.h>
+
+#define KM_THREADS 128
+#define KM_KEYS 128              // of a block's step, 32 a warp
+#define KM_MAX_SEQS 1024
+
+struct Kv4MmaArgs {
+  const bf16* q; bf16* out; const uint8_t* k; const uint8_t* v;
+  const int* table; const int* cu_tokens; const int* context_lens; const float* sinks; float* lse; float* scratch; int* err;
+  long q_stride, out_stride;
+  int max_pages, S, n_q, n_kv, page_size, num_pages, window;
+  float scale, softcap;
+  int min_rows, max_rows;
+};
+
+__device__ __forceinline__ void km_mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+               : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+               : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
+}
+__device__ __forceinline__ uint32_t km_turn(uint32_t x) {      // an 8 x 8 matrix of 16-bit numbers, rows for columns
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+__device__ __forceinline__ float km_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t km_half2(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *(const uint32_t*)&h;
+}
+__device__ __forceinline__ uint32_t km_mul2(uint32_t a, uint32_t b) {
+  const __half2 h = __hmul2(*(const __half2*)&a, *(const __half2*)&b);
+  return *(const uint32_t*)&h;
+}
+template <int WORDS>
+__device__ __forceinline__ void km_load(uint32_t* x, const uint8_t* p) {      // read once: not kept in the first cache
+  if constexpr (WORDS == 4) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "l"(p));
+  else if constexpr (WORDS == 2) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "l"(p));
+  else asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(x[0]) : "l"(p));
+}
+__device__ __forceinline__ uint32_t km_load16(const uint8_t* p) {
+  uint16_t x;
+  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(x) : "l"(p));
+  return x;
+}
+
+// A request's place in the work: rows, row tiles, keys from..to (from a multiple of 8), steps of 128 keys.
+struct KmRequest { int first, n, ctx, rows, row_tiles, from, steps; };
+template <int RT>
+__device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
+  KmRequest r;
+  r.first = a.cu_tokens[s];
+  r.n = a.cu_tokens[s + 1] - r.first;
+  r.ctx = a.context_lens[s];
+  r.rows = r.n * (a.n_q / a.n_kv);
+  if (r.rows <= a.min_rows || r.rows > a.max_rows) r.rows = 0;
+  r.row_tiles = (r.rows + RT - 1) / RT;
+  const int lo = a.window > 0 ? max(0, r.ctx - r.n - a.window + 1) : 0;
+  r.from = lo & ~7;
+  r.steps = r.rows > 0 ? max(1, (r.ctx - r.from + KM_KEYS - 1) / KM_KEYS) : 0;
+  return r;
+}
+
+// GROUPS: of 32 numbers of a head (2 or 4); NT: tiles of 8 rows.
+template <int GROUPS, int NT>
+__global__ void __launch_bounds__(KM_THREADS, NT == 1 ? 3 : 2)
+kv4_mma_kernel(const Kv4MmaArgs a) {
+  constexpr int D = GROUPS * 32, RT = 8 * NT, KW = GROUPS, VW = GROUPS / 2;      // words of a key's and of a value's piece
+  extern __shared__ __align__(16) float smem[];
+  float* o_s = smem;                                  // [4][RT][D]
+  float* m_s = o_s + 4 * RT * D;                      // [4][RT]
+  float* l_s = m_s + 4 * RT;
+  int* before_s = (int*)(l_s + 4 * RT);               // [S + 1] units' steps in front of a request
+  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  pdl_wait();
+  if (warp == 0) {
+    int sum = 0;
+    for (int s0 = 0; s0 < a.S; s0 += 32) {
+      int x = 0;
+      if (s0 + lane < a.S) { const KmRequest r = km_request<RT>(a, s0 + lane); x = r.steps * r.row_tiles * a.n_kv; }
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      if (s0 + lane < a.S) before_s[s0 + lane + 1] = sum + x;
+      sum += __shfl_sync(0xffffffffu, x, 31);
+    }
+    if (lane == 0) before_s[0] = 0;
+  }
+  __syncthreads();
+  const int total = before_s[a.S], N = gridDim.x;
+  const int begin = (int)((long)total * blockIdx.x / N), end = (int)((long)total * (blockIdx.x + 1) / N);
+  if (begin >= end) return;
+  int s = 0;
+  {                                                   // the request of the first step: the last one that begins at or before it and is not empty
+    int lo = 0, hi = a.S;
+    while (hi - lo > 1) { const int mid = (lo + hi) >> 1; if (before_s[mid] <= begin) lo = mid; else hi = mid; }
+    s = lo;
+  }
+  const int G = a.n_q / a.n_kv;
+  const long page_bytes = (long)a.page_size * GROUPS * 17;
+  for (int pos = begin; pos < end;) {
+    while (before_s[s + 1] <= pos) ++s;
+    const KmRequest R = km_request<RT>(a, s);
+    const int at = pos - before_s[s], unit = at / R.steps, step0 = at - unit * R.steps, step1 = min(R.steps, step0 + end - pos);
+    const int head = unit / R.row_tiles, row0 = (unit - head * R.row_tiles) * RT, rows = min(RT, R.rows - row0), base = R.ctx - R.n;
+    // ---- the queries
+    uint32_t qb[NT][GROUPS][4];
+    float init[NT][GROUPS][2], factor[NT][2];
+    int place[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const int row = row0 + 8 * x + g;
+      const bool there = 8 * x + g < rows;
+      const bf16* q = a.q + (there ? (R.first + row / G) * a.q_stride + (long)(head * G + row % G) * D : 0);
+      float v[GROUPS][8];
+      uint32_t top = 0;
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          v[j][i] = there ? __bfloat162float(q[32 * j + 8 * t + i]) : 0.f;
+          top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
+        }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const bool odd = top >= 0x7f800000u;
+      const int e = top == 0 || odd ? 0 : ilogbf(__uint_as_float(top));
+      const float f = ldexpf(a.scale * (a.softcap > 0.f ? 1.f : 1.4426950408889634f), e - 14 + 24);
+      float sums[GROUPS];
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        float w[8];
+        sums[j] = 0.f;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {                 // the odd ones meet the second nibbles, which are 16 times as large
+          const float y = odd ? __int_as_float(0x7fc00000) : ldexpf(v[j][i], 14 - e - (i & 1) * 4);
+          w[i] = __half2float(__float2half_rn(y));
+          sums[j] += i & 1 ? 16.f * w[i] : w[i];
+        }
+        qb[x][j][0] = km_half2(w[0], w[4]);
+        qb[x][j][1] = km_half2(w[1], w[5]);
+        qb[x][j][2] = km_half2(w[2], w[6]);
+        qb[x][j][3] = km_half2(w[3], w[7]);
+        sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 1);
+        sums[j] += __shfl_xor_sync(0xffffffffu, sums[j], 2);
+        sums[j] *= -8.f / 16777216.f;
+#pragma unroll
+        for (int c = 0; c < 2; ++c) init[x][j][c] = __shfl_sync(0xffffffffu, sums[j], (2 * t + c) * 4);
+      }
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        factor[x][c] = __shfl_sync(0xffffffffu, f, (2 * t + c) * 4);
+        const int r = 8 * x + 2 * t + c;
+        place[x][c] = r < rows ? base + (row0 + r) / G : -1;
+      }
+    }
+    const int first_place = base + row0 / G, last_place = base + (row0 + rows - 1) / G;
+    const int clear_from = a.window > 0 ? last_place - a.window + 1 : 0, clear_to = first_place;      // keys that all rows see
+    const int low = a.window > 0 ? max(0, first_place - a.window + 1) : 0;
+    float acc[NT][GROUPS][2][4], ones[NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) { m[x][c] = -INFINITY; l[x][c] = 0.f; }
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        ones[x][i] = 0.f;
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) acc[x][j][0][i] = acc[x][j][1][i] = 0.f;
+      }
+    }
+    uint32_t bad[NT] = {};                            // bit j: row 8 x + g sees a value of group j that is no number
+    uint32_t seen_scales = 0;                         // all the values' scales below 2 so far, or-ed
+    int lift[GROUPS], tops[GROUPS];                   // powers of two; the largest scale from 2 on
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) lift[j] = tops[j] = 0;
+
+    // ---- where the keys are: lane 4 i + o has the 8 keys o of the warp's 32 of step i, 8 steps at a time
+    const int key_w = R.from + warp * 32;
+    uint32_t off16 = 0, off16_next = 0, ok = 0, ok_next = 0;
+    int slot = 0, slot_next = 0;
+    auto find = [&](int step, uint32_t& off, int& sl, uint32_t& mask) {
+      const int i = step + (lane >> 2), key = key_w + i * KM_KEYS + (lane & 3) * 8;
+      const int pidx = key / a.page_size;
+      int page = -1;
+      sl = key - pidx * a.page_size;
+      if (i < step1 && key <= last_place) {
+        page = pidx < a.max_pages ? a.table[(long)s * a.max_pages + pidx] : -1;
+        if (page < 0 || page >= a.num_pages) { report_error(a.err, PHOTON_DEV_BAD_PAGE, s, key, page); page = -1; }
+      }
+      const bool good = page >= 0;
+      off = good ? (uint32_t)((((long)page * a.n_kv + head) * page_bytes + (long)sl * (D / 2)) >> 4) : 0u;
+      if (!good) sl = 0;
+      mask = __ballot_sync(0xffffffffu, good);
+    };
+    find(step0, off16, slot, ok);
+    uint32_t kw[4][KW], vw[4][2][VW], ks[4], vs[4][2];
+    auto load_k = [&](int i) {                         // i: the step's place among the 8 that are known
+#pragma unroll
+      for (int o = 0; o < 4; ++o) {
+        const uint8_t* p = a.k + ((unsigned long long)__shfl_sync(0xffffffffu, off16, 4 * i + o) << 4);
+        const int sl = __shfl_sync(0xffffffffu, slot, 4 * i + o);
+        km_load<KW>(kw[o], p + g * (D / 2) + 4 * GROUPS * t);
+        const uint8_t* sc = p + (a.page_size - sl) * (D / 2) + (sl + g) * GROUPS;
+        if constexpr (GROUPS == 4) km_load<1>(&ks[o], sc); else ks[o] = km_load16(sc);
+      }
+    };
+    auto load_v = [&](int i) {
+#pragma unroll
+      for (int o = 0; o < 4; ++o) {
+        const uint8_t* p = a.v + ((unsigned long long)__shfl_sync(0xffffffffu, off16, 4 * i + o) << 4);
+        const int sl = __shfl_sync(0xffffffffu, slot, 4 * i + o);
+        km_load<VW>(vw[o][0], p + (2 * t) * (D / 2) + 2 * GROUPS * g);
+        km_load<VW>(vw[o][1], p + (2 * t + 1) * (D / 2) + 2 * GROUPS * g);
+        const uint8_t* sc = p + (a.page_size - sl) * (D / 2) + (sl + 2 * t) * GROUPS;
+        if constexpr (GROUPS == 4) km_load<2>(vs[o], sc);
+        else { uint32_t both; km_load<1>(&both, sc); vs[o][0] = both & 0xffffu; vs[o][1] = both >> 16; }
+      }
+    };
+    load_k(0);
+    load_v(0);
+    for (int step = step0; step < step1; ++step) {
+      const int i8 = (step - step0) & 7;
+      const uint32_t here = ok >> (4 * i8) & 15u;
+      if (i8 == 0) find(step + 8, off16_next, slot_next, ok_next);
+      const int key0 = key_w + step * KM_KEYS;
+      // ---- scores
+      float sc[NT][2][4];
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) sc[x][0][i] = sc[x][1][i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int jj = 0; jj < GROUPS; jj += 2) {
+          // two groups' scales of the keys g and 8 + g of this half
+          uint32_t h0 = __byte_perm(ks[2 * i], 0, jj ? 0x3424 : 0x1404) >> 1, h1 = __byte_perm(ks[2 * i + 1], 0, jj ? 0x3424 : 0x1404) >> 1;
+          const float2 s0 = __half22float2(*(const __half2*)&h0), s1 = __half22float2(*(const __half2*)&h1);
+#pragma unroll
+          for (int jx = 0; jx < 2; ++jx) {
+            const int j = jj + jx;
+            const uint32_t w0 = kw[2 * i][j], w1 = kw[2 * i + 1][j], u0 = w0 >> 8, u1 = w1 >> 8;
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+              float d[4];
+              km_mma(d, w0 & 0x000F000Fu, w1 & 0x000F000Fu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qb[x][j][0], qb[x][j][1], init[x][j][0], init[x][j][1], init[x][j][0],
+                     init[x][j][1]);
+              km_mma(d, u0 & 0x000F000Fu, u1 & 0x000F000Fu, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qb[x][j][2], qb[x][j][3], d[0], d[1], d[2], d[3]);
+              const float a0 = jx ? s0.y : s0.x, a1 = jx ? s1.y : s1.x;
+              sc[x][i][0] += a0 * d[0];
+              sc[x][i][1] += a0 * d[1];
+              sc[x][i][2] += a1 * d[2];
+              sc[x][i][3] += a1 * d[3];
+            }
+          }
+        }
+      }
+      const bool more = step + 1 < step1;
+      const bool turn = i8 == 7;
+      if (more) {
+        if (turn) { off16 = off16_next; slot = slot_next; }
+        load_k((i8 + 1) & 7);
+      }
+      // ---- the softmax
+      const bool masked = here != 15u || key0 < clear_from || key0 + 31 > clear_to;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            sc[x][i][c] *= factor[x][c & 1];
+            if (a.softcap > 0.f) {                     // tanh y = 1 - 2 / (1 + e^2y)
+              const float y = km_exp2(sc[x][i][c] * (2.f * 1.4426950408889634f / a.softcap));
+              sc[x][i][c] = a.softcap * 1.4426950408889634f * (1.f - __fdividef(2.f, 1.f + y));
+            }
+          }
+      uint32_t hidden = 0;                             // bit (8 x + 4 i + c): this thread's score is no key of its row
+      if (masked) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int key = key0 + 16 * i + 8 * (c >> 1) + g, at_place = place[x][c & 1];
+              const bool sees = (here >> (2 * i + (c >> 1)) & 1u) && key <= at_place && (a.window <= 0 || key > at_place - a.window);
+              if (!sees) { sc[x][i][c] = -INFINITY; hidden |= 1u << (8 * x + 4 * i + c); }
+            }
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int key = key0 + 8 * o + 2 * t + b;
+            if (!(here >> o & 1u) || key > last_place || key < low) vs[o][b] = 0;      // whatever lies there
+          }
+      }
+      float alpha[NT][2], ref[NT][2];
+      bool grown = false;
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          float top = fmaxf(fmaxf(sc[x][0][c], sc[x][0][c + 2]), fmaxf(sc[x][1][c], sc[x][1][c + 2]));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+          top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          top = fmaxf(top, m[x][c]);
+          alpha[x][c] = m[x][c] == -INFINITY ? 1.f : km_exp2(m[x][c] - top);
+          grown |= top > m[x][c];
+          m[x][c] = top;
+          ref[x][c] = top == -INFINITY ? 0.f : top - 15.f;
+        }
+      // The largest product has to stay below 65,504 and small values should not lose bits: a group whose scales so far are below 2 and not below 2^-7 stays as it is.  Scales
+      // from 2 on are looked at one by one; a NaN among them lifts nothing.
+      uint32_t all = __reduce_or_sync(0xffffffffu, (vs[0][0] | vs[0][1] | vs[1][0]) | (vs[1][1] | vs[2][0] | vs[2][1]) | (vs[3][0] | vs[3][1]));
+      bool odd_scales = false, new_tops = false;
+      if (all & 0x80808080u) {
+        uint32_t low = 0;
+        int big[GROUPS];
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) big[j] = 0;
+#pragma unroll
+        for (int w = 0; w < 8; ++w)
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) {
+            const int byte = vs[w >> 1][w & 1] >> (8 * j) & 255;
+            if (byte < 128) low |= (uint32_t)byte << (8 * j);
+            else if (byte < 248) big[j] = max(big[j], byte);
+            else odd_scales = true;
+          }
+        odd_scales = __any_sync(0xffffffffu, odd_scales);
+        all = __reduce_or_sync(0xffffffffu, low);
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) {
+          const int most = __reduce_max_sync(0xffffffffu, big[j]);
+          if (most > tops[j]) { tops[j] = most; new_tops = true; }
+        }
+      }
+      if ((all & ~seen_scales) || new_tops) {
+        seen_scales |= all;
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) {
+          const int e = tops[j] > 0 ? tops[j] >> 3 : seen_scales >> (8 * j + 3) & 15, to = e > 15 || e < 8 ? 15 - e : 0;
+          if (to != lift[j]) {
+            const float f = ldexpf(1.f, to - lift[j]);
+            lift[j] = to;
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+#pragma unroll
+              for (int i = 0; i < 4; ++i) { acc[x][j][0][i] *= f; acc[x][j][1][i] *= f; }
+              if (g == j) { ones[x][0] *= f; ones[x][1] *= f; }
+            }
+          }
+        }
+      }
+      if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+        for (int x = 0; x < NT; ++x)
+#pragma unroll
+          for (int c = 0; c < 2; ++c) {
+            l[x][c] *= alpha[x][c];
+            ones[x][c] *= alpha[x][c];
+#pragma unroll
+            for (int j = 0; j < GROUPS; ++j)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) { acc[x][j][h][c] *= alpha[x][c]; acc[x][j][h][c + 2] *= alpha[x][c]; }
+          }
+      }
+      uint32_t pb[NT][4];
+#pragma unroll
+      for (int x = 0; x < NT; ++x)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          float p[4];
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            p[c] = km_exp2(sc[x][i][c] - ref[x][c & 1]);
+            if (hidden >> (8 * x + 4 * i + c) & 1u) p[c] = -0.f;
+            l[x][c & 1] += p[c];
+          }
+          pb[x][2 * i] = km_turn(km_half2(p[0], p[1]));
+          pb[x][2 * i + 1] = km_turn(km_half2(p[2], p[3]));
+        }
+      // ---- the values
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) {
+          uint32_t r[2], s2[2];
+#pragma unroll
+          for (int b = 0; b < 2; ++b) {
+            const int o = 2 * u + b;
+            r[b] = __byte_perm(vw[o][0][j / 2], vw[o][1][j / 2], j & 1 ? 0x7632 : 0x5410);
+            s2[b] = __byte_perm(vs[o][0], vs[o][1], j == 0 ? 0x4000 : j == 1 ? 0x5010 : j == 2 ? 0x6020 : 0x7030) >> 1 & 0x7F807F80u;
+            if (lift[j] != 0) { const float f = ldexpf(1.f, lift[j]); s2[b] = km_mul2(s2[b], km_half2(f, f)); }
+          }
+          const uint32_t t0 = r[0] >> 8, t1 = r[1] >> 8, one = g == j ? 0x3C003C00u : 0u;
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            uint32_t b0 = km_mul2(pb[x][2 * u], s2[0]), b1 = km_mul2(pb[x][2 * u + 1], s2[1]);
+            if (odd_scales) {                          // no number goes into the sums, where it would meet the zeros beside the ones: who sees it is noted
+              const uint32_t w[2] = {pb[x][2 * u], pb[x][2 * u + 1]};
+              uint32_t keep[2] = {0u, 0u};
+#pragma unroll
+              for (int b = 0; b < 2; ++b)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                  const bool none = ((s2[b] >> (16 * h)) & 0x7fffu) > 0x7c00u;
+                  if (none && ((w[b] >> (16 * h)) & 0xffffu) != 0x8000u) bad[x] |= 1u << j;      // a weight of -0: the row does not see the key
+                  if (!none) keep[b] |= 0xffffu << (16 * h);
+                }
+              b0 &= keep[0];
+              b1 &= keep[1];
+            }
+            float* c0 = acc[x][j][0];
+            float* c1 = acc[x][j][1];
+            km_mma(c0, r[0] & 0x000F000Fu, r[0] & 0x00F000F0u, r[1] & 0x000F000Fu, r[1] & 0x00F000F0u, b0, b1, c0[0], c0[1], c0[2], c0[3]);
+            km_mma(c1, t0 & 0x000F000Fu, t0 & 0x00F000F0u, t1 & 0x000F000Fu, t1 & 0x00F000F0u, b0, b1, c1[0], c1[1], c1[2], c1[3]);
+            km_mma(ones[x], one, 0u, one, 0u, b0, b1, ones[x][0], ones[x][1], ones[x][2], ones[x][3]);
+          }
+        }
+      }
+      if (more) {
+        load_v((i8 + 1) & 7);
+        if (turn) ok = ok_next;
+      }
+    }
+    // ---- the warps' results side by side
+    __syncthreads();
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      bad[x] |= __shfl_xor_sync(0xffffffffu, bad[x], 1);
+      bad[x] |= __shfl_xor_sync(0xffffffffu, bad[x], 2);
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const uint32_t none = __shfl_sync(0xffffffffu, bad[x], (2 * t + c) * 4);
+        l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], 4);
+        l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], 8);
+        l[x][c] += __shfl_xor_sync(0xffffffffu, l[x][c], 16);
+        const int row = 8 * x + 2 * t + c;
+        if (g == 0) { m_s[warp * RT + row] = m[x][c]; l_s[warp * RT + row] = l[x][c]; }
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) {
+          const float eight = 8.f * __shfl_sync(0xffffffffu, ones[x][c], 4 * j + t), f = none >> j & 1u ? NAN : ldexpf(1.f, -lift[j]);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+            *(float2*)&o_s[(warp * RT + row) * D + 32 * j + 4 * g + 2 * h] = make_float2((acc[x][j][h][c] * 16777216.f - eight) * f, (acc[x][j][h][c + 2] * 1048576.f - eight) * f);
+        }
+      }
+    }
+    __syncthreads();
+    const bool whole = step0 == 0 && step1 == R.steps;
+    const long part = 2L * blockIdx.x + (pos == begin ? 0 : 1);
+    float* part_o = a.scratch + part * RT * D;
+    float* part_ml = a.scratch + 2L * N * RT * D + part * RT * 2;
+    for (int i = tid; i < rows * (D / 4); i += KM_THREADS) {
+      const int r = i / (D / 4), d4 = i - r * (D / 4), row = row0 + r, h = head * G + row % G;
+      const long token = R.first + row / G;
+      const float m0 = fmaxf(fmaxf(m_s[r], m_s[RT + r]), fmaxf(m_s[2 * RT + r], m_s[3 * RT + r]));
+      float top = m0;
+      if (whole && a.sinks != nullptr) top = fmaxf(top, a.sinks[h] * 1.4426950408889634f);
+      const float zero = top == -INFINITY ? 0.f : top;
+      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+      float total_l = 0.f;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const float lw = l_s[w * RT + r];
+        if (lw == 0.f) continue;
+        const float f = m_s[w * RT + r] == -INFINITY ? 1.f : exp2f(m_s[w * RT + r] - zero);
+        const float4 o = *(const float4*)&o_s[(w * RT + r) * D + 4 * d4];
+        total_l += lw * f;
+        sum.x += o.x * f; sum.y += o.y * f; sum.z += o.z * f; sum.w += o.w * f;
+      }
+      if (whole) {
+        if (a.sinks != nullptr) total_l += exp2f(a.sinks[h] * 1.4426950408889634f - zero + 15.f);
+        if (d4 == 0 && a.lse != nullptr) a.lse[token * a.n_q + h] = total_l == 0.f ? -INFINITY : (zero - 15.f + log2f(total_l)) * 0.6931471805599453f;
+        const float f = total_l == 0.f ? 0.f : 1.f / total_l;
+        bf16* to = a.out + token * a.out_stride + (long)h * D + 4 * d4;
+        to[0] = __float2bfloat16_rn(sum.x * f);
+        to[1] = __float2bfloat16_rn(sum.y * f);
+        to[2] = __float2bfloat16_rn(sum.z * f);
+        to[3] = __float2bfloat16_rn(sum.w * f);
+      } else {
+        *(float4*)&part_o[r * D + 4 * d4] = sum;
+        if (d4 == 0) { part_ml[2 * r] = top; part_ml[2 * r + 1] = total_l; }
+      }
+    }
+    pos += step1 - step0;
+    __syncthreads();
+  }
+}
+
+// Units that lie in several blocks.  A block has one row of a unit's tile.
+template <int GROUPS, int NT>
+__global__ void __launch_bounds__(GROUPS * 32)
+kv4_mma_join_kernel(const Kv4MmaArgs a, int N) {
+  constexpr int D = GROUPS * 32, RT = 8 * NT;
+  __shared__ int sums[2][GROUPS];
+  pdl_wait();
+  const int s = blockIdx.z, head = blockIdx.y, row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const KmRequest R = km_request<RT>(a, s);
+  if (row >= R.rows) return;
+  int before = 0, total = 0;
+  for (int i = tid; i < a.S; i += D) {
+    const KmRequest r = km_request<RT>(a, i);
+    const int x = r.steps * r.row_tiles * a.n_kv;
+    total += x;
+    if (i < s) before += x;
+  }
+  before = __reduce_add_sync(0xffffffffu, before);
+  total = __reduce_add_sync(0xffffffffu, total);
+  if (lane == 0) { sums[0][warp] = before; sums[1][warp] = total; }
+  __syncthreads();
+  before = total = 0;
+#pragma unroll
+  for (int i = 0; i < GROUPS; ++i) { before += sums[0][i]; total += sums[1][i]; }
+  const int from = before + (head * R.row_tiles + row / RT) * R.steps, to = from + R.steps;
+  // the block that has step x: the last one that begins at or before it
+  auto block_of = [&](int x) {
+    int b = (int)((long)x * N / total);
+    while (b + 1 < N && (long)total * (b + 1) / N <= x) ++b;
+    while ((long)total * b / N > x) --b;
+    return b;
+  };
+  const int b0 = block_of(from), b1 = block_of(to - 1);
+  if (b0 == b1) return;
+  const int r = row % RT, G = a.n_q / a.n_kv, h = head * G + row % G;
+  const float* part_ml = a.scratch + 2L * N * RT * D;
+  const float sink = a.sinks != nullptr ? a.sinks[h] * 1.4426950408889634f : -INFINITY;
+  auto part_of = [&](int b) { return 2L * b + ((long)total * b / N >= from ? 0 : 1); };
+  float m = sink;
+  for (int b = b0; b <= b1; ++b) if ((long)total * b / N < (long)total * (b + 1) / N) m = fmaxf(m, part_ml[(part_of(b) * RT + r) * 2]);
+  const float zero = m == -INFINITY ? 0.f : m;
+  float l = a.sinks != nullptr ? exp2f(sink - zero + 15.f) : 0.f, sum = 0.f;
+  for (int b = b0; b <= b1; ++b) {
+    if ((long)total * b / N >= (long)total * (b + 1) / N) continue;
+    const long part = part_of(b);
+    const float pm = part_ml[(part * RT + r) * 2], pl = part_ml[(part * RT + r) * 2 + 1], o = a.scratch[(part * RT + r) * D + tid];
+    if (pl == 0.f) continue;
+    const float f = pm == -INFINITY ? 1.f : exp2f(pm - zero);
+    l += pl * f;
+    sum += o * f;
+  }
+  const long token = R.first + row / G;
+  if (tid == 0 && a.lse != nullptr) a.lse[token * a.n_q + h] = l == 0.f ? -INFINITY : (zero - 15.f + log2f(l)) * 0.6931471805599453f;
+  a.out[token * a.out_stride + (long)h * D + tid] = __float2bfloat16_rn(l == 0.f ? 0.f : sum / l);
+}
+
+template <int GROUPS, int NT>
+static int km_launch(const Kv4MmaArgs& a, int N, int max_rows, cudaStream_t stream) {
+  constexpr int RT = 8 * NT;
+  const size_t smem = (4 * RT * GROUPS * 32 + 8 * RT) * sizeof(float) + (a.S + 1) * sizeof(int);
+  static bool set = false;
+  if (!set) {
+    const cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (4 * RT * GROUPS * 32 + 8 * RT) * 4 + (KM_MAX_SEQS + 1) * 4);
+    if (e != cudaSuccess) return (int)e;
+    set = true;
+  }
+  int status = launch_pdl(kv4_mma_kernel<GROUPS, NT>, dim3(N), dim3(KM_THREADS), smem, stream, a);
+  if (status != 0) return status;
+  return launch_pdl(kv4_mma_join_kernel<GROUPS, NT>, dim3(max_rows, a.n_kv, a.S), dim3(GROUPS * 32), 0, stream, a, N);
+}
+
+// parts: blocks; scratch: 2 * parts * RT * (d + 2) floats, RT = 8 for up to 8 rows, else 16.
+PHOTON_API int photon_kv4_attention_mma(const photon_kv4_attention_call* c, cudaStream_t stream) {
+  if (c->S <= 0 || c->max_tokens_per_seq <= 0) return 0;
+  if (c->dtype != PHOTON_BF16 || c->n_kv <= 0 || c->n_q <= 0 || c->n_q % c->n_kv || c->max_pages <= 0) return PHOTON_ERR_ARGUMENT;
+  if (!kv4_sizes_ok(c->page_size, c->d) || (c->d != 64 && c->d != 128) || c->page_size % 8 || c->num_pages <= 0) return PHOTON_ERR_UNSUPPORTED;
+  if (c->S > KM_MAX_SEQS || c->n_kv > 65535 || c->scale <= 0.f || ((uintptr_t)c->k_cache | (uintptr_t)c->v_cache) % 16) return PHOTON_ERR_UNSUPPORTED;
+  if (kv4_page_bytes(c->page_size, c->d) / 16 * c->num_pages * c->n_kv > 0xffffffffL) return PHOTON_ERR_UNSUPPORTED;      // a key's place in 16 bytes: 32 bits
+  if (c->parts < 1 || c->scratch == nullptr) return PHOTON_ERR_ARGUMENT;
+  const int rows = c->max_tokens_per_seq * (c->n_q / c->n_kv), most = rows < c->max_rows ? rows : c->max_rows;
+  const Kv4MmaArgs a = {(const bf16*)c->q, (bf16*)c->out, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->block_table, c->cu_tokens, c->context_lens, c->sinks, c->lse,
+                        c->scratch, c->err, c->q_stride, c->out_stride, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, c->min_rows,
+                        c->max_rows};
+  if (c->d == 64) return most <= 8 ? km_launch<2, 1>(a, c->parts, most, stream) : km_launch<2, 2>(a, c->parts, most, stream);
+  return most <= 8 ? km_launch<4, 1>(a, c->parts, most, stream) : km_launch<4, 2>(a, c->parts, most, stream);
+}

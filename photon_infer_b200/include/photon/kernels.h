@@ -660,6 +660,11 @@ typedef struct {
 } photon_kv4_attention_call;
 PHOTON_EXPORT int photon_kv4_attention(const photon_kv4_attention_call* call, cudaStream_t stream);
 
+/* ------------------------------------------------------------------ kv4_attention_mma.cu: the same on the tensor cores, bfloat16, d 64 or 128 */
+/* At most 1,024 requests, pages of a multiple of 8 tokens, caches of up to 64 GB each.  parts: blocks of the grid; scratch: 2 * parts * R * (d + 2) floats, R = 8 for at most 8
+ * rows a request, else 16. */
+PHOTON_EXPORT int photon_kv4_attention_mma(const photon_kv4_attention_call* call, cudaStream_t stream);
+
 /* ------------------------------------------------------------------ key_weights.cu */
 /* weights [num_pages][n_kv][page_size]: what the keys below context_lens[s] got of the softmax of request s's rows is added; keys from held[s] on (held null: the call's own tokens)
  * are set.  k_cache: of dtype, [num_pages][n_kv][page_size][d], or with packed 4 bits a number.  Rows and masks as in photon_kv4_attention; lse as that leaves it, or null:

@@ -2938,15 +2938,26 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
         most = KV4_FEW_ROWS
     tokens = -(-most // group)
     keys = min(max_keys, window + tokens) if window else max_keys
-    tiles, blocks = -(-keys // 128), num_seqs * n_kv * -(-tokens * group // 8)
-    parts = max(1, min(tiles, 4 * sm_count(q.device) // blocks, 64))
-    scratch = torch.empty(T * n_q * parts * (head_dim + 2), dtype=torch.float32, device=q.device) if parts > 1 else None
+    name, parts, floats = _kv4_route(q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, num_seqs, n_kv, most, keys, T * n_q, sm_count(q.device))
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     call = _KV4_ATTENTION_CALL.pack(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(),
                                     _data(sink), _data(lse), _data(scratch), _data(err), q.stride(0), out.stride(0), _dtype_code(q), pages, num_seqs, tokens, n_q, n_kv,
                                     head_dim, page_size, k_cache.shape[0], window, parts, 0, most, scale, softcap or 0.0)
-    _check(_plain_fn("kv4_attention", "photon_kv4_attention", _CALL_ARGS)(call, _stream()), "kv4_attention")
-    if parts > 1:
+    _check(_plain_fn(name, "photon_" + name, _CALL_ARGS)(call, _stream()), "kv4_attention")
+    if floats:
         _count_launches(1)
+
+
+def _kv4_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: int, num_seqs: int, n_kv: int, rows: int, keys: int, all_rows: int, sms: int):
+    """(kernel, parts, floats of scratch) for requests of at most ``rows`` rows (tokens x query heads per key/value head) and ``keys`` visible keys."""
+    if dtype == torch.bfloat16 and head_dim in (64, 128) and page_size % 8 == 0 and 0 < page_heads * kv4_page_bytes(page_size, head_dim) < 1 << 36 and num_seqs <= 1024:
+        tile = 8 if rows <= 8 else 16
+        units = num_seqs * n_kv * -(-rows // tile)
+        parts = min((3 if tile == 8 else 2) * sms, units * (-(-keys // 128) + 1))
+        return "kv4_attention_mma", parts, 2 * parts * tile * (head_dim + 2)
+    tiles, blocks = -(-keys // 128), num_seqs * n_kv * -(-rows // 8)
+    parts = max(1, min(tiles, 4 * sms // blocks, 64))
+    return "kv4_attention", parts, all_rows * parts * (head_dim + 2) if parts > 1 else 0
 
 
 _KV4_SPOIL_ARGS = [c_char_p, c_void_p, c_long, c_int, c_void_p]
