@@ -30,13 +30,13 @@ struct Kv4MmaArgs {
 };
 
 __device__ __forceinline__ void km_mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1, float c0, float c1, float c2, float c3) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%11,%12,%13};"
                : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
                : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c0), "f"(c1), "f"(c2), "f"(c3));
 }
 __device__ __forceinline__ uint32_t km_turn(uint32_t x) {      // an 8 x 8 matrix of 16-bit numbers, rows for columns
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 __device__ __forceinline__ float km_exp2(float x) {
@@ -44,6 +44,8 @@ __device__ __forceinline__ float km_exp2(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+__device__ __forceinline__ float km_power(int e) { return __int_as_float((127 + e) << 23); }      // 2^e, -126 <= e <= 127
+__device__ __forceinline__ float km_scaled(float x, int e) { return x * km_power(e / 2) * km_power(e - e / 2); }
 __device__ __forceinline__ uint32_t km_half2(float lo, float hi) {
   const __half2 h = __floats2half2_rn(lo, hi);
   return *(const uint32_t*)&h;
@@ -51,6 +53,12 @@ __device__ __forceinline__ uint32_t km_half2(float lo, float hi) {
 __device__ __forceinline__ uint32_t km_mul2(uint32_t a, uint32_t b) {
   const __half2 h = __hmul2(*(const __half2*)&a, *(const __half2*)&b);
   return *(const uint32_t*)&h;
+}
+// Bytes of two words by a selector's nibbles; 8 + i: eight times byte i's first bit.
+__device__ __forceinline__ uint32_t km_bytes(uint32_t a, uint32_t b, uint32_t selector) {
+  uint32_t y;
+  asm("prmt.b32 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(selector));
+  return y;
 }
 template <int WORDS>
 __device__ __forceinline__ void km_load(uint32_t* x, const uint8_t* p) {      // read once: not kept in the first cache
@@ -81,8 +89,8 @@ __device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
   return r;
 }
 
-// GROUPS: of 32 numbers of a head (2 or 4); NT: tiles of 8 rows.
-template <int GROUPS, int NT>
+// GROUPS: of 32 numbers of a head (2 or 4); NT: tiles of 8 rows; CAP: bounded scores.
+template <int GROUPS, int NT, bool CAP>
 __global__ void __launch_bounds__(KM_THREADS, NT == 1 ? 3 : 2)
 kv4_mma_kernel(const Kv4MmaArgs a) {
   constexpr int D = GROUPS * 32, RT = 8 * NT, KW = GROUPS, VW = GROUPS / 2;      // words of a key's and of a value's piece
@@ -120,6 +128,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
   }
   const int G = a.n_q / a.n_kv;
   const long page_bytes = (long)a.page_size * GROUPS * 17;
+  const float cap_in = 2.f * 1.4426950408889634f / a.softcap, cap_out = a.softcap * 1.4426950408889634f;
   for (int pos = begin; pos < end;) {
     while (before_s[s + 1] <= pos) ++s;
     const KmRequest R = km_request<RT>(a, s);
@@ -146,8 +155,8 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
       const bool odd = top >= 0x7f800000u;
-      const int e = top == 0 || odd ? 0 : ilogbf(__uint_as_float(top));
-      const float f = ldexpf(a.scale * (a.softcap > 0.f ? 1.f : 1.4426950408889634f), e - 14 + 24);
+      const int e = top == 0 || odd ? 0 : max((int)(top >> 23), 1) - 127;
+      const float f = fmaxf(km_scaled(a.scale * (CAP ? 1.f : 1.4426950408889634f), e - 14 + 24), 1e-37f);
       float sums[GROUPS];
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
@@ -155,7 +164,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         sums[j] = 0.f;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {                 // the odd ones meet the second nibbles, which are 16 times as large
-          const float y = odd ? __int_as_float(0x7fc00000) : ldexpf(v[j][i], 14 - e - (i & 1) * 4);
+          const float y = odd ? __int_as_float(0x7fc00000) : km_scaled(v[j][i], 14 - e - (i & 1) * 4);
           w[i] = __half2float(__float2half_rn(y));
           sums[j] += i & 1 ? 16.f * w[i] : w[i];
         }
@@ -196,47 +205,53 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
     int lift[GROUPS], tops[GROUPS];                   // powers of two; the largest scale from 2 on
 #pragma unroll
     for (int j = 0; j < GROUPS; ++j) lift[j] = tops[j] = 0;
+    bool lifted = false;                              // some group is or was
+    uint32_t one[GROUPS];                             // row j of the first operand
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) one[j] = g == j ? 0x3C003C00u : 0u;
 
     // ---- where the keys are: lane 4 i + o has the 8 keys o of the warp's 32 of step i, 8 steps at a time
     const int key_w = R.from + warp * 32;
-    uint32_t off16 = 0, off16_next = 0, ok = 0, ok_next = 0;
-    int slot = 0, slot_next = 0;
-    auto find = [&](int step, uint32_t& off, int& sl, uint32_t& mask) {
+    // off: where the 8 keys' codes begin, in 16 bytes; sc: where their scales do
+    uint32_t off = 0, off_next = 0, sc16 = 0, sc16_next = 0, ok = 0, ok_next = 0;
+    auto find = [&](int step, uint32_t& to, uint32_t& scales, uint32_t& mask) {
       const int i = step + (lane >> 2), key = key_w + i * KM_KEYS + (lane & 3) * 8;
       const int pidx = key / a.page_size;
-      int page = -1;
-      sl = key - pidx * a.page_size;
+      int page = -1, sl = key - pidx * a.page_size;
       if (i < step1 && key <= last_place) {
         page = pidx < a.max_pages ? a.table[(long)s * a.max_pages + pidx] : -1;
         if (page < 0 || page >= a.num_pages) { report_error(a.err, PHOTON_DEV_BAD_PAGE, s, key, page); page = -1; }
       }
       const bool good = page >= 0;
-      off = good ? (uint32_t)((((long)page * a.n_kv + head) * page_bytes + (long)sl * (D / 2)) >> 4) : 0u;
-      if (!good) sl = 0;
+      if (!good) page = sl = 0;                       // some page of the pool: what is read there is not used
+      const uint32_t begin16 = ((uint32_t)page * a.n_kv + head) * (uint32_t)(page_bytes >> 4);
+      to = begin16 + sl * (D / 32);
+      scales = begin16 + a.page_size * (D / 32) + sl * GROUPS / 16;
       mask = __ballot_sync(0xffffffffu, good);
     };
-    find(step0, off16, slot, ok);
+    find(step0, off, sc16, ok);
     uint32_t kw[4][KW], vw[4][2][VW], ks[4], vs[4][2];
+    const uint8_t* k_codes = a.k + g * (D / 2) + 4 * GROUPS * t;
+    const uint8_t* k_scales = a.k + g * GROUPS;
+    const uint8_t* v_codes = a.v + 2 * t * (D / 2) + 2 * GROUPS * g;
+    const uint8_t* v_scales = a.v + 2 * t * GROUPS;
     auto load_k = [&](int i) {                         // i: the step's place among the 8 that are known
 #pragma unroll
       for (int o = 0; o < 4; ++o) {
-        const uint8_t* p = a.k + ((unsigned long long)__shfl_sync(0xffffffffu, off16, 4 * i + o) << 4);
-        const int sl = __shfl_sync(0xffffffffu, slot, 4 * i + o);
-        km_load<KW>(kw[o], p + g * (D / 2) + 4 * GROUPS * t);
-        const uint8_t* sc = p + (a.page_size - sl) * (D / 2) + (sl + g) * GROUPS;
-        if constexpr (GROUPS == 4) km_load<1>(&ks[o], sc); else ks[o] = km_load16(sc);
+        km_load<KW>(kw[o], k_codes + __shfl_sync(0xffffffffu, off, 4 * i + o) * 16ull);
+        const uint8_t* p = k_scales + __shfl_sync(0xffffffffu, sc16, 4 * i + o) * 16ull;
+        if constexpr (GROUPS == 4) km_load<1>(&ks[o], p); else ks[o] = km_load16(p);
       }
     };
     auto load_v = [&](int i) {
 #pragma unroll
       for (int o = 0; o < 4; ++o) {
-        const uint8_t* p = a.v + ((unsigned long long)__shfl_sync(0xffffffffu, off16, 4 * i + o) << 4);
-        const int sl = __shfl_sync(0xffffffffu, slot, 4 * i + o);
-        km_load<VW>(vw[o][0], p + (2 * t) * (D / 2) + 2 * GROUPS * g);
-        km_load<VW>(vw[o][1], p + (2 * t + 1) * (D / 2) + 2 * GROUPS * g);
-        const uint8_t* sc = p + (a.page_size - sl) * (D / 2) + (sl + 2 * t) * GROUPS;
-        if constexpr (GROUPS == 4) km_load<2>(vs[o], sc);
-        else { uint32_t both; km_load<1>(&both, sc); vs[o][0] = both & 0xffffu; vs[o][1] = both >> 16; }
+        const uint8_t* p = v_codes + __shfl_sync(0xffffffffu, off, 4 * i + o) * 16ull;
+        km_load<VW>(vw[o][0], p);
+        km_load<VW>(vw[o][1], p + D / 2);
+        p = v_scales + __shfl_sync(0xffffffffu, sc16, 4 * i + o) * 16ull;
+        if constexpr (GROUPS == 4) km_load<2>(vs[o], p);
+        else { uint32_t both; km_load<1>(&both, p); vs[o][0] = both & 0xffffu; vs[o][1] = both >> 16; }
       }
     };
     load_k(0);
@@ -244,14 +259,10 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
     for (int step = step0; step < step1; ++step) {
       const int i8 = (step - step0) & 7;
       const uint32_t here = ok >> (4 * i8) & 15u;
-      if (i8 == 0) find(step + 8, off16_next, slot_next, ok_next);
+      if (i8 == 0) find(step + 8, off_next, sc16_next, ok_next);
       const int key0 = key_w + step * KM_KEYS;
       // ---- scores
       float sc[NT][2][4];
-#pragma unroll
-      for (int x = 0; x < NT; ++x)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) sc[x][0][i] = sc[x][1][i] = 0.f;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
 #pragma unroll
@@ -270,10 +281,8 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
                      init[x][j][1]);
               km_mma(d, u0 & 0x000F000Fu, u1 & 0x000F000Fu, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qb[x][j][2], qb[x][j][3], d[0], d[1], d[2], d[3]);
               const float a0 = jx ? s0.y : s0.x, a1 = jx ? s1.y : s1.x;
-              sc[x][i][0] += a0 * d[0];
-              sc[x][i][1] += a0 * d[1];
-              sc[x][i][2] += a1 * d[2];
-              sc[x][i][3] += a1 * d[3];
+#pragma unroll
+              for (int c = 0; c < 4; ++c) sc[x][i][c] = j == 0 ? (c < 2 ? a0 : a1) * d[c] : fmaf(c < 2 ? a0 : a1, d[c], sc[x][i][c]);
             }
           }
         }
@@ -281,24 +290,22 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       const bool more = step + 1 < step1;
       const bool turn = i8 == 7;
       if (more) {
-        if (turn) { off16 = off16_next; slot = slot_next; }
+        if (turn) { off = off_next; sc16 = sc16_next; }
         load_k((i8 + 1) & 7);
       }
       // ---- the softmax
       const bool masked = here != 15u || key0 < clear_from || key0 + 31 > clear_to;
+      if constexpr (CAP) {                              // tanh y = 1 - 2 / (1 + e^2y); the factor is in it then
 #pragma unroll
-      for (int x = 0; x < NT; ++x)
+        for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+          for (int i = 0; i < 2; ++i)
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            sc[x][i][c] *= factor[x][c & 1];
-            if (a.softcap > 0.f) {                     // tanh y = 1 - 2 / (1 + e^2y)
-              const float y = km_exp2(sc[x][i][c] * (2.f * 1.4426950408889634f / a.softcap));
-              sc[x][i][c] = a.softcap * 1.4426950408889634f * (1.f - __fdividef(2.f, 1.f + y));
+            for (int c = 0; c < 4; ++c) {
+              const float y = km_exp2(sc[x][i][c] * (factor[x][c & 1] * cap_in));
+              sc[x][i][c] = fmaf(-cap_out, __fdividef(2.f, 1.f + y), cap_out);
             }
-          }
-      uint32_t hidden = 0;                             // bit (8 x + 4 i + c): this thread's score is no key of its row
+      }
       if (masked) {
 #pragma unroll
         for (int x = 0; x < NT; ++x)
@@ -308,7 +315,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
             for (int c = 0; c < 4; ++c) {
               const int key = key0 + 16 * i + 8 * (c >> 1) + g, at_place = place[x][c & 1];
               const bool sees = (here >> (2 * i + (c >> 1)) & 1u) && key <= at_place && (a.window <= 0 || key > at_place - a.window);
-              if (!sees) { sc[x][i][c] = -INFINITY; hidden |= 1u << (8 * x + 4 * i + c); }
+              if (!sees) sc[x][i][c] = -INFINITY;
             }
 #pragma unroll
         for (int o = 0; o < 4; ++o)
@@ -328,6 +335,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
           top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+          if constexpr (!CAP) top *= factor[x][c];
           top = fmaxf(top, m[x][c]);
           alpha[x][c] = m[x][c] == -INFINITY ? 1.f : km_exp2(m[x][c] - top);
           grown |= top > m[x][c];
@@ -366,8 +374,9 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         for (int j = 0; j < GROUPS; ++j) {
           const int e = tops[j] > 0 ? tops[j] >> 3 : seen_scales >> (8 * j + 3) & 15, to = e > 15 || e < 8 ? 15 - e : 0;
           if (to != lift[j]) {
-            const float f = ldexpf(1.f, to - lift[j]);
+            const float f = km_power(to - lift[j]);
             lift[j] = to;
+            lifted = true;
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
 #pragma unroll
@@ -398,49 +407,55 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
           float p[4];
 #pragma unroll
           for (int c = 0; c < 4; ++c) {
-            p[c] = km_exp2(sc[x][i][c] - ref[x][c & 1]);
-            if (hidden >> (8 * x + 4 * i + c) & 1u) p[c] = -0.f;
+            p[c] = km_exp2(CAP ? sc[x][i][c] - ref[x][c & 1] : fmaf(sc[x][i][c], factor[x][c & 1], -ref[x][c & 1]));
             l[x][c & 1] += p[c];
           }
           pb[x][2 * i] = km_turn(km_half2(p[0], p[1]));
           pb[x][2 * i + 1] = km_turn(km_half2(p[2], p[3]));
         }
       // ---- the values
+      uint32_t s2[4][GROUPS];                          // scales of the keys 2 t and 2 t + 1 of each 8; the bytes between are a scale's first bit, 0 below 2
+#pragma unroll
+      for (int o = 0; o < 4; ++o)
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) s2[o][j] = km_bytes(vs[o][0], vs[o][1], j == 0 ? 0x4C08 : j == 1 ? 0x5D19 : j == 2 ? 0x6E2A : 0x7F3B) >> 1;
+      if (lifted || odd_scales) {
+#pragma unroll
+        for (int o = 0; o < 4; ++o)
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) {
+            uint32_t y = s2[o][j] & 0x7F807F80u;
+            if (odd_scales) {                          // no number goes into the sums, where it would meet the zeros beside the ones: who sees it is noted
+#pragma unroll
+              for (int b = 0; b < 2; ++b)
+                if (((y >> (16 * b)) & 0x7fffu) >= 0x7c00u) {
+                  y &= b ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+                  for (int x = 0; x < NT; ++x) {
+                    const int r = 8 * x + g, key = key0 + 8 * o + 2 * t + b, at_place = base + (row0 + r) / G;
+                    if (r < rows && key <= at_place && (a.window <= 0 || key > at_place - a.window)) bad[x] |= 1u << j;
+                  }
+                }
+            }
+            const float f = km_power(lift[j]);
+            s2[o][j] = km_mul2(y, km_half2(f, f));
+          }
+      }
 #pragma unroll
       for (int u = 0; u < 2; ++u) {
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j) {
-          uint32_t r[2], s2[2];
-#pragma unroll
-          for (int b = 0; b < 2; ++b) {
-            const int o = 2 * u + b;
-            r[b] = __byte_perm(vw[o][0][j / 2], vw[o][1][j / 2], j & 1 ? 0x7632 : 0x5410);
-            s2[b] = __byte_perm(vs[o][0], vs[o][1], j == 0 ? 0x4000 : j == 1 ? 0x5010 : j == 2 ? 0x6020 : 0x7030) >> 1 & 0x7F807F80u;
-            if (lift[j] != 0) { const float f = ldexpf(1.f, lift[j]); s2[b] = km_mul2(s2[b], km_half2(f, f)); }
-          }
-          const uint32_t t0 = r[0] >> 8, t1 = r[1] >> 8, one = g == j ? 0x3C003C00u : 0u;
+          const uint32_t r0 = __byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410);
+          const uint32_t r1 = __byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410);
+          const uint32_t t0 = r0 >> 8, t1 = r1 >> 8;
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
-            uint32_t b0 = km_mul2(pb[x][2 * u], s2[0]), b1 = km_mul2(pb[x][2 * u + 1], s2[1]);
-            if (odd_scales) {                          // no number goes into the sums, where it would meet the zeros beside the ones: who sees it is noted
-              const uint32_t w[2] = {pb[x][2 * u], pb[x][2 * u + 1]};
-              uint32_t keep[2] = {0u, 0u};
-#pragma unroll
-              for (int b = 0; b < 2; ++b)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                  const bool none = ((s2[b] >> (16 * h)) & 0x7fffu) > 0x7c00u;
-                  if (none && ((w[b] >> (16 * h)) & 0xffffu) != 0x8000u) bad[x] |= 1u << j;      // a weight of -0: the row does not see the key
-                  if (!none) keep[b] |= 0xffffu << (16 * h);
-                }
-              b0 &= keep[0];
-              b1 &= keep[1];
-            }
+            const uint32_t b0 = km_mul2(pb[x][2 * u], s2[2 * u][j]), b1 = km_mul2(pb[x][2 * u + 1], s2[2 * u + 1][j]);
             float* c0 = acc[x][j][0];
             float* c1 = acc[x][j][1];
-            km_mma(c0, r[0] & 0x000F000Fu, r[0] & 0x00F000F0u, r[1] & 0x000F000Fu, r[1] & 0x00F000F0u, b0, b1, c0[0], c0[1], c0[2], c0[3]);
+            km_mma(c0, r0 & 0x000F000Fu, r0 & 0x00F000F0u, r1 & 0x000F000Fu, r1 & 0x00F000F0u, b0, b1, c0[0], c0[1], c0[2], c0[3]);
             km_mma(c1, t0 & 0x000F000Fu, t0 & 0x00F000F0u, t1 & 0x000F000Fu, t1 & 0x00F000F0u, b0, b1, c1[0], c1[1], c1[2], c1[3]);
-            km_mma(ones[x], one, 0u, one, 0u, b0, b1, ones[x][0], ones[x][1], ones[x][2], ones[x][3]);
+            km_mma(ones[x], one[j], 0u, one[j], 0u, b0, b1, ones[x][0], ones[x][1], ones[x][2], ones[x][3]);
           }
         }
       }
@@ -465,7 +480,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         if (g == 0) { m_s[warp * RT + row] = m[x][c]; l_s[warp * RT + row] = l[x][c]; }
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j) {
-          const float eight = 8.f * __shfl_sync(0xffffffffu, ones[x][c], 4 * j + t), f = none >> j & 1u ? NAN : ldexpf(1.f, -lift[j]);
+          const float eight = 8.f * __shfl_sync(0xffffffffu, ones[x][c], 4 * j + t), f = none >> j & 1u ? NAN : km_power(-lift[j]);
 #pragma unroll
           for (int h = 0; h < 2; ++h)
             *(float2*)&o_s[(warp * RT + row) * D + 32 * j + 4 * g + 2 * h] = make_float2((acc[x][j][h][c] * 16777216.f - eight) * f, (acc[x][j][h][c + 2] * 1048576.f - eight) * f);
@@ -570,17 +585,17 @@ kv4_mma_join_kernel(const Kv4MmaArgs a, int N) {
   a.out[token * a.out_stride + (long)h * D + tid] = __float2bfloat16_rn(l == 0.f ? 0.f : sum / l);
 }
 
-template <int GROUPS, int NT>
+template <int GROUPS, int NT, bool CAP>
 static int km_launch(const Kv4MmaArgs& a, int N, int max_rows, cudaStream_t stream) {
   constexpr int RT = 8 * NT;
   const size_t smem = (4 * RT * GROUPS * 32 + 8 * RT) * sizeof(float) + (a.S + 1) * sizeof(int);
   static bool set = false;
   if (!set) {
-    const cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (4 * RT * GROUPS * 32 + 8 * RT) * 4 + (KM_MAX_SEQS + 1) * 4);
+    const cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (4 * RT * GROUPS * 32 + 8 * RT) * 4 + (KM_MAX_SEQS + 1) * 4);
     if (e != cudaSuccess) return (int)e;
     set = true;
   }
-  int status = launch_pdl(kv4_mma_kernel<GROUPS, NT>, dim3(N), dim3(KM_THREADS), smem, stream, a);
+  int status = launch_pdl(kv4_mma_kernel<GROUPS, NT, CAP>, dim3(N), dim3(KM_THREADS), smem, stream, a);
   if (status != 0) return status;
   return launch_pdl(kv4_mma_join_kernel<GROUPS, NT>, dim3(max_rows, a.n_kv, a.S), dim3(GROUPS * 32), 0, stream, a, N);
 }
@@ -597,6 +612,8 @@ PHOTON_API int photon_kv4_attention_mma(const photon_kv4_attention_call* c, cuda
   const Kv4MmaArgs a = {(const bf16*)c->q, (bf16*)c->out, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->block_table, c->cu_tokens, c->context_lens, c->sinks, c->lse,
                         c->scratch, c->err, c->q_stride, c->out_stride, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, c->min_rows,
                         c->max_rows};
-  if (c->d == 64) return most <= 8 ? km_launch<2, 1>(a, c->parts, most, stream) : km_launch<2, 2>(a, c->parts, most, stream);
-  return most <= 8 ? km_launch<4, 1>(a, c->parts, most, stream) : km_launch<4, 2>(a, c->parts, most, stream);
+#define ATTEND(GROUPS, NT) (c->softcap > 0.f ? km_launch<GROUPS, NT, true>(a, c->parts, most, stream) : km_launch<GROUPS, NT, false>(a, c->parts, most, stream))
+  if (c->d == 64) return most <= 8 ? ATTEND(2, 1) : ATTEND(2, 2);
+  return most <= 8 ? ATTEND(4, 1) : ATTEND(4, 2);
+#undef ATTEND
 }
