@@ -2951,9 +2951,9 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
 def _kv4_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: int, num_seqs: int, n_kv: int, rows: int, keys: int, all_rows: int, sms: int):
     """(kernel, parts, floats of scratch) for requests of at most ``rows`` rows (tokens x query heads per key/value head) and ``keys`` visible keys."""
     if dtype == torch.bfloat16 and head_dim in (64, 128) and page_size % 8 == 0 and 0 < page_heads * kv4_page_bytes(page_size, head_dim) < 1 << 36 and num_seqs <= 1024:
-        tile = 8 if rows <= 8 else 16
+        tile = 4 if rows <= 4 else 8
         units = num_seqs * n_kv * -(-rows // tile)
-        parts = min((3 if tile == 8 else 2) * sms, units * (-(-keys // 128) + 1))
+        parts = min((5 - head_dim // 64 - (tile == 8)) * sms, units * (-(-keys // 128) + 1))
         return "kv4_attention_mma", parts, 2 * parts * tile * (head_dim + 2)
     tiles, blocks = -(-keys // 128), num_seqs * n_kv * -(-rows // 8)
     parts = max(1, min(tiles, 4 * sms // blocks, 64))
