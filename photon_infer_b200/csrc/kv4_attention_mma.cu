@@ -7,35 +7,41 @@
 // where the last factor has two parts, two 16-bit floats, in neighbouring columns of the second operand, so that four rows (tokens x query heads of a key/value head) fill its
 // eight columns; a value's behind the sum, since two rows of the result are the sums over c0 + 16 c1 and 16 c1.
 //   score[key][row] = factor[row] sum over groups  scale[key][group] (sum over the group  c q  -  8 sum over the group  q),
-// the last sum being what the product's result begins with.  The weights, as 16-bit floats, are turned over in registers and multiplied by the values' scales,
-//   out[number][row] = sum over keys  c (p scale)[key][group(number)][row]  -  8 sum over keys (p scale)[key][group][row],
-// where the last sums of all groups are one more product, with ones in a row of the first operand for each group.  Weights are lifted by 2^15, and the scales of a group
+// the last sum known beforehand.  The weights, as 16-bit floats, are turned over in registers and multiplied by the values' scales,
+//   out[number][row] = sum over keys  (c - 8) (p scale)[key][group(number)][row],
+// where pairs of codes under the mask get the exponent of 1,024 with it and 1,024 and the eights are taken off by an addition, which is exact.  Weights are lifted by 2^15, and the scales of a group
 // whose largest so far is 2 or more, or below 2^-7, by the power of two that brings it to [1, 2).  All sums and the softmax are in 32 bits.
 //
-// Every warp walks keys of its own, 32 at a time, straight from the cache into registers, the next keys' codes asked for as soon as these are in the operands.  All
-// blocks have equal runs of the requests' tiles of 128 keys; results of a unit (request, head, 4 or 8 rows) that lies in one block are written, others are joined by a
-// second kernel in ascending order.
+// All warps have equal runs of the requests' tiles of 32 keys, wherever units (a request, a head, 4 or 8 rows) begin and end, and nothing to do with one another: a tile's
+// bytes come through three stages of the warp's own in shared memory, two of them on their way.  Results of a unit that lies in one warp are written, the others' parts are joined by a
+// second kernel, in the same order every time.
 #include "kv4.cuh"
 #include <math.h>
 
 #define KM_THREADS 128
-#define KM_KEYS 128              // of a block's step, 32 a warp
+#define KM_KEYS 32               // of a warp's step
 #define KM_MAX_SEQS 1024
+#define KM_STAGES 3              // of a warp's 32 keys and values in shared memory
 
 struct Kv4MmaArgs {
   const bf16* q; bf16* out; const uint8_t* k; const uint8_t* v;
-  const int* table; const int* cu_tokens; const int* context_lens; const float* sinks; float* lse; float* scratch; int* err;
+  const int* table; const int* cu_tokens; const int* context_lens; const float* sinks; float* lse; float* scratch; int* before; int* err;      // before [S + 1]: behind the scratch
   long q_stride, out_stride;
   int max_pages, S, n_q, n_kv, page_size, num_pages, window;
   float scale, softcap;
-  int min_rows, max_rows, q_vec;      // q_vec: rows of q on 16-byte boundaries
+  int min_rows, max_rows, q_vec, out_vec;      // rows of q on 16-byte boundaries, of out on 8-byte ones
 };
 
-// d += a b: 16 x 16 and 16 x 8 numbers of 16 bits.
+// d += a b: 16 x 16 and 16 x 8 numbers of 16 bits; and d = a b.
 __device__ __forceinline__ void km_mma(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void km_mma0(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t km_turn(uint32_t x) {      // an 8 x 8 matrix of 16-bit numbers, rows for columns
   uint32_t y;
@@ -63,19 +69,37 @@ __device__ __forceinline__ uint32_t km_bytes(uint32_t a, uint32_t b, uint32_t se
   asm("prmt.b32 %0, %1, %2, %3;" : "=r"(y) : "r"(a), "r"(b), "r"(selector));
   return y;
 }
-template <int WORDS>
-__device__ __forceinline__ void km_load(uint32_t* x, const uint8_t* p) {      // read once: not kept in the first cache
-  if constexpr (WORDS == 4) asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "l"(p));
-  else if constexpr (WORDS == 2) asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "l"(p));
-  else asm volatile("ld.global.nc.L1::no_allocate.u32 %0, [%1];" : "=r"(x[0]) : "l"(p));
+__device__ __forceinline__ void km_copy(uint32_t to, const uint8_t* from) {      // 16 bytes to shared memory
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
-__device__ __forceinline__ uint32_t km_load16(const uint8_t* p) {
+__device__ __forceinline__ uint32_t km_add2(uint32_t a, uint32_t b) {
+  const __half2 h = __hadd2(*(const __half2*)&a, *(const __half2*)&b);
+  return *(const uint32_t*)&h;
+}
+template <int WORDS>
+__device__ __forceinline__ void km_read(uint32_t* x, uint32_t at) {
+  if constexpr (WORDS == 4) asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(at));
+  else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(x[0]), "=r"(x[1]) : "r"(at));
+  else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(x[0]) : "r"(at));
+}
+__device__ __forceinline__ uint32_t km_read16(uint32_t at) {
   uint16_t x;
-  asm volatile("ld.global.nc.u16 %0, [%1];" : "=h"(x) : "l"(p));
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(x) : "r"(at));
   return x;
 }
+__device__ __forceinline__ const uint8_t* km_at(const uint8_t* base, uint32_t sixteens) {
+  const uint8_t* p;
+  asm("mad.wide.u32 %0, %1, 16, %2;" : "=l"(p) : "r"(sixteens), "l"(base));
+  return p;
+}
+// Where 16 bytes `c` of row r of 8 rows lie in a stage: no two of the lanes that read together, 8 rows' pieces by turns (keys) or every other row's (values), meet in a bank.
+template <int GROUPS>
+__device__ __forceinline__ int km_place(int r, int c) {
+  if constexpr (GROUPS == 4) return (r ^ (r >> 1 & 1)) * 64 + ((c ^ (r >> 2 & 1) << 1) * 16);
+  else return (r & 1 ? 4 + (r >> 1 ^ 2) : r >> 1) * 32 + c * 16;
+}
 
-// A request's place in the work: rows, row tiles, keys from..to (from a multiple of 8), steps of 128 keys.
+// A request's place in the work: rows, row tiles, keys from..to (from a multiple of 8), steps of 32 keys.
 struct KmRequest { int first, n, ctx, rows, row_tiles, from, steps; };
 template <int RT>
 __device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
@@ -94,15 +118,13 @@ __device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
 
 // GROUPS: of 32 numbers of a head (2 or 4); NT: tiles of 4 rows; CAP: bounded scores.
 template <int GROUPS, int NT, bool CAP>
-__global__ void __launch_bounds__(KM_THREADS, (GROUPS == 4 ? 3 : 4) - (NT - 1))
+__global__ void __launch_bounds__(KM_THREADS, 5 - NT)
 kv4_mma_kernel(const Kv4MmaArgs a) {
   constexpr int D = GROUPS * 32, RT = 4 * NT, KW = GROUPS, VW = GROUPS / 2;      // words of a key's and of a value's piece
-  extern __shared__ __align__(16) float smem[];
-  float* o_s = smem;                                  // [4][RT][D]
-  float* m_s = o_s + 4 * RT * D;                      // [4][RT]
-  float* l_s = m_s + 4 * RT;
-  int* before_s = (int*)(l_s + 4 * RT);               // [S + 1] units' steps in front of a request
-  const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+  constexpr int ROW = D / 2, STAGE = 64 * ROW + 64 * GROUPS;      // codes of 32 keys, of 32 values, their scales
+  extern __shared__ __align__(16) uint8_t smem[];     // the four warps' stages
+  int* before_s = (int*)(smem + 4 * KM_STAGES * STAGE);      // [S + 1] units' steps in front of a request
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   pdl_wait();
   if (warp == 0) {
     int sum = 0;
@@ -118,10 +140,15 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       sum += __shfl_sync(0xffffffffu, x, 31);
     }
     if (lane == 0) before_s[0] = 0;
+    if (blockIdx.x == 0) {                            // for the second kernel
+      __syncwarp();
+      for (int i = lane; i <= a.S; i += 32) a.before[i] = before_s[i];
+    }
   }
   __syncthreads();
-  const int total = before_s[a.S], N = gridDim.x;
-  const int begin = (int)((long)total * blockIdx.x / N), end = (int)((long)total * (blockIdx.x + 1) / N);
+  pdl_launch_dependents();
+  const int total = before_s[a.S], N = gridDim.x * 4, me = blockIdx.x * 4 + warp;
+  const int begin = (int)((long)total * me / N), end = (int)((long)total * (me + 1) / N);
   if (begin >= end) return;
   int s = 0;
   {                                                   // the request of the first step: the last one that begins at or before it
@@ -132,9 +159,6 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
   const int G = a.n_q / a.n_kv;
   const long page_bytes = (long)a.page_size * GROUPS * 17;
   const float cap_in = 2.f * 1.4426950408889634f / a.softcap, cap_out = a.softcap * 1.4426950408889634f;
-  uint32_t one[GROUPS];                               // row j of the first operand: ones
-#pragma unroll
-  for (int j = 0; j < GROUPS; ++j) one[j] = g == j ? 0x3C003C00u : 0u;
   for (int pos = begin; pos < end;) {
     while (before_s[s + 1] <= pos) ++s;
     const KmRequest R = km_request<RT>(a, s);
@@ -144,82 +168,105 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
     const int low = a.window > 0 ? max(0, first_place - a.window + 1) : 0;                            // keys from here to last_place some row sees
     const int clear_from = a.window > 0 ? last_place - a.window + 1 : 0, clear_to = first_place;      // keys that all rows see
 
-    // ---- where the keys are: lane 4 i + o has the 8 keys o of the warp's 32 of step i, 8 steps at a time
-    const int key_w = R.from + warp * 32;
+    // ---- where the keys are: lane 4 i + o has the 8 keys o of step i's 32, 8 steps at a time
     // off: where the 8 keys' codes begin, in 16 bytes; sc: where their scales do
-    uint32_t off = 0, off_next = 0, sc16 = 0, sc16_next = 0, ok = 0, ok_next = 0;
-    auto find = [&](int step, uint32_t& to, uint32_t& scales, uint32_t& mask) {
-      const int i = step + (lane >> 2), key = key_w + i * KM_KEYS + (lane & 3) * 8;
-      const int pidx = key / a.page_size;
-      int page = -1, sl = key - pidx * a.page_size;
-      if (i < step1 && key <= last_place) {
-        page = pidx < a.max_pages ? a.table[(long)s * a.max_pages + pidx] : -1;
-        if (page < 0 || page >= a.num_pages) { report_error(a.err, PHOTON_DEV_BAD_PAGE, s, key, page); page = -1; }
+    uint32_t off = 0, sc16 = 0, ok = 0;
+    int entry = -1;                                   // of the block table, for the 8 steps behind those that are known
+    auto look = [&](int step) {
+      const int key = R.from + (step + (lane >> 2)) * KM_KEYS + (lane & 3) * 8, pidx = key / a.page_size;
+      entry = -1;
+      if (step + (lane >> 2) < step1 && key <= last_place) {
+        if (pidx < a.max_pages) entry = a.table[(long)s * a.max_pages + pidx];
+        if (pidx >= a.max_pages) report_error(a.err, PHOTON_DEV_BAD_PAGE, s, key, -1);
       }
-      const bool good = page >= 0;
-      if (!good) page = sl = 0;                       // some page of the pool: what is read there is not used
+    };
+    auto found = [&](int step) {
+      const int key = R.from + (step + (lane >> 2)) * KM_KEYS + (lane & 3) * 8, pidx = key / a.page_size;
+      const bool asked = step + (lane >> 2) < step1 && key <= last_place && pidx < a.max_pages, good = asked && entry >= 0 && entry < a.num_pages;
+      if (asked && !good) report_error(a.err, PHOTON_DEV_BAD_PAGE, s, key, entry);
+      const int page = good ? entry : 0, sl = good ? key - pidx * a.page_size : 0;      // else some page of the pool: what is read there is not used
       const uint32_t begin16 = ((uint32_t)page * a.n_kv + head) * (uint32_t)(page_bytes >> 4);
-      to = begin16 + sl * (D / 32);
-      scales = begin16 + a.page_size * (D / 32) + sl * GROUPS / 16;
-      mask = __ballot_sync(0xffffffffu, good);
+      off = begin16 + sl * (D / 32);
+      sc16 = begin16 + a.page_size * (D / 32) + sl * GROUPS / 16;
+      ok = __ballot_sync(0xffffffffu, good);
     };
-    find(step0, off, sc16, ok);
-    // keys 8 o + g and values 8 o + 2 t, + 1; the scales of keys 8 o + g and of values 8 o + 2 t, + 1 for o = 2 u + (g & 1)
-    uint32_t kw[4][KW], vw[4][2][VW], ks[4], vs[2][2];
-    const uint8_t* k_codes = a.k + g * (D / 2) + 4 * GROUPS * t;
-    const uint8_t* v_codes = a.v + 2 * t * (D / 2) + 2 * GROUPS * g;
-    auto load_k = [&](int i) {                         // i: the step's place among the 8 that are known
+    look(step0);
+    uint32_t ok_use = 0;
+    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (KM_STAGES * STAGE);
+    int given = 0;                                     // steps asked for, stages in turn
+    uint32_t give_to = ring;
+    auto ask = [&]() {
+      if (step0 + given < step1) {
+        if ((given & 7) == 0) {
+          found(step0 + given);
+          look(step0 + given + 8);
+        }
+        const int i = given & 7;
+        if constexpr (GROUPS == 4) {
+          const uint32_t to = give_to + km_place<4>(lane >> 2, lane & 3);
 #pragma unroll
-      for (int o = 0; o < 4; ++o) {
-        km_load<KW>(kw[o], k_codes + __shfl_sync(0xffffffffu, off, 4 * i + o) * 16ull);
-        const uint8_t* p = a.k + g * GROUPS + __shfl_sync(0xffffffffu, sc16, 4 * i + o) * 16ull;
-        if constexpr (GROUPS == 4) km_load<1>(&ks[o], p); else ks[o] = km_load16(p);
+          for (int o = 0; o < 4; ++o) {
+            const uint32_t x = __shfl_sync(0xffffffffu, off, 4 * i + o) + lane;
+            km_copy(to + o * 512, km_at(a.k, x));
+            km_copy(to + 2048 + o * 512, km_at(a.v, x));
+          }
+          const uint32_t x = __shfl_sync(0xffffffffu, sc16, 4 * i + (lane >> 1 & 3)) + (lane & 1);
+          if (lane < 16) km_copy(give_to + 4096 + lane * 16, km_at(lane < 8 ? a.k : a.v, x));
+        } else {
+          const uint32_t to = give_to + (lane >> 4) * 256 + km_place<2>(lane >> 1 & 7, lane & 1);
+#pragma unroll
+          for (int o = 0; o < 4; o += 2) {
+            const uint32_t x = __shfl_sync(0xffffffffu, off, 4 * i + o + (lane >> 4)) + (lane & 15);
+            km_copy(to + o * 256, km_at(a.k, x));
+            km_copy(to + 1024 + o * 256, km_at(a.v, x));
+          }
+          const uint32_t x = __shfl_sync(0xffffffffu, sc16, 4 * i + (lane & 3));
+          if (lane < 8) km_copy(give_to + 2048 + lane * 16, km_at(lane < 4 ? a.k : a.v, x));
+        }
+        ++given;
+        give_to = give_to == ring + (KM_STAGES - 1) * STAGE ? ring : give_to + STAGE;
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto load_v = [&](int i) {
-#pragma unroll
-      for (int o = 0; o < 4; ++o) {
-        const uint8_t* p = v_codes + __shfl_sync(0xffffffffu, off, 4 * i + o) * 16ull;
-        km_load<VW>(vw[o][0], p);
-        km_load<VW>(vw[o][1], p + D / 2);
-      }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint8_t* p = a.v + 2 * t * GROUPS + __shfl_sync(0xffffffffu, sc16, 4 * i + 2 * u + (g & 1)) * 16ull;
-        if constexpr (GROUPS == 4) km_load<2>(vs[u], p);
-        else { uint32_t both; km_load<1>(&both, p); vs[u][0] = both & 0xffffu; vs[u][1] = both >> 16; }
-      }
-    };
-    load_k(0);
-    load_v(0);
-
     // ---- the queries: column g of the second operand is part g & 1 of row 4 x + g / 2
+    uint4 raw[NT][GROUPS];
+#pragma unroll
+    for (int x = 0; x < NT; ++x) {
+      const int r = 4 * x + (g >> 1), row = row0 + r;
+      const bf16* q = a.q + (R.first + row / G) * a.q_stride + (long)(head * G + row % G) * D + 8 * t;
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) {
+        raw[x][j] = make_uint4(0u, 0u, 0u, 0u);
+        if (r >= rows) continue;
+        if (a.q_vec) {
+          raw[x][j] = *(const uint4*)(q + 32 * j);
+        } else {
+          uint32_t w[4];
+          const uint16_t* p = (const uint16_t*)(q + 32 * j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[i] = p[2 * i] | (uint32_t)p[2 * i + 1] << 16;
+          raw[x][j] = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < KM_STAGES - 1; ++i) ask();
+
     uint32_t qb[NT][GROUPS][4];
     float init[NT][GROUPS], factor[NT];
     int place[NT];                                     // of row 4 x + t
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
-      const int r = 4 * x + (g >> 1), row = row0 + r;
-      const bool there = r < rows, second = g & 1;
-      const bf16* q = a.q + (there ? (R.first + row / G) * a.q_stride + (long)(head * G + row % G) * D : 0) + 8 * t;
+      const bool second = g & 1;
       float v[GROUPS][8];
       uint32_t top = 0;
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
-        if (a.q_vec) {
-          const uint4 u = *(const uint4*)(q + 32 * j);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        const uint32_t w[4] = {raw[x][j].x, raw[x][j].y, raw[x][j].z, raw[x][j].w};
 #pragma unroll
-          for (int i = 0; i < 4; ++i) { v[j][2 * i] = __uint_as_float(w[i] << 16); v[j][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-        } else {
+        for (int i = 0; i < 4; ++i) { v[j][2 * i] = __uint_as_float(w[i] << 16); v[j][2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) v[j][i] = __bfloat162float(q[32 * j + i]);
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          if (!there) v[j][i] = 0.f;
-          top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
-        }
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(v[j][i]) & 0x7fffffffu);
       }
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
@@ -251,30 +298,40 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       factor[x] = __shfl_sync(0xffffffffu, f, 8 * t);
       place[x] = 4 * x + t < rows ? base + (row0 + 4 * x + t) / G : -1;
     }
-    float acc[NT][GROUPS][2][4], ones[NT][4], m[NT], l[NT];
+    float acc[NT][GROUPS][2][4], m[NT], l[NT];
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
       m[x] = -INFINITY;
       l[x] = 0.f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        ones[x][i] = 0.f;
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j) acc[x][j][0][i] = acc[x][j][1][i] = 0.f;
       }
     }
     uint32_t bad[NT] = {};                             // bit j: row 4 x + g / 2 sees a value of group j that is no number
-    int top_e[GROUPS];                                 // the exponent of the largest scale so far: 15 is that of 1
+    uint32_t tops = 0x01010101u;                       // the exponents of each group's largest scale so far: 15 is that of 1
     uint32_t room = 0;                                 // what makes a byte with a larger exponent set its first bit, where that matters
     bool lifted = false;
-#pragma unroll
-    for (int j = 0; j < GROUPS; ++j) top_e[j] = 1;
 
+    uint32_t stage = ring;
+    const uint32_t k_at = km_place<GROUPS>(g, GROUPS == 4 ? t : t >> 1) + (GROUPS == 4 ? 0 : (t & 1) * 8);
+    const uint32_t v_at0 = 32 * ROW + km_place<GROUPS>(2 * t, GROUPS == 4 ? g >> 1 : g >> 2) + (GROUPS == 4 ? (g & 1) * 8 : (g & 3) * 4);
+    const uint32_t v_at1 = 32 * ROW + km_place<GROUPS>(2 * t + 1, GROUPS == 4 ? g >> 1 : g >> 2) + (GROUPS == 4 ? (g & 1) * 8 : (g & 3) * 4);
     for (int step = step0; step < step1; ++step) {
+      asm volatile("cp.async.wait_group %0;" ::"n"(KM_STAGES - 2) : "memory");
+      __syncwarp();                                    // this step's bytes are there, and the stage before it has been read by all
       const int i8 = (step - step0) & 7;
-      const uint32_t here = ok >> (4 * i8) & 15u;
-      if (i8 == 0) find(step + 8, off_next, sc16_next, ok_next);
-      const int key0 = key_w + step * KM_KEYS;
+      if (i8 == 0) ok_use = ok;
+      const uint32_t here = ok_use >> (4 * i8) & 15u;
+      ask();
+      const int key0 = R.from + step * KM_KEYS;
+      uint32_t kw[4][KW], ks[4];                       // keys 8 o + g and their scales
+#pragma unroll
+      for (int o = 0; o < 4; ++o) {
+        km_read<KW>(kw[o], stage + k_at + o * 8 * ROW);
+        if constexpr (GROUPS == 4) km_read<1>(&ks[o], stage + 64 * ROW + (8 * o + g) * 4); else ks[o] = km_read16(stage + 64 * ROW + (8 * o + g) * 2);
+      }
       // ---- scores of the keys 8 o + g for row 4 x + t
       float sc[NT][4];
 #pragma unroll
@@ -291,21 +348,22 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
             const uint32_t u0 = __byte_perm(w0, 0, 0x4341), u1 = __byte_perm(w1, 0, 0x4341);
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
-              float d[4] = {init[x][j], 0.f, init[x][j], 0.f};
-              km_mma(d, w0 & 0x00FF00FFu, w1 & 0x00FF00FFu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qb[x][j][0], qb[x][j][1]);
+              float d[4];
+              km_mma0(d, w0 & 0x00FF00FFu, w1 & 0x00FF00FFu, w0 & 0x00F000F0u, w1 & 0x00F000F0u, qb[x][j][0], qb[x][j][1]);
               km_mma(d, u0, u1, u0 & 0x00F000F0u, u1 & 0x00F000F0u, qb[x][j][2], qb[x][j][3]);
-              const float d0 = d[0] + d[1], d1 = d[2] + d[3];
+              const float d0 = d[0] + (d[1] + init[x][j]), d1 = d[2] + (d[3] + init[x][j]);
               sc[x][2 * i] = j == 0 ? (jx ? s0.y : s0.x) * d0 : fmaf(jx ? s0.y : s0.x, d0, sc[x][2 * i]);
               sc[x][2 * i + 1] = j == 0 ? (jx ? s1.y : s1.x) * d1 : fmaf(jx ? s1.y : s1.x, d1, sc[x][2 * i + 1]);
             }
           }
         }
       }
-      const bool more = step + 1 < step1;
-      const bool turn = i8 == 7;
-      if (more) {
-        if (turn) { off = off_next; sc16 = sc16_next; }
-        load_k((i8 + 1) & 7);
+      uint32_t vs[2][2];                               // scales of the values 8 o + 2 t, + 1 for o = 2 u + (g & 1)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t from = stage + 64 * ROW + 32 * GROUPS + (8 * (2 * u + (g & 1)) + 2 * t) * GROUPS;
+        if constexpr (GROUPS == 4) km_read<2>(vs[u], from);
+        else { uint32_t both; km_read<1>(&both, from); vs[u][0] = both & 0xffffu; vs[u][1] = both >> 16; }
       }
       // ---- the softmax
       const bool masked = here != 15u || key0 < clear_from || key0 + 31 > clear_to;
@@ -366,15 +424,14 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
             if (byte < 248) most = max(most, byte); else odd_scales = true;
           }
           most = __reduce_max_sync(0xffffffffu, most) >> 3;
-          const int was = top_e[j], to = max(was, most), old_lift = was > 15 || was < 8 ? 15 - was : 0, new_lift = to > 15 || to < 8 ? 15 - to : 0;
-          top_e[j] = to;
+          const int was = tops >> (8 * j) & 255, to = max(was, most), old_lift = was > 15 || was < 8 ? 15 - was : 0, new_lift = to > 15 || to < 8 ? 15 - to : 0;
+          tops += (uint32_t)(to - was) << (8 * j);
           if (new_lift != old_lift) {
             const float f = km_power(new_lift - old_lift);
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
 #pragma unroll
               for (int i = 0; i < 4; ++i) { acc[x][j][0][i] *= f; acc[x][j][1][i] *= f; }
-              if (g == j) { ones[x][0] *= f; ones[x][1] *= f; }
             }
           }
           lifted |= new_lift != 0;
@@ -388,7 +445,6 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
           l[x] *= alpha[x];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            ones[x][i] *= alpha[x];
 #pragma unroll
             for (int j = 0; j < GROUPS; ++j) { acc[x][j][0][i] *= alpha[x]; acc[x][j][1][i] *= alpha[x]; }
           }
@@ -416,6 +472,12 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
           pe[x] = g & 1 ? 0u : y;
           po[x] = g & 1 ? y : 0u;
         }
+        uint32_t vw[2][2][VW];                         // values 8 (2 u + o) + 2 t, + 1
+#pragma unroll
+        for (int o = 0; o < 2; ++o) {
+          km_read<VW>(vw[o][0], stage + v_at0 + (2 * u + o) * 8 * ROW);
+          km_read<VW>(vw[o][1], stage + v_at1 + (2 * u + o) * 8 * ROW);
+        }
 #pragma unroll
         for (int j = 0; j < GROUPS; ++j) {
           // the scales of its keys 2 t and 2 t + 1; the bytes between are a scale's first bit, 0 below 2
@@ -434,162 +496,169 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
                   }
                 }
             }
-            const float f = km_power(top_e[j] > 15 || top_e[j] < 8 ? 15 - top_e[j] : 0);
+            const int e = tops >> (8 * j) & 255;
+            const float f = km_power(e > 15 || e < 8 ? 15 - e : 0);
             s2 = km_mul2(s2, km_half2(f, f));
           }
-          const uint32_t r0 = __byte_perm(vw[2 * u][0][j / 2], vw[2 * u][1][j / 2], j & 1 ? 0x7632 : 0x5410);
-          const uint32_t r1 = __byte_perm(vw[2 * u + 1][0][j / 2], vw[2 * u + 1][1][j / 2], j & 1 ? 0x7632 : 0x5410);
-          const uint32_t t0 = __byte_perm(r0, 0, 0x4341), t1 = __byte_perm(r1, 0, 0x4341);
+          // of two keys each: numbers 0 and 1 of this lane's four, then 2 and 3, as 1024 + c0 + 16 c1 and 1024 + 16 c1; less what makes them c - 8
+          const uint32_t r0 = __byte_perm(vw[0][0][j / 2], vw[0][1][j / 2], j & 1 ? 0x7632 : 0x5410);
+          const uint32_t r1 = __byte_perm(vw[1][0][j / 2], vw[1][1][j / 2], j & 1 ? 0x7632 : 0x5410);
+          const uint32_t t0 = __byte_perm(r0, 0x64646464u, 0x4341), t1 = __byte_perm(r1, 0x64646464u, 0x4341);
+          const uint32_t e0 = km_add2((r0 & 0x00FF00FFu) | 0x64006400u, 0xE488E488u), h0 = km_add2((r0 & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
+          const uint32_t e1 = km_add2((r1 & 0x00FF00FFu) | 0x64006400u, 0xE488E488u), h1 = km_add2((r1 & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
+          const uint32_t e2 = km_add2(t0, 0xE488E488u), h2 = km_add2((t0 & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
+          const uint32_t e3 = km_add2(t1, 0xE488E488u), h3 = km_add2((t1 & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
             const uint32_t b0 = km_mul2(pe[x], s2), b1 = km_mul2(po[x], s2);
-            km_mma(acc[x][j][0], r0 & 0x00FF00FFu, r0 & 0x00F000F0u, r1 & 0x00FF00FFu, r1 & 0x00F000F0u, b0, b1);
-            km_mma(acc[x][j][1], t0, t0 & 0x00F000F0u, t1, t1 & 0x00F000F0u, b0, b1);
-            km_mma(ones[x], one[j], 0u, one[j], 0u, b0, b1);
+            km_mma(acc[x][j][0], e0, h0, e1, h1, b0, b1);
+            km_mma(acc[x][j][1], e2, h2, e3, h3, b0, b1);
           }
         }
       }
-      if (more) {
-        load_v((i8 + 1) & 7);
-        if (turn) ok = ok_next;
-      }
+      stage = stage == ring + (KM_STAGES - 1) * STAGE ? ring : stage + STAGE;
     }
-    // ---- the warps' results side by side
-    __syncthreads();
+    // ---- the results: the unit's, or a part of them
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    const bool whole = step0 == 0 && step1 == R.steps;
+    const long part = 2L * me + (pos == begin ? 0 : 1);
 #pragma unroll
     for (int x = 0; x < NT; ++x) {
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 4);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 8);
       l[x] += __shfl_xor_sync(0xffffffffu, l[x], 16);
       bad[x] = __reduce_or_sync(0xffffffffu, bad[x] << (8 * (g >> 1))) >> (8 * t);
-      const int row = 4 * x + t;
-      if (g == 0) { m_s[warp * RT + row] = m[x]; l_s[warp * RT + row] = l[x]; }
-      const float both = ones[x][0] + ones[x][1];
+      const int r = 4 * x + t, row = row0 + r, h = head * G + row % G;
+      const long token = R.first + row / G;
+      const bool there = r < rows;
+      float mul = 1.f;
+      if (whole) {
+        float top = m[x], total_l = l[x];
+        if (a.sinks != nullptr && there) {
+          const float sink = a.sinks[h] * 1.4426950408889634f;
+          top = fmaxf(top, sink);
+          mul = m[x] == -INFINITY ? 1.f : exp2f(m[x] - top);
+          total_l = total_l * mul + exp2f(sink - top + 15.f);
+        }
+        if (g == 0 && there && a.lse != nullptr) a.lse[token * a.n_q + h] = total_l == 0.f ? -INFINITY : (top - 15.f + log2f(total_l)) * 0.6931471805599453f;
+        mul = total_l == 0.f ? 0.f : mul / total_l;
+      } else if (g == 0) {
+        float* ml = a.scratch + 2L * N * RT * D + (part * RT + r) * 2;
+        ml[0] = m[x];
+        ml[1] = l[x];
+      }
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
-        const float eight = 8.f * __shfl_sync(0xffffffffu, both, 4 * j + t), f = bad[x] >> j & 1u ? NAN : km_power(top_e[j] > 15 || top_e[j] < 8 ? top_e[j] - 15 : 0);
+        const int e = tops >> (8 * j) & 255;
+        const float f = (bad[x] >> j & 1u ? NAN : km_power(e > 15 || e < 8 ? e - 15 : 0)) * mul;
+        float y[4];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          const float* c = acc[x][j][h];
+        for (int i = 0; i < 2; ++i) {
+          const float* c = acc[x][j][i];
           const float c1 = c[2] + c[3], c0 = c[0] + c[1] - c1;
-          *(float2*)&o_s[(warp * RT + row) * D + 32 * j + 4 * g + 2 * h] = make_float2((c0 * 16777216.f - eight) * f, (c1 * 1048576.f - eight) * f);
+          y[2 * i] = c0 * f;
+          y[2 * i + 1] = c1 * (0.0625f * f);
+        }
+        if (!whole) {
+          *(float4*)&a.scratch[(part * RT + r) * D + 32 * j + 4 * g] = make_float4(y[0], y[1], y[2], y[3]);
+        } else if (there) {
+          bf16* to = a.out + token * a.out_stride + (long)h * D + 32 * j + 4 * g;
+          const __nv_bfloat162 lo = __floats2bfloat162_rn(y[0], y[1]), hi = __floats2bfloat162_rn(y[2], y[3]);
+          if (a.out_vec) *(uint2*)to = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
+          else { to[0] = lo.x; to[1] = lo.y; to[2] = hi.x; to[3] = hi.y; }
         }
       }
     }
-    __syncthreads();
-    const bool whole = step0 == 0 && step1 == R.steps;
-    const long part = 2L * blockIdx.x + (pos == begin ? 0 : 1);
-    float* part_o = a.scratch + part * RT * D;
-    float* part_ml = a.scratch + 2L * N * RT * D + part * RT * 2;
-    for (int i = tid; i < rows * (D / 4); i += KM_THREADS) {
-      const int r = i / (D / 4), d4 = i - r * (D / 4), row = row0 + r, h = head * G + row % G;
-      const long token = R.first + row / G;
-      const float m0 = fmaxf(fmaxf(m_s[r], m_s[RT + r]), fmaxf(m_s[2 * RT + r], m_s[3 * RT + r]));
-      float top = m0;
-      if (whole && a.sinks != nullptr) top = fmaxf(top, a.sinks[h] * 1.4426950408889634f);
-      const float zero = top == -INFINITY ? 0.f : top;
-      float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
-      float total_l = 0.f;
-#pragma unroll
-      for (int w = 0; w < 4; ++w) {
-        const float lw = l_s[w * RT + r];
-        if (lw == 0.f) continue;
-        const float f = m_s[w * RT + r] == -INFINITY ? 1.f : exp2f(m_s[w * RT + r] - zero);
-        const float4 o = *(const float4*)&o_s[(w * RT + r) * D + 4 * d4];
-        total_l += lw * f;
-        sum.x += o.x * f; sum.y += o.y * f; sum.z += o.z * f; sum.w += o.w * f;
-      }
-      if (whole) {
-        if (a.sinks != nullptr) total_l += exp2f(a.sinks[h] * 1.4426950408889634f - zero + 15.f);
-        if (d4 == 0 && a.lse != nullptr) a.lse[token * a.n_q + h] = total_l == 0.f ? -INFINITY : (zero - 15.f + log2f(total_l)) * 0.6931471805599453f;
-        const float f = total_l == 0.f ? 0.f : 1.f / total_l;
-        bf16* to = a.out + token * a.out_stride + (long)h * D + 4 * d4;
-        to[0] = __float2bfloat16_rn(sum.x * f);
-        to[1] = __float2bfloat16_rn(sum.y * f);
-        to[2] = __float2bfloat16_rn(sum.z * f);
-        to[3] = __float2bfloat16_rn(sum.w * f);
-      } else {
-        *(float4*)&part_o[r * D + 4 * d4] = sum;
-        if (d4 == 0) { part_ml[2 * r] = top; part_ml[2 * r + 1] = total_l; }
-      }
-    }
     pos += step1 - step0;
-    __syncthreads();
   }
 }
 
-// Units that lie in several blocks.  A block has one row of a unit's tile.
+// Units that lie in several warps: a block has one.  A thread has four numbers of a row in every `pars`-th part, in ascending order; then the threads' sums are joined.
 template <int GROUPS, int NT>
-__global__ void __launch_bounds__(GROUPS * 32)
+__global__ void __launch_bounds__(1024, 1)
 kv4_mma_join_kernel(const Kv4MmaArgs a, int N) {
-  constexpr int D = GROUPS * 32, RT = 4 * NT;
-  __shared__ int sums[2][GROUPS];
+  constexpr int D = GROUPS * 32, RT = 4 * NT, ITEMS = RT * D / 4;
+  extern __shared__ __align__(16) float join_s[];     // [pars][ITEMS] of {4 sums}, then {maximum, sum of weights}
   pdl_wait();
-  const int s = blockIdx.z, head = blockIdx.y, row = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+  const int s = blockIdx.z, head = blockIdx.y, tile = blockIdx.x, tid = threadIdx.x, pars = blockDim.x / ITEMS, item = tid % ITEMS, par = tid / ITEMS;
+  const int before = a.before[s], after = a.before[s + 1], total = a.before[a.S];
   const KmRequest R = km_request<RT>(a, s);
-  if (row >= R.rows) return;
-  int before = 0, total = 0;
-  for (int i = tid; i < a.S; i += D) {
-    const KmRequest r = km_request<RT>(a, i);
-    const int x = r.steps * r.row_tiles * a.n_kv;
-    total += x;
-    if (i < s) before += x;
-  }
-  before = __reduce_add_sync(0xffffffffu, before);
-  total = __reduce_add_sync(0xffffffffu, total);
-  if (lane == 0) { sums[0][warp] = before; sums[1][warp] = total; }
-  __syncthreads();
-  before = total = 0;
-#pragma unroll
-  for (int i = 0; i < GROUPS; ++i) { before += sums[0][i]; total += sums[1][i]; }
-  const int from = before + (head * R.row_tiles + row / RT) * R.steps, to = from + R.steps;
-  // the block that has step x: the last one that begins at or before it
-  auto block_of = [&](int x) {
-    int b = (int)((long)x * N / total);
-    while (b + 1 < N && (long)total * (b + 1) / N <= x) ++b;
-    while ((long)total * b / N > x) --b;
-    return b;
+  if (after == before || tile >= R.row_tiles) return;
+  const int from = before + (head * R.row_tiles + tile) * R.steps, to = from + R.steps;
+  // the warp that has step x: the last one that begins at or before it
+  auto warp_of = [&](int x) {
+    int w = (int)((long)x * N / total);
+    while (w + 1 < N && (long)total * (w + 1) / N <= x) ++w;
+    while ((long)total * w / N > x) --w;
+    return w;
   };
-  const int b0 = block_of(from), b1 = block_of(to - 1);
-  if (b0 == b1) return;
-  const int r = row % RT, G = a.n_q / a.n_kv, h = head * G + row % G;
+  const int w0 = warp_of(from), w1 = warp_of(to - 1);
+  if (w0 == w1) return;
+  const int r = item / (D / 4), d4 = item - r * (D / 4), row0 = tile * RT, row = row0 + r, G = a.n_q / a.n_kv, h = head * G + row % G;
+  const bool there = row < R.rows;
   const float* part_ml = a.scratch + 2L * N * RT * D;
-  const float sink = a.sinks != nullptr ? a.sinks[h] * 1.4426950408889634f : -INFINITY;
-  auto part_of = [&](int b) { return 2L * b + ((long)total * b / N >= from ? 0 : 1); };
-  float m = sink;
-  for (int b = b0; b <= b1; ++b) if ((long)total * b / N < (long)total * (b + 1) / N) m = fmaxf(m, part_ml[(part_of(b) * RT + r) * 2]);
-  const float zero = m == -INFINITY ? 0.f : m;
-  float l = a.sinks != nullptr ? exp2f(sink - zero + 15.f) : 0.f, sum = 0.f;
-  for (int b = b0; b <= b1; ++b) {
-    if ((long)total * b / N >= (long)total * (b + 1) / N) continue;
-    const long part = part_of(b);
-    const float pm = part_ml[(part * RT + r) * 2], pl = part_ml[(part * RT + r) * 2 + 1], o = a.scratch[(part * RT + r) * D + tid];
-    if (pl == 0.f) continue;
-    const float f = pm == -INFINITY ? 1.f : exp2f(pm - zero);
-    l += pl * f;
-    sum += o * f;
+  float m = -INFINITY, l = 0.f;
+  float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float pm, float pl, float4 o) {
+    if (pl == 0.f) return;                            // a part of which the row sees nothing
+    const float top = fmaxf(m, pm);
+    const float f = m == -INFINITY ? 1.f : exp2f(m - top), k = pm == -INFINITY ? 1.f : exp2f(pm - top);      // no maximum and yet a sum: it is no number
+    l = l * f + pl * k;
+    sum.x = sum.x * f + o.x * k; sum.y = sum.y * f + o.y * k; sum.z = sum.z * f + o.z * k; sum.w = sum.w * f + o.w * k;
+    m = top;
+  };
+#pragma unroll 4
+  for (int w = w0 + par; w <= w1; w += pars) {
+    const long begin = (long)total * w / N, end = (long)total * (w + 1) / N;
+    if (begin >= end) continue;
+    const long part = (2L * w + (begin >= from ? 0 : 1)) * RT + r;
+    const float2 ml = *(const float2*)&part_ml[part * 2];
+    add(ml.x, ml.y, *(const float4*)&a.scratch[part * D + 4 * d4]);
+  }
+  float2* ml_s = (float2*)(join_s + 4 * pars * ITEMS);
+  ((float4*)join_s)[tid] = sum;
+  ml_s[tid] = make_float2(m, l);
+  __syncthreads();
+  if (par > 0 || !there) return;
+  for (int p = 1; p < pars; ++p) add(ml_s[p * ITEMS + item].x, ml_s[p * ITEMS + item].y, ((float4*)join_s)[p * ITEMS + item]);
+  float mul = 1.f;
+  if (a.sinks != nullptr) {
+    const float sink = a.sinks[h] * 1.4426950408889634f, top = fmaxf(m, sink);
+    mul = m == -INFINITY ? 1.f : exp2f(m - top);
+    l = l * mul + exp2f(sink - top + 15.f);
+    m = top;
   }
   const long token = R.first + row / G;
-  if (tid == 0 && a.lse != nullptr) a.lse[token * a.n_q + h] = l == 0.f ? -INFINITY : (zero - 15.f + log2f(l)) * 0.6931471805599453f;
-  a.out[token * a.out_stride + (long)h * D + tid] = __float2bfloat16_rn(l == 0.f ? 0.f : sum / l);
+  if (d4 == 0 && a.lse != nullptr) a.lse[token * a.n_q + h] = l == 0.f ? -INFINITY : (m - 15.f + log2f(l)) * 0.6931471805599453f;
+  mul = l == 0.f ? 0.f : mul / l;
+  bf16* out = a.out + token * a.out_stride + (long)h * D + 4 * d4;
+  const __nv_bfloat162 lo = __floats2bfloat162_rn(sum.x * mul, sum.y * mul), hi = __floats2bfloat162_rn(sum.z * mul, sum.w * mul);
+  if (a.out_vec) *(uint2*)out = make_uint2(*(const uint32_t*)&lo, *(const uint32_t*)&hi);
+  else { out[0] = lo.x; out[1] = lo.y; out[2] = hi.x; out[3] = hi.y; }
 }
 
 template <int GROUPS, int NT, bool CAP>
-static int km_launch(const Kv4MmaArgs& a, int N, int max_rows, cudaStream_t stream) {
+static int km_launch(const Kv4MmaArgs& a, int blocks, int max_rows, cudaStream_t stream) {
   constexpr int RT = 4 * NT;
-  const size_t smem = (4 * RT * GROUPS * 32 + 8 * RT) * sizeof(float) + (a.S + 1) * sizeof(int);
+  constexpr size_t stages = 4 * KM_STAGES * (64 * GROUPS * 16 + 64 * GROUPS);
   static bool set = false;
   if (!set) {
-    const cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (4 * RT * GROUPS * 32 + 8 * RT) * 4 + (KM_MAX_SEQS + 1) * 4);
+    cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages + (KM_MAX_SEQS + 1) * sizeof(int)));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     if (e != cudaSuccess) return (int)e;
     set = true;
   }
-  int status = launch_pdl(kv4_mma_kernel<GROUPS, NT, CAP>, dim3(N), dim3(KM_THREADS), smem, stream, a);
+  const int status = launch_pdl(kv4_mma_kernel<GROUPS, NT, CAP>, dim3(blocks), dim3(KM_THREADS), stages + (a.S + 1) * sizeof(int), stream, a);
   if (status != 0) return status;
-  return launch_pdl(kv4_mma_join_kernel<GROUPS, NT>, dim3(max_rows, a.n_kv, a.S), dim3(GROUPS * 32), 0, stream, a, N);
+  // threads by the parts that a unit has, about
+  const int tiles = (max_rows + RT - 1) / RT;
+  const long parts = 4L * blocks / ((long)a.S * a.n_kv * tiles);
+  const int threads = parts > 24 ? 1024 : 256;
+  return launch_pdl(kv4_mma_join_kernel<GROUPS, NT>, dim3(tiles, a.n_kv, a.S), dim3(threads), threads * 6 * sizeof(float), stream, a, 4 * blocks);
 }
 
-// parts: blocks; scratch: 2 * parts * RT * (d + 2) floats, RT = 4 for up to 4 rows, else 8.
+// parts: blocks; scratch: 8 * parts * RT * (d + 2) + S + 1 words, RT = 4 for up to 4 rows, else 8.
 PHOTON_API int photon_kv4_attention_mma(const photon_kv4_attention_call* c, cudaStream_t stream) {
   if (c->S <= 0 || c->max_tokens_per_seq <= 0) return 0;
   if (c->dtype != PHOTON_BF16 || c->n_kv <= 0 || c->n_q <= 0 || c->n_q % c->n_kv || c->max_pages <= 0) return PHOTON_ERR_ARGUMENT;
@@ -598,9 +667,11 @@ PHOTON_API int photon_kv4_attention_mma(const photon_kv4_attention_call* c, cuda
   if (kv4_page_bytes(c->page_size, c->d) / 16 * c->num_pages * c->n_kv > 0xffffffffL) return PHOTON_ERR_UNSUPPORTED;      // a key's place in 16 bytes: 32 bits
   if (c->parts < 1 || c->scratch == nullptr) return PHOTON_ERR_ARGUMENT;
   const int rows = c->max_tokens_per_seq * (c->n_q / c->n_kv), most = rows < c->max_rows ? rows : c->max_rows;
+  const long words = 8L * c->parts * (most <= 4 ? 4 : 8) * (c->d + 2);
   const Kv4MmaArgs a = {(const bf16*)c->q, (bf16*)c->out, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->block_table, c->cu_tokens, c->context_lens, c->sinks, c->lse,
-                        c->scratch, c->err, c->q_stride, c->out_stride, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, c->min_rows,
-                        c->max_rows, (uintptr_t)c->q % 16 == 0 && c->q_stride % 8 == 0};
+                        c->scratch, (int*)c->scratch + words, c->err, c->q_stride, c->out_stride, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, c->min_rows,
+                        c->max_rows, (uintptr_t)c->q % 16 == 0 && c->q_stride % 8 == 0,
+                        (uintptr_t)c->out % 8 == 0 && c->out_stride % 4 == 0};
 #define ATTEND(GROUPS, NT) (c->softcap > 0.f ? km_launch<GROUPS, NT, true>(a, c->parts, most, stream) : km_launch<GROUPS, NT, false>(a, c->parts, most, stream))
   if (c->d == 64) return most <= 4 ? ATTEND(2, 1) : ATTEND(2, 2);
   return most <= 4 ? ATTEND(4, 1) : ATTEND(4, 2);

@@ -661,8 +661,8 @@ typedef struct {
 PHOTON_EXPORT int photon_kv4_attention(const photon_kv4_attention_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ kv4_attention_mma.cu: the same on the tensor cores, bfloat16, d 64 or 128 */
-/* At most 1,024 requests, pages of a multiple of 8 tokens, caches of up to 64 GB each.  parts: blocks of the grid; scratch: 2 * parts * R * (d + 2) floats, R = 4 for at most 4
- * rows a request, else 8. */
+/* At most 1,024 requests, pages of a multiple of 8 tokens, caches of up to 64 GB each.  parts: blocks of the grid; scratch: 8 * parts * R * (d + 2) + S + 1 words, R = 4 for at
+ * most 4 rows a request, else 8. */
 PHOTON_EXPORT int photon_kv4_attention_mma(const photon_kv4_attention_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ key_weights.cu */
