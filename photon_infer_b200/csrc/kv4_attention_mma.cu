@@ -21,6 +21,8 @@
 #define KM_THREADS 128
 #define KM_KEYS 32               // of a warp's step
 #define KM_MAX_SEQS 1024
+// Blocks an SM: what their registers leave room for.
+#define KM_BLOCKS(GROUPS, NT) ((GROUPS == 4 ? 4 : 5) - NT)
 #define KM_STAGES 3              // of a warp's 32 keys and values in shared memory
 
 struct Kv4MmaArgs {
@@ -29,6 +31,7 @@ struct Kv4MmaArgs {
   long q_stride, out_stride;
   int max_pages, S, n_q, n_kv, page_size, num_pages, window;
   float scale, softcap;
+  int page_shift;                // of page_size / 8, or -1
   int min_rows, max_rows, q_vec, out_vec;      // rows of q on 16-byte boundaries, of out on 8-byte ones
 };
 
@@ -118,7 +121,7 @@ __device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
 
 // GROUPS: of 32 numbers of a head (2 or 4); NT: tiles of 4 rows; CAP: bounded scores.
 template <int GROUPS, int NT, bool CAP>
-__global__ void __launch_bounds__(KM_THREADS, 5 - NT)
+__global__ void __launch_bounds__(KM_THREADS, KM_BLOCKS(GROUPS, NT))
 kv4_mma_kernel(const Kv4MmaArgs a) {
   constexpr int D = GROUPS * 32, RT = 4 * NT, KW = GROUPS, VW = GROUPS / 2;      // words of a key's and of a value's piece
   constexpr int ROW = D / 2, STAGE = 64 * ROW + 64 * GROUPS;      // codes of 32 keys, of 32 values, their scales
@@ -157,8 +160,14 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
     s = lo;
   }
   const int G = a.n_q / a.n_kv;
-  const long page_bytes = (long)a.page_size * GROUPS * 17;
+  const uint32_t page16 = (uint32_t)a.page_size * GROUPS * 17 / 16;
   const float cap_in = 2.f * 1.4426950408889634f / a.softcap, cap_out = a.softcap * 1.4426950408889634f;
+  // constants that stay in registers: two of them in one instruction do not fit, and the compiler would make them again for each
+  uint32_t c_1024, c_64, c_both, c_high;
+  asm volatile("mov.u32 %0, 0x64006400;" : "=r"(c_1024));
+  asm volatile("mov.u32 %0, 0x64646464;" : "=r"(c_64));
+  asm volatile("mov.u32 %0, 0xE488E488;" : "=r"(c_both));      // -1160 twice
+  asm volatile("mov.u32 %0, 0xE480E480;" : "=r"(c_high));      // -1152 twice
   for (int pos = begin; pos < end;) {
     while (before_s[s + 1] <= pos) ++s;
     const KmRequest R = km_request<RT>(a, s);
@@ -171,24 +180,22 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
     // ---- where the keys are: lane 4 i + o has the 8 keys o of step i's 32, 8 steps at a time
     // off: where the 8 keys' codes begin, in 16 bytes; sc: where their scales do
     uint32_t off = 0, sc16 = 0, ok = 0;
-    int entry = -1;                                   // of the block table, for the 8 steps behind those that are known
+    int entry = -1, place8 = 0;                       // the block table's entry and which 8 of the page
+    const int eight0 = (R.from >> 3) + lane;
     auto look = [&](int step) {
-      const int key = R.from + (step + (lane >> 2)) * KM_KEYS + (lane & 3) * 8, pidx = key / a.page_size;
-      entry = -1;
-      if (step + (lane >> 2) < step1 && key <= last_place) {
-        if (pidx < a.max_pages) entry = a.table[(long)s * a.max_pages + pidx];
-        if (pidx >= a.max_pages) report_error(a.err, PHOTON_DEV_BAD_PAGE, s, key, -1);
-      }
+      const int eight = eight0 + step * 4;
+      const int pidx = a.page_shift >= 0 ? eight >> a.page_shift : eight / (a.page_size >> 3);
+      place8 = eight - pidx * (a.page_size >> 3);
+      entry = -2;                                     // not asked for
+      if (step + (lane >> 2) < step1 && eight * 8 <= last_place) entry = pidx < a.max_pages ? a.table[(long)s * a.max_pages + pidx] : -1;
     };
     auto found = [&](int step) {
-      const int key = R.from + (step + (lane >> 2)) * KM_KEYS + (lane & 3) * 8, pidx = key / a.page_size;
-      const bool asked = step + (lane >> 2) < step1 && key <= last_place && pidx < a.max_pages, good = asked && entry >= 0 && entry < a.num_pages;
-      if (asked && !good) report_error(a.err, PHOTON_DEV_BAD_PAGE, s, key, entry);
-      const int page = good ? entry : 0, sl = good ? key - pidx * a.page_size : 0;      // else some page of the pool: what is read there is not used
-      const uint32_t begin16 = ((uint32_t)page * a.n_kv + head) * (uint32_t)(page_bytes >> 4);
-      off = begin16 + sl * (D / 32);
-      sc16 = begin16 + a.page_size * (D / 32) + sl * GROUPS / 16;
+      const bool good = entry >= 0 && entry < a.num_pages;
       ok = __ballot_sync(0xffffffffu, good);
+      if (!good && entry != -2) report_error(a.err, PHOTON_DEV_BAD_PAGE, s, (eight0 + step * 4) * 8, entry);
+      const uint32_t begin16 = ((uint32_t)(good ? entry : 0) * a.n_kv + head) * page16;      // else some page of the pool: what is read there is not used
+      off = begin16 + place8 * (D / 4);
+      sc16 = begin16 + a.page_size * (D / 32) + place8 * GROUPS / 2;
     };
     look(step0);
     uint32_t ok_use = 0;
@@ -439,6 +446,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         }
         odd_scales = __any_sync(0xffffffffu, odd_scales);
       }
+      const bool special = rare || lifted;
       if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
@@ -478,17 +486,19 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
           km_read<VW>(vw[o][0], stage + v_at0 + (2 * u + o) * 8 * ROW);
           km_read<VW>(vw[o][1], stage + v_at1 + (2 * u + o) * 8 * ROW);
         }
+        // the scales of its keys 2 t and 2 t + 1; the bytes between are a scale's first bit, 0 below 2
+        uint32_t s2[GROUPS];
 #pragma unroll
-        for (int j = 0; j < GROUPS; ++j) {
-          // the scales of its keys 2 t and 2 t + 1; the bytes between are a scale's first bit, 0 below 2
-          uint32_t s2 = km_bytes(vs[u][0], vs[u][1], j == 0 ? 0x4C08 : j == 1 ? 0x5D19 : j == 2 ? 0x6E2A : 0x7F3B) >> 1;
-          if (rare || lifted) {
-            s2 &= 0x7F807F80u;
-            if (odd_scales) {                          // no number goes into the sums, where it would meet the zeros beside the ones: who sees it is noted
+        for (int j = 0; j < GROUPS; ++j) s2[j] = km_bytes(vs[u][0], vs[u][1], j == 0 ? 0x4C08 : j == 1 ? 0x5D19 : j == 2 ? 0x6E2A : 0x7F3B) >> 1;
+        if (special) {
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) {
+            s2[j] &= 0x7F807F80u;
+            if (odd_scales) {                          // no number goes into the products, where it would meet rows that do not see it: who does is noted
 #pragma unroll
               for (int h = 0; h < 2; ++h)
-                if ((s2 >> (16 * h) & 0x7fffu) >= 0x7c00u) {
-                  s2 &= h ? 0x0000ffffu : 0xffff0000u;
+                if ((s2[j] >> (16 * h) & 0x7fffu) >= 0x7c00u) {
+                  s2[j] &= h ? 0x0000ffffu : 0xffff0000u;
 #pragma unroll
                   for (int x = 0; x < NT; ++x) {
                     const int r = 4 * x + (g >> 1), key = key0 + 16 * u + 8 * (g & 1) + 2 * t + h, at_place = base + (row0 + r) / G;
@@ -498,19 +508,22 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
             }
             const int e = tops >> (8 * j) & 255;
             const float f = km_power(e > 15 || e < 8 ? 15 - e : 0);
-            s2 = km_mul2(s2, km_half2(f, f));
+            s2[j] = km_mul2(s2[j], km_half2(f, f));
           }
+        }
+#pragma unroll
+        for (int j = 0; j < GROUPS; ++j) {
           // of two keys each: numbers 0 and 1 of this lane's four, then 2 and 3, as 1024 + c0 + 16 c1 and 1024 + 16 c1; less what makes them c - 8
           const uint32_t r0 = __byte_perm(vw[0][0][j / 2], vw[0][1][j / 2], j & 1 ? 0x7632 : 0x5410);
           const uint32_t r1 = __byte_perm(vw[1][0][j / 2], vw[1][1][j / 2], j & 1 ? 0x7632 : 0x5410);
-          const uint32_t t0 = __byte_perm(r0, 0x64646464u, 0x4341), t1 = __byte_perm(r1, 0x64646464u, 0x4341);
-          const uint32_t e0 = km_add2((r0 & 0x00FF00FFu) | 0x64006400u, 0xE488E488u), h0 = km_add2((r0 & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
-          const uint32_t e1 = km_add2((r1 & 0x00FF00FFu) | 0x64006400u, 0xE488E488u), h1 = km_add2((r1 & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
-          const uint32_t e2 = km_add2(t0, 0xE488E488u), h2 = km_add2((t0 & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
-          const uint32_t e3 = km_add2(t1, 0xE488E488u), h3 = km_add2((t1 & 0x00F000F0u) | 0x64006400u, 0xE480E480u);
+          const uint32_t t0 = __byte_perm(r0, c_64, 0x4341), t1 = __byte_perm(r1, c_64, 0x4341);
+          const uint32_t e0 = km_add2((r0 & 0x00FF00FFu) | c_1024, c_both), h0 = km_add2((r0 & 0x00F000F0u) | c_1024, c_high);
+          const uint32_t e1 = km_add2((r1 & 0x00FF00FFu) | c_1024, c_both), h1 = km_add2((r1 & 0x00F000F0u) | c_1024, c_high);
+          const uint32_t e2 = km_add2(t0, c_both), h2 = km_add2((t0 & 0x00F000F0u) | c_1024, c_high);
+          const uint32_t e3 = km_add2(t1, c_both), h3 = km_add2((t1 & 0x00F000F0u) | c_1024, c_high);
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
-            const uint32_t b0 = km_mul2(pe[x], s2), b1 = km_mul2(po[x], s2);
+            const uint32_t b0 = km_mul2(pe[x], s2[j]), b1 = km_mul2(po[x], s2[j]);
             km_mma(acc[x][j][0], e0, h0, e1, h1, b0, b1);
             km_mma(acc[x][j][1], e2, h2, e3, h3, b0, b1);
           }
@@ -667,10 +680,12 @@ PHOTON_API int photon_kv4_attention_mma(const photon_kv4_attention_call* c, cuda
   if (kv4_page_bytes(c->page_size, c->d) / 16 * c->num_pages * c->n_kv > 0xffffffffL) return PHOTON_ERR_UNSUPPORTED;      // a key's place in 16 bytes: 32 bits
   if (c->parts < 1 || c->scratch == nullptr) return PHOTON_ERR_ARGUMENT;
   const int rows = c->max_tokens_per_seq * (c->n_q / c->n_kv), most = rows < c->max_rows ? rows : c->max_rows;
+  int shift = -1;
+  for (int i = 0; i < 28; ++i) if (c->page_size == 8 << i) shift = i;
   const long words = 8L * c->parts * (most <= 4 ? 4 : 8) * (c->d + 2);
   const Kv4MmaArgs a = {(const bf16*)c->q, (bf16*)c->out, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->block_table, c->cu_tokens, c->context_lens, c->sinks, c->lse,
-                        c->scratch, (int*)c->scratch + words, c->err, c->q_stride, c->out_stride, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, c->min_rows,
-                        c->max_rows, (uintptr_t)c->q % 16 == 0 && c->q_stride % 8 == 0,
+                        c->scratch, (int*)c->scratch + words, c->err, c->q_stride, c->out_stride, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, shift,
+                        c->min_rows, c->max_rows, (uintptr_t)c->q % 16 == 0 && c->q_stride % 8 == 0,
                         (uintptr_t)c->out % 8 == 0 && c->out_stride % 4 == 0};
 #define ATTEND(GROUPS, NT) (c->softcap > 0.f ? km_launch<GROUPS, NT, true>(a, c->parts, most, stream) : km_launch<GROUPS, NT, false>(a, c->parts, most, stream))
   if (c->d == 64) return most <= 4 ? ATTEND(2, 1) : ATTEND(2, 2);

@@ -2953,7 +2953,7 @@ def _kv4_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: in
     if dtype == torch.bfloat16 and head_dim in (64, 128) and page_size % 8 == 0 and 0 < page_heads * kv4_page_bytes(page_size, head_dim) < 1 << 36 and num_seqs <= 1024:
         tile = 4 if rows <= 4 else 8
         units = num_seqs * n_kv * -(-rows // tile)
-        parts = min((4 if tile == 4 else 3) * sms, -(-units * (-(-keys // 32) + 1) // 4))
+        parts = min((5 - head_dim // 64 - (tile == 8)) * sms, -(-units * (-(-keys // 32) + 1) // 4))
         return "kv4_attention_mma", parts, 8 * parts * tile * (head_dim + 2) + num_seqs + 1
     tiles, blocks = -(-keys // 128), num_seqs * n_kv * -(-rows // 8)
     parts = max(1, min(tiles, 4 * sms // blocks, 64))
