@@ -119,6 +119,17 @@ __device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
   return r;
 }
 
+// Steps in equal runs, the first ones a step longer.
+struct KmRuns {
+  int each, longer;
+  __device__ __forceinline__ KmRuns(int total, int warps) : each(total / warps), longer(total - total / warps * warps) {}
+  __device__ __forceinline__ int begin(int w) const { return w * each + min(w, longer); }
+  __device__ __forceinline__ int warp_of(int step) const {
+    const int first = longer * (each + 1);
+    return step < first ? step / (each + 1) : longer + (step - first) / each;
+  }
+};
+
 // GROUPS: of 32 numbers of a head (2 or 4); NT: tiles of 4 rows; CAP: bounded scores.
 template <int GROUPS, int NT, bool CAP>
 __global__ void __launch_bounds__(KM_THREADS, KM_BLOCKS(GROUPS, NT))
@@ -151,7 +162,8 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
   __syncthreads();
   pdl_launch_dependents();
   const int total = before_s[a.S], N = gridDim.x * 4, me = blockIdx.x * 4 + warp;
-  const int begin = (int)((long)total * me / N), end = (int)((long)total * (me + 1) / N);
+  const KmRuns runs(total, N);
+  const int begin = runs.begin(me), end = runs.begin(me + 1);
   if (begin >= end) return;
   int s = 0;
   {                                                   // the request of the first step: the last one that begins at or before it
@@ -599,14 +611,8 @@ kv4_mma_join_kernel(const Kv4MmaArgs a, int N) {
   const KmRequest R = km_request<RT>(a, s);
   if (after == before || tile >= R.row_tiles) return;
   const int from = before + (head * R.row_tiles + tile) * R.steps, to = from + R.steps;
-  // the warp that has step x: the last one that begins at or before it
-  auto warp_of = [&](int x) {
-    int w = (int)((long)x * N / total);
-    while (w + 1 < N && (long)total * (w + 1) / N <= x) ++w;
-    while ((long)total * w / N > x) --w;
-    return w;
-  };
-  const int w0 = warp_of(from), w1 = warp_of(to - 1);
+  const KmRuns runs(total, N);
+  const int w0 = runs.warp_of(from), w1 = runs.warp_of(to - 1);
   if (w0 == w1) return;
   const int r = item / (D / 4), d4 = item - r * (D / 4), row0 = tile * RT, row = row0 + r, G = a.n_q / a.n_kv, h = head * G + row % G;
   const bool there = row < R.rows;
@@ -621,13 +627,21 @@ kv4_mma_join_kernel(const Kv4MmaArgs a, int N) {
     sum.x = sum.x * f + o.x * k; sum.y = sum.y * f + o.y * k; sum.z = sum.z * f + o.z * k; sum.w = sum.w * f + o.w * k;
     m = top;
   };
-#pragma unroll 4
-  for (int w = w0 + par; w <= w1; w += pars) {
-    const long begin = (long)total * w / N, end = (long)total * (w + 1) / N;
-    if (begin >= end) continue;
-    const long part = (2L * w + (begin >= from ? 0 : 1)) * RT + r;
-    const float2 ml = *(const float2*)&part_ml[part * 2];
-    add(ml.x, ml.y, *(const float4*)&a.scratch[part * D + 4 * d4]);
+  for (int w = w0 + par; w <= w1; w += 8 * pars) {   // eight parts under way
+    float2 ml[8];
+    float4 o[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const int at = w + i * pars;
+      ml[i] = make_float2(-INFINITY, 0.f);
+      if (at <= w1) {
+        const long part = (2L * at + (runs.begin(at) >= from ? 0 : 1)) * RT + r;
+        ml[i] = *(const float2*)&part_ml[part * 2];
+        o[i] = *(const float4*)&a.scratch[part * D + 4 * d4];
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) add(ml[i].x, ml[i].y, o[i]);
   }
   float2* ml_s = (float2*)(join_s + 4 * pars * ITEMS);
   ((float4*)join_s)[tid] = sum;
