@@ -18,6 +18,8 @@
 #include "kv4.cuh"
 #include <math.h>
 
+#pragma nv_diag_suppress 128      // what keys got has no use for the second half of the loop
+
 #define KM_THREADS 128
 #define KM_KEYS 32               // of a warp's step
 #define KM_MAX_SEQS 1024
@@ -32,6 +34,7 @@ struct Kv4MmaArgs {
   int max_pages, S, n_q, n_kv, page_size, num_pages, window;
   float scale, softcap;
   int page_shift;                // of page_size / 8, or -1
+  float* weights; const int* held;      // the second use: what keys got, beside them
   int min_rows, max_rows, q_vec, out_vec;      // rows of q on 16-byte boundaries, of out on 8-byte ones
 };
 
@@ -104,7 +107,7 @@ __device__ __forceinline__ int km_place(int r, int c) {
 
 // A request's place in the work: rows, row tiles, keys from..to (from a multiple of 8), steps of 32 keys.
 struct KmRequest { int first, n, ctx, rows, row_tiles, from, steps; };
-template <int RT>
+template <int RT, bool WEIGH>
 __device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
   KmRequest r;
   r.first = a.cu_tokens[s];
@@ -113,7 +116,8 @@ __device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
   r.rows = r.n * (a.n_q / a.n_kv);
   if (r.rows <= a.min_rows || r.rows > a.max_rows) r.rows = 0;
   r.row_tiles = (r.rows + RT - 1) / RT;
-  const int lo = a.window > 0 ? max(0, r.ctx - r.n - a.window + 1) : 0;
+  int lo = a.window > 0 ? max(0, r.ctx - r.n - a.window + 1) : 0;
+  if (WEIGH) lo = max(0, min(lo, a.held != nullptr ? a.held[s] : r.ctx - r.n));      // keys without a sum get one
   r.from = lo & ~7;
   r.steps = r.rows > 0 ? max(1, (r.ctx - r.from + KM_KEYS - 1) / KM_KEYS) : 0;
   return r;
@@ -131,11 +135,12 @@ struct KmRuns {
 };
 
 // GROUPS: of 32 numbers of a head (2 or 4); NT: tiles of 4 rows; CAP: bounded scores.
-template <int GROUPS, int NT, bool CAP>
-__global__ void __launch_bounds__(KM_THREADS, KM_BLOCKS(GROUPS, NT))
+// WEIGH: no values.  With every row's logarithm known, a key's sum over the rows is added to the one beside it: lane (g, t) has key 8 t + g of a step.
+template <int GROUPS, int NT, bool CAP, bool WEIGH>
+__global__ void __launch_bounds__(KM_THREADS, WEIGH ? 4 : KM_BLOCKS(GROUPS, NT))
 kv4_mma_kernel(const Kv4MmaArgs a) {
   constexpr int D = GROUPS * 32, RT = 4 * NT, KW = GROUPS, VW = GROUPS / 2;      // words of a key's and of a value's piece
-  constexpr int ROW = D / 2, STAGE = 64 * ROW + 64 * GROUPS;      // codes of 32 keys, of 32 values, their scales
+  constexpr int ROW = D / 2, CODES = (WEIGH ? 32 : 64) * ROW, STAGE = CODES + CODES / 16;      // codes of 32 keys, of 32 values, their scales
   extern __shared__ __align__(16) uint8_t smem[];     // the four warps' stages
   int* before_s = (int*)(smem + 4 * KM_STAGES * STAGE);      // [S + 1] units' steps in front of a request
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
@@ -144,7 +149,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
     int sum = 0;
     for (int s0 = 0; s0 < a.S; s0 += 32) {
       int x = 0;
-      if (s0 + lane < a.S) { const KmRequest r = km_request<RT>(a, s0 + lane); x = r.steps * r.row_tiles * a.n_kv; }
+      if (s0 + lane < a.S) { const KmRequest r = km_request<RT, WEIGH>(a, s0 + lane); x = r.steps * r.row_tiles * a.n_kv; }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, x, o);
@@ -154,7 +159,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       sum += __shfl_sync(0xffffffffu, x, 31);
     }
     if (lane == 0) before_s[0] = 0;
-    if (blockIdx.x == 0) {                            // for the second kernel
+    if (!WEIGH && blockIdx.x == 0) {                  // for the second kernel
       __syncwarp();
       for (int i = lane; i <= a.S; i += 32) a.before[i] = before_s[i];
     }
@@ -182,7 +187,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
   asm volatile("mov.u32 %0, 0xE480E480;" : "=r"(c_high));      // -1152 twice
   for (int pos = begin; pos < end;) {
     while (before_s[s + 1] <= pos) ++s;
-    const KmRequest R = km_request<RT>(a, s);
+    const KmRequest R = km_request<RT, WEIGH>(a, s);
     const int at = pos - before_s[s], unit = at / R.steps, step0 = at - unit * R.steps, step1 = min(R.steps, step0 + end - pos);
     const int head = unit / R.row_tiles, row0 = (unit - head * R.row_tiles) * RT, rows = min(RT, R.rows - row0), base = R.ctx - R.n;
     const int first_place = base + row0 / G, last_place = base + (row0 + rows - 1) / G;
@@ -191,7 +196,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
 
     // ---- where the keys are: lane 4 i + o has the 8 keys o of step i's 32, 8 steps at a time
     // off: where the 8 keys' codes begin, in 16 bytes; sc: where their scales do
-    uint32_t off = 0, sc16 = 0, ok = 0;
+    uint32_t off = 0, sc16 = 0, ok = 0, w8 = 0;       // w8: where the 8 keys' sums are, in eights
     int entry = -1, place8 = 0;                       // the block table's entry and which 8 of the page
     const int eight0 = (R.from >> 3) + lane;
     auto look = [&](int step) {
@@ -208,7 +213,11 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       const uint32_t begin16 = ((uint32_t)(good ? entry : 0) * a.n_kv + head) * page16;      // else some page of the pool: what is read there is not used
       off = begin16 + place8 * (D / 4);
       sc16 = begin16 + a.page_size * (D / 32) + place8 * GROUPS / 2;
+      if (WEIGH) w8 = ((uint32_t)(good ? entry : 0) * a.n_kv + head) * (uint32_t)(a.page_size >> 3) + place8;
     };
+    const int known = WEIGH ? (a.held != nullptr ? a.held[s] : base) : 0;
+    float old_a = 0.f, old_b = 0.f, old_c = 0.f;       // the sums so far of this lane's key: of this step, the next and the one behind it
+    float *at_a = nullptr, *at_b = nullptr, *at_c = nullptr;
     look(step0);
     uint32_t ok_use = 0;
     const uint32_t ring = (uint32_t)__cvta_generic_to_shared(smem) + warp * (KM_STAGES * STAGE);
@@ -227,20 +236,26 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
           for (int o = 0; o < 4; ++o) {
             const uint32_t x = __shfl_sync(0xffffffffu, off, 4 * i + o) + lane;
             km_copy(to + o * 512, km_at(a.k, x));
-            km_copy(to + 2048 + o * 512, km_at(a.v, x));
+            if (!WEIGH) km_copy(to + 2048 + o * 512, km_at(a.v, x));
           }
           const uint32_t x = __shfl_sync(0xffffffffu, sc16, 4 * i + (lane >> 1 & 3)) + (lane & 1);
-          if (lane < 16) km_copy(give_to + 4096 + lane * 16, km_at(lane < 8 ? a.k : a.v, x));
+          if (lane < (WEIGH ? 8 : 16)) km_copy(give_to + CODES + lane * 16, km_at(lane < 8 ? a.k : a.v, x));
         } else {
           const uint32_t to = give_to + (lane >> 4) * 256 + km_place<2>(lane >> 1 & 7, lane & 1);
 #pragma unroll
           for (int o = 0; o < 4; o += 2) {
             const uint32_t x = __shfl_sync(0xffffffffu, off, 4 * i + o + (lane >> 4)) + (lane & 15);
             km_copy(to + o * 256, km_at(a.k, x));
-            km_copy(to + 1024 + o * 256, km_at(a.v, x));
+            if (!WEIGH) km_copy(to + 1024 + o * 256, km_at(a.v, x));
           }
           const uint32_t x = __shfl_sync(0xffffffffu, sc16, 4 * i + (lane & 3));
-          if (lane < 8) km_copy(give_to + 2048 + lane * 16, km_at(lane < 4 ? a.k : a.v, x));
+          if (lane < (WEIGH ? 4 : 8)) km_copy(give_to + CODES + lane * 16, km_at(lane < 4 ? a.k : a.v, x));
+        }
+        if constexpr (WEIGH) {
+          const int key = R.from + (step0 + given) * KM_KEYS + 8 * t + g;
+          float* p = a.weights + __shfl_sync(0xffffffffu, w8, 4 * i + t) * 8ull + g;
+          at_c = (ok >> (4 * i + t) & 1u) && key < R.ctx ? p : nullptr;
+          old_c = at_c != nullptr && key < known ? *p : 0.f;
         }
         ++given;
         give_to = give_to == ring + (KM_STAGES - 1) * STAGE ? ring : give_to + STAGE;
@@ -269,7 +284,10 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       }
     }
 #pragma unroll
-    for (int i = 0; i < KM_STAGES - 1; ++i) ask();
+    for (int i = 0; i < KM_STAGES - 1; ++i) {
+      ask();
+      if (i == 0) { at_a = at_c; old_a = old_c; } else { at_b = at_c; old_b = old_c; }
+    }
 
     uint32_t qb[NT][GROUPS][4];
     float init[NT][GROUPS], factor[NT];
@@ -328,6 +346,16 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         for (int j = 0; j < GROUPS; ++j) acc[x][j][0][i] = acc[x][j][1][i] = 0.f;
       }
     }
+    float lse2[NT];                                    // WEIGH: of row 4 x + t, in powers of two
+    if constexpr (WEIGH) {
+#pragma unroll
+      for (int x = 0; x < NT; ++x) {
+        const int row = 4 * x + t;
+        lse2[x] = INFINITY;
+        if (row < rows) lse2[x] = a.lse[(long)(R.first + row / G) * a.n_q + head * G + row % G] * 1.4426950408889634f;
+        if (lse2[x] == -INFINITY) lse2[x] = INFINITY;   // a row that sees nothing
+      }
+    }
     uint32_t bad[NT] = {};                             // bit j: row 4 x + g / 2 sees a value of group j that is no number
     uint32_t tops = 0x01010101u;                       // the exponents of each group's largest scale so far: 15 is that of 1
     uint32_t room = 0;                                 // what makes a byte with a larger exponent set its first bit, where that matters
@@ -349,7 +377,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
 #pragma unroll
       for (int o = 0; o < 4; ++o) {
         km_read<KW>(kw[o], stage + k_at + o * 8 * ROW);
-        if constexpr (GROUPS == 4) km_read<1>(&ks[o], stage + 64 * ROW + (8 * o + g) * 4); else ks[o] = km_read16(stage + 64 * ROW + (8 * o + g) * 2);
+        if constexpr (GROUPS == 4) km_read<1>(&ks[o], stage + CODES + (8 * o + g) * 4); else ks[o] = km_read16(stage + CODES + (8 * o + g) * 2);
       }
       // ---- scores of the keys 8 o + g for row 4 x + t
       float sc[NT][4];
@@ -377,13 +405,6 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
           }
         }
       }
-      uint32_t vs[2][2];                               // scales of the values 8 o + 2 t, + 1 for o = 2 u + (g & 1)
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const uint32_t from = stage + 64 * ROW + 32 * GROUPS + (8 * (2 * u + (g & 1)) + 2 * t) * GROUPS;
-        if constexpr (GROUPS == 4) km_read<2>(vs[u], from);
-        else { uint32_t both; km_read<1>(&both, from); vs[u][0] = both & 0xffffu; vs[u][1] = both >> 16; }
-      }
       // ---- the softmax
       const bool masked = here != 15u || key0 < clear_from || key0 + 31 > clear_to;
       if constexpr (CAP) {                              // tanh y = 1 - 2 / (1 + e^2y); the factor is in it then
@@ -403,6 +424,33 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
             const int key = key0 + 8 * o + g;
             if (!((here >> o & 1u) && key <= place[x] && (a.window <= 0 || key > place[x] - a.window))) sc[x][o] = -INFINITY;
           }
+      }
+      if constexpr (WEIGH) {
+        float sum[4];
+#pragma unroll
+        for (int o = 0; o < 4; ++o) {
+          sum[o] = 0.f;
+#pragma unroll
+          for (int x = 0; x < NT; ++x) sum[o] += sc[x][o] == -INFINITY ? 0.f : km_exp2(CAP ? sc[x][o] - lse2[x] : fmaf(sc[x][o], factor[x], -lse2[x]));
+        }
+        // over the four lanes with a key's rows, so that lane t has key 8 t + g
+        const float y0 = (t & 1 ? sum[1] : sum[0]) + __shfl_xor_sync(0xffffffffu, t & 1 ? sum[0] : sum[1], 1);
+        const float y1 = (t & 1 ? sum[3] : sum[2]) + __shfl_xor_sync(0xffffffffu, t & 1 ? sum[2] : sum[3], 1);
+        const float y = (t & 2 ? y1 : y0) + __shfl_xor_sync(0xffffffffu, t & 2 ? y0 : y1, 2);
+        if (at_a != nullptr) *at_a = old_a + y;
+        at_a = at_b; old_a = old_b;
+        at_b = at_c; old_b = old_c;
+        stage = stage == ring + (KM_STAGES - 1) * STAGE ? ring : stage + STAGE;
+        continue;
+      }
+      uint32_t vs[2][2];                               // scales of the values 8 o + 2 t, + 1 for o = 2 u + (g & 1)
+#pragma unroll
+      for (int u = 0; u < 2; ++u) {
+        const uint32_t from = stage + CODES + 32 * GROUPS + (8 * (2 * u + (g & 1)) + 2 * t) * GROUPS;
+        if constexpr (GROUPS == 4) km_read<2>(vs[u], from);
+        else { uint32_t both; km_read<1>(&both, from); vs[u][0] = both & 0xffffu; vs[u][1] = both >> 16; }
+      }
+      if (masked) {
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
@@ -546,6 +594,10 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
     // ---- the results: the unit's, or a part of them
     asm volatile("cp.async.wait_group 0;" ::: "memory");
     __syncwarp();
+    if constexpr (WEIGH) {
+      pos += step1 - step0;
+      continue;
+    }
     const bool whole = step0 == 0 && step1 == R.steps;
     const long part = 2L * me + (pos == begin ? 0 : 1);
 #pragma unroll
@@ -608,7 +660,7 @@ kv4_mma_join_kernel(const Kv4MmaArgs a, int N) {
   pdl_wait();
   const int s = blockIdx.z, head = blockIdx.y, tile = blockIdx.x, tid = threadIdx.x, pars = blockDim.x / ITEMS, item = tid % ITEMS, par = tid / ITEMS;
   const int before = a.before[s], after = a.before[s + 1], total = a.before[a.S];
-  const KmRequest R = km_request<RT>(a, s);
+  const KmRequest R = km_request<RT, false>(a, s);
   if (after == before || tile >= R.row_tiles) return;
   const int from = before + (head * R.row_tiles + tile) * R.steps, to = from + R.steps;
   const KmRuns runs(total, N);
@@ -671,12 +723,12 @@ static int km_launch(const Kv4MmaArgs& a, int blocks, int max_rows, cudaStream_t
   constexpr size_t stages = 4 * KM_STAGES * (64 * GROUPS * 16 + 64 * GROUPS);
   static bool set = false;
   if (!set) {
-    cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages + (KM_MAX_SEQS + 1) * sizeof(int)));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages + (KM_MAX_SEQS + 1) * sizeof(int)));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP, false>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
     if (e != cudaSuccess) return (int)e;
     set = true;
   }
-  const int status = launch_pdl(kv4_mma_kernel<GROUPS, NT, CAP>, dim3(blocks), dim3(KM_THREADS), stages + (a.S + 1) * sizeof(int), stream, a);
+  const int status = launch_pdl(kv4_mma_kernel<GROUPS, NT, CAP, false>, dim3(blocks), dim3(KM_THREADS), stages + (a.S + 1) * sizeof(int), stream, a);
   if (status != 0) return status;
   // threads by the parts that a unit has, about
   const int tiles = (max_rows + RT - 1) / RT;
@@ -698,11 +750,43 @@ PHOTON_API int photon_kv4_attention_mma(const photon_kv4_attention_call* c, cuda
   for (int i = 0; i < 28; ++i) if (c->page_size == 8 << i) shift = i;
   const long words = 8L * c->parts * (most <= 4 ? 4 : 8) * (c->d + 2);
   const Kv4MmaArgs a = {(const bf16*)c->q, (bf16*)c->out, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->block_table, c->cu_tokens, c->context_lens, c->sinks, c->lse,
-                        c->scratch, (int*)c->scratch + words, c->err, c->q_stride, c->out_stride, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, shift,
+                        c->scratch, (int*)c->scratch + words, c->err, c->q_stride, c->out_stride, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, shift, nullptr, nullptr,
                         c->min_rows, c->max_rows, (uintptr_t)c->q % 16 == 0 && c->q_stride % 8 == 0,
                         (uintptr_t)c->out % 8 == 0 && c->out_stride % 4 == 0};
 #define ATTEND(GROUPS, NT) (c->softcap > 0.f ? km_launch<GROUPS, NT, true>(a, c->parts, most, stream) : km_launch<GROUPS, NT, false>(a, c->parts, most, stream))
   if (c->d == 64) return most <= 4 ? ATTEND(2, 1) : ATTEND(2, 2);
   return most <= 4 ? ATTEND(4, 1) : ATTEND(4, 2);
 #undef ATTEND
+}
+
+template <int GROUPS, int NT, bool CAP>
+static int km_weigh(const Kv4MmaArgs& a, int blocks, cudaStream_t stream) {
+  constexpr size_t stages = 4 * KM_STAGES * (32 * GROUPS * 17);
+  static bool set = false;
+  if (!set) {
+    cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages + (KM_MAX_SEQS + 1) * sizeof(int)));
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP, true>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
+    if (e != cudaSuccess) return (int)e;
+    set = true;
+  }
+  return launch_pdl(kv4_mma_kernel<GROUPS, NT, CAP, true>, dim3(blocks), dim3(KM_THREADS), stages + (a.S + 1) * sizeof(int), stream, a);
+}
+
+PHOTON_API int photon_kv4_key_weights(const photon_key_weights_call* c, cudaStream_t stream) {
+  if (c->S <= 0 || c->max_keys <= 0 || c->max_tokens_per_seq <= 0) return 0;
+  if (c->dtype != PHOTON_BF16 || !c->packed || c->n_kv <= 0 || c->n_q <= 0 || c->n_q % c->n_kv || c->max_pages <= 0 || c->lse == nullptr || c->parts < 1) return PHOTON_ERR_ARGUMENT;
+  if (!kv4_sizes_ok(c->page_size, c->d) || (c->d != 64 && c->d != 128) || c->page_size % 8 || c->num_pages <= 0) return PHOTON_ERR_UNSUPPORTED;
+  if (c->S > KM_MAX_SEQS || c->n_kv > 65535 || c->scale <= 0.f || (uintptr_t)c->k_cache % 16) return PHOTON_ERR_UNSUPPORTED;
+  if (kv4_page_bytes(c->page_size, c->d) / 16 * c->num_pages * c->n_kv > 0xffffffffL) return PHOTON_ERR_UNSUPPORTED;
+  const int rows = c->max_tokens_per_seq * (c->n_q / c->n_kv);
+  if (rows > 8) return PHOTON_ERR_UNSUPPORTED;        // a key's rows are one warp's
+  int shift = -1;
+  for (int i = 0; i < 28; ++i) if (c->page_size == 8 << i) shift = i;
+  const Kv4MmaArgs a = {(const bf16*)c->q, nullptr, (const uint8_t*)c->k_cache, nullptr, c->block_table, c->cu_tokens, c->context_lens, nullptr, (float*)c->lse, nullptr, nullptr, c->err,
+                        c->q_stride, 0, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, shift, c->weights, c->held, 0, rows,
+                        (uintptr_t)c->q % 16 == 0 && c->q_stride % 8 == 0, 0};
+#define WEIGH(GROUPS, NT) (c->softcap > 0.f ? km_weigh<GROUPS, NT, true>(a, c->parts, stream) : km_weigh<GROUPS, NT, false>(a, c->parts, stream))
+  if (c->d == 64) return rows <= 4 ? WEIGH(2, 1) : WEIGH(2, 2);
+  return rows <= 4 ? WEIGH(4, 1) : WEIGH(4, 2);
+#undef WEIGH
 }

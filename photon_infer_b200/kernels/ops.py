@@ -2833,7 +2833,7 @@ def _kv4_cache(what: str, cache: torch.Tensor, n_kv: int, head_dim: int) -> int:
 _KV4_WRITE_CALL = struct.Struct("6q2q6i")
 _KV4_UNPACK_CALL = struct.Struct("11q1q9i4x")
 _KV4_ATTENTION_CALL = struct.Struct("11q2q13i2f4x")
-_KEY_WEIGHTS_CALL = struct.Struct("11q1q13i2f4x")
+_KEY_WEIGHTS_CALL = struct.Struct("11q2q13i2f4x")
 _EVICT_CALL = struct.Struct("7q12i")
 
 
@@ -3029,15 +3029,32 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
     _check_lse("key_weights", lse, T, n_q)
     if num_seqs == 0 or max_keys <= 0:
         return
-    tiles = -(-max_keys // 128)
-    parts = max(1, min(tiles, 8 * sm_count(q.device) // (num_seqs * n_kv)))
-    scratch = torch.empty(max(T, 1) * n_q * parts * 2, dtype=torch.float32, device=q.device) if lse is None else None
+    if T == 0:
+        return
+    if q.dtype == torch.bfloat16 and head_dim in (64, 128) and (q.stride(0) % 8 or q.data_ptr() % 16):
+        q = q.contiguous() if q.stride(0) != q.shape[1] else q.clone()      # rows on 16-byte boundaries: a copy of the queries is little beside the keys
+    name, parts, floats = _key_weights_route(q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, packed, lse is not None, num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv),
+                                             max_keys, T * n_q, sm_count(q.device))
+    scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if lse is None else None
     call = _KEY_WEIGHTS_CALL.pack(q.data_ptr(), weights.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), _data(held),
-                                  _data(sink), _data(lse), _data(scratch), _data(err), q.stride(0), _dtype_code(q), int(packed), pages, num_seqs, max_keys, n_q, n_kv, head_dim,
+                                  _data(sink), _data(lse), _data(scratch), _data(err), q.stride(0), T, _dtype_code(q), int(packed), pages, num_seqs, max_keys, n_q, n_kv, head_dim,
                                   page_size, k_cache.shape[0], min(window or 0, 0x7fffffff), parts, max_tokens_per_seq, scale, softcap or 0.0)
-    _check(_plain_fn("key_weights", "photon_key_weights", _CALL_ARGS)(call, _stream()), "key_weights")
+    module = "kv4_attention_mma" if name == "kv4_key_weights" else name
+    _check(_plain_fn(module, "photon_" + name, _CALL_ARGS)(call, _stream()), "key_weights")
     if lse is None:
-        _count_launches(1)
+        _count_launches(2 if name == "key_weights_mma" else 1)
+
+
+def _key_weights_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: int, packed: bool, known: bool, num_seqs: int, n_kv: int, rows: int, keys: int, all_rows: int,
+                       sms: int):
+    """(kernel, parts, floats of scratch where the logarithms are not ``known``)."""
+    parts = -(-keys // 128)
+    if dtype != torch.bfloat16 or head_dim not in (64, 128) or page_heads <= 0:
+        parts = max(1, min(parts, 8 * sms // max(1, num_seqs * n_kv)))
+        return "key_weights", parts, 2 * all_rows * parts
+    if packed and known and rows <= 8 and page_size % 8 == 0 and num_seqs <= 1024 and page_heads * kv4_page_bytes(page_size, head_dim) < 1 << 36:
+        return "kv4_key_weights", min(4 * sms, -(-num_seqs * n_kv * (-(-keys // 32) + 1) // 4)), 0
+    return "key_weights_mma", parts, all_rows * (2 * parts + 1)
 
 
 def cache_evict(kv: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor, num_seqs: int,
