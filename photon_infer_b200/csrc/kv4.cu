@@ -1,30 +1,48 @@
 // Rows of keys and values rounded to 4 bits into the paged cache, and pages of it read back (the format: kv4.cuh).
 //
-// kv4_write: four lanes have a group of 32 numbers, 8 each; two exchanges give its largest magnitude.  The rounding is the definition's, to the last tie: max / 7 is cut
-// to 24 bits with its last bit set where something was cut off, which rounds to 4 bits as the whole quotient would; a number's multiple comes from a product with 1 /
-// scale and is put right by what is left over, x - n scale, which is exact.
-// kv4_unpack: a thread reads 8 numbers and writes them where they belong.
+// kv4_write: two lanes have a group of 32 numbers, 16 each; an exchange gives its largest magnitude.  The rounding is the definition's, to the last tie.  In 32 bits max / 7 is
+// cut to 24 bits with its last bit set where something was cut off, which rounds to 4 bits as the whole quotient would.  A bfloat16 number's quotient by the scale, 8 bits by 4, is a
+// half and something or at least 2^-10 away from one: x / scale rounded to multiples of 2^-12 lies where the quotient lies, and a half on the half (max / 7 likewise, to 2^-9 of a
+// step, where 2^-6 is the least).  For 32 bits the multiple from that product is put right by what is left over, x - n scale, which is exact.
+// kv4_unpack: a thread reads a quarter of a row, 8 numbers of every group, and writes them where they belong.
 #include "kv4.cuh"
 
 #define KV4_THREADS 256
 
 // The scale of a group whose largest magnitude is `top`, finite.
+template <typename T>
 __device__ __forceinline__ float kv4_scale_of(float top) {
-  float q = __fdiv_rz(top, 7.f);
-  if (fmaf(-q, 7.f, top) != 0.f) q = __uint_as_float(__float_as_uint(q) | 1u);
+  float q;
+  if constexpr (sizeof(T) == 2) {
+    q = __fmul_rn(top, 0.14285714924335479736328125f);
+  } else {
+    q = __fdiv_rz(top, 7.f);
+    if (fmaf(-q, 7.f, top) != 0.f) q = __uint_as_float(__float_as_uint(q) | 1u);
+  }
   q = fminf(q, 61440.f);
   const uint32_t e = max(__float_as_uint(q) >> 23, 113u);          // the exponent, 2^-14 at least: steps of 2^-17
   const float magic = __uint_as_float((e + 20u) << 23 | 0x400000u);
+  if constexpr (sizeof(T) == 2) {                                   // to 2^-9 of a step first
+    const float fine = __uint_as_float((e + 11u) << 23 | 0x400000u);
+    q = __fsub_rn(__fadd_rn(q, fine), fine);
+  }
   return __fsub_rn(__fadd_rn(q, magic), magic);
 }
 
-// x / scale to the nearest whole number, halves to the even one, in -7 .. 7; scale > 0.
-__device__ __forceinline__ int kv4_round(float x, float scale, float inv, float half) {
-  float n = rintf(fminf(fmaxf(__fmul_rn(x, inv), -8.f), 8.f));
-  const float left = fmaf(-n, scale, x), away = fabsf(left);       // exact: x and n scale are as near as that
-  const bool odd = (int)n & 1;
-  if (away > half || (away == half && odd)) n += left > 0.f ? 1.f : -1.f;
-  return (int)fminf(fmaxf(n, -7.f), 7.f) + 8;
+// x / scale to the nearest whole number, halves to the even one, -7 to 7, plus 8, as a number; scale > 0, inv = 1 / scale.
+template <typename T>
+__device__ __forceinline__ float kv4_round(float x, float scale, float inv) {
+  constexpr float WHOLE = 12582912.f;                              // 1.5 * 2^23: its last bit is 1
+  if constexpr (sizeof(T) == 2) {
+    constexpr float FINE = 1.5f * 2048.f;                          // its last bit is 2^-12
+    const float y = __fsub_rn(__fmaf_rn(x, inv, FINE), FINE);
+    return __fsub_rn(__fadd_rn(fminf(fmaxf(y, -7.f), 7.f), WHOLE), WHOLE - 8.f);
+  } else {
+    float n = __fsub_rn(__fadd_rn(fminf(fmaxf(__fmul_rn(x, inv), -8.f), 8.f), WHOLE), WHOLE);
+    const float left = fmaf(-n, scale, x), away = fabsf(left), half = 0.5f * scale;      // exact: x and n scale are as near as that
+    if (away > half || (away == half && ((int)n & 1))) n += left > 0.f ? 1.f : -1.f;
+    return fminf(fmaxf(n, -7.f), 7.f) + 8.f;
+  }
 }
 
 template <typename T, bool VEC>
@@ -43,55 +61,94 @@ __device__ __forceinline__ void load8(const T* p, float* x) {
   }
 }
 
-template <typename T, bool VEC>
+// A token's items: (plane, head, group, half of the group); `tokens` of them a block.
+template <typename T, bool VEC, int GROUPS>
 __global__ void __launch_bounds__(KV4_THREADS)
 kv4_write_kernel(const T* __restrict__ k, long k_stride, const T* __restrict__ v, long v_stride, const int* __restrict__ slot_mapping, uint8_t* __restrict__ k_cache,
-                 uint8_t* __restrict__ v_cache, long items, int n_kv, int groups, int page_size, long num_slots, int* err) {
+                 uint8_t* __restrict__ v_cache, int T_all, int n_kv, int page_size, int page_shift, long num_slots, int per_token, int* err) {
   pdl_wait();
   pdl_launch_dependents();
-  const long at = (long)blockIdx.x * (KV4_THREADS / 4) + threadIdx.x / 4;      // (token, plane, head, group)
-  const int t = threadIdx.x & 3;
-  const bool live = at < items;                      // a warp's lanes stay together for the exchanges
-  const long of = live ? at : items - 1;
-  const int j = (int)(of % groups);
-  const long row = of / groups;
-  const int h = (int)(row % n_kv), plane = (int)(row / n_kv % 2);
-  const long token = row / n_kv / 2;
-  long slot = slot_mapping[token];
+  // several tokens a block (threadIdx.y), or a token's items in rounds of the block's threads (blockIdx.y)
+  const int token = blockIdx.x * blockDim.y + threadIdx.y, item = blockIdx.y * blockDim.x + threadIdx.x;
+  const bool there = token < T_all;
+  long slot = there ? slot_mapping[token] : -1;
   if (slot >= num_slots || slot < -1) {
-    if (live && t == 0 && j == 0 && h == 0 && plane == 0) report_error(err, PHOTON_DEV_BAD_SLOT, (int)token, (int)slot, (int)min(num_slots, 0x7fffffffL));
+    if (item == 0) report_error(err, PHOTON_DEV_BAD_SLOT, token, (int)slot, (int)min(num_slots, 0x7fffffffL));
     slot = -1;
   }
-  float x[8];
-  load8<T, VEC>((plane ? v + token * v_stride : k + token * k_stride) + (h * groups + j) * 32 + 8 * t, x);
+  const bool live = there && item < per_token;         // a warp's lanes stay together for the exchanges
+  const int half = item & 1, j = (item >> 1) % GROUPS, row = (item >> 1) / GROUPS, plane = row >= n_kv, h = row - plane * n_kv;
+  float x[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = 0.f;
+  if (live) {
+    const T* from = (plane ? v + token * v_stride : k + token * k_stride) + (h * GROUPS + j) * 32 + 16 * half;
+    load8<T, VEC>(from, x);
+    load8<T, VEC>(from + 8, x + 8);
+  }
   uint32_t top = 0;                                  // magnitudes as whole numbers: a NaN is the largest
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+  for (int i = 0; i < 16; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
   top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-  uint32_t word = 0x88888888u, byte = 255;
+  uint32_t word[2] = {0x88888888u, 0x88888888u}, byte = 255;
   if (top < 0x7f800000u) {
-    const float scale = kv4_scale_of(__uint_as_float(top));
+    const float scale = kv4_scale_of<T>(__uint_as_float(top));
     byte = __half_as_ushort(__float2half_rn(scale)) >> 7;
     if (scale > 0.f) {
-      const float inv = __frcp_rn(scale), half = 0.5f * scale;
-      word = 0;
+      float inv;
+      asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(inv) : "f"(scale));
 #pragma unroll
-      for (int i = 0; i < 8; ++i) word |= (uint32_t)kv4_round(x[i], scale, inv, half) << (4 * i);
+      for (int w = 0; w < 2; ++w) {
+        uint32_t part[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {                  // four codes as one whole number below 2^16
+          const float* y = x + 8 * w + 4 * q;
+          float sum = kv4_round<T>(y[3], scale, inv);
+#pragma unroll
+          for (int i = 2; i >= 0; --i) sum = __fmaf_rn(sum, 16.f, kv4_round<T>(y[i], scale, inv));
+          part[q] = __float_as_uint(__fadd_rn(sum, 8388608.f));
+        }
+        word[w] = __byte_perm(part[0], part[1], 0x5410);
+      }
     }
   }
-  if (!live || slot < 0) return;
-  const long page = slot / page_size;
-  const int place = (int)(slot - page * page_size), d2 = groups * 16;
-  uint8_t* base = (plane ? v_cache : k_cache) + (page * n_kv + h) * kv4_page_bytes(page_size, groups * 32);
-  uint8_t* codes = base + (long)place * d2;
-  if (plane == 0) {
-    *(uint32_t*)(codes + 4 * (t * groups + j)) = word;
-  } else {
-    *(uint16_t*)(codes + 2 * (2 * t * groups + j)) = (uint16_t)word;
-    *(uint16_t*)(codes + 2 * ((2 * t + 1) * groups + j)) = (uint16_t)(word >> 16);
+  uint8_t *base = nullptr, *codes = nullptr;
+  const int d2 = GROUPS * 16;
+  int place = 0;
+  if (live && slot >= 0) {
+    const int at = (int)slot, page = page_shift >= 0 ? at >> page_shift : at / page_size;
+    place = at - page * page_size;
+    base = (plane ? v_cache : k_cache) + ((long)page * n_kv + h) * ((long)page_size * GROUPS * 17);
+    codes = base + place * d2;
   }
-  if (t == 0) base[(long)page_size * d2 + place * groups + j] = (uint8_t)byte;
+  if constexpr (GROUPS % 2 == 0) {
+    // the neighbouring group's half words beside this one's: the even group has the values' first two eights, the odd one the others
+    // half words of g = 4 half + 0, 1 | 2, 3: word[0] has 0 and 1, word[1] has 2 and 3
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, j & 1 ? word[0] : word[1], 2);
+    if (codes != nullptr) {
+      if (plane == 0) {
+        *(uint32_t*)(codes + 4 * (2 * half * GROUPS + j)) = word[0];
+        *(uint32_t*)(codes + 4 * ((2 * half + 1) * GROUPS + j)) = word[1];
+      } else {
+        const uint32_t a = j & 1 ? other : word[0], b = j & 1 ? word[1] : other;      // of the even group, of the odd one
+        const int g = 4 * half + 2 * (j & 1);
+        *(uint32_t*)(codes + 2 * (g * GROUPS + (j & ~1))) = __byte_perm(a, b, 0x5410);
+        *(uint32_t*)(codes + 2 * ((g + 1) * GROUPS + (j & ~1))) = __byte_perm(a, b, 0x7632);
+      }
+    }
+  } else if (codes != nullptr) {
+#pragma unroll
+    for (int w = 0; w < 2; ++w) {
+      const int t = 2 * half + w;
+      if (plane == 0) {
+        *(uint32_t*)(codes + 4 * (t * GROUPS + j)) = word[w];
+      } else {
+        *(uint16_t*)(codes + 2 * (2 * t * GROUPS + j)) = (uint16_t)word[w];
+        *(uint16_t*)(codes + 2 * ((2 * t + 1) * GROUPS + j)) = (uint16_t)(word[w] >> 16);
+      }
+    }
+  }
+  if (codes != nullptr && half == 0) base[(long)page_size * d2 + place * GROUPS + j] = (uint8_t)byte;
 }
 
 template <typename T>
@@ -110,68 +167,98 @@ __device__ __forceinline__ void store8(T* p, const float* x) {      // 16-byte a
   }
 }
 
-// Page i of the outputs is page table[i / per * stride + i % per] of the caches.  With cu_tokens: i / per is a request, and only the requests with more than min_rows
-// rows (tokens x group) and their pages below context_lens count, and what lies behind their keys is zero; new_table (per wide) gets the outputs' page, or -1;
-// positions gets every token's place in its request.  A value that is not finite is laid out as zero then (a weight of 0 would make it a NaN in rows that do not see it), and
-// flags [S * per * parts] tells where there was one: kv4_spoil_kernel gives it to the rows that see it.
-template <typename T>
+// Page blockIdx.x of the outputs is page table[i / per * stride + i % per] of the caches; blockIdx.y has a part of its (plane, head, slot, t).  With cu_tokens: i / per is a request, and
+// only the requests with more than min_rows rows (tokens x group) and their pages below context_lens count, and what lies behind their keys is zero; new_table (per wide) gets the
+// outputs' page, or -1; positions gets every token's place in its request.  A value that is not finite is laid out as zero then (a weight of 0 would make it a NaN in rows that
+// do not see it), and flags [S * per * gridDim.y] tells where there was one: kv4_spoil_kernel gives it to the rows that see it.
+template <typename T, int GROUPS>
 __global__ void __launch_bounds__(KV4_THREADS)
 kv4_unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int* __restrict__ table, int per, long stride, T* __restrict__ k_out,
-                  T* __restrict__ v_out, int n_kv, int groups, int page_size, int num_pages, int parts, const int* __restrict__ cu_tokens,
-                  const int* __restrict__ context_lens, int group, int min_rows, int* __restrict__ new_table, int* __restrict__ positions,
-                  int* __restrict__ flags, int* err) {
+                  T* __restrict__ v_out, int n_kv, int page_size, int page_shift, int num_pages, const int* __restrict__ cu_tokens, const int* __restrict__ context_lens, int group,
+                  int min_rows, int* __restrict__ new_table, int* __restrict__ positions, int* __restrict__ flags, int* err) {
+  constexpr int D = GROUPS * 32;
   pdl_wait();
   pdl_launch_dependents();
-  const long i = blockIdx.x / parts;
-  const int part = (int)(blockIdx.x - i * parts), s = (int)(i / per), p = (int)(i - (long)s * per);
+  const int i = blockIdx.x, s = per == (int)gridDim.x ? 0 : i / per, p = i - s * per;
   int end = 0x7fffffff;                              // keys of the request
   if (cu_tokens != nullptr) {
     const int first = cu_tokens[s], n = cu_tokens[s + 1] - first;
     end = context_lens[s];
-    if (positions != nullptr && p == 0 && part == 0)
+    if (positions != nullptr && p == 0 && blockIdx.y == 0)
       for (int x = threadIdx.x; x < n; x += KV4_THREADS) positions[first + x] = end - n + x;
     if ((long)n * group <= min_rows || (long)p * page_size >= end) {
-      if (new_table != nullptr && part == 0 && threadIdx.x == 0) new_table[i] = -1;
+      if (new_table != nullptr && blockIdx.y == 0 && threadIdx.x == 0) new_table[i] = -1;
       return;
     }
   }
   const int page = table[s * stride + p];
   const bool bad = page < 0 || page >= num_pages;
-  if (part == 0 && threadIdx.x == 0) {
-    if (new_table != nullptr) new_table[i] = bad ? -1 : (int)i;
+  if (blockIdx.y == 0 && threadIdx.x == 0) {
+    if (new_table != nullptr) new_table[i] = bad ? -1 : i;
     if (bad) report_error(err, PHOTON_DEV_BAD_PAGE, s, p, page);
   }
-  if (bad) return;
-  const int words = groups * 4, rows = n_kv * page_size, d = groups * 32;
-  const long bytes = kv4_page_bytes(page_size, d);
-  const int unit = part * KV4_THREADS + threadIdx.x;            // (plane, head and slot, word)
-  const bool live = unit < 2 * rows * words;
-  const int plane = live && unit >= rows * words, at = live ? unit - plane * rows * words : 0, row = at / words, w = at - row * words;
-  const int h = row / page_size, slot = row - h * page_size;
-  const uint8_t* base = (plane ? v_cache : k_cache) + ((long)page * n_kv + h) * bytes;
-  const uint8_t* codes = base + (long)slot * groups * 16;
-  const int t = w / groups, j = w - t * groups;
-  const uint32_t word = plane == 0 ? *(const uint32_t*)(codes + 4 * w)
-                                   : *(const uint16_t*)(codes + 2 * (2 * t * groups + j)) | (uint32_t)*(const uint16_t*)(codes + 2 * ((2 * t + 1) * groups + j)) << 16;
-  const float scale = kv4_scale(base[(long)page_size * groups * 16 + slot * groups + j]);
-  float x[8];
-#pragma unroll
-  for (int b = 0; b < 8; ++b) x[b] = (long)p * page_size + slot < end ? kv4_code(word, b) * scale : 0.f;
-  if (flags != nullptr) {
-    const bool odd = live && plane && (long)p * page_size + slot < end && !isfinite(scale);
-#pragma unroll
-    for (int b = 0; b < 8; ++b) if (odd) x[b] = 0.f;
-    const int any = __syncthreads_or(odd);
-    if (threadIdx.x == 0) flags[blockIdx.x] = any;
+  if (bad) {
+    if (flags != nullptr && threadIdx.x == 0) flags[(long)i * gridDim.y + blockIdx.y] = 0;
+    return;
   }
-  if (live) store8((plane ? v_out : k_out) + ((i * n_kv + h) * page_size + slot) * d + 32 * j + 8 * t, x);
+  // lane t of four has bytes 4 t GROUPS .. of a row: 8 numbers of every group, whichever plane
+  const int unit = blockIdx.y * KV4_THREADS + threadIdx.x, t = unit & 3, row = unit >> 2, ph = page_shift >= 0 ? row >> page_shift : row / page_size, slot = row - ph * page_size;
+  bool odd = false;
+  if (ph < 2 * n_kv) {
+    const bool plane = ph >= n_kv;
+    const int h = plane ? ph - n_kv : ph;
+    const uint8_t* base = (plane ? v_cache : k_cache) + ((long)page * n_kv + h) * ((long)page_size * GROUPS * 17);
+    const uint8_t* codes = base + (long)slot * (GROUPS * 16) + 4 * GROUPS * t;
+    const uint8_t* scales = base + (long)page_size * GROUPS * 16 + slot * GROUPS;
+    T* out = (plane ? v_out : k_out) + (((long)i * n_kv + h) * page_size + slot) * D + 8 * t;
+    uint32_t w[GROUPS];
+    uint8_t b[GROUPS];
+    if constexpr (GROUPS % 4 == 0) {
+#pragma unroll
+      for (int j = 0; j < GROUPS; j += 4) {
+        const uint4 u = *(const uint4*)(codes + 4 * j);
+        w[j] = u.x; w[j + 1] = u.y; w[j + 2] = u.z; w[j + 3] = u.w;
+        const uint32_t x = *(const uint32_t*)(scales + j);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) b[j + c] = (uint8_t)(x >> (8 * c));
+      }
+    } else if constexpr (GROUPS == 2) {
+      const uint2 u = *(const uint2*)codes;
+      w[0] = u.x; w[1] = u.y;
+      const uint16_t x = *(const uint16_t*)scales;
+      b[0] = (uint8_t)x; b[1] = (uint8_t)(x >> 8);
+    } else {
+#pragma unroll
+      for (int j = 0; j < GROUPS; ++j) { w[j] = *(const uint32_t*)(codes + 4 * j); b[j] = scales[j]; }
+    }
+    const bool behind = (long)p * page_size + slot >= end;
+#pragma unroll
+    for (int j = 0; j < GROUPS; ++j) {
+      uint32_t word = w[j];
+      if (plane) {                                   // half word j of the first half, half word j of the second
+        const uint32_t lo = w[j / 2] >> (16 * (j & 1)), hi = w[(GROUPS + j) / 2] >> (16 * ((GROUPS + j) & 1));
+        word = __byte_perm(lo, hi, 0x5410);
+      }
+      const float scale = kv4_scale(b[j]);
+      const bool none = flags != nullptr && plane && !behind && !isfinite(scale);
+      odd |= none;
+      float y[8];
+#pragma unroll
+      for (int c = 0; c < 8; ++c) y[c] = behind || none ? 0.f : kv4_code(word, c) * scale;
+      store8(out + 32 * j, y);
+    }
+  }
+  if (flags != nullptr) {
+    const int any = __syncthreads_or(odd);
+    if (threadIdx.x == 0) flags[(long)i * gridDim.y + blockIdx.y] = any;
+  }
 }
 
 // The rows of the requests with more than min_rows rows that see a value which is not finite: its group's numbers are none either.  One block for each (request, head), which has
 // nothing to do but read the flags as a rule.
 __global__ void __launch_bounds__(1024)
-kv4_spoil_kernel(const uint8_t* __restrict__ v_cache, const int* __restrict__ table, int per, long stride, int n_kv, int groups, int page_size, int num_pages, int parts,
-                 const int* __restrict__ cu_tokens, const int* __restrict__ context_lens, int group, int min_rows, const int* __restrict__ flags, bf16* __restrict__ out,
+kv4_spoil_kernel(const uint8_t* __restrict__ v_cache, const int* __restrict__ table, int per, long stride, int n_kv, int groups, int page_size, int num_pages,
+                 const int* __restrict__ cu_tokens, const int* __restrict__ context_lens, int group, int min_rows, int parts, const int* __restrict__ flags, bf16* __restrict__ out,
                  long out_stride, int window) {
   pdl_wait();
   const int head = blockIdx.x, s = blockIdx.y, first = cu_tokens[s], n = cu_tokens[s + 1] - first, len = context_lens[s], base = len - n;
@@ -198,28 +285,57 @@ PHOTON_API int photon_kv4_write(const photon_kv4_write_call* c, cudaStream_t str
   if (c->T <= 0) return 0;
   if ((c->dtype != PHOTON_F32 && c->dtype != PHOTON_BF16) || c->n_kv <= 0 || c->num_pages < 0) return PHOTON_ERR_ARGUMENT;
   if (!kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_UNSUPPORTED;
-  const int groups = c->d / 32, size = c->dtype == PHOTON_F32 ? 4 : 2;
-  const long items = (long)c->T * 2 * c->n_kv * groups, blocks = (items + KV4_THREADS / 4 - 1) / (KV4_THREADS / 4);
-  if (blocks > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
+  const int groups = c->d / 32, size = c->dtype == PHOTON_F32 ? 4 : 2, per_token = 4 * c->n_kv * groups, tokens = per_token <= KV4_THREADS / 2 && c->T > 1 ? KV4_THREADS / 32 * 32 / per_token : 1;
+  const long slots = (long)c->num_pages * c->page_size;
+  if (c->n_kv > 65536 || slots > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
   const bool vec = ((uintptr_t)c->k | (uintptr_t)c->v | (uintptr_t)(c->k_stride * size) | (uintptr_t)(c->v_stride * size)) % 16 == 0;
-#define WRITE(T, VEC) launch_pdl(kv4_write_kernel<T, VEC>, dim3((unsigned)blocks), dim3(KV4_THREADS), 0, stream, (const T*)c->k, c->k_stride, (const T*)c->v, c->v_stride, \
-                                 c->slot_mapping, (uint8_t*)c->k_cache, (uint8_t*)c->v_cache, items, c->n_kv, groups, c->page_size, (long)c->num_pages * c->page_size, c->err)
-  if (c->dtype == PHOTON_F32) return vec ? WRITE(float, true) : WRITE(float, false);
-  return vec ? WRITE(bf16, true) : WRITE(bf16, false);
+  const dim3 grid((c->T + tokens - 1) / tokens, tokens > 1 ? 1 : (per_token + KV4_THREADS - 1) / KV4_THREADS), block(tokens > 1 ? per_token : KV4_THREADS, tokens);
+  int shift = -1;
+  for (int i = 0; i < 31; ++i) if (c->page_size == 1 << i) shift = i;
+#define WRITE(TYPE, VEC, G) launch_pdl(kv4_write_kernel<TYPE, VEC, G>, grid, block, 0, stream, (const TYPE*)c->k, c->k_stride, (const TYPE*)c->v, c->v_stride, c->slot_mapping, \
+                                    (uint8_t*)c->k_cache, (uint8_t*)c->v_cache, c->T, c->n_kv, c->page_size, shift, slots, per_token, c->err)
+#define WRITE_OF(G) (c->dtype == PHOTON_F32 ? vec ? WRITE(float, true, G) : WRITE(float, false, G) : vec ? WRITE(bf16, true, G) : WRITE(bf16, false, G))
+  switch (groups) {
+    case 1: return WRITE_OF(1);
+    case 2: return WRITE_OF(2);
+    case 3: return WRITE_OF(3);
+    case 4: return WRITE_OF(4);
+    case 5: return WRITE_OF(5);
+    case 6: return WRITE_OF(6);
+    case 7: return WRITE_OF(7);
+    default: return WRITE_OF(8);
+  }
+#undef WRITE_OF
 #undef WRITE
 }
+
+// Blocks of a page.
+static int kv4_unpack_parts(const photon_kv4_unpack_call* c) { return (int)((8L * c->n_kv * c->page_size + KV4_THREADS - 1) / KV4_THREADS); }
 
 PHOTON_API int photon_kv4_unpack(const photon_kv4_unpack_call* c, cudaStream_t stream) {
   if (c->S <= 0 || c->per <= 0) return 0;
   if ((c->dtype != PHOTON_F32 && c->dtype != PHOTON_BF16) || c->n_kv <= 0 || c->num_pages < 0) return PHOTON_ERR_ARGUMENT;
   if (!kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_UNSUPPORTED;
   if (((uintptr_t)c->k_out | (uintptr_t)c->v_out) % 16) return PHOTON_ERR_ARGUMENT;
-  const long units = 2L * c->n_kv * c->page_size * (c->d / 8), parts = (units + KV4_THREADS - 1) / KV4_THREADS, blocks = parts * c->S * c->per;
-  if (units > 0x7fffffffL || blocks > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
-#define UNPACK(T) launch_pdl(kv4_unpack_kernel<T>, dim3((unsigned)blocks), dim3(KV4_THREADS), 0, stream, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->table, \
-                             c->per, c->stride, (T*)c->k_out, (T*)c->v_out, c->n_kv, c->d / 32, c->page_size, c->num_pages, (int)parts, c->cu_tokens, c->context_lens, \
-                             c->group, c->min_rows, c->new_table, c->positions, c->cu_tokens != nullptr ? c->flags : nullptr, c->err)
-  return c->dtype == PHOTON_F32 ? UNPACK(float) : UNPACK(bf16);
+  if ((long)c->S * c->per > 0x7fffffffL || 8L * c->n_kv * c->page_size > 65535L * KV4_THREADS) return PHOTON_ERR_UNSUPPORTED;
+  const dim3 grid(c->S * c->per, kv4_unpack_parts(c));
+  int shift = -1;
+  for (int i = 0; i < 31; ++i) if (c->page_size == 1 << i) shift = i;
+#define UNPACK(T, G) launch_pdl(kv4_unpack_kernel<T, G>, grid, dim3(KV4_THREADS), 0, stream, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->table, c->per, c->stride, \
+                                (T*)c->k_out, (T*)c->v_out, c->n_kv, c->page_size, shift, c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, c->new_table, c->positions, \
+                                c->cu_tokens != nullptr ? c->flags : nullptr, c->err)
+#define UNPACK_OF(G) (c->dtype == PHOTON_F32 ? UNPACK(float, G) : UNPACK(bf16, G))
+  switch (c->d / 32) {
+    case 1: return UNPACK_OF(1);
+    case 2: return UNPACK_OF(2);
+    case 3: return UNPACK_OF(3);
+    case 4: return UNPACK_OF(4);
+    case 5: return UNPACK_OF(5);
+    case 6: return UNPACK_OF(6);
+    case 7: return UNPACK_OF(7);
+    default: return UNPACK_OF(8);
+  }
+#undef UNPACK_OF
 #undef UNPACK
 }
 
@@ -227,7 +343,6 @@ PHOTON_API int photon_kv4_spoil(const photon_kv4_unpack_call* c, void* out, long
   if (c->S <= 0 || c->per <= 0) return 0;
   if (c->dtype != PHOTON_BF16 || c->flags == nullptr || c->cu_tokens == nullptr || !kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_ARGUMENT;
   if (c->S > 65535) return PHOTON_ERR_UNSUPPORTED;
-  const long units = 2L * c->n_kv * c->page_size * (c->d / 8), parts = (units + KV4_THREADS - 1) / KV4_THREADS;
   return launch_pdl(kv4_spoil_kernel, dim3(c->n_kv, c->S), dim3(1024), 0, stream, (const uint8_t*)c->v_cache, c->table, c->per, c->stride, c->n_kv, c->d / 32, c->page_size,
-                    c->num_pages, (int)parts, c->cu_tokens, c->context_lens, c->group, c->min_rows, (const int*)c->flags, (bf16*)out, out_stride, window);
+                    c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, kv4_unpack_parts(c), (const int*)c->flags, (bf16*)out, out_stride, window);
 }

@@ -636,7 +636,7 @@ PHOTON_EXPORT int photon_kv4_write(const photon_kv4_write_call* call, cudaStream
 /* Pages read back, k_out and v_out [S * per][n_kv][page_size][d], 16-byte aligned: page s * per + p is page table[s * stride + p]; one outside the pool is left out.  With cu_tokens
  * (else null): of request s only the pages below context_lens[s], and only where it has more than min_rows rows (tokens x group), with zeros behind the last key; new_table
  * [S * per] (may be null) gets each output page's own number, or -1, positions [T] (may be null) each token's place in its request;
- * with flags [S * per * ceil(2 * n_kv * page_size * d / 2048)] (may be null) values that are not finite are laid out as zero and marked there for photon_kv4_spoil. */
+ * with flags [S * per * ceil(n_kv * page_size / 32)] (may be null) values that are not finite are laid out as zero and marked there for photon_kv4_spoil. */
 typedef struct {
   const void* k_cache; const void* v_cache; const int* table; void* k_out; void* v_out; const int* cu_tokens; const int* context_lens; int* new_table; int* positions;
   int* flags; int* err;

@@ -2977,9 +2977,9 @@ def _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, 
     one = per * n_kv * page_size * head_dim * 4
     some = max(1, min(num_seqs, KV4_PROMPT_BYTES // one, 65535 // -(-max_tokens // (128 // (n_q // n_kv)))))
     numbers = torch.empty((2, some * per, n_kv, page_size, head_dim), dtype=q.dtype, device=device)
-    parts = -(-2 * n_kv * page_size * head_dim // 2048)
-    where = torch.empty(some * per * (1 + parts) + T, dtype=torch.int32, device=device)
-    table, flags, positions = where[:some * per].view(some, per), where[some * per:some * per * (1 + parts)], where[some * per * (1 + parts):]
+    marks = some * per * (1 + -(-n_kv * page_size // 32))
+    where = torch.empty(marks + T, dtype=torch.int32, device=device)
+    table, flags, positions = where[:some * per].view(some, per), where[some * per:marks], where[marks:]
     for s0 in range(0, num_seqs, some):
         n = min(some, num_seqs - s0)
         cu, lens = cu_tokens[s0:s0 + n + 1], context_lens[s0:s0 + n]
