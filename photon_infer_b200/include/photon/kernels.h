@@ -687,10 +687,11 @@ PHOTON_EXPORT int photon_kv4_key_weights(const photon_key_weights_call* call, cu
 /* ------------------------------------------------------------------ cache_evict.cu */
 /* kv [entries][planes][num_pages][n_kv][page_size * (row_bytes + scale_bytes)], rows first, then scales; weights [entries][num_pages][n_kv][page_size].  Requests with more than
  * `keep` keys keep that many: in every entry and head the first `first`, the last `last` and those with the largest weights (of equal ones the lower place), moved to the
- * front in their order, the weights with them.  kept [entries][S][n_kv][keep]: their old places (of requests that lose keys).  new_lens [S] = min(context_lens, keep), another array than context_lens. */
+ * front in their order, the weights with them.  kept [entries][S][n_kv][keep]: their old places (of requests that lose keys).  new_lens [S] = min(context_lens, keep), another array than
+ * context_lens; a request has at most max_keys keys. */
 typedef struct {
   void* kv; float* weights; const int* block_table; const int* context_lens; int* new_lens; int* kept; int* err;
-  int entries, planes, num_pages, n_kv, page_size, max_pages, S, keep, first, last, row_bytes, scale_bytes;
+  int entries, planes, num_pages, n_kv, page_size, max_pages, S, max_keys, keep, first, last, row_bytes, scale_bytes;
 } photon_evict_call;
 PHOTON_EXPORT int photon_cache_evict(const photon_evict_call* call, cudaStream_t stream);
 

@@ -2834,7 +2834,7 @@ _KV4_WRITE_CALL = struct.Struct("6q2q6i")
 _KV4_UNPACK_CALL = struct.Struct("11q1q9i4x")
 _KV4_ATTENTION_CALL = struct.Struct("11q2q13i2f4x")
 _KEY_WEIGHTS_CALL = struct.Struct("11q2q13i2f4x")
-_EVICT_CALL = struct.Struct("7q12i")
+_EVICT_CALL = struct.Struct("7q13i4x")
 
 
 def _data(t: Optional[torch.Tensor]) -> int:
@@ -3091,8 +3091,8 @@ def cache_evict(kv: torch.Tensor, weights: torch.Tensor, block_table: torch.Tens
     table = block_table.shape
     if len(table) != 2 or num_seqs < 0 or table[0] < num_seqs or context_lens.numel() < num_seqs or new_lens.numel() < num_seqs or table[0] * table[1] < 1:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_evict: block_table, context_lens and new_lens must cover every request")
-    if keep < 0 or keep_first < 0 or keep_last < 0:
-        raise PhotonError(ErrorCode.INVALID_ARGUMENT, "cache_evict: keep, keep_first and keep_last must not be negative")
+    if keep < 0 or keep_first < 0 or keep_last < 0 or max_keys < 0:
+        raise PhotonError(ErrorCode.INVALID_ARGUMENT, "cache_evict: max_keys, keep, keep_first and keep_last must not be negative")
     if num_seqs and new_lens.data_ptr() < context_lens.data_ptr() + 4 * num_seqs and context_lens.data_ptr() < new_lens.data_ptr() + 4 * num_seqs:
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, "cache_evict: new_lens must be another tensor than context_lens, which is read while it is written")
     if kept is None:
@@ -3102,7 +3102,7 @@ def cache_evict(kv: torch.Tensor, weights: torch.Tensor, block_table: torch.Tens
         if kept.shape != (entries, num_seqs, n_kv, keep):
             raise PhotonError(ErrorCode.SHAPE_MISMATCH, "cache_evict: kept must be [entries, requests, n_kv, keep]")
     call = _EVICT_CALL.pack(kv.data_ptr(), weights.data_ptr(), block_table.data_ptr(), context_lens.data_ptr(), new_lens.data_ptr(), kept.data_ptr(), _data(err), entries,
-                            shape[1], pages, n_kv, page_size, table[1], num_seqs, keep, keep_first, keep_last, row_bytes, scale_bytes)
+                            shape[1], pages, n_kv, page_size, table[1], num_seqs, max_keys, keep, keep_first, keep_last, row_bytes, scale_bytes)
     _check(_plain_fn("cache_evict", "photon_cache_evict", _CALL_ARGS)(call, _stream()), "cache_evict")
     if keep:
         _count_launches(1)

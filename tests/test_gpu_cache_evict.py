@@ -162,3 +162,14 @@ def test_captured_and_replayed():
         graph.replay()
         want = _want(case[0], case[1], case[2], lengths, 150, 4, 10, True, 16, 64)
         assert torch.equal(kv.cpu(), want[0]) and torch.equal(w.cpu(), want[1]) and lens.tolist() == [min(x, 150) for x in lengths]
+
+
+def test_more_keys_than_announced():
+    """max_keys only decides where the sums are kept."""
+    from photon_infer_b200.kernels import ops
+    kv, w, table, _ = _case([2000, 90], 1, 2, 64, 16, True, torch.bfloat16, seed=31)
+    want = _want(kv, w, table, [2000, 90], 700, 3, 5, True, 16, 64)
+    for announced in (0, 100, 2000, 1 << 20):
+        got, sums, lens = kv.to(DEV), w.to(DEV), torch.zeros(2, dtype=torch.int32, device=DEV)
+        ops.cache_evict(got, sums, table.to(DEV), torch.tensor([2000, 90], dtype=torch.int32, device=DEV), lens, 2, announced, 700, 3, 5, None)
+        assert torch.equal(got.cpu(), want[0]) and torch.equal(sums.cpu(), want[1]) and lens.tolist() == [700, 90]
