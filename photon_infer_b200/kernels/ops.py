@@ -2801,32 +2801,54 @@ def kv4_page_bytes(page_size: int, head_dim: int) -> int:
     return page_size * (head_dim // 32) * _KV4_GROUP
 
 
-def _on_device(what: str, *tensors: Optional[torch.Tensor]) -> None:
-    """All on the current CUDA device, whose stream the kernels run on."""
-    index = None
+def _on_device(what: str, *tensors: Optional[torch.Tensor]) -> int:
+    """All on the current CUDA device, whose stream the kernels run on; returns its index."""
+    index = -1
     for t in tensors:
         if t is None:
             continue
-        if not t.is_cuda:
+        at = t.get_device()                             # -1: the host
+        if at != index or at < 0:
             _cuda(t)
-        if index is None:
-            index = torch._C._cuda_getDevice()
-        if t.get_device() != index:
-            raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"{what}: a tensor is on another device than the current one")
+            if index >= 0 or at != torch._C._cuda_getDevice():
+                raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"{what}: a tensor is on another device than the current one")
+            index = at
+    return index
 
 
-def _kv4_cache(what: str, cache: torch.Tensor, n_kv: int, head_dim: int) -> int:
-    """Checks a cache in 4 bits; returns its page size."""
-    shape, row = cache.shape, head_dim // 32 * _KV4_GROUP
+@functools.lru_cache(maxsize=256)
+def _kv4_page_size(what: str, page_bytes: int, head_dim: int) -> int:
     if head_dim <= 0 or head_dim % 32 or head_dim > 256:
         raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, f"{what}: heads of {head_dim} are not supported (multiples of 32 up to 256)")
-    if cache.dtype is not torch.uint8 or len(shape) != 3 or shape[1] != n_kv or shape[2] == 0 or shape[2] % row or not cache.is_contiguous():
+    row = head_dim // 32 * _KV4_GROUP
+    if page_bytes <= 0 or page_bytes % row:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: {page_bytes} bytes are no page in 4 bits (kv4_page_bytes)")
+    kv4_page_bytes(page_bytes // row, head_dim)
+    return page_bytes // row
+
+
+def _kv4_caches(what: str, n_kv: int, head_dim: int, k_cache: torch.Tensor, v_cache: Optional[torch.Tensor]):
+    """Checks caches in 4 bits, one or two of one shape; returns (page size, pages)."""
+    shape, uint8 = k_cache.shape, torch.uint8
+    if k_cache.dtype is not uint8 or len(shape) != 3 or shape[1] != n_kv or not k_cache.is_contiguous():
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: a cache in 4 bits must be contiguous uint8 [pages, n_kv, kv4_page_bytes(page_size, head_dim)]")
-    if cache.data_ptr() % 16:
+    page_size = _kv4_page_size(what, shape[2], head_dim)
+    if v_cache is not None and (v_cache.dtype is not uint8 or v_cache.shape != shape or not v_cache.is_contiguous()):
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: the caches must have one shape")
+    if k_cache.data_ptr() % 16 or (v_cache is not None and v_cache.data_ptr() % 16):
         raise PhotonError(ErrorCode.INVALID_ARGUMENT, f"{what}: a cache in 4 bits must begin on a 16-byte boundary")
-    page_size = shape[2] // row
-    kv4_page_bytes(page_size, head_dim)
-    return page_size
+    return page_size, shape[0]
+
+
+_sms_by_index = {}
+
+
+def _sms(index: int, device: torch.device) -> int:
+    """``sm_count`` by a device's index."""
+    n = _sms_by_index.get(index)
+    if n is None:
+        n = _sms_by_index[index] = sm_count(device)
+    return n
 
 
 #: photon_kv4_write_call, photon_kv4_unpack_call, photon_kv4_attention_call, photon_key_weights_call, photon_evict_call
@@ -2847,17 +2869,14 @@ def kv4_write(k: torch.Tensor, v: torch.Tensor, slot_mapping: torch.Tensor, k_ca
     twice) in a paged cache in 4 bits (``kv4_page_bytes``).  A group of 32 numbers gets the scale nearest to its largest magnitude / 7 and each number the nearest multiple of
     it, halves the even one; magnitudes above 430,080 are held as that, a group with a number that is not finite reads as NaN."""
     _on_device("kv4_write", k, v, slot_mapping, k_cache, v_cache, err)
-    page_size = _kv4_cache("kv4_write", k_cache, n_kv, head_dim)
-    T = slot_mapping.numel()
-    for name, t in (("k", k), ("v", v)):
-        if t.shape != (T, n_kv * head_dim) or (t.stride(1) != 1 and T) or t.dtype != k.dtype:
-            raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"kv4_write: {name} must be [T, {n_kv} * {head_dim}] with contiguous heads, of one type")
-    _int32(slot_mapping, "slot_mapping")
-    if v_cache.shape != k_cache.shape:
-        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_write: the caches must have one shape")
-    _kv4_cache("kv4_write", v_cache, n_kv, head_dim)
-    call = _KV4_WRITE_CALL.pack(k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), _data(err), k.stride(0), v.stride(0),
-                                _dtype_code(k), T, n_kv, head_dim, page_size, k_cache.shape[0])
+    page_size, pages = _kv4_caches("kv4_write", n_kv, head_dim, k_cache, v_cache)
+    T, dtype, (k_stride, k_inner), (v_stride, v_inner) = slot_mapping.numel(), k.dtype, k.stride(), v.stride()
+    if k.shape != (T, n_kv * head_dim) or v.shape != k.shape or ((k_inner != 1 or v_inner != 1) and T) or v.dtype is not dtype:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"kv4_write: k and v must be [T, {n_kv} * {head_dim}] with contiguous heads, of one type")
+    if slot_mapping.dtype is not torch.int32 or not slot_mapping.is_contiguous():
+        _int32(slot_mapping, "slot_mapping")
+    call = _KV4_WRITE_CALL.pack(k.data_ptr(), v.data_ptr(), slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), 0 if err is None else err.data_ptr(), k_stride,
+                                v_stride, _dtype_code(k), T, n_kv, head_dim, page_size, pages)
     _check(_plain_fn("kv4", "photon_kv4_write", _CALL_ARGS)(call, _stream()), "kv4_write")
 
 
@@ -2867,14 +2886,14 @@ def kv4_unpack(k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor
     _on_device("kv4_unpack", k_cache, v_cache, pages, k_out, v_out, err)
     _int32(pages, "pages")
     shape = k_out.shape
-    if len(shape) != 4 or shape[0] != pages.numel() or v_out.shape != shape or v_out.dtype != k_out.dtype or not k_out.is_contiguous() or not v_out.is_contiguous():
+    if len(shape) != 4 or shape[0] != pages.numel() or v_out.shape != shape or v_out.dtype is not k_out.dtype or not k_out.is_contiguous() or not v_out.is_contiguous():
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_unpack: the outputs must be contiguous [pages, n_kv, page_size, head_dim], of one type")
     N, n_kv, page_size, head_dim = shape
-    if _kv4_cache("kv4_unpack", k_cache, n_kv, head_dim) != page_size or v_cache.shape != k_cache.shape:
+    size, pool = _kv4_caches("kv4_unpack", n_kv, head_dim, k_cache, v_cache)
+    if size != page_size:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_unpack: the outputs' pages must be those of the caches")
-    _kv4_cache("kv4_unpack", v_cache, n_kv, head_dim)
-    call = _KV4_UNPACK_CALL.pack(k_cache.data_ptr(), v_cache.data_ptr(), pages.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), 0, 0, 0, 0, 0, _data(err), N,
-                                 _dtype_code(k_out), 1, N, n_kv, head_dim, page_size, k_cache.shape[0], 1, 0)
+    call = _KV4_UNPACK_CALL.pack(k_cache.data_ptr(), v_cache.data_ptr(), pages.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), 0, 0, 0, 0, 0,
+                                 0 if err is None else err.data_ptr(), N, _dtype_code(k_out), 1, N, n_kv, head_dim, page_size, pool, 1, 0)
     _check(_plain_fn("kv4", "photon_kv4_unpack", _CALL_ARGS)(call, _stream()), "kv4_unpack")
 
 
@@ -2910,44 +2929,45 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
     token's position as long as none has left it.  A row that sees nothing is zero.  ``q`` and ``out [T, n_q * d]`` may be views with a row stride; ``sink``, ``softcap``: as in
     ``paged_attention``.  ``lse`` (float32 ``[T, n_q]``): gets the logarithm of the sum of each row's exponentials (the sink's among them; -inf where there is nothing), which
     ``key_weights`` takes.  A query that is not finite makes its row NaN."""
-    _on_device("kv4_attention", q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, sink, lse, err)
+    index = _on_device("kv4_attention", q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, sink, lse, err)
     if sink is not None:
         _check_sink(sink, n_q)
     _check_heads("kv4_attention", n_q, n_kv, scale, softcap, window)
-    _rows_view("kv4_attention", q, n_q, head_dim)
-    _rows_view("kv4_attention", out, n_q, head_dim)
-    T, width = q.shape
-    if out.shape[0] != T or out.dtype != q.dtype:
-        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_attention: q and out must have one shape and type")
-    if T > 1 and out.stride(0) < width:
+    shape, dtype = q.shape, q.dtype
+    if len(shape) != 2 or shape[1] != n_q * head_dim or out.shape != shape or out.dtype is not dtype:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_attention: q and out must be [T, n_q * head_dim], of one type")
+    (T, width), (q_stride, q_inner), (out_stride, out_inner) = shape, q.stride(), out.stride()
+    if (q_inner != 1 or out_inner != 1) and T:
+        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_attention: rows of q and out must be contiguous")
+    if T > 1 and out_stride < width:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_attention: rows of out must not overlap")
-    page_size = _kv4_cache("kv4_attention", k_cache, n_kv, head_dim)
-    if v_cache.shape != k_cache.shape:
-        raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_attention: the caches must have one shape")
-    _kv4_cache("kv4_attention", v_cache, n_kv, head_dim)
+    page_size, pool = _kv4_caches("kv4_attention", n_kv, head_dim, k_cache, v_cache)
     _int32s("cu_tokens context_lens block_table", cu_tokens, context_lens, block_table)
     pages = _check_step("kv4_attention", num_seqs, cu_tokens, context_lens, block_table)
-    _check_lse("kv4_attention", lse, T, n_q)
+    if lse is not None:
+        _check_lse("kv4_attention", lse, T, n_q)
     if T == 0 or num_seqs == 0 or max_tokens_per_seq <= 0 or max_keys <= 0:
         return
     group, window = n_q // n_kv, min(window or 0, 0x7fffffff)
     most = max_tokens_per_seq * group                   # rows of a request
-    if most > KV4_FEW_ROWS and lse is None and attention_tc_supported(q.dtype, head_dim, group, page_size):
+    if most > KV4_FEW_ROWS and lse is None and attention_tc_supported(dtype, head_dim, group, page_size):
         _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, num_seqs, max_tokens_per_seq, max_keys, n_q, n_kv, head_dim, page_size, window,
                     scale, err, sink, softcap)
         most = KV4_FEW_ROWS
     tokens = -(-most // group)
     keys = min(max_keys, window + tokens) if window else max_keys
-    name, parts, floats = _kv4_route(q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, num_seqs, n_kv, most, keys, T * n_q, sm_count(q.device))
+    name, parts, floats = _kv4_route(dtype, head_dim, page_size, pool * n_kv, num_seqs, n_kv, most, keys, T * n_q, _sms(index, q.device))
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     call = _KV4_ATTENTION_CALL.pack(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(),
-                                    _data(sink), _data(lse), _data(scratch), _data(err), q.stride(0), out.stride(0), _dtype_code(q), pages, num_seqs, tokens, n_q, n_kv,
-                                    head_dim, page_size, k_cache.shape[0], window, parts, 0, most, scale, softcap or 0.0)
+                                    0 if sink is None else sink.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
+                                    0 if err is None else err.data_ptr(), q_stride, out_stride, _dtype_code(q), pages, num_seqs, tokens, n_q, n_kv, head_dim, page_size, pool,
+                                    window, parts, 0, most, scale, softcap or 0.0)
     _check(_plain_fn(name, "photon_" + name, _CALL_ARGS)(call, _stream()), "kv4_attention")
     if floats:
         _count_launches(1)
 
 
+@functools.lru_cache(maxsize=4096)
 def _kv4_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: int, num_seqs: int, n_kv: int, rows: int, keys: int, all_rows: int, sms: int):
     """(kernel, parts, floats of scratch) for requests of at most ``rows`` rows (tokens x query heads per key/value head) and ``keys`` visible keys."""
     if dtype == torch.bfloat16 and head_dim in (64, 128) and page_size % 8 == 0 and 0 < page_heads * kv4_page_bytes(page_size, head_dim) < 1 << 36 and num_seqs <= 1024:
@@ -3003,14 +3023,14 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
     queries may be a step's, or the last ones of a prompt (``cu_tokens`` then counts those).  Keys from ``held[s]`` (int32) on have no sum yet and get this one; without
     ``held`` those are the given tokens' own keys.  ``k_cache``: a plain one of the type of ``q`` (``[pages, n_kv, page_size, d]``, ``d`` a multiple of 8 up to 256) or one in 4 bits.
     ``lse``: as ``kv4_attention`` leaves it for the same queries; without it the keys are read twice."""
-    _on_device("key_weights", q, weights, k_cache, block_table, cu_tokens, context_lens, held, sink, lse, err)
+    index = _on_device("key_weights", q, weights, k_cache, block_table, cu_tokens, context_lens, held, sink, lse, err)
     if sink is not None:
         _check_sink(sink, n_q)
     _check_heads("key_weights", n_q, n_kv, scale, softcap, window)
     _rows_view("key_weights", q, n_q, head_dim)
     T, packed = q.shape[0], k_cache.dtype is torch.uint8
     if packed:
-        page_size = _kv4_cache("key_weights", k_cache, n_kv, head_dim)
+        page_size, _ = _kv4_caches("key_weights", n_kv, head_dim, k_cache, None)
     else:
         if head_dim % 8 or not 0 < head_dim <= 256:
             raise PhotonError(ErrorCode.UNSUPPORTED_SIZE, f"key_weights: heads of {head_dim} are not supported (multiples of 8 up to 256)")
@@ -3034,7 +3054,7 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
     if q.dtype == torch.bfloat16 and head_dim in (64, 128) and (q.stride(0) % 8 or q.data_ptr() % 16):
         q = q.contiguous() if q.stride(0) != q.shape[1] else q.clone()      # rows on 16-byte boundaries: a copy of the queries is little beside the keys
     name, parts, floats = _key_weights_route(q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, packed, lse is not None, num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv),
-                                             max_keys, T * n_q, sm_count(q.device))
+                                             max_keys, T * n_q, _sms(index, q.device))
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if lse is None else None
     call = _KEY_WEIGHTS_CALL.pack(q.data_ptr(), weights.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), _data(held),
                                   _data(sink), _data(lse), _data(scratch), _data(err), q.stride(0), T, _dtype_code(q), int(packed), pages, num_seqs, max_keys, n_q, n_kv, head_dim,
@@ -3045,6 +3065,7 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
         _count_launches(2 if name == "key_weights_mma" else 1)
 
 
+@functools.lru_cache(maxsize=4096)
 def _key_weights_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: int, packed: bool, known: bool, num_seqs: int, n_kv: int, rows: int, keys: int, all_rows: int,
                        sms: int):
     """(kernel, parts, floats of scratch where the logarithms are not ``known``)."""
