@@ -673,13 +673,14 @@ typedef struct {
   const void* q; float* weights; const void* k_cache; const int* block_table; const int* cu_tokens; const int* context_lens; const int* held; const float* sinks;
   const float* lse; float* scratch; int* err;
   long q_stride, scratch_rows;          /* scratch_rows: T, for the second form */
-  int dtype, packed, max_pages, S, max_keys, n_q, n_kv, d, page_size, num_pages, window, parts, max_tokens_per_seq;
+  int dtype, packed, max_pages, S, max_keys, n_q, n_kv, d, page_size, num_pages, window, parts, max_tokens_per_seq, keep_scores;
   float scale, softcap;
 } photon_key_weights_call;
 PHOTON_EXPORT int photon_key_weights(const photon_key_weights_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ key_weights_mma.cu: the same on the tensor cores, bfloat16, d 64 or 128 */
-/* 16-byte aligned rows of q; at most max_tokens_per_seq tokens a request; parts = ceil(max_keys / 128); without lse, scratch: T * n_q * (2 * parts + 1) floats. */
+/* 16-byte aligned rows of q; at most max_tokens_per_seq tokens and max_keys keys a request.  parts: runs of a request's keys.  Without lse, scratch: T * n_q * (2 * parts + 1)
+ * floats, and with keep_scores (at most 16 rows a request: the keys are read once) T * n_q * max_keys more. */
 PHOTON_EXPORT int photon_key_weights_mma(const photon_key_weights_call* call, cudaStream_t stream);
 /* kv4_attention_mma.cu: with lse, for a cache in 4 bits and at most 8 rows (max_tokens_per_seq * n_q / n_kv), pages of a multiple of 8 tokens, 1,024 requests.  parts: blocks. */
 PHOTON_EXPORT int photon_kv4_key_weights(const photon_key_weights_call* call, cudaStream_t stream);

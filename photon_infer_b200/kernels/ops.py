@@ -2855,7 +2855,7 @@ def _sms(index: int, device: torch.device) -> int:
 _KV4_WRITE_CALL = struct.Struct("6q2q6i")
 _KV4_UNPACK_CALL = struct.Struct("11q1q9i4x")
 _KV4_ATTENTION_CALL = struct.Struct("11q2q13i2f4x")
-_KEY_WEIGHTS_CALL = struct.Struct("11q2q13i2f4x")
+_KEY_WEIGHTS_CALL = struct.Struct("11q2q14i2f")
 _EVICT_CALL = struct.Struct("7q13i4x")
 
 
@@ -2950,7 +2950,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
         return
     group, window = n_q // n_kv, min(window or 0, 0x7fffffff)
     most = max_tokens_per_seq * group                   # rows of a request
-    if most > KV4_FEW_ROWS and lse is None and attention_tc_supported(dtype, head_dim, group, page_size):
+    if most > KV4_FEW_ROWS and lse is None and attention_tc_supported(dtype, head_dim, group, page_size) \
+            and not _kv4_few(head_dim, page_size, num_seqs, n_kv, most, min(max_keys, window + max_tokens_per_seq) if window else max_keys):
         _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, num_seqs, max_tokens_per_seq, max_keys, n_q, n_kv, head_dim, page_size, window,
                     scale, err, sink, softcap)
         most = KV4_FEW_ROWS
@@ -2965,6 +2966,17 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
     _check(_plain_fn(name, "photon_" + name, _CALL_ARGS)(call, _stream()), "kv4_attention")
     if floats:
         _count_launches(1)
+
+
+def _kv4_few(head_dim: int, page_size: int, num_seqs: int, n_kv: int, rows: int, keys: int) -> bool:
+    """Whether requests of up to ``rows`` rows go to the kernel that reads the codes, eight rows at a time, rather than have their pages laid out for the tcgen05 kernel, whose blocks
+    walk a request's keys one tile behind the other.  In us, the two sides of the comparison and 9 to 12 each.  Measured (pages laid out, codes), 32/8 heads of 128, 1 request of 8
+    tokens behind 1,500 39 and 23, behind 6,000 99 and 28; of 64 39 and 36, 109 and 81; of 128 40 and 51, 111 and 141; 4 of 16 44 and 36, 123 and 81; 4 of 33 45 and 53, 132 and 148; 16 of 8
+    75 and 51, 193 and 142; 16 of 16 75 and 85, 193 and 266; of 64, 1 of 33 30 and 21, 82 and 33; 4 of 64 33 and 54, 95 and 160; 16 of 8 44 and 33, 145 and 87."""
+    if head_dim not in (64, 128) or page_size % 8 or num_seqs > 1024:
+        return False
+    codes = num_seqs * n_kv * -(-rows // 8) * -(-keys // 32) * (1.33e-3 if head_dim == 128 else 0.78e-3) + 3
+    return codes <= keys * (15.5e-3 if head_dim == 128 else 11.8e-3) + num_seqs * n_kv * keys * head_dim * 1.37e-6
 
 
 @functools.lru_cache(maxsize=4096)
@@ -3053,12 +3065,12 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
         return
     if q.dtype == torch.bfloat16 and head_dim in (64, 128) and (q.stride(0) % 8 or q.data_ptr() % 16):
         q = q.contiguous() if q.stride(0) != q.shape[1] else q.clone()      # rows on 16-byte boundaries: a copy of the queries is little beside the keys
-    name, parts, floats = _key_weights_route(q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, packed, lse is not None, num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv),
+    name, parts, floats, keep = _key_weights_route(q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, packed, lse is not None, num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv),
                                              max_keys, T * n_q, _sms(index, q.device))
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if lse is None else None
     call = _KEY_WEIGHTS_CALL.pack(q.data_ptr(), weights.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), _data(held),
                                   _data(sink), _data(lse), _data(scratch), _data(err), q.stride(0), T, _dtype_code(q), int(packed), pages, num_seqs, max_keys, n_q, n_kv, head_dim,
-                                  page_size, k_cache.shape[0], min(window or 0, 0x7fffffff), parts, max_tokens_per_seq, scale, softcap or 0.0)
+                                  page_size, k_cache.shape[0], min(window or 0, 0x7fffffff), parts, max_tokens_per_seq, int(keep), scale, softcap or 0.0)
     module = "kv4_attention_mma" if name == "kv4_key_weights" else name
     _check(_plain_fn(module, "photon_" + name, _CALL_ARGS)(call, _stream()), "key_weights")
     if lse is None:
@@ -3068,14 +3080,17 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
 @functools.lru_cache(maxsize=4096)
 def _key_weights_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: int, packed: bool, known: bool, num_seqs: int, n_kv: int, rows: int, keys: int, all_rows: int,
                        sms: int):
-    """(kernel, parts, floats of scratch where the logarithms are not ``known``)."""
-    parts = -(-keys // 128)
+    """(kernel, parts, floats of scratch where the logarithms are not ``known``, whether the scores are kept)."""
+    tiles = -(-keys // 128)
     if dtype != torch.bfloat16 or head_dim not in (64, 128) or page_heads <= 0:
-        parts = max(1, min(parts, 8 * sms // max(1, num_seqs * n_kv)))
-        return "key_weights", parts, 2 * all_rows * parts
+        parts = max(1, min(tiles, 8 * sms // max(1, num_seqs * n_kv)))
+        return "key_weights", parts, 2 * all_rows * parts, False
     if packed and known and rows <= 8 and page_size % 8 == 0 and num_seqs <= 1024 and page_heads * kv4_page_bytes(page_size, head_dim) < 1 << 36:
-        return "kv4_key_weights", min(4 * sms, -(-num_seqs * n_kv * (-(-keys // 32) + 1) // 4)), 0
-    return "key_weights_mma", parts, all_rows * (2 * parts + 1)
+        return "kv4_key_weights", min(4 * sms, -(-num_seqs * n_kv * (-(-keys // 32) + 1) // 4)), 0, False
+    # two blocks an SM: runs of keys for as many blocks as fill them, twice over for few rows, where a request that is shorter than the longest costs most
+    parts = max(1, min(tiles, (4 if rows <= 16 else 2) * sms // max(1, num_seqs * n_kv)))
+    keep = not known and rows <= 16 and all_rows * keys <= 1 << 26
+    return "key_weights_mma", parts, all_rows * (2 * parts + 1 + (keys if keep else 0)), keep
 
 
 def cache_evict(kv: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor, num_seqs: int,
