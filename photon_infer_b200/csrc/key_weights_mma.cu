@@ -8,6 +8,7 @@
 // row, and a third kernel turns them into weights; for more rows the keys are read again.
 #include "kv4.cuh"
 #include <math.h>
+#include <type_traits>
 
 #define KX_KEYS 128
 #define KX_THREADS 256
@@ -196,62 +197,86 @@ key_weights_mma_kernel(const KeyWeightsMmaArgs a) {
       const uint32_t* there = there_s[tile & 1];
       const bool clear = (there[0] & there[1] & there[2] & there[3]) == 0xffffffffu && key0 + KX_KEYS - 1 <= base && (a.window <= 0 || key0 > last_place - a.window);      // all rows see all
       const uint32_t k_at = (uint32_t)__cvta_generic_to_shared(k_s) + ((tile & 1) * KX_KEYS + (lane & 15)) * PITCH + (lane >> 4) * 16;
-      for (int part = my_k; part < KX_KEYS / 16; part += wk) {
-        if (part * 16 >= keys || !busy) break;
-        float d[2][4] = {};
+      // 16 keys, or twice 16 side by side: the second ones' products fill the first ones' waits
+      auto work = [&](auto several, int part0) {
+        constexpr int P = decltype(several)::value;
+        float d[P][2][4] = {};
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
-          uint32_t k4[4];
-          kx_matrices(k4, k_at + part * 16 * PITCH + 32 * i);
-          kx_mma(d[0], k4, b[i][0], b[i][1]);
-          if (two) kx_mma(d[1], k4, b[i][2], b[i][3]);
-        }
-        float x[4][2];                                 // rows as above, keys g and 8 + g
+          uint32_t k4[P][4];
 #pragma unroll
-        for (int c = 0; c < 4; ++c)
+          for (int p = 0; p < P; ++p) kx_matrices(k4[p], k_at + (part0 + p * wk) * 16 * PITCH + 32 * i);
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const float y = d[c >> 1][2 * h + (c & 1)];
-            x[c][h] = a.softcap > 0.f ? cap_out * (1.f - __fdividef(2.f, 1.f + kx_exp2(y * cap_in))) : y * scale2;
-          }
-        if (!clear) {
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const int k = part * 16 + 8 * h + g, key = key0 + k;
-            const bool is = there[k >> 5] >> (k & 31) & 1u;
-#pragma unroll
-            for (int c = 0; c < 4; ++c) if (!(is && key <= at_place[c] && (a.window <= 0 || key > at_place[c] - a.window))) x[c][h] = -INFINITY;
+          for (int p = 0; p < P; ++p) {
+            kx_mma(d[p][0], k4[p], b[i][0], b[i][1]);
+            if (two) kx_mma(d[p][1], k4[p], b[i][2], b[i][3]);
           }
         }
-        if constexpr (FINAL) {
 #pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            float sum = 0.f;
+        for (int p = 0; p < P; ++p) {
+          const int part = part0 + p * wk;
+          float x[4][2];                               // rows as above, keys g and 8 + g
 #pragma unroll
-            for (int c = 0; c < 4; ++c) if (c < 2 || two) sum += x[c][h] == -INFINITY ? 0.f : kx_exp2(x[c][h] - ref[c]);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 1);
-            sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-            if (t == 0) sum_s[my_r][part * 16 + 8 * h + g] = sum;
+          for (int c = 0; c < 4; ++c)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) x[c][h] = d[p][c >> 1][2 * h + (c & 1)];
+          if (a.softcap > 0.f) {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) x[c][h] = cap_out * (1.f - __fdividef(2.f, 1.f + kx_exp2(x[c][h] * cap_in)));
+          } else {
+#pragma unroll
+            for (int c = 0; c < 4; ++c)
+#pragma unroll
+              for (int h = 0; h < 2; ++h) x[c][h] *= scale2;
           }
-        } else {
+          if (!clear) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            if (c >= 2 && !two) continue;
-            const float top = fmaxf(m[c], fmaxf(x[c][0], x[c][1])), zero = top == -INFINITY ? 0.f : top;
-            l[c] = (m[c] == -INFINITY ? l[c] : l[c] * kx_exp2(m[c] - zero)) + kx_exp2(x[c][0] - zero) + kx_exp2(x[c][1] - zero);
-            m[c] = top;
+            for (int h = 0; h < 2; ++h) {
+              const int k = part * 16 + 8 * h + g, key = key0 + k;
+              const bool is = there[k >> 5] >> (k & 31) & 1u;
+#pragma unroll
+              for (int c = 0; c < 4; ++c) if (!(is && key <= at_place[c] && (a.window <= 0 || key > at_place[c] - a.window))) x[c][h] = -INFINITY;
+            }
           }
-          if (a.scores != nullptr) {
+          if constexpr (FINAL) {
+            float sum[2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+              sum[h] = 0.f;
+              // a hidden key's weight is 0 whatever the row's logarithm is
+#pragma unroll
+              for (int c = 0; c < 4; ++c) if (c < 2 || two) sum[h] += !clear && x[c][h] == -INFINITY ? 0.f : kx_exp2(x[c][h] - ref[c]);
+            }
+            // the four lanes with a key's rows: an even lane has key g in the end, an odd one key 8 + g
+            const float y = (t & 1 ? sum[1] : sum[0]) + __shfl_xor_sync(0xffffffffu, t & 1 ? sum[0] : sum[1], 1), z = y + __shfl_xor_sync(0xffffffffu, y, 2);
+            if (t < 2) sum_s[my_r][part * 16 + 8 * t + g] = z;
+          } else {
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-              const int row = r0 + my_r * 16 + (c >> 1) * 8 + 2 * t + (c & 1);
-              if (row >= rows) continue;
-              float* to = a.scores + ((long)(first + row / G) * a.n_q + head * G + row % G) * a.width + key0 + part * 16 + g;
+              if (c >= 2 && !two) continue;
+              const float top = fmaxf(m[c], fmaxf(x[c][0], x[c][1])), zero = top == -INFINITY ? 0.f : top;
+              l[c] = (m[c] == -INFINITY ? l[c] : l[c] * kx_exp2(m[c] - zero)) + kx_exp2(x[c][0] - zero) + kx_exp2(x[c][1] - zero);
+              m[c] = top;
+            }
+            if (a.scores != nullptr) {
 #pragma unroll
-              for (int h = 0; h < 2; ++h) if (part * 16 + 8 * h + g < keys && key0 + part * 16 + 8 * h + g < a.width) to[8 * h] = x[c][h];
+              for (int c = 0; c < 4; ++c) {
+                const int row = r0 + my_r * 16 + (c >> 1) * 8 + 2 * t + (c & 1);
+                if (row >= rows) continue;
+                float* to = a.scores + ((long)(first + row / G) * a.n_q + head * G + row % G) * a.width + key0 + part * 16 + g;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) if (part * 16 + 8 * h + g < keys && key0 + part * 16 + 8 * h + g < a.width) to[8 * h] = x[c][h];
+              }
             }
           }
         }
+      };
+      if (busy) {
+        int part = my_k;
+        for (; (part + wk) * 16 < keys; part += 2 * wk) work(std::integral_constant<int, 2>(), part);
+        if (part * 16 < keys) work(std::integral_constant<int, 1>(), part);
       }
       if (more) put(tile + 1);
       if constexpr (FINAL) {
