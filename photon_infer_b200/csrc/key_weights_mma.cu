@@ -6,32 +6,13 @@
 // with its key, and a key's sum over the rows lies in the lanes of one row.  Every key is one block's: no atomics, the same bits every time.
 // Without the rows' logarithms a first kernel leaves each run's maxima and sums and a second one joins them.  Up to 16 rows' scores are kept as well, 4 bytes for 2 d of a key's
 // row, and a third kernel turns them into weights; for more rows the keys are read again.
-#include "kv4.cuh"
-#include <math.h>
+#include "key_weights.cuh"
 #include <type_traits>
 
-#define KX_KEYS 128
 #define KX_THREADS 256
 #define KX_WARPS 8
 #define KX_ROWS 128              // query rows in shared memory at a time, at most
 
-struct KeyWeightsMmaArgs {
-  const bf16* q; float* weights; const void* k; const int* table; const int* cu_tokens; const int* context_lens; const int* held; const float* sinks; const float* lse;
-  float* scratch; int* err;
-  long q_stride;
-  float* scores;                 // [T * n_q][width] in powers of two, or null
-  long width;
-  int max_pages, S, n_q, n_kv, page_size, num_pages, window;
-  int parts, each;               // runs of a request, and tiles of 128 keys in a run
-  int room;                      // for query rows: a multiple of 16
-  float scale, softcap;
-};
-
-__device__ __forceinline__ float kx_exp2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 __device__ __forceinline__ void kx_matrices(uint32_t* r, uint32_t at) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(at) : "memory");
 }
@@ -40,12 +21,6 @@ __device__ __forceinline__ void kx_mma(float* d, const uint32_t* a, uint32_t b0,
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ uint32_t kx_scaled(uint32_t word, int shift, __nv_bfloat162 scale) {      // codes at `shift` and 16 bits behind it, as numbers
-  const uint32_t x = (word >> shift & 0x000F000Fu) | 0x43004300u;                                     // 128 + c
-  const __nv_bfloat162 y = __hmul2(__hsub2(*(const __nv_bfloat162*)&x, __float2bfloat162_rn(136.f)), scale);
-  return *(const uint32_t*)&y;
-}
-
 // FINAL: the weights; else the maxima and sums of the run.
 template <int D, bool PACKED, bool FINAL>
 __global__ void __launch_bounds__(KX_THREADS, 2)
@@ -349,29 +324,6 @@ key_weights_scores_kernel(const KeyWeightsMmaArgs a) {
       if (x != -INFINITY) sum += kx_exp2(x - lse_s[r]);
     }
   *w = sum;
-}
-
-// A warp joins the maxima and sums of one (token, head).
-__global__ void __launch_bounds__(128)
-key_weights_lse_kernel(const KeyWeightsMmaArgs a, float* __restrict__ lse) {
-  pdl_wait();
-  const int seq = blockIdx.y, lane = threadIdx.x & 31, at = blockIdx.x * 4 + (threadIdx.x >> 5);
-  const int first = a.cu_tokens[seq], n = a.cu_tokens[seq + 1] - first, i = at / a.n_q, h = at - i * a.n_q;
-  if (i >= n) return;
-  const int parts = a.parts;
-  const long of = (long)(first + i) * a.n_q + h;
-  const float2* ml = (const float2*)(a.scratch + of * a.parts * 2);
-  float m = a.sinks != nullptr && lane == 0 ? a.sinks[h] * 1.4426950408889634f : -INFINITY, l = m == -INFINITY ? 0.f : 1.f;
-  for (int p = lane; p < parts; p += 32) {
-    const float2 x = ml[p];
-    if (x.y == 0.f) continue;
-    const float top = fmaxf(m, x.x);
-    l = (m == -INFINITY ? l : l * exp2f(m - top)) + (x.x == -INFINITY ? x.y : x.y * exp2f(x.x - top));
-    m = top;
-  }
-  const float top = warp_max(m);
-  l = warp_sum(m == -INFINITY ? l : l * exp2f(m - top));
-  if (lane == 0) lse[of] = l == 0.f ? -INFINITY : ((top == -INFINITY ? 0.f : top) + log2f(l)) * 0.6931471805599453f;
 }
 
 template <int D, bool PACKED, bool FINAL>

@@ -682,6 +682,8 @@ PHOTON_EXPORT int photon_key_weights(const photon_key_weights_call* call, cudaSt
 /* 16-byte aligned rows of q; at most max_tokens_per_seq tokens and max_keys keys a request.  parts: runs of a request's keys.  Without lse, scratch: T * n_q * (2 * parts + 1)
  * floats, and with keep_scores (at most 16 rows a request: the keys are read once) T * n_q * max_keys more. */
 PHOTON_EXPORT int photon_key_weights_mma(const photon_key_weights_call* call, cudaStream_t stream);
+/* key_weights_tc.cu: the same on tcgen05, for many rows; without keep_scores. */
+PHOTON_EXPORT int photon_key_weights_tc(const photon_key_weights_call* call, cudaStream_t stream);
 /* kv4_attention_mma.cu: with lse, for a cache in 4 bits and at most 8 rows (max_tokens_per_seq * n_q / n_kv), pages of a multiple of 8 tokens, 1,024 requests.  parts: blocks. */
 PHOTON_EXPORT int photon_kv4_key_weights(const photon_key_weights_call* call, cudaStream_t stream);
 

@@ -3074,7 +3074,7 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
     module = "kv4_attention_mma" if name == "kv4_key_weights" else name
     _check(_plain_fn(module, "photon_" + name, _CALL_ARGS)(call, _stream()), "key_weights")
     if lse is None:
-        _count_launches(2 if name == "key_weights_mma" else 1)
+        _count_launches(1 if name == "key_weights" else 2)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -3090,7 +3090,8 @@ def _key_weights_route(dtype: torch.dtype, head_dim: int, page_size: int, page_h
     # two blocks an SM: runs of keys for as many blocks as fill them, twice over for few rows, where a request that is shorter than the longest costs most
     parts = max(1, min(tiles, (4 if rows <= 16 else 2) * sms // max(1, num_seqs * n_kv)))
     keep = not known and rows <= 16 and all_rows * keys <= 1 << 26
-    return "key_weights_mma", parts, all_rows * (2 * parts + 1 + (keys if keep else 0)), keep
+    # tcgen05 has tiles of 128 rows: 32 rows of 8,000 keys take 20.7 us there and 19.9 us on the other kernel, 80 rows of four times 4,000 keys 34.6 and 50.2
+    return "key_weights_tc" if rows > 32 else "key_weights_mma", parts, all_rows * (2 * parts + 1 + (keys if keep else 0)), keep
 
 
 def cache_evict(kv: torch.Tensor, weights: torch.Tensor, block_table: torch.Tensor, context_lens: torch.Tensor, new_lens: torch.Tensor, num_seqs: int,
