@@ -2944,6 +2944,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
     page_size, pool = _kv4_caches("kv4_attention", n_kv, head_dim, k_cache, v_cache)
     _int32s("cu_tokens context_lens block_table", cu_tokens, context_lens, block_table)
     pages = _check_step("kv4_attention", num_seqs, cu_tokens, context_lens, block_table)
+    max_tokens_per_seq, max_keys = min(max_tokens_per_seq, T), min(max_keys, pages * page_size)
     if lse is not None:
         _check_lse("kv4_attention", lse, T, n_q)
     if T == 0 or num_seqs == 0 or max_tokens_per_seq <= 0 or max_keys <= 0:
@@ -3034,7 +3035,8 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
     gets, for its key/value head, the sum over the request's rows of ``exp(score - lse)``.  Tokens, keys, masks, ``sink`` and ``softcap`` as in ``kv4_attention``; the
     queries may be a step's, or the last ones of a prompt (``cu_tokens`` then counts those).  Keys from ``held[s]`` (int32) on have no sum yet and get this one; without
     ``held`` those are the given tokens' own keys.  ``k_cache``: a plain one of the type of ``q`` (``[pages, n_kv, page_size, d]``, ``d`` a multiple of 8 up to 256) or one in 4 bits.
-    ``lse``: as ``kv4_attention`` leaves it for the same queries; without it the keys are read twice."""
+    ``lse``: as ``kv4_attention`` leaves it for the same queries; without it the keys are read twice.  No page may be two requests' of a call, which would
+    add to one sum at once: requests that share a prefix are given one call after the other."""
     index = _on_device("key_weights", q, weights, k_cache, block_table, cu_tokens, context_lens, held, sink, lse, err)
     if sink is not None:
         _check_sink(sink, n_q)
@@ -3054,19 +3056,18 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "key_weights: weights must be contiguous float32 [pages, n_kv, page_size]")
     _int32s("cu_tokens context_lens block_table", cu_tokens, context_lens, block_table)
     pages = _check_step("key_weights", num_seqs, cu_tokens, context_lens, block_table)
+    max_tokens_per_seq, max_keys = min(max_tokens_per_seq, T), min(max_keys, pages * page_size)
     if held is not None:
         _int32(held, "held")
         if held.numel() < num_seqs:
             raise PhotonError(ErrorCode.SHAPE_MISMATCH, "key_weights: held must cover every request")
     _check_lse("key_weights", lse, T, n_q)
-    if num_seqs == 0 or max_keys <= 0:
-        return
-    if T == 0:
+    if T == 0 or num_seqs == 0 or max_tokens_per_seq <= 0 or max_keys <= 0:
         return
     if q.dtype == torch.bfloat16 and head_dim in (64, 128) and (q.stride(0) % 8 or q.data_ptr() % 16):
         q = q.contiguous() if q.stride(0) != q.shape[1] else q.clone()      # rows on 16-byte boundaries: a copy of the queries is little beside the keys
     name, parts, floats, keep = _key_weights_route(q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, packed, lse is not None, num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv),
-                                             max_keys, T * n_q, _sms(index, q.device))
+                                                   max_keys, T * n_q, _sms(index, q.device))
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if lse is None else None
     call = _KEY_WEIGHTS_CALL.pack(q.data_ptr(), weights.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), _data(held),
                                   _data(sink), _data(lse), _data(scratch), _data(err), q.stride(0), T, _dtype_code(q), int(packed), pages, num_seqs, max_keys, n_q, n_kv, head_dim,
@@ -3101,7 +3102,8 @@ def cache_evict(kv: torch.Tensor, weights: torch.Tensor, block_table: torch.Tens
     move to the front of the request's pages in their order; where ``keep`` is too small for that, the first ones come before the last ones.  ``kv``: ``[entries, planes, pages, n_kv,
     page_size, d]``, or uint8 ``[entries, planes, pages, n_kv, kv4_page_bytes]`` in 4 bits; ``weights`` (float32 ``[entries, pages, n_kv, page_size]``, as ``key_weights``
     leaves them) move along.  ``new_lens [S]``: the tokens that are left; what lies behind them stays as it was.  ``kept`` (int32 ``[entries, S, n_kv, keep]``): gets the old places
-    of the rows of requests that lose some.  Heads keep different tokens, so a request's later tokens take their positions from its text and their slots from the cache."""
+    of the rows of requests that lose some.  Heads keep different tokens, so a request's later tokens take their positions from its text and their slots from the cache.
+    The pages are rewritten in place: none may be another request's too (a shared prefix, a fork), inside the call or outside it."""
     _on_device("cache_evict", kv, weights, block_table, context_lens, new_lens, kept, err)
     shape, wanted = kv.shape, weights.shape
     if weights.dtype != torch.float32 or len(wanted) != 4 or not weights.is_contiguous() or weights.numel() == 0:
