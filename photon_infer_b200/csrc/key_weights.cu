@@ -4,8 +4,7 @@
 // held[seq] on have no sum yet and get this one.  lse [T, n_q]: the natural logarithm of each row's sum of exponentials; where there is none, a first kernel leaves
 // the maximum and the sum of every share of the keys, and the second joins them.  Every key is one thread's: no sums over blocks, no atomics.
 // The cache: 4 bits (kv4.cuh), bfloat16 or 32 bits.
-#include "kv4.cuh"
-#include <math.h>
+#include "key_weights.cuh"
 
 #define KW_THREADS 128
 #define KW_ROWS 8
@@ -17,25 +16,6 @@ struct KeyWeightsArgs {
   int max_pages, n_q, n_kv, d, page_size, num_pages, window, parts;
   float scale, softcap;
 };
-
-__device__ __forceinline__ float key_score(float x, float scale, float softcap) {      // in powers of two
-  constexpr float LOG2E = 1.4426950408889634f;
-  return softcap > 0.f ? softcap * tanhf(x * scale / softcap) * LOG2E : x * (scale * LOG2E);
-}
-
-// Numbers 8 x .. 8 x + 7 of a key's row in its own order.
-template <typename C>
-__device__ __forceinline__ void key_numbers(const C* row, int x, float* c) {
-  if constexpr (sizeof(C) == 2) {
-    const uint4 u = ((const uint4*)row)[x];
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) { c[2 * i] = __uint_as_float(w[i] << 16); c[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
-  } else {
-    const float4 a = ((const float4*)row)[2 * x], b = ((const float4*)row)[2 * x + 1];
-    c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w; c[4] = b.x; c[5] = b.y; c[6] = b.z; c[7] = b.w;
-  }
-}
 
 // T: the queries' type, C: the cache's; FINAL: the weights, else the shares' maxima and sums.
 template <typename T, typename C, bool FINAL>

@@ -1,4 +1,4 @@
-// What the tensor-core kernels of key_weights_mma.cu and key_weights_tc.cu share: their arguments, codes as bfloat16 numbers, and the join of the runs' maxima and sums.
+// What the kernels of key_weights*.cu share: their arguments, numbers of keys, scores, and the join of the runs' maxima and sums.
 #pragma once
 #include "kv4.cuh"
 #include <math.h>
@@ -26,6 +26,25 @@ __device__ __forceinline__ uint32_t kx_scaled(uint32_t word, int shift, __nv_bfl
   const uint32_t x = (word >> shift & 0x000F000Fu) | 0x43004300u;                                     // 128 + c
   const __nv_bfloat162 y = __hmul2(__hsub2(*(const __nv_bfloat162*)&x, __float2bfloat162_rn(136.f)), scale);
   return *(const uint32_t*)&y;
+}
+
+__device__ __forceinline__ float key_score(float x, float scale, float softcap) {      // in powers of two
+  constexpr float LOG2E = 1.4426950408889634f;
+  return softcap > 0.f ? softcap * tanhf(x * scale / softcap) * LOG2E : x * (scale * LOG2E);
+}
+
+// Numbers 8 x .. 8 x + 7 of a key's row in its own order.
+template <typename C>
+__device__ __forceinline__ void key_numbers(const C* row, int x, float* c) {
+  if constexpr (sizeof(C) == 2) {
+    const uint4 u = ((const uint4*)row)[x];
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) { c[2 * i] = __uint_as_float(w[i] << 16); c[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u); }
+  } else {
+    const float4 a = ((const float4*)row)[2 * x], b = ((const float4*)row)[2 * x + 1];
+    c[0] = a.x; c[1] = a.y; c[2] = a.z; c[3] = a.w; c[4] = b.x; c[5] = b.y; c[6] = b.z; c[7] = b.w;
+  }
 }
 
 // A warp joins the maxima and sums of one (token, head).

@@ -672,11 +672,15 @@ PHOTON_EXPORT int photon_kv4_attention_mma(const photon_kv4_attention_call* call
 typedef struct {
   const void* q; float* weights; const void* k_cache; const int* block_table; const int* cu_tokens; const int* context_lens; const int* held; const float* sinks;
   const float* lse; float* scratch; int* err;
-  long q_stride, scratch_rows;          /* scratch_rows: T, for the second form */
+  long q_stride, scratch_rows;          /* scratch_rows: T */
   int dtype, packed, max_pages, S, max_keys, n_q, n_kv, d, page_size, num_pages, window, parts, max_tokens_per_seq, keep_scores;
   float scale, softcap;
 } photon_key_weights_call;
 PHOTON_EXPORT int photon_key_weights(const photon_key_weights_call* call, cudaStream_t stream);
+
+/* ------------------------------------------------------------------ key_weights_rows.cu: the same for many rows */
+/* At most max_tokens_per_seq tokens a request.  parts: runs of a request's keys.  Without lse, scratch: T * n_q * (2 * parts + 1) floats. */
+PHOTON_EXPORT int photon_key_weights_rows(const photon_key_weights_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ key_weights_mma.cu: the same on the tensor cores, bfloat16, d 64 or 128 */
 /* 16-byte aligned rows of q; at most max_tokens_per_seq tokens and max_keys keys a request.  parts: runs of a request's keys.  Without lse, scratch: T * n_q * (2 * parts + 1)

@@ -38,9 +38,10 @@ def test_weights():
         assert parts >= 1
         if name == "kv4_key_weights":
             assert packed and known and rows <= 8 and page % 8 == 0 and seqs <= 1024 and floats == 0
-        elif name == "key_weights":
-            assert (dtype, d) not in ((torch.bfloat16, 64), (torch.bfloat16, 128)) and floats == 2 * all_rows * parts and not keep
+        elif name in ("key_weights", "key_weights_rows"):
+            assert (dtype, d) not in ((torch.bfloat16, 64), (torch.bfloat16, 128)) and not keep
+            assert (name == "key_weights") == (rows <= 8) and floats == all_rows * (2 * parts + (0 if rows <= 8 else 1))
         else:
             assert dtype == torch.bfloat16 and d in (64, 128) and (name == "key_weights_tc") == (rows > 32)
             assert floats == all_rows * (2 * parts + 1 + (keys if keep else 0)) and (not keep or (rows <= 16 and not known and floats <= (1 << 26) + all_rows * (2 * parts + 1)))
-    assert seen == {"key_weights", "key_weights_mma", "key_weights_tc", "kv4_key_weights"}
+    assert seen == {"key_weights", "key_weights_rows", "key_weights_mma", "key_weights_tc", "kv4_key_weights"}
