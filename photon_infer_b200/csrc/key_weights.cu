@@ -4,6 +4,9 @@
 // held[seq] on have no sum yet and get this one.  lse [T, n_q]: the natural logarithm of each row's sum of exponentials; where there is none, a first kernel leaves
 // the maximum and the sum of every share of the keys, and the second joins them.  Every key is one thread's: no sums over blocks, no atomics.
 // The cache: 4 bits (kv4.cuh), bfloat16 or 32 bits.
+//
+// For up to 8 rows, 8 at a time, in 32 bits: what bounds it is the reading, since a thread has a key and reads its row by itself, and every number meets 8 rows' whether they are there or not.  4
+// rows beside 4,000 keys, 8 heads of 128, 32 bits: 30 us; key_weights_rows.cu takes 35 for them and from 9 rows on less.
 #include "key_weights.cuh"
 
 #define KW_THREADS 128
