@@ -5,9 +5,9 @@
 // First the rows are the first operand: two threads have a row, and its maximum and its sum over the keys stay in registers.  Then, with the rows' logarithms, the keys
 // are: two threads have a key and add up what the rows give it.  No score leaves tensor memory but into the registers of the thread that needs it, and a sum has one order.
 //
-// What bounds it: the exponentials, two for a score at 16 a cycle on an SM, take 1.1 us of the 2.6 us that a pass needs for two blocks' tiles; the rest is waiting inside a
+// What bounds it: the exponentials, two for a score at 16 a cycle on an SM, take 1.1 us of the 2 to 2.5 us that a pass needs for two blocks' tiles; the rest is waiting inside a
 // tile, with 16 warps on an SM, which tensor memory (2 x 128 columns a block) and shared memory allow no more of.  Two requests of 32 tokens beside 8,009 keys, 32 query heads on 8,
-// heads of 128: 41 us, where key_weights_mma.cu takes 60; 8 of 64 beside 4,000: 118 and 197; up to 32 rows key_weights_mma.cu is the faster by 1 to 3 us.
+// heads of 128: 37 us, where key_weights_mma.cu takes 60; 8 of 64 beside 4,000: 118 and 197; up to 32 rows key_weights_mma.cu is the faster by 1 to 3 us.
 #include "key_weights.cuh"
 #include "tcgen05.cuh"
 #include <type_traits>
@@ -65,20 +65,30 @@ key_weights_tc_kernel(const KeyWeightsMmaArgs a) {
   bool fine = true;
   float m = -INFINITY, l = 0.f;                       // of row block_r0 + own, in this thread's columns; m in unscaled scores where nothing bounds them
   if (tile0 < tile1) {
-    // ---- places: thread `tid` < 128 has key `tid` of a tile, and the block table's entry of the next one
-    auto entry_of = [&](int tile) {
-      const int key = tile * KX_KEYS + tid, pidx = key / a.page_size;
-      return half == 0 && tile < tile1 && key < ctx ? (pidx < a.max_pages ? a.table[(long)seq * a.max_pages + pidx] : -1) : -2;      // -2: not asked for
+    // ---- places: thread `tid` < 128 has key `tid` of a tile; the block table's entries come a tile ahead, and a tile's page and place follow from those of the one in front
+    const int first_key = tile0 * KX_KEYS + own, step_pages = KX_KEYS / a.page_size, step_slots = KX_KEYS - step_pages * a.page_size;
+    int next_page = 0, next_slot = 0, next_key = 0;
+    struct Place { int entry, slot; };                 // entry -2: not asked for
+    auto look = [&]() {                                // the tiles one behind the other; what is not there reads some entry of the table, too
+      const int entry = a.table[(long)seq * a.max_pages + min(next_page, a.max_pages - 1)];
+      const Place p = {half != 0 || next_key >= min(ctx, tile1 * KX_KEYS) ? -2 : next_page < a.max_pages ? entry : -1, next_slot};
+      next_key += KX_KEYS;
+      next_page += step_pages;
+      next_slot += step_slots;
+      if (next_slot >= a.page_size) {
+        next_slot -= a.page_size;
+        ++next_page;
+      }
+      return p;
     };
-    auto settle = [&](int tile, int entry) {           // the tile's places, from its entries
+    auto settle = [&](int tile, Place p) {             // the tile's places
       if (half != 0 || tile >= tile1) return;
-      const int key = tile * KX_KEYS + tid, slot = key - key / a.page_size * a.page_size;
-      const bool good = entry >= 0 && entry < a.num_pages;
-      if (FINAL && !good && entry != -2) report_error(a.err, PHOTON_DEV_BAD_PAGE, seq, key, entry);
+      const bool good = p.entry >= 0 && p.entry < a.num_pages;
+      if (FINAL && !good && p.entry != -2) report_error(a.err, PHOTON_DEV_BAD_PAGE, seq, tile * KX_KEYS + tid, p.entry);
       const uint32_t votes = __ballot_sync(0xffffffffu, good);
       if (lane == 0) there_s[tile & 3][warp] = votes;
-      row_s[tile & 3][tid] = ((long)(good ? entry : 0) * a.n_kv + head) * a.page_size + (good ? slot : 0);      // else some row of the pool: what is read is not used
-      slot_s[tile & 3][tid] = good ? slot : 0;
+      row_s[tile & 3][tid] = ((long)(good ? p.entry : 0) * a.n_kv + head) * a.page_size + (good ? p.slot : 0);      // else some row of the pool: what is read is not used
+      if (PACKED) slot_s[tile & 3][tid] = good ? p.slot : 0;
     };
     auto piece_at = [&](uint8_t* tile, int row, int piece) { return tile + (piece >> 3) * (128 * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4); };
     constexpr int ROUNDS = KX_KEYS * PIECES / KT_THREADS;                  // of a thread, 16 bytes each
@@ -120,29 +130,38 @@ key_weights_tc_kernel(const KeyWeightsMmaArgs a) {
       }
     };
     auto stage_rows = [&](int r0) {
-      for (int x = tid; x < 128 * (D / 8); x += KT_THREADS) {
-        const int r = x / (D / 8), piece = x - r * (D / 8), row = r0 + r;
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        if (row < rows) v = *(const uint4*)(a.q + (first + row / G) * a.q_stride + (long)(head * G + row % G) * D + 8 * piece);
-        *(uint4*)piece_at(q_s, r, piece) = v;
+      constexpr int EACH = 128 * (D / 8) / KT_THREADS;
+      uint4 v[EACH];
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {                 // all are asked for before the first is put
+        const int x = i * KT_THREADS + tid, r = x / (D / 8), piece = x - r * (D / 8), row = r0 + r, token = row / G;
+        v[i] = make_uint4(0u, 0u, 0u, 0u);
+        if (row < rows) v[i] = *(const uint4*)(a.q + (first + token) * a.q_stride + (long)(head * G + row - token * G) * D + 8 * piece);
+      }
+      const int row = r0 + own, token = min(row, rows - 1) / G;
+      const float lse = FINAL && row < rows ? a.lse[(long)(first + token) * a.n_q + head * G + row - token * G] * 1.4426950408889634f : INFINITY;
+#pragma unroll
+      for (int i = 0; i < EACH; ++i) {
+        const int x = i * KT_THREADS + tid, r = x / (D / 8), piece = x - r * (D / 8);
+        *(uint4*)piece_at(q_s, r, piece) = v[i];
       }
       if (half != 0) return;
-      const int row = r0 + tid;
-      place_s[tid] = row < rows ? base + row / G : -1;
-      lse_s[tid] = FINAL && row < rows ? a.lse[(long)(first + row / G) * a.n_q + head * G + row % G] * 1.4426950408889634f : INFINITY;
+      place_s[tid] = row < rows ? base + token : -1;
+      lse_s[tid] = lse;
     };
     const float scale2 = a.scale * 1.4426950408889634f, cap_in = 2.f * 1.4426950408889634f * a.scale / a.softcap, cap_out = a.softcap * 1.4426950408889634f;
     auto bounded = [&](float x) { return cap_out * (1.f - __fdividef(2.f, 1.f + kx_exp2(x * cap_in))); };
     // The products of a tile run while the scores of the one in front of it are worked on, and the keys behind it are on their way.
+    const uint64_t k_desc = tc_desc(tc_smem(k_s)), q_desc = tc_desc(tc_smem(q_s));
     auto multiply = [&](int tile, int width) {
       if (warp == 0 && tile < tile1 && tc_elect()) {
         tc_fence_after();
-        const uint32_t k_addr = tc_smem(k_s + (tile & 1) * TILE), q_addr = tc_smem(q_s), to = tmem + 128 * (tile & 1);
+        const uint32_t to = tmem + 128 * (tile & 1), idesc = FINAL ? tc_idesc(128, width) : tc_idesc(128, 128);
+        const uint64_t kt = k_desc + (tile & 1) * (TILE >> 4);
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t kd = tc_desc(k_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32), qd = tc_desc(q_addr + (kk >> 2) * (128 * 128) + (kk & 3) * 32);
-          if (FINAL) tc_mma(to, kd, qd, tc_idesc(128, width), kk > 0 ? 1u : 0u);
-          else tc_mma(to, qd, kd, tc_idesc(128, 128), kk > 0 ? 1u : 0u);
+        for (int kk = 0; kk < D / 16; ++kk) {          // in 16 bytes: 16 numbers of a row, a panel
+          const int at = ((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4;
+          tc_mma(to, FINAL ? kt + at : q_desc + at, FINAL ? q_desc + at : kt + at, idesc, kk > 0 ? 1u : 0u);
         }
         tc_commit(&done);
       }
@@ -156,11 +175,14 @@ key_weights_tc_kernel(const KeyWeightsMmaArgs a) {
     uint32_t parity = 0;
     for (int r0 = block_r0; r0 < (FINAL ? rows : block_r0 + 1) && fine; r0 += 128) {
       const int width = min(128, (rows - r0 + 15) / 16 * 16);             // columns of rows
-      int entry = entry_of(tile0), entry1 = entry_of(tile0 + 1);
+      next_page = first_key / a.page_size;
+      next_slot = first_key - next_page * a.page_size;
+      next_key = first_key;
+      const Place place0 = look(), place1 = look();
+      Place ahead = look();
       stage_rows(r0);
-      settle(tile0, entry);
-      settle(tile0 + 1, entry1);
-      entry = entry_of(tile0 + 2);
+      settle(tile0, place0);
+      settle(tile0 + 1, place1);
       __syncthreads();
       ask(tile0);
       put(tile0);
@@ -177,8 +199,8 @@ key_weights_tc_kernel(const KeyWeightsMmaArgs a) {
         const int key0 = tile * KX_KEYS;
         float had = 0.f;
         if (FINAL && half == 0 && (there_s[tile & 3][warp & 3] >> lane & 1u) && (r0 > 0 || key0 + tid < known)) had = a.weights[row_s[tile & 3][tid]];
-        settle(tile + 2, entry);
-        entry = entry_of(tile + 3);
+        settle(tile + 2, ahead);
+        ahead = look();
         arrived();
         const bool ok = tc_wait_warp(&done, parity, &abort_s);
         parity ^= 1;

@@ -18,7 +18,7 @@
 //
 // What bounds it: instructions.  A warp's tile of 32 keys and values, heads of 128, has some 620, of which 290 run at half rate: 47 us of the 68 that 64 requests of up to 6,000 keys take (24
 // query heads on 8; 253 MB, 0.57 of the copy rate); 20 us are begin, end and join.  Two requests of 100,003 keys, 32 on 8: 63 us, 0.53.  One of 640, heads of 64: 7.5 us, a chain of
-// latencies.  Equal runs instead of a block for each share of a request: 94 to 79 us for the 64; units of 8 rows take 1.3 times a unit of 4.  8-bit products were slower.
+// latencies.  Equal runs instead of a block for each share of a request: 94 to 79 us for the 64.  8-bit products were slower.
 #include "kv4.cuh"
 #include <math.h>
 
