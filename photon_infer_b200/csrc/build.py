@@ -32,7 +32,7 @@ BASE_FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-shared", "-Xcompiler", "-fPIC"
 ALL_MODULES = ("elementwise", "rope_kv", "qk_norm", "attention", "attention_rows", "latent", "hyper", "gla", "delta", "delta_chunked", "attention_talk", "attention_diff", "linrec", "linrec_segments", "linrec_chunks", "row_norms", "moe", "gemm_f32", "gemm_f32_tc", "gemm_skinny", "gemm_skinny_fused",
                "gemm_skinny_static",
                "gemm_tc", "gemm_tc2", "sampling", "tree_attention", "tree_attention_tc", "tree_attention_few", "tree_accept", "cache_rows",
-               "kv4", "kv4_attention", "kv4_attention_mma", "key_weights", "key_weights_rows", "key_weights_mma", "key_weights_tc", "cache_evict")
+               "kv4", "kv4_attention", "kv4_attention_rows", "kv4_attention_mma", "key_weights", "key_weights_rows", "key_weights_mma", "key_weights_tc", "cache_evict")
 
 _loaded: Dict[Tuple[str, Tuple[Tuple[str, str], ...]], ctypes.CDLL] = {}
 _lock = threading.Lock()

@@ -659,6 +659,8 @@ typedef struct {
   float scale, softcap;
 } photon_kv4_attention_call;
 PHOTON_EXPORT int photon_kv4_attention(const photon_kv4_attention_call* call, cudaStream_t stream);
+/* kv4_attention_rows.cu: the same for many rows. */
+PHOTON_EXPORT int photon_kv4_attention_rows(const photon_kv4_attention_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ kv4_attention_mma.cu: the same on the tensor cores, bfloat16, d 64 or 128 */
 /* At most 1,024 requests, pages of a multiple of 8 tokens, caches of up to 64 GB each.  parts: blocks of the grid; scratch: 8 * parts * R * (d + 2) + S + 1 words, R = 4 for at

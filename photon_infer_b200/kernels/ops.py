@@ -2988,9 +2988,14 @@ def _kv4_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: in
         units = num_seqs * n_kv * -(-rows // tile)
         parts = min((5 - head_dim // 64 - (tile == 8)) * sms, -(-units * (-(-keys // 32) + 1) // 4))
         return "kv4_attention_mma", parts, 8 * parts * tile * (head_dim + 2) + num_seqs + 1
-    tiles, blocks = -(-keys // 128), num_seqs * n_kv * -(-rows // 8)
-    parts = max(1, min(tiles, 4 * sms // blocks, 64))
-    return "kv4_attention", parts, all_rows * parts * (head_dim + 2) if parts > 1 else 0
+    # In 32 bits, 32/8 heads of 128, us on the first kernel and the second: 12 rows of 8 requests behind 2,000 keys 135 and 182, 24 of 2 behind 3,000 90 and 99, 32 of 2 behind 3,000
+    # 115 and 100, of 8 behind 2,000 257 and 184; where the first has a tile of rows and keys for a block or so, it is the faster: 32 rows behind 500 keys 26 and 37, 160 behind 500
+    # (640 tiles on 148 SMs) 55 and 39.
+    tiles, few_blocks = -(-keys // 128), num_seqs * n_kv * -(-rows // 8)
+    many = rows > 24 and few_blocks * tiles > 4 * sms
+    blocks = num_seqs * n_kv * -(-rows // 64) if many else few_blocks
+    parts = max(1, min(tiles, (2 if many else 4) * sms // blocks, 64))
+    return "kv4_attention_rows" if many else "kv4_attention", parts, all_rows * parts * (head_dim + 2) if parts > 1 else 0
 
 
 _KV4_SPOIL_ARGS = [c_char_p, c_void_p, c_long, c_int, c_void_p]

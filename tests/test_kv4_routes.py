@@ -18,7 +18,8 @@ def test_attention():
             # eight warps of a block, each with a tile of rows and a place for what it leaves, and the requests' sums in front
             assert parts <= 4 * 148 and floats == 8 * parts * (4 if rows <= 4 else 8) * (d + 2) + seqs + 1
         else:
-            assert name == "kv4_attention" and parts <= 64 and floats == (tokens * parts * (d + 2) if parts > 1 else 0)
+            assert (name == "kv4_attention_rows") == (rows > 24 and seqs * n_kv * -(-rows // 8) * -(-keys // 128) > 4 * 148) and name in ("kv4_attention", "kv4_attention_rows")
+            assert parts <= 64 and floats == (tokens * parts * (d + 2) if parts > 1 else 0)
 
 
 def test_few_rows_stay_with_the_codes():
