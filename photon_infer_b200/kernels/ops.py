@@ -2977,7 +2977,10 @@ def _kv4_few(head_dim: int, page_size: int, num_seqs: int, n_kv: int, rows: int,
     if head_dim not in (64, 128) or page_size % 8 or num_seqs > 1024:
         return False
     codes = num_seqs * n_kv * -(-rows // 8) * -(-keys // 32) * (1.33e-3 if head_dim == 128 else 0.78e-3) + 3
-    return codes <= keys * (15.5e-3 if head_dim == 128 else 11.8e-3) + num_seqs * n_kv * keys * head_dim * 1.37e-6
+    laid_out = keys * (15.5e-3 if head_dim == 128 else 11.8e-3) + num_seqs * n_kv * keys * head_dim * 1.37e-6
+    # Short prompts are bound by the host, since the framework launches prompt portions from Python: the five launches with laid out pages take it 77 to 88 us, the two with the codes 18
+    # to 28.  128 tokens behind 500: 87 and 42 us a call (captured in a graph 21 and 40), heads of 64 80 and 23 (17 and 21); 64 behind 200: 89 and 28 (17 and 21).
+    return codes <= max(laid_out, 15)
 
 
 @functools.lru_cache(maxsize=4096)
@@ -3014,20 +3017,20 @@ def _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, 
         into = into.clone(memory_format=torch.contiguous_format)
     one = per * n_kv * page_size * head_dim * 4
     some = max(1, min(num_seqs, KV4_PROMPT_BYTES // one, 65535 // -(-max_tokens // (128 // (n_q // n_kv)))))
-    numbers = torch.empty((2, some * per, n_kv, page_size, head_dim), dtype=q.dtype, device=device)
-    marks = some * per * (1 + -(-n_kv * page_size // 32))
-    where = torch.empty(marks + T, dtype=torch.int32, device=device)
-    table, flags, positions = where[:some * per].view(some, per), where[some * per:marks], where[marks:]
+    k_numbers, v_numbers = torch.empty((2, some * per, n_kv, page_size, head_dim), dtype=q.dtype, device=device).unbind()
+    marks = some * per * -(-n_kv * page_size // 32)
+    table, flags, positions = torch.empty(some * per + marks + T, dtype=torch.int32, device=device).split((some * per, marks, T))
+    table, k_at, v_at, table_at, positions_at, flags_at = table.view(some, per), k_numbers.data_ptr(), v_numbers.data_ptr(), table.data_ptr(), positions.data_ptr(), flags.data_ptr()
+    pages, pool, group = block_table.shape[1], k_cache.shape[0], n_q // n_kv
+    unpack, spoil = _plain_fn("kv4", "photon_kv4_unpack", _CALL_ARGS), _plain_fn("kv4", "photon_kv4_spoil", _KV4_SPOIL_ARGS)
     for s0 in range(0, num_seqs, some):
         n = min(some, num_seqs - s0)
-        cu, lens = cu_tokens[s0:s0 + n + 1], context_lens[s0:s0 + n]
-        call = _KV4_UNPACK_CALL.pack(k_cache.data_ptr(), v_cache.data_ptr(), block_table[s0:].data_ptr(), numbers[0].data_ptr(), numbers[1].data_ptr(), cu.data_ptr(),
-                                     lens.data_ptr(), table.data_ptr(), positions.data_ptr(), flags.data_ptr(), _data(err), block_table.shape[1], _dtype_code(q), n, per, n_kv, head_dim,
-                                     page_size, k_cache.shape[0], n_q // n_kv, KV4_FEW_ROWS)
-        _check(_plain_fn("kv4", "photon_kv4_unpack", _CALL_ARGS)(call, _stream()), "kv4_attention")
-        attention_tc(q, into, numbers[0], numbers[1], table[:n], cu, positions, n, max_tokens, n_q, n_kv, head_dim, window, scale, err, sink=sink, softcap=softcap,
-                     keys=max_keys)
-        _check(_plain_fn("kv4", "photon_kv4_spoil", _KV4_SPOIL_ARGS)(call, into.data_ptr(), into.stride(0), window, _stream()), "kv4_attention")
+        cu = cu_tokens[s0:s0 + n + 1] if s0 else cu_tokens
+        call = _KV4_UNPACK_CALL.pack(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr() + 4 * s0 * pages, k_at, v_at, cu.data_ptr(), context_lens.data_ptr() + 4 * s0,
+                                     table_at, positions_at, flags_at, _data(err), pages, _dtype_code(q), n, per, n_kv, head_dim, page_size, pool, group, KV4_FEW_ROWS)
+        _check(unpack(call, _stream()), "kv4_attention")
+        attention_tc(q, into, k_numbers, v_numbers, table, cu, positions, n, max_tokens, n_q, n_kv, head_dim, window, scale, err, sink=sink, softcap=softcap, keys=max_keys)
+        _check(spoil(call, into.data_ptr(), into.stride(0), window, _stream()), "kv4_attention")
     if into is not out:
         out.copy_(into)
 
