@@ -30,6 +30,7 @@
 // Blocks an SM: what their registers leave room for.
 #define KM_BLOCKS(GROUPS, NT) ((GROUPS == 4 ? 4 : 5) - NT)
 #define KM_STAGES 3              // of a warp's 32 keys and values in shared memory
+#define KM_MOST 0x7fffffffu      // steps of a call: so many or more are counted as this, and not taken
 
 struct Kv4MmaArgs {
   const bf16* q; bf16* out; const uint8_t* k; const uint8_t* v;
@@ -123,7 +124,7 @@ __device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
   int lo = a.window > 0 ? max(0, r.ctx - r.n - a.window + 1) : 0;
   if (WEIGH) lo = max(0, min(lo, a.held != nullptr ? a.held[s] : r.ctx - r.n));      // keys without a sum get one
   r.from = lo & ~7;
-  r.steps = r.rows > 0 ? max(1, (r.ctx - r.from + KM_KEYS - 1) / KM_KEYS) : 0;
+  r.steps = r.rows <= 0 ? 0 : r.ctx <= r.from ? 1 : (int)(((unsigned)(r.ctx - r.from) + KM_KEYS - 1) / KM_KEYS);
   return r;
 }
 
@@ -150,17 +151,20 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t = lane & 3;
   pdl_wait();
   if (warp == 0) {
-    int sum = 0;
+    uint32_t sum = 0;                                 // a sum of two such counts fits 32 bits
     for (int s0 = 0; s0 < a.S; s0 += 32) {
-      int x = 0;
-      if (s0 + lane < a.S) { const KmRequest r = km_request<RT, WEIGH>(a, s0 + lane); x = r.steps * r.row_tiles * a.n_kv; }
+      uint32_t x = 0;
+      if (s0 + lane < a.S) {
+        const KmRequest r = km_request<RT, WEIGH>(a, s0 + lane);
+        x = (uint32_t)min((unsigned long long)r.steps * r.row_tiles * a.n_kv, (unsigned long long)KM_MOST);
+      }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
+        const uint32_t y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x = min(x + y, KM_MOST);
       }
-      if (s0 + lane < a.S) before_s[s0 + lane + 1] = sum + x;
-      sum += __shfl_sync(0xffffffffu, x, 31);
+      if (s0 + lane < a.S) before_s[s0 + lane + 1] = (int)min(sum + x, KM_MOST);
+      sum = min(sum + __shfl_sync(0xffffffffu, x, 31), KM_MOST);
     }
     if (lane == 0) before_s[0] = 0;
     if (!WEIGH && blockIdx.x == 0) {                  // for the second kernel
@@ -171,6 +175,10 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
   __syncthreads();
   pdl_launch_dependents();
   const int total = before_s[a.S], N = gridDim.x * 4, me = blockIdx.x * 4 + warp;
+  if ((uint32_t)total == KM_MOST) {                   // lengths that the call's limits do not cover: the host gives no such call to this kernel
+    if (blockIdx.x == 0 && threadIdx.x == 0) report_error(a.err, PHOTON_DEV_TOO_LONG, a.S, a.n_kv, 0);
+    return;
+  }
   const KmRuns runs(total, N);
   const int begin = runs.begin(me), end = runs.begin(me + 1);
   if (begin >= end) return;
@@ -665,7 +673,7 @@ kv4_mma_join_kernel(const Kv4MmaArgs a, int N) {
   const int s = blockIdx.z, head = blockIdx.y, tile = blockIdx.x, tid = threadIdx.x, pars = blockDim.x / ITEMS, item = tid % ITEMS, par = tid / ITEMS;
   const int before = a.before[s], after = a.before[s + 1], total = a.before[a.S];
   const KmRequest R = km_request<RT, false>(a, s);
-  if (after == before || tile >= R.row_tiles) return;
+  if (after == before || tile >= R.row_tiles || (uint32_t)total == KM_MOST) return;
   const int from = before + (head * R.row_tiles + tile) * R.steps, to = from + R.steps;
   const KmRuns runs(total, N);
   const int w0 = runs.warp_of(from), w1 = runs.warp_of(to - 1);

@@ -97,7 +97,8 @@ def graph_batch_size(n: int) -> int:
 _DEVICE_ERRORS = {1: "token id {1} at token {0} of the step is outside the vocabulary of {2}",
                   2: "token {0} of the step was given cache slot {1}, outside the pool of {2} slots",
                   3: "token {0} of the step needs key {1}, whose block-table entry is {2}",
-                  4: "a kernel gave up waiting (stage {0}, {1}, {2})"}
+                  4: "a kernel gave up waiting (stage {0}, {1}, {2})",
+                  5: "the lengths of {0} requests are more work than a kernel counts"}
 
 
 class ModelRunner:

@@ -49,6 +49,7 @@ extern "C" {
 #define PHOTON_DEV_BAD_SLOT 2
 #define PHOTON_DEV_BAD_PAGE 3
 #define PHOTON_DEV_WAIT_TIMEOUT 4
+#define PHOTON_DEV_TOO_LONG 5          /* lengths on the device that are more work than a kernel counts: it did nothing */
 /* activations of the gated feed-forward kernels: silu, and the tanh form of gelu */
 #define PHOTON_ACT_SILU 0
 #define PHOTON_ACT_GELU_TANH 1
@@ -663,7 +664,8 @@ PHOTON_EXPORT int photon_kv4_attention(const photon_kv4_attention_call* call, cu
 PHOTON_EXPORT int photon_kv4_attention_rows(const photon_kv4_attention_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ kv4_attention_mma.cu: the same on the tensor cores, bfloat16, d 64 or 128 */
-/* At most 1,024 requests, pages of a multiple of 8 tokens, caches of up to 64 GB each.  parts: blocks of the grid; scratch: 8 * parts * R * (d + 2) + S + 1 words, R = 4 for at
+/* At most 1,024 requests, pages of a multiple of 8 tokens, caches of up to 64 GB each, and fewer than 2^31 - 1 steps: of a request, (tokens * n_q / n_kv / R, rounded up) * n_kv * (keys /
+ * 32, rounded up).  Of more, counted on the device, nothing is done and PHOTON_DEV_TOO_LONG is recorded.  parts: blocks of the grid; scratch: 8 * parts * R * (d + 2) + S + 1 words, R = 4 for at
  * most 4 rows a request, else 8. */
 PHOTON_EXPORT int photon_kv4_attention_mma(const photon_kv4_attention_call* call, cudaStream_t stream);
 

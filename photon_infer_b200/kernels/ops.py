@@ -2987,10 +2987,11 @@ def _kv4_few(head_dim: int, page_size: int, num_seqs: int, n_kv: int, rows: int,
 def _kv4_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: int, num_seqs: int, n_kv: int, rows: int, keys: int, all_rows: int, sms: int):
     """(kernel, parts, floats of scratch) for requests of at most ``rows`` rows (tokens x query heads per key/value head) and ``keys`` visible keys."""
     if dtype == torch.bfloat16 and head_dim in (64, 128) and page_size % 8 == 0 and 0 < page_heads * kv4_page_bytes(page_size, head_dim) < 1 << 36 and num_seqs <= 1024:
-        tile = 4 if rows <= 4 else 8
-        units = num_seqs * n_kv * -(-rows // tile)
-        parts = min((5 - head_dim // 64 - (tile == 8)) * sms, -(-units * (-(-keys // 32) + 1) // 4))
-        return "kv4_attention_mma", parts, 8 * parts * tile * (head_dim + 2) + num_seqs + 1
+        tile, steps = 4 if rows <= 4 else 8, -(-keys // 32) + 1
+        # the kernel counts the call's steps in 31 bits: row tiles, a request's last one not full, by the longest request's keys
+        if (all_rows // tile + num_seqs * n_kv) * steps < (1 << 31) - 1:
+            parts = min((5 - head_dim // 64 - (tile == 8)) * sms, -(-num_seqs * n_kv * -(-rows // tile) * steps // 4))
+            return "kv4_attention_mma", parts, 8 * parts * tile * (head_dim + 2) + num_seqs + 1
     # In 32 bits, 32/8 heads of 128, us on the first kernel and the second: 12 rows of 8 requests behind 2,000 keys 135 and 182, 24 of 2 behind 3,000 90 and 99, 32 of 2 behind 3,000
     # 115 and 100, of 8 behind 2,000 257 and 184; where the first has a tile of rows and keys for a block or so, it is the faster: 32 rows behind 500 keys 26 and 37, 160 behind 500
     # (640 tiles on 148 SMs) 55 and 39.
