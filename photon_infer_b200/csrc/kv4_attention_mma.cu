@@ -9,8 +9,9 @@
 //   score[key][row] = factor[row] sum over groups  scale[key][group] (sum over the group  c q  -  8 sum over the group  q),
 // the last sum known beforehand.  The weights, as 16-bit floats, are turned over in registers and multiplied by the values' scales,
 //   out[number][row] = sum over keys  (c - 8) (p scale)[key][group(number)][row],
-// where pairs of codes under the mask get the exponent of 1,024 with it and 1,024 and the eights are taken off by an addition, which is exact.  Weights are lifted by 2^15, and the scales of a group
-// whose largest so far is 2 or more, or below 2^-7, by the power of two that brings it to [1, 2).  All sums and the softmax are in 32 bits.
+// where pairs of codes under the mask get the exponent of 1,024 with it and 1,024 and the eights are taken off by an addition, which is exact.  Weights are lifted by 2^15, and scales of 2
+// or more, or below 2^-9, meet them by themselves, lifted by a power of two.  All sums and the softmax are in 32 bits; the first number of a pair is the difference of two sums and so off
+// by some 2^-20 of the second one's, where its own rounding to 4 bits was off by half a scale.
 //
 // All warps have equal runs of the requests' tiles of 32 keys, wherever units (a request, a head, 4 or 8 rows) begin and end, and nothing to do with one another: a tile's
 // bytes come through three stages of the warp's own in shared memory, two of them on their way.  Results of a unit that lies in one warp are written, the others' parts are joined by a
@@ -369,9 +370,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       }
     }
     uint32_t bad[NT] = {};                             // bit j: row 4 x + g / 2 sees a value of group j that is no number
-    uint32_t tops = 0x01010101u;                       // the exponents of each group's largest scale so far: 15 is that of 1
-    uint32_t room = 0;                                 // what makes a byte with a larger exponent set its first bit, where that matters
-    bool lifted = false;
+    int held = 0;                                      // the sums in acc are multiplied by 2^held
 
     uint32_t stage = ring;
     const uint32_t k_at = km_place<GROUPS>(g, GROUPS == 4 ? t : t >> 1) + (GROUPS == 4 ? 0 : (t & 1) * 8);
@@ -468,7 +467,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
 #pragma unroll
           for (int b = 0; b < 2; ++b) {
             const int o = 2 * u + (g & 1), key = key0 + 8 * o + 2 * t + b;
-            if (!(here >> o & 1u) || key > last_place || key < low) vs[u][b] = 0;      // whatever lies there
+            if (!(here >> o & 1u) || key > last_place || key < low) vs[u][b] = GROUPS == 4 ? 0x78787878u : 0x7878u;      // 1, whatever lies there: its weight is 0
           }
       }
       float alpha[NT], ref[NT];
@@ -486,39 +485,26 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         m[x] = top;
         ref[x] = top == -INFINITY ? 0.f : top - 15.f;
       }
-      // scales that call for another power of two, or no numbers
-      const uint32_t high = ((vs[0][0] + room) | vs[0][0] | (vs[0][1] + room) | vs[0][1] | (vs[1][0] + room) | vs[1][0] | (vs[1][1] + room) | vs[1][1]) &
-                            (GROUPS == 4 ? 0x80808080u : 0x8080u);
-      const bool rare = __any_sync(0xffffffffu, high != 0 || step == step0);
+      // scales that call for another power of two (a byte of 48 is 2^-9, one of 128 is 2), or no numbers
+      constexpr uint32_t FIRST = GROUPS == 4 ? 0x80808080u : 0x8080u, UP = GROUPS == 4 ? 0x50505050u : 0x5050u;
+      const uint32_t some = vs[0][0] | vs[0][1] | vs[1][0] | vs[1][1], all = (vs[0][0] + UP) & (vs[0][1] + UP) & (vs[1][0] + UP) & (vs[1][1] + UP);
+      const bool rare = __any_sync(0xffffffffu, ((some | ~all) & FIRST) != 0 || held != 0);
+      uint32_t bands = 2;
       bool odd_scales = false;
       if (rare) {
-        room = 0;
-        lifted = false;
+        uint32_t mine = 0;
 #pragma unroll
-        for (int j = 0; j < GROUPS; ++j) {
-          int most = 0;
+        for (int j = 0; j < GROUPS; ++j)
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const int byte = vs[w >> 1][w & 1] >> (8 * j) & 255;
-            if (byte < 248) most = max(most, byte); else odd_scales = true;
+            const uint32_t byte = vs[w >> 1][w & 1] >> (8 * j) & 255u;
+            mine |= byte == 0 ? 0u : byte < 48 ? 1u : byte < 128 ? 2u : byte < 192 ? 4u : byte < 248 ? 8u : 16u;
           }
-          most = __reduce_max_sync(0xffffffffu, most) >> 3;
-          const int was = tops >> (8 * j) & 255, to = max(was, most), old_lift = was > 15 || was < 8 ? 15 - was : 0, new_lift = to > 15 || to < 8 ? 15 - to : 0;
-          tops += (uint32_t)(to - was) << (8 * j);
-          if (new_lift != old_lift) {
-            const float f = km_power(new_lift - old_lift);
-#pragma unroll
-            for (int x = 0; x < NT; ++x) {
-#pragma unroll
-              for (int i = 0; i < 4; ++i) { acc[x][j][0][i] *= f; acc[x][j][1][i] *= f; }
-            }
-          }
-          lifted |= new_lift != 0;
-          if (to < 8) room |= (uint32_t)(0x7F - (8 * to + 7)) << (8 * j);
-        }
-        odd_scales = __any_sync(0xffffffffu, odd_scales);
+        bands = __reduce_or_sync(0xffffffffu, mine);
+        odd_scales = bands & 16u;
+        bands &= 15u;
+        if (bands == 0) bands = 2;
       }
-      const bool special = rare || lifted;
       if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
@@ -542,65 +528,87 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         p2[x][0] = km_half2(p[0], p[1]);
         p2[x][1] = km_half2(p[2], p[3]);
       }
-      // ---- the values.  Column g of the second operand has the weights of row 4 x + g / 2 for the 8 keys 2 u + (g & 1), and nothing for the 8 beside them
+      // ---- the values.  Column g of the second operand has the weights of row 4 x + g / 2 for the 8 keys 2 u + (g & 1), and nothing for the 8 beside them.
+      // Scales from 2^-9 to 2 meet the weights as they are; others, a band of 2^8 at a time, by the power of two that brings them there, and the sums with them: a weight times a scale
+      // keeps its bits whatever lies beside it.  As a rule there is one band.
+#pragma unroll 1
+      do {
+        uint32_t from = 0, size = 0, lift2 = 0;        // the band's scales as 16-bit floats, the power of two
+        if (rare) {
+          const int band = __ffs(bands) - 1, lift = 8 * (1 - band);
+          from = band == 0 ? 1u : band == 1 ? 48u << 7 : band == 2 ? 128u << 7 : 192u << 7;
+          size = (band == 0 ? 48u << 7 : band == 1 ? 128u << 7 : band == 2 ? 192u << 7 : 248u << 7) - from;
+          lift2 = km_half2(km_power(lift), km_power(lift));
+          if (lift != held) {
+            const float f = km_power(lift - held);
 #pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        uint32_t pe[NT], po[NT];
+            for (int x = 0; x < NT; ++x)
 #pragma unroll
-        for (int x = 0; x < NT; ++x) {
-          const uint32_t y = km_turn(p2[x][u]);
-          pe[x] = g & 1 ? 0u : y;
-          po[x] = g & 1 ? y : 0u;
-        }
-        uint32_t vw[2][2][VW];                         // values 8 (2 u + o) + 2 t, + 1
+              for (int j = 0; j < GROUPS; ++j)
 #pragma unroll
-        for (int o = 0; o < 2; ++o) {
-          km_read<VW>(vw[o][0], stage + v_at0 + (2 * u + o) * 8 * ROW);
-          km_read<VW>(vw[o][1], stage + v_at1 + (2 * u + o) * 8 * ROW);
-        }
-        // the scales of its keys 2 t and 2 t + 1; the bytes between are a scale's first bit, 0 below 2
-        uint32_t s2[GROUPS];
-#pragma unroll
-        for (int j = 0; j < GROUPS; ++j) s2[j] = km_bytes(vs[u][0], vs[u][1], j == 0 ? 0x4C08 : j == 1 ? 0x5D19 : j == 2 ? 0x6E2A : 0x7F3B) >> 1;
-        if (special) {
-#pragma unroll
-          for (int j = 0; j < GROUPS; ++j) {
-            s2[j] &= 0x7F807F80u;
-            if (odd_scales) {                          // no number goes into the products, where it would meet rows that do not see it: who does is noted
-#pragma unroll
-              for (int h = 0; h < 2; ++h)
-                if ((s2[j] >> (16 * h) & 0x7fffu) >= 0x7c00u) {
-                  s2[j] &= h ? 0x0000ffffu : 0xffff0000u;
-#pragma unroll
-                  for (int x = 0; x < NT; ++x) {
-                    const int r = 4 * x + (g >> 1), key = key0 + 16 * u + 8 * (g & 1) + 2 * t + h, at_place = base + (row0 + r) / G;
-                    if (r < rows && key <= at_place && (a.window <= 0 || key > at_place - a.window)) bad[x] |= 1u << j;
-                  }
-                }
-            }
-            const int e = tops >> (8 * j) & 255;
-            const float f = km_power(e > 15 || e < 8 ? 15 - e : 0);
-            s2[j] = km_mul2(s2[j], km_half2(f, f));
+                for (int i = 0; i < 4; ++i) { acc[x][j][0][i] *= f; acc[x][j][1][i] *= f; }
+            held = lift;
           }
         }
+        bands &= bands - 1;
 #pragma unroll
-        for (int j = 0; j < GROUPS; ++j) {
-          // of two keys each: numbers 0 and 1 of this lane's four, then 2 and 3, as 1024 + c0 + 16 c1 and 1024 + 16 c1; less what makes them c - 8
-          const uint32_t r0 = __byte_perm(vw[0][0][j / 2], vw[0][1][j / 2], j & 1 ? 0x7632 : 0x5410);
-          const uint32_t r1 = __byte_perm(vw[1][0][j / 2], vw[1][1][j / 2], j & 1 ? 0x7632 : 0x5410);
-          const uint32_t t0 = __byte_perm(r0, c_64, 0x4341), t1 = __byte_perm(r1, c_64, 0x4341);
-          const uint32_t e0 = km_add2((r0 & 0x00FF00FFu) | c_1024, c_both), h0 = km_add2((r0 & 0x00F000F0u) | c_1024, c_high);
-          const uint32_t e1 = km_add2((r1 & 0x00FF00FFu) | c_1024, c_both), h1 = km_add2((r1 & 0x00F000F0u) | c_1024, c_high);
-          const uint32_t e2 = km_add2(t0, c_both), h2 = km_add2((t0 & 0x00F000F0u) | c_1024, c_high);
-          const uint32_t e3 = km_add2(t1, c_both), h3 = km_add2((t1 & 0x00F000F0u) | c_1024, c_high);
+        for (int u = 0; u < 2; ++u) {
+          uint32_t pe[NT], po[NT];
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
-            const uint32_t b0 = km_mul2(pe[x], s2[j]), b1 = km_mul2(po[x], s2[j]);
-            km_mma(acc[x][j][0], e0, h0, e1, h1, b0, b1);
-            km_mma(acc[x][j][1], e2, h2, e3, h3, b0, b1);
+            const uint32_t y = km_turn(p2[x][u]);
+            pe[x] = g & 1 ? 0u : y;
+            po[x] = g & 1 ? y : 0u;
+          }
+          uint32_t vw[2][2][VW];                         // values 8 (2 u + o) + 2 t, + 1
+#pragma unroll
+          for (int o = 0; o < 2; ++o) {
+            km_read<VW>(vw[o][0], stage + v_at0 + (2 * u + o) * 8 * ROW);
+            km_read<VW>(vw[o][1], stage + v_at1 + (2 * u + o) * 8 * ROW);
+          }
+          // the scales of its keys 2 t and 2 t + 1; the bytes between are a scale's first bit, 0 below 2
+          uint32_t s2[GROUPS];
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) s2[j] = km_bytes(vs[u][0], vs[u][1], j == 0 ? 0x4C08 : j == 1 ? 0x5D19 : j == 2 ? 0x6E2A : 0x7F3B) >> 1;
+          if (rare) {
+#pragma unroll
+            for (int j = 0; j < GROUPS; ++j) {
+              s2[j] &= 0x7F807F80u;
+              if (odd_scales) {                          // no number goes into the products, where it would meet rows that do not see it: who does is noted
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                  if ((s2[j] >> (16 * h) & 0x7fffu) >= 0x7c00u) {
+                    s2[j] &= h ? 0x0000ffffu : 0xffff0000u;
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                      const int r = 4 * x + (g >> 1), key = key0 + 16 * u + 8 * (g & 1) + 2 * t + h, at_place = base + (row0 + r) / G;
+                      if (r < rows && key <= at_place && (a.window <= 0 || key > at_place - a.window)) bad[x] |= 1u << j;
+                    }
+                  }
+              }
+              s2[j] &= ((s2[j] & 0xffffu) - from < size ? 0x0000ffffu : 0u) | ((s2[j] >> 16) - from < size ? 0xffff0000u : 0u);
+              s2[j] = km_mul2(s2[j], lift2);
+            }
+          }
+#pragma unroll
+          for (int j = 0; j < GROUPS; ++j) {
+            // of two keys each: numbers 0 and 1 of this lane's four, then 2 and 3, as 1024 + c0 + 16 c1 and 1024 + 16 c1; less what makes them c - 8
+            const uint32_t r0 = __byte_perm(vw[0][0][j / 2], vw[0][1][j / 2], j & 1 ? 0x7632 : 0x5410);
+            const uint32_t r1 = __byte_perm(vw[1][0][j / 2], vw[1][1][j / 2], j & 1 ? 0x7632 : 0x5410);
+            const uint32_t t0 = __byte_perm(r0, c_64, 0x4341), t1 = __byte_perm(r1, c_64, 0x4341);
+            const uint32_t e0 = km_add2((r0 & 0x00FF00FFu) | c_1024, c_both), h0 = km_add2((r0 & 0x00F000F0u) | c_1024, c_high);
+            const uint32_t e1 = km_add2((r1 & 0x00FF00FFu) | c_1024, c_both), h1 = km_add2((r1 & 0x00F000F0u) | c_1024, c_high);
+            const uint32_t e2 = km_add2(t0, c_both), h2 = km_add2((t0 & 0x00F000F0u) | c_1024, c_high);
+            const uint32_t e3 = km_add2(t1, c_both), h3 = km_add2((t1 & 0x00F000F0u) | c_1024, c_high);
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+              const uint32_t b0 = km_mul2(pe[x], s2[j]), b1 = km_mul2(po[x], s2[j]);
+              km_mma(acc[x][j][0], e0, h0, e1, h1, b0, b1);
+              km_mma(acc[x][j][1], e2, h2, e3, h3, b0, b1);
+            }
           }
         }
-      }
+      } while (bands != 0);
       stage = stage == ring + (KM_STAGES - 1) * STAGE ? ring : stage + STAGE;
     }
     // ---- the results: the unit's, or a part of them
@@ -639,8 +647,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       }
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
-        const int e = tops >> (8 * j) & 255;
-        const float f = (bad[x] >> j & 1u ? NAN : km_power(e > 15 || e < 8 ? e - 15 : 0)) * mul;
+        const float f = (bad[x] >> j & 1u ? NAN : km_power(-held)) * mul;
         float y[4];
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
