@@ -150,7 +150,7 @@ kv4_attention_kernel(const Kv4Args a) {
         if (a.sinks != nullptr) {
           const float sink = a.sinks[h] * 1.4426950408889634f, top = fmaxf(m, sink);
           mul = m == -INFINITY ? 1.f : exp2f(m - top);
-          total = total * mul + exp2f(sink - top);
+          if (sink != -INFINITY) total = total * mul + exp2f(sink - top);
           m = top;
         }
         if (tid == 0 && a.lse != nullptr) a.lse[of] = total == 0.f ? -INFINITY : (m + log2f(total)) * 0.6931471805599453f;

@@ -636,7 +636,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
           const float sink = a.sinks[h] * 1.4426950408889634f;
           top = fmaxf(top, sink);
           mul = m[x] == -INFINITY ? 1.f : exp2f(m[x] - top);
-          total_l = total_l * mul + exp2f(sink - top + 15.f);
+          if (sink != -INFINITY) total_l = total_l * mul + exp2f(sink - top + 15.f);
         }
         if (g == 0 && there && a.lse != nullptr) a.lse[token * a.n_q + h] = total_l == 0.f ? -INFINITY : (top - 15.f + log2f(total_l)) * 0.6931471805599453f;
         mul = total_l == 0.f ? 0.f : mul / total_l;
@@ -724,7 +724,7 @@ kv4_mma_join_kernel(const Kv4MmaArgs a, int N) {
   if (a.sinks != nullptr) {
     const float sink = a.sinks[h] * 1.4426950408889634f, top = fmaxf(m, sink);
     mul = m == -INFINITY ? 1.f : exp2f(m - top);
-    l = l * mul + exp2f(sink - top + 15.f);
+    if (sink != -INFINITY) l = l * mul + exp2f(sink - top + 15.f);
     m = top;
   }
   const long token = R.first + row / G;

@@ -232,7 +232,7 @@ kv4_attention_rows_kernel(const Kv4Args a) {
       if (a.sinks != nullptr) {
         const float sink = a.sinks[h] * 1.4426950408889634f, both = fmaxf(top, sink);
         mul = top == -INFINITY ? 1.f : exp2f(top - both);
-        total = total * mul + exp2f(sink - both);
+        if (sink != -INFINITY) total = total * mul + exp2f(sink - both);
         top = both;
       }
       if (kt == 0 && a.lse != nullptr) a.lse[of] = total == 0.f ? -INFINITY : (top + log2f(total)) * 0.6931471805599453f;
