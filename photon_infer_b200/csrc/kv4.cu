@@ -11,6 +11,7 @@
 #include "kv4.cuh"
 
 #define KV4_THREADS 256
+#define KV4_SPOIL_TOKENS 64      // of a block: two of a lane
 
 // The scale of a group whose largest magnitude is `top`, finite.
 template <typename T>
@@ -257,30 +258,52 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict
   }
 }
 
-// The rows of the requests with more than min_rows rows that see a value which is not finite: its group's numbers are none either.  One block for each (request, head), which has
-// nothing to do but read the flags as a rule.
-__global__ void __launch_bounds__(1024)
+// The rows of the requests with more than min_rows rows that see a value which is not finite: its group's numbers are none either.  A block has 64 tokens of a (request, head), and nothing to
+// do but read its keys' flags as a rule.  Else it finds, for every group and token, the last such key at or before the token's place, which decides for any window, and writes each number once.
+__global__ void __launch_bounds__(KV4_THREADS)
 kv4_spoil_kernel(const uint8_t* __restrict__ v_cache, const int* __restrict__ table, int per, long stride, int n_kv, int groups, int page_size, int num_pages,
                  const int* __restrict__ cu_tokens, const int* __restrict__ context_lens, int group, int min_rows, int parts, const int* __restrict__ flags, bf16* __restrict__ out,
                  long out_stride, int window) {
+  __shared__ int last_s[8][KV4_SPOIL_TOKENS];
   pdl_wait();
-  const int head = blockIdx.x, s = blockIdx.y, first = cu_tokens[s], n = cu_tokens[s + 1] - first, len = context_lens[s], base = len - n;
+  const int head = blockIdx.x, s = blockIdx.y, first = cu_tokens[s], n = cu_tokens[s + 1] - first, len = context_lens[s], base = len - n, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if ((long)n * group <= min_rows) return;
-  const int pages = min(per, (len + page_size - 1) / page_size);
-  int any = 0;
-  for (int i = threadIdx.x; i < pages * parts; i += 1024) any |= flags[(long)s * per * parts + i];
-  if (!__syncthreads_or(any)) return;
-  for (int key = threadIdx.x; key < min(len, pages * page_size); key += 1024) {
-    const int page = table[s * stride + key / page_size];
-    if (page < 0 || page >= num_pages) continue;
-    const uint8_t* scales = v_cache + ((long)page * n_kv + head) * kv4_page_bytes(page_size, groups * 32) + (long)page_size * groups * 16 + key % page_size * groups;
-    for (int j = 0; j < groups; ++j) {
-      if (scales[j] < 248) continue;
-      const int last = window > 0 && window < n + base - key ? key + window - 1 - base : n - 1;
-      for (int i = max(0, key - base); i <= last; ++i)
-        for (int x = 0; x < group * 32; ++x)
-          out[(first + i) * out_stride + (head * group + x / 32) * groups * 32 + 32 * j + x % 32] = __float2bfloat16_rn(__int_as_float(0x7fc00000));
+  const int pages = min(per, (max(len, 0) + page_size - 1) / page_size);
+  for (int t0 = blockIdx.z * KV4_SPOIL_TOKENS; t0 < n; t0 += gridDim.z * KV4_SPOIL_TOKENS) {
+    const int tokens = min(KV4_SPOIL_TOKENS, n - t0), place0 = base + t0, place1 = place0 + tokens - 1;
+    if (place1 < 0) continue;
+    const int low = window > 0 ? max(0, place0 - window + 1) : 0, page0 = low / page_size, page1 = min(pages, place1 / page_size + 1);
+    int any = 0;
+    for (long i = ((long)s * per + page0) * parts + tid; i < ((long)s * per + page1) * parts; i += KV4_THREADS) any |= flags[i];
+    if (!__syncthreads_or(any)) continue;
+    for (int i = tid; i < groups * KV4_SPOIL_TOKENS; i += KV4_THREADS) last_s[i / KV4_SPOIL_TOKENS][i % KV4_SPOIL_TOKENS] = -1;
+    __syncthreads();
+    for (int key = low + tid; key <= place1 && key / page_size < page1; key += KV4_THREADS) {
+      const int page = table[s * stride + key / page_size];
+      if (page < 0 || page >= num_pages) continue;
+      const uint8_t* scales = v_cache + ((long)page * n_kv + head) * kv4_page_bytes(page_size, groups * 32) + (long)page_size * groups * 16 + key % page_size * groups;
+      for (int j = 0; j < groups; ++j) if (scales[j] >= 248) atomicMax(&last_s[j][max(0, key - place0)], key);
     }
+    __syncthreads();
+    if (warp < groups) {                               // the largest up to every token: a lane has two
+      const int a = last_s[warp][2 * lane], b = max(a, last_s[warp][2 * lane + 1]);
+      int upto = b;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int x = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto = max(upto, x);
+      }
+      const int before = __shfl_up_sync(0xffffffffu, upto, 1);
+      last_s[warp][2 * lane] = lane > 0 ? max(a, before) : a;
+      last_s[warp][2 * lane + 1] = upto;
+    }
+    __syncthreads();
+    for (int i = tid; i < tokens * group * groups * 4; i += KV4_THREADS) {      // 8 numbers of a (token, query head, group)
+      const int at = i >> 2, j = at % groups, row = at / groups, t = row / group, last = last_s[j][t];
+      if (last < 0 || (window > 0 && last <= place0 + t - window)) continue;
+      *(uint4*)(out + (first + t0 + t) * out_stride + ((long)(head * group + row - t * group) * groups + j) * 32 + 8 * (i & 3)) = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+    }
+    __syncthreads();                                   // what was found is done with
   }
 }
 
@@ -342,10 +365,11 @@ PHOTON_API int photon_kv4_unpack(const photon_kv4_unpack_call* c, cudaStream_t s
 #undef UNPACK
 }
 
-PHOTON_API int photon_kv4_spoil(const photon_kv4_unpack_call* c, void* out, long out_stride, int window, cudaStream_t stream) {
-  if (c->S <= 0 || c->per <= 0) return 0;
-  if (c->dtype != PHOTON_BF16 || c->flags == nullptr || c->cu_tokens == nullptr || !kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_ARGUMENT;
-  if (c->S > 65535) return PHOTON_ERR_UNSUPPORTED;
-  return launch_pdl(kv4_spoil_kernel, dim3(c->n_kv, c->S), dim3(1024), 0, stream, (const uint8_t*)c->v_cache, c->table, c->per, c->stride, c->n_kv, c->d / 32, c->page_size,
-                    c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, kv4_unpack_parts(c), (const int*)c->flags, (bf16*)out, out_stride, window);
+PHOTON_API int photon_kv4_spoil(const photon_kv4_unpack_call* c, void* out, long out_stride, int max_tokens, int window, cudaStream_t stream) {
+  if (c->S <= 0 || c->per <= 0 || max_tokens <= 0) return 0;
+  if (c->dtype != PHOTON_BF16 || c->flags == nullptr || c->cu_tokens == nullptr || c->n_kv <= 0 || c->group <= 0 || !kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_ARGUMENT;
+  if (c->S > 65535 || (uintptr_t)out % 16 || out_stride % 8) return PHOTON_ERR_UNSUPPORTED;
+  const int chunks = (max_tokens + KV4_SPOIL_TOKENS - 1) / KV4_SPOIL_TOKENS;
+  return launch_pdl(kv4_spoil_kernel, dim3(c->n_kv, c->S, chunks < 65535 ? chunks : 65535), dim3(KV4_THREADS), 0, stream, (const uint8_t*)c->v_cache, c->table, c->per, c->stride, c->n_kv,
+                    c->d / 32, c->page_size, c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, kv4_unpack_parts(c), (const int*)c->flags, (bf16*)out, out_stride, window);
 }
