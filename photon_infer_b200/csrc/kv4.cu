@@ -258,13 +258,15 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict
   }
 }
 
-// The rows of the requests with more than min_rows rows that see a value which is not finite: its group's numbers are none either.  A block has 64 tokens of a (request, head), and nothing to
-// do but read its keys' flags as a rule.  Else it finds, for every group and token, the last such key at or before the token's place, which decides for any window, and writes each number once.
+// The rows of the requests with more than min_rows rows that see a value which is not finite: its group's numbers are none either.  Rows whose query is not finite, too, where scores of minus
+// infinity look like keys that are not seen: all their numbers, if they see a key.  A block has 64 tokens of a (request, head), and nothing to do but read its keys' flags and its queries as a rule.  Else it finds,
+// for every group and token, the last such key at or before the token's place, which decides for any window, and writes each number once.
 __global__ void __launch_bounds__(KV4_THREADS)
 kv4_spoil_kernel(const uint8_t* __restrict__ v_cache, const int* __restrict__ table, int per, long stride, int n_kv, int groups, int page_size, int num_pages,
                  const int* __restrict__ cu_tokens, const int* __restrict__ context_lens, int group, int min_rows, int parts, const int* __restrict__ flags, bf16* __restrict__ out,
-                 long out_stride, int window) {
+                 long out_stride, const bf16* __restrict__ q, long q_stride, int window) {
   __shared__ int last_s[8][KV4_SPOIL_TOKENS];
+  __shared__ uint32_t odd_s[KV4_SPOIL_TOKENS * 128 / 32];      // rows (tokens x query heads, at most 128) whose query is not finite
   pdl_wait();
   const int head = blockIdx.x, s = blockIdx.y, first = cu_tokens[s], n = cu_tokens[s + 1] - first, len = context_lens[s], base = len - n, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   if ((long)n * group <= min_rows) return;
@@ -273,8 +275,24 @@ kv4_spoil_kernel(const uint8_t* __restrict__ v_cache, const int* __restrict__ ta
     const int tokens = min(KV4_SPOIL_TOKENS, n - t0), place0 = base + t0, place1 = place0 + tokens - 1;
     if (place1 < 0) continue;
     const int low = window > 0 ? max(0, place0 - window + 1) : 0, page0 = low / page_size, page1 = min(pages, place1 / page_size + 1);
+    for (int i = tid; i < (tokens * group + 31) / 32; i += KV4_THREADS) odd_s[i] = 0;
+    __syncthreads();
     int any = 0;
     for (long i = ((long)s * per + page0) * parts + tid; i < ((long)s * per + page1) * parts; i += KV4_THREADS) any |= flags[i];
+    const int pieces = group * groups * 4;             // 16 bytes of a token's query heads
+#pragma unroll 4
+    for (int i = tid; i < tokens * pieces; i += KV4_THREADS) {
+      const int t = i / pieces, piece = i - t * pieces;
+      const uint4 u = *(const uint4*)(q + (first + t0 + t) * q_stride + (long)head * group * groups * 32 + 8 * piece);
+      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+      bool odd = false;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) odd |= (w[c] & 0x7f80u) == 0x7f80u || (w[c] & 0x7f800000u) == 0x7f800000u;
+      if (!odd) continue;
+      const int row = t * group + piece / (groups * 4);
+      atomicOr(&odd_s[row >> 5], 1u << (row & 31));
+      any = 1;
+    }
     if (!__syncthreads_or(any)) continue;
     for (int i = tid; i < groups * KV4_SPOIL_TOKENS; i += KV4_THREADS) last_s[i / KV4_SPOIL_TOKENS][i % KV4_SPOIL_TOKENS] = -1;
     __syncthreads();
@@ -299,9 +317,19 @@ kv4_spoil_kernel(const uint8_t* __restrict__ v_cache, const int* __restrict__ ta
     }
     __syncthreads();
     for (int i = tid; i < tokens * group * groups * 4; i += KV4_THREADS) {      // 8 numbers of a (token, query head, group)
-      const int at = i >> 2, j = at % groups, row = at / groups, t = row / group, last = last_s[j][t];
-      if (last < 0 || (window > 0 && last <= place0 + t - window)) continue;
-      *(uint4*)(out + (first + t0 + t) * out_stride + ((long)(head * group + row - t * group) * groups + j) * 32 + 8 * (i & 3)) = make_uint4(0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u);
+      const int at = i >> 2, j = at % groups, row = at / groups, t = row / group, last = last_s[j][t], place = place0 + t;
+      uint32_t is = 0x7fc07fc0u;
+      if (odd_s[row >> 5] >> (row & 31) & 1u) {
+        bool sees = false;                             // a key that is there
+        for (int p = place < 0 ? -1 : min(place / page_size, pages - 1); !sees && p >= (window > 0 ? max(0, place - window + 1) : 0) / page_size; --p) {
+          const int page = table[s * stride + p];
+          sees = page >= 0 && page < num_pages;
+        }
+        if (!sees) is = 0u;
+      } else if (last < 0 || (window > 0 && last <= place - window)) {
+        continue;
+      }
+      *(uint4*)(out + (first + t0 + t) * out_stride + ((long)(head * group + row - t * group) * groups + j) * 32 + 8 * (i & 3)) = make_uint4(is, is, is, is);
     }
     __syncthreads();                                   // what was found is done with
   }
@@ -365,11 +393,12 @@ PHOTON_API int photon_kv4_unpack(const photon_kv4_unpack_call* c, cudaStream_t s
 #undef UNPACK
 }
 
-PHOTON_API int photon_kv4_spoil(const photon_kv4_unpack_call* c, void* out, long out_stride, int max_tokens, int window, cudaStream_t stream) {
+PHOTON_API int photon_kv4_spoil(const photon_kv4_unpack_call* c, void* out, long out_stride, const void* q, long q_stride, int max_tokens, int window, cudaStream_t stream) {
   if (c->S <= 0 || c->per <= 0 || max_tokens <= 0) return 0;
   if (c->dtype != PHOTON_BF16 || c->flags == nullptr || c->cu_tokens == nullptr || c->n_kv <= 0 || c->group <= 0 || !kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_ARGUMENT;
-  if (c->S > 65535 || (uintptr_t)out % 16 || out_stride % 8) return PHOTON_ERR_UNSUPPORTED;
+  if (c->S > 65535 || c->group > 128 || ((uintptr_t)out | (uintptr_t)q) % 16 || out_stride % 8 || q_stride % 8) return PHOTON_ERR_UNSUPPORTED;
   const int chunks = (max_tokens + KV4_SPOIL_TOKENS - 1) / KV4_SPOIL_TOKENS;
   return launch_pdl(kv4_spoil_kernel, dim3(c->n_kv, c->S, chunks < 65535 ? chunks : 65535), dim3(KV4_THREADS), 0, stream, (const uint8_t*)c->v_cache, c->table, c->per, c->stride, c->n_kv,
-                    c->d / 32, c->page_size, c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, kv4_unpack_parts(c), (const int*)c->flags, (bf16*)out, out_stride, window);
+                    c->d / 32, c->page_size, c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, kv4_unpack_parts(c), (const int*)c->flags, (bf16*)out, out_stride,
+                    (const bf16*)q, q_stride, window);
 }

@@ -37,7 +37,7 @@ kv4_attention_kernel(const Kv4Args a) {
   for (int i = tid; i < ROWS * d; i += KA_THREADS) {                 // the query rows, in the order of a key's row
     const int r = i / d, p = i - r * d, w = p / 8, t = w / a.groups, j = w - t * a.groups;
     const int row = row0 + r, token = first + row / G, h = head * G + row % G;
-    qs[r * 256 + p] = r < rows ? to_f32(((const T*)a.q)[token * a.q_stride + h * d + 32 * j + 8 * t + p % 8]) : 0.f;
+    qs[r * 256 + p] = r < rows ? kv4_query(((const T*)a.q)[token * a.q_stride + h * d + 32 * j + 8 * t + p % 8]) : 0.f;
   }
   if (tid < ROWS) m_s[tid] = -INFINITY;
   const int subsets = KA_THREADS / words, sub = tid / words, w = tid - sub * words;      // the second half's share: word w, keys sub, sub + subsets ..

@@ -323,7 +323,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       const bool odd = top >= 0x7f800000u;
       const int e = top == 0 || odd ? 0 : max((int)(top >> 23), 1) - 127;
       const float up1 = km_power((14 - e) / 2), up2 = km_power(14 - e - (14 - e) / 2);      // the largest number to [2^14, 2^15)
-      const float f = odd ? NAN : fmaxf(km_scaled(a.scale * (CAP ? 1.f : 1.4426950408889634f), e - 14 + 24), 1e-37f);
+      const float f = fmaxf(km_scaled(a.scale * (CAP ? 1.f : 1.4426950408889634f), e - 14 + 24), 1e-37f);
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
         float sum = 0.f, y[8];
@@ -343,7 +343,8 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         }
         sum += __shfl_xor_sync(0xffffffffu, sum, 1);
         sum += __shfl_xor_sync(0xffffffffu, sum, 2);
-        init[x][j] = __shfl_sync(0xffffffffu, sum, 8 * t) * (-8.f / 16777216.f);
+        // a query that is not finite: no score is a number, but for those that a mask takes out behind this
+        init[x][j] = __shfl_sync(0xffffffffu, odd ? NAN : sum, 8 * t) * (-8.f / 16777216.f);
       }
       factor[x] = __shfl_sync(0xffffffffu, f, 8 * t);
       place[x] = 4 * x + t < rows ? base + (row0 + 4 * x + t) / G : -1;

@@ -89,7 +89,7 @@ kv4_attention_rows_kernel(const Kv4Args a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int r = 8 * warp + i, row = row0 + min(r, rows - 1), token = row / G;
-          x[i] = r < rows ? to_f32(((const T*)a.q)[(first + token) * a.q_stride + (long)(head * G + row - token * G) * d + KR_PIECE * c + lane]) : 0.f;
+          x[i] = r < rows ? kv4_query(((const T*)a.q)[(first + token) * a.q_stride + (long)(head * G + row - token * G) * d + KR_PIECE * c + lane]) : 0.f;
         }
       };
 #pragma unroll
