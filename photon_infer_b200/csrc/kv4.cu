@@ -258,13 +258,14 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict
   }
 }
 
-// The rows of the requests with more than min_rows rows that see a value which is not finite: its group's numbers are none either.  Rows whose query is not finite, too, where scores of minus
-// infinity look like keys that are not seen: all their numbers, if they see a key.  A block has 64 tokens of a (request, head), and nothing to do but read its keys' flags and its queries as a rule.  Else it finds,
-// for every group and token, the last such key at or before the token's place, which decides for any window, and writes each number once.
+// The rows of the requests with more than min_rows rows that see a value which is not finite: its group's numbers are none either.  Rows whose query is not finite, too, if they see a key, and
+// else none: where all their scores are minus infinity they are zero now, else NaN, which is what is looked for; where scores are bounded they can be any number, so that all queries are looked at.
+// A block has 64 tokens of a (request, head), and nothing to do but read its keys' flags and the rows' first numbers as a rule: 5 of the 187 us of 2,048 tokens behind 6,144 keys.  Else it finds, for every group and
+// token, the last broken key at or before the token's place, which decides for any window, and writes each number once.
 __global__ void __launch_bounds__(KV4_THREADS)
 kv4_spoil_kernel(const uint8_t* __restrict__ v_cache, const int* __restrict__ table, int per, long stride, int n_kv, int groups, int page_size, int num_pages,
-                 const int* __restrict__ cu_tokens, const int* __restrict__ context_lens, int group, int min_rows, int parts, const int* __restrict__ flags, bf16* __restrict__ out,
-                 long out_stride, const bf16* __restrict__ q, long q_stride, int window) {
+                 const int* __restrict__ cu_tokens, const int* __restrict__ context_lens, int group, int min_rows, int parts, const int* __restrict__ flags, bf16* out,
+                 long out_stride, const bf16* __restrict__ q, long q_stride, int window, bool bounded) {
   __shared__ int last_s[8][KV4_SPOIL_TOKENS];
   __shared__ uint32_t odd_s[KV4_SPOIL_TOKENS * 128 / 32];      // rows (tokens x query heads, at most 128) whose query is not finite
   pdl_wait();
@@ -278,21 +279,24 @@ kv4_spoil_kernel(const uint8_t* __restrict__ v_cache, const int* __restrict__ ta
     for (int i = tid; i < (tokens * group + 31) / 32; i += KV4_THREADS) odd_s[i] = 0;
     __syncthreads();
     int any = 0;
-    for (long i = ((long)s * per + page0) * parts + tid; i < ((long)s * per + page1) * parts; i += KV4_THREADS) any |= flags[i];
-    const int pieces = group * groups * 4;             // 16 bytes of a token's query heads
+    for (int row = tid; row < tokens * group; row += KV4_THREADS) {
+      const int t = row / group, h = head * group + row - t * group;
+      if (!bounded) {
+        const uint4 u = *(const uint4*)(out + (first + t0 + t) * out_stride + (long)h * groups * 32);
+        if (((u.x | u.y | u.z | u.w) & 0x7fff7fffu) != 0 && (u.x & 0x7fffu) <= 0x7f80u) continue;
+      }
+      const uint4* query = (const uint4*)(q + (first + t0 + t) * q_stride + (long)h * groups * 32);
+      uint32_t carry = 0;                              // the exponent's bits all set: one more of them carries into the bit in front of them, which the mask has cleared
 #pragma unroll 4
-    for (int i = tid; i < tokens * pieces; i += KV4_THREADS) {
-      const int t = i / pieces, piece = i - t * pieces;
-      const uint4 u = *(const uint4*)(q + (first + t0 + t) * q_stride + (long)head * group * groups * 32 + 8 * piece);
-      const uint32_t w[4] = {u.x, u.y, u.z, u.w};
-      bool odd = false;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) odd |= (w[c] & 0x7f80u) == 0x7f80u || (w[c] & 0x7f800000u) == 0x7f800000u;
-      if (!odd) continue;
-      const int row = t * group + piece / (groups * 4);
+      for (int i = 0; i < groups * 4; ++i) {
+        const uint4 u = query[i];
+        carry |= ((u.x & 0x7f807f80u) + 0x00800080u) | ((u.y & 0x7f807f80u) + 0x00800080u) | ((u.z & 0x7f807f80u) + 0x00800080u) | ((u.w & 0x7f807f80u) + 0x00800080u);
+      }
+      if ((carry & 0x80008000u) == 0) continue;
       atomicOr(&odd_s[row >> 5], 1u << (row & 31));
       any = 1;
     }
+    for (long i = ((long)s * per + page0) * parts + tid; i < ((long)s * per + page1) * parts; i += KV4_THREADS) any |= flags[i];
     if (!__syncthreads_or(any)) continue;
     for (int i = tid; i < groups * KV4_SPOIL_TOKENS; i += KV4_THREADS) last_s[i / KV4_SPOIL_TOKENS][i % KV4_SPOIL_TOKENS] = -1;
     __syncthreads();
@@ -393,12 +397,12 @@ PHOTON_API int photon_kv4_unpack(const photon_kv4_unpack_call* c, cudaStream_t s
 #undef UNPACK
 }
 
-PHOTON_API int photon_kv4_spoil(const photon_kv4_unpack_call* c, void* out, long out_stride, const void* q, long q_stride, int max_tokens, int window, cudaStream_t stream) {
+PHOTON_API int photon_kv4_spoil(const photon_kv4_unpack_call* c, void* out, long out_stride, const void* q, long q_stride, int max_tokens, int window, int bounded, cudaStream_t stream) {
   if (c->S <= 0 || c->per <= 0 || max_tokens <= 0) return 0;
   if (c->dtype != PHOTON_BF16 || c->flags == nullptr || c->cu_tokens == nullptr || c->n_kv <= 0 || c->group <= 0 || !kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_ARGUMENT;
   if (c->S > 65535 || c->group > 128 || ((uintptr_t)out | (uintptr_t)q) % 16 || out_stride % 8 || q_stride % 8) return PHOTON_ERR_UNSUPPORTED;
   const int chunks = (max_tokens + KV4_SPOIL_TOKENS - 1) / KV4_SPOIL_TOKENS;
   return launch_pdl(kv4_spoil_kernel, dim3(c->n_kv, c->S, chunks < 65535 ? chunks : 65535), dim3(KV4_THREADS), 0, stream, (const uint8_t*)c->v_cache, c->table, c->per, c->stride, c->n_kv,
                     c->d / 32, c->page_size, c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, kv4_unpack_parts(c), (const int*)c->flags, (bf16*)out, out_stride,
-                    (const bf16*)q, q_stride, window);
+                    (const bf16*)q, q_stride, window, bounded != 0);
 }

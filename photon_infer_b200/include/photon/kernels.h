@@ -646,9 +646,10 @@ typedef struct {
 } photon_kv4_unpack_call;
 PHOTON_EXPORT int photon_kv4_unpack(const photon_kv4_unpack_call* call, cudaStream_t stream);
 /* Behind an attention over what that call laid out: rows of out (bfloat16 [T, n_kv * group * d], 16-byte aligned rows) that see a marked value become NaN in its group's numbers, and
- * rows whose query (q, as out) is not finite and that see a key in all.  At most 128 query heads per key/value head; requests of at most max_tokens tokens in the step, or of more, which
+ * rows whose query (q, as out) is not finite and that see a key in all (bounded: the scores were).  At most 128 query heads per key/value head; requests of at most max_tokens tokens in the step, or of more, which
  * take turns. */
-PHOTON_EXPORT int photon_kv4_spoil(const photon_kv4_unpack_call* call, void* out, long out_stride, const void* q, long q_stride, int max_tokens, int window, cudaStream_t stream);
+PHOTON_EXPORT int photon_kv4_spoil(const photon_kv4_unpack_call* call, void* out, long out_stride, const void* q, long q_stride, int max_tokens, int window, int bounded,
+                                   cudaStream_t stream);
 
 /* ------------------------------------------------------------------ kv4_attention.cu */
 /* The tokens cu_tokens[s] .. cu_tokens[s + 1] - 1 of the step are the last of request s's context_lens[s] keys; the one at place p sees keys p - window + 1 .. p (window 0:

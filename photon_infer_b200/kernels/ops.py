@@ -3002,7 +3002,7 @@ def _kv4_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: in
     return "kv4_attention_rows" if many else "kv4_attention", parts, all_rows * parts * (head_dim + 2) if parts > 1 else 0
 
 
-_KV4_SPOIL_ARGS = [c_char_p, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_void_p]
+_KV4_SPOIL_ARGS = [c_char_p, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_int, c_void_p]
 
 
 def _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, num_seqs, max_tokens, max_keys, n_q, n_kv, head_dim, page_size, window, scale, err,
@@ -3031,7 +3031,7 @@ def _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, 
                                      table_at, positions_at, flags_at, _data(err), pages, _dtype_code(q), n, per, n_kv, head_dim, page_size, pool, group, KV4_FEW_ROWS)
         _check(unpack(call, _stream()), "kv4_attention")
         attention_tc(q, into, k_numbers, v_numbers, table, cu, positions, n, max_tokens, n_q, n_kv, head_dim, window, scale, err, sink=sink, softcap=softcap, keys=max_keys)
-        _check(spoil(call, into.data_ptr(), into.stride(0), q.data_ptr(), q.stride(0), max_tokens, window, _stream()), "kv4_attention")
+        _check(spoil(call, into.data_ptr(), into.stride(0), q.data_ptr(), q.stride(0), max_tokens, window, int(bool(softcap)), _stream()), "kv4_attention")
     if into is not out:
         out.copy_(into)
 
