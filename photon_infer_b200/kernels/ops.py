@@ -2914,6 +2914,14 @@ def _check_lse(what: str, lse: Optional[torch.Tensor], T: int, n_q: int) -> None
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, f"{what}: lse must be contiguous float32 [T, n_q]")
 
 
+def _rows_on_16_bytes(x: torch.Tensor) -> torch.Tensor:
+    """``x [T, width]`` (``width`` a multiple of 8, 16 bits a number) if every row begins on a 16-byte boundary, else a copy.  Not ``contiguous()``, for which the stride of a single row and
+    where a tensor begins are all the same."""
+    if x.stride(0) >= x.shape[1] and x.stride(0) % 8 == 0 and x.data_ptr() % 16 == 0:
+        return x
+    return torch.empty(x.shape, dtype=x.dtype, device=x.device).copy_(x)
+
+
 #: Rows (tokens x query heads per key/value head) up to which ``attention_tc`` leaves a request to other kernels.
 KV4_FEW_ROWS = 16
 #: Bytes of a prompt portion's keys and values in bfloat16 that are laid out at a time.
@@ -3011,11 +3019,8 @@ def _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, 
     products are many times the bytes: 2,048 tokens of 32/8 heads of 128 behind 4,096 keys are 86 GFLOP and 25 MB laid out."""
     per = min(-(-max_keys // page_size), block_table.shape[1])
     device, (T, width) = q.device, q.shape
-    if q.stride(0) < width or q.stride(0) % 8 or q.data_ptr() % 16:
-        q = q.contiguous()
-    into = out if out.is_contiguous() and out.data_ptr() % 16 == 0 else out.contiguous()
-    if into.data_ptr() % 16:
-        into = into.clone(memory_format=torch.contiguous_format)
+    q = _rows_on_16_bytes(q)
+    into = out if out.stride(0) == width and out.data_ptr() % 16 == 0 else torch.empty((T, width), dtype=out.dtype, device=device).copy_(out)
     one = per * n_kv * page_size * head_dim * 4
     some = max(1, min(num_seqs, KV4_PROMPT_BYTES // one, 65535 // -(-max_tokens // (128 // (n_q // n_kv)))))
     k_numbers, v_numbers = torch.empty((2, some * per, n_kv, page_size, head_dim), dtype=q.dtype, device=device).unbind()
