@@ -3079,7 +3079,7 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
     if T == 0 or num_seqs == 0 or max_tokens_per_seq <= 0 or max_keys <= 0:
         return
     if q.dtype == torch.bfloat16 and head_dim in (64, 128) and (q.stride(0) % 8 or q.data_ptr() % 16):
-        q = q.contiguous() if q.stride(0) != q.shape[1] else q.clone()      # rows on 16-byte boundaries: a copy of the queries is little beside the keys
+        q = _rows_on_16_bytes(q)                        # a copy of the queries is little beside the keys
     name, parts, floats, keep = _key_weights_route(q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, packed, lse is not None, num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv),
                                                    max_keys, T * n_q, _sms(index, q.device))
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if lse is None else None
