@@ -10,6 +10,7 @@
 // rows that may move.  With little to move two chains of latencies: one request, 1,152 to 1,024, 16 layers, 8 heads of 64 in 4 bits, 17.5 us.  Sums that stay in shared memory and places
 // found once for a batch of rows: 684 to 445 us.
 #include "common.cuh"
+#include "limits.cuh"
 
 #define EV_THREADS 512
 #define EV_MOVERS 256
@@ -229,12 +230,9 @@ PHOTON_API int photon_cache_evict(const photon_evict_call* c, cudaStream_t strea
   const int kinds = c->planes * (c->scale_bytes > 0 ? 2 : 1) + 1;
   const long blocks = units * kinds * slices;
   if (blocks > 0x7fffffffL) return PHOTON_ERR_UNSUPPORTED;
-  static bool set = false;
-  if (!set) {
-    const cudaError_t e = cudaFuncSetAttribute(evict_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, EV_SHARED);
-    if (e != cudaSuccess) return (int)e;
-    set = true;
-  }
+  static bool ready[64] = {};
+  const int limit = smem_limit((const void*)evict_select_kernel, EV_SHARED, false, ready);
+  if (limit != 0) return limit;
   const int status = launch_pdl(evict_select_kernel, dim3((unsigned)units), dim3(EV_THREADS), (size_t)room * 4, stream, a);
   if (status != 0 || c->keep == 0) return status;
   return launch_pdl(evict_move_kernel, dim3((unsigned)blocks), dim3(EV_MOVERS), 0, stream, a, slices, slice_pieces, kinds);

@@ -333,13 +333,9 @@ template <int D, bool PACKED, bool FINAL>
 static int kx_launch(const KeyWeightsMmaArgs& a, dim3 grid, cudaStream_t stream) {
   constexpr size_t most = (2 * KX_KEYS + KX_ROWS) * (2 * D + 16);
   const size_t smem = (2 * KX_KEYS + a.room) * (2 * D + 16);
-  static bool set = false;
-  if (!set) {
-    cudaError_t e = cudaFuncSetAttribute(key_weights_mma_kernel<D, PACKED, FINAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)most);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(key_weights_mma_kernel<D, PACKED, FINAL>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-    if (e != cudaSuccess) return (int)e;
-    set = true;
-  }
+  static bool ready[64] = {};
+  const int limit = smem_limit((const void*)key_weights_mma_kernel<D, PACKED, FINAL>, (int)most, true, ready);
+  if (limit != 0) return limit;
   return launch_pdl(key_weights_mma_kernel<D, PACKED, FINAL>, grid, dim3(KX_THREADS), smem, stream, a);
 }
 

@@ -323,13 +323,9 @@ key_weights_tc_kernel(const KeyWeightsMmaArgs a) {
 template <int D, bool PACKED, bool FINAL>
 static int kt_launch(const KeyWeightsMmaArgs& a, dim3 grid, cudaStream_t stream) {
   constexpr size_t smem = 3 * 128 * D * 2 + 1024;
-  static bool set = false;
-  if (!set) {
-    cudaError_t e = cudaFuncSetAttribute(key_weights_tc_kernel<D, PACKED, FINAL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(key_weights_tc_kernel<D, PACKED, FINAL>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-    if (e != cudaSuccess) return (int)e;
-    set = true;
-  }
+  static bool ready[64] = {};
+  const int limit = smem_limit((const void*)key_weights_tc_kernel<D, PACKED, FINAL>, (int)smem, true, ready);
+  if (limit != 0) return limit;
   return launch_pdl(key_weights_tc_kernel<D, PACKED, FINAL>, grid, dim3(KT_THREADS), smem, stream, a);
 }
 

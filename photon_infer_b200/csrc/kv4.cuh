@@ -11,6 +11,7 @@
 // 8 lanes that share the rows of a product's result read one run each and get 4 numbers of every group.
 #pragma once
 #include "common.cuh"
+#include "limits.cuh"
 #include <cuda_fp16.h>
 
 __host__ __device__ __forceinline__ long kv4_page_bytes(int page_size, int d) { return (long)page_size * (d / 32) * 17; }

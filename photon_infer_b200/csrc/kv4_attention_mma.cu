@@ -741,13 +741,9 @@ template <int GROUPS, int NT, bool CAP>
 static int km_launch(const Kv4MmaArgs& a, int blocks, int max_rows, cudaStream_t stream) {
   constexpr int RT = 4 * NT;
   constexpr size_t stages = 4 * KM_STAGES * (64 * GROUPS * 16 + 64 * GROUPS);
-  static bool set = false;
-  if (!set) {
-    cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages + (KM_MAX_SEQS + 1) * sizeof(int)));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP, false>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-    if (e != cudaSuccess) return (int)e;
-    set = true;
-  }
+  static bool ready[64] = {};
+  const int limit = smem_limit((const void*)kv4_mma_kernel<GROUPS, NT, CAP, false>, (int)(stages + (KM_MAX_SEQS + 1) * sizeof(int)), true, ready);
+  if (limit != 0) return limit;
   const int status = launch_pdl(kv4_mma_kernel<GROUPS, NT, CAP, false>, dim3(blocks), dim3(KM_THREADS), stages + (a.S + 1) * sizeof(int), stream, a);
   if (status != 0) return status;
   // threads by the parts that a unit has, about
@@ -782,13 +778,9 @@ PHOTON_API int photon_kv4_attention_mma(const photon_kv4_attention_call* c, cuda
 template <int GROUPS, int NT, bool CAP>
 static int km_weigh(const Kv4MmaArgs& a, int blocks, cudaStream_t stream) {
   constexpr size_t stages = 4 * KM_STAGES * (32 * GROUPS * 17);
-  static bool set = false;
-  if (!set) {
-    cudaError_t e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(stages + (KM_MAX_SEQS + 1) * sizeof(int)));
-    if (e == cudaSuccess) e = cudaFuncSetAttribute(kv4_mma_kernel<GROUPS, NT, CAP, true>, cudaFuncAttributePreferredSharedMemoryCarveout, 100);
-    if (e != cudaSuccess) return (int)e;
-    set = true;
-  }
+  static bool ready[64] = {};
+  const int limit = smem_limit((const void*)kv4_mma_kernel<GROUPS, NT, CAP, true>, (int)(stages + (KM_MAX_SEQS + 1) * sizeof(int)), true, ready);
+  if (limit != 0) return limit;
   return launch_pdl(kv4_mma_kernel<GROUPS, NT, CAP, true>, dim3(blocks), dim3(KM_THREADS), stages + (a.S + 1) * sizeof(int), stream, a);
 }
 

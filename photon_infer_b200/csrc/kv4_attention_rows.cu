@@ -254,12 +254,9 @@ kv4_attention_rows_kernel(const Kv4Args a) {
 template <typename T, int NV>
 static int kr_launch(const Kv4Args& a, dim3 grid, cudaStream_t stream) {
   constexpr size_t smem = (KR_KEYS * KR_PITCH + KR_PIECE * (KR_KEY_PITCH + KR_PITCH)) * sizeof(float);
-  static bool set = false;
-  if (!set) {
-    const cudaError_t e = cudaFuncSetAttribute(kv4_attention_rows_kernel<T, NV>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    if (e != cudaSuccess) return (int)e;
-    set = true;
-  }
+  static bool ready[64] = {};
+  const int limit = smem_limit((const void*)kv4_attention_rows_kernel<T, NV>, (int)smem, false, ready);
+  if (limit != 0) return limit;
   return launch_pdl(kv4_attention_rows_kernel<T, NV>, grid, dim3(KR_THREADS), smem, stream, a);
 }
 
