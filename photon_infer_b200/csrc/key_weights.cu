@@ -5,7 +5,7 @@
 // the maximum and the sum of every share of the keys, and the second joins them.  Every key is one thread's: no sums over blocks, no atomics.
 // The cache: 4 bits (kv4.cuh), bfloat16 or 32 bits.
 //
-// For up to 8 rows, 8 at a time, in 32 bits: what bounds it is the reading, since a thread has a key and reads its row by itself, and every number meets 8 rows' whether they are there or not.  4
+// For up to 8 rows, in 32 bits: what bounds it is the reading, since a thread has a key and reads its row by itself, and every number meets 8 rows' whether they are there or not.  4
 // rows beside 4,000 keys, 8 heads of 128, 32 bits: 30 us; key_weights_rows.cu takes 35 for them and from 9 rows on less.
 #include "key_weights.cuh"
 
@@ -30,124 +30,117 @@ key_weights_kernel(const KeyWeightsArgs a) {
   pdl_wait();
   const int seq = blockIdx.z, head = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int first = a.cu_tokens[seq], n = a.cu_tokens[seq + 1] - first, ctx = a.context_lens[seq];
-  const int G = a.n_q / a.n_kv, rows = n * G, d = a.d, groups = d / 32, words = d / 8, base = ctx - n;
+  const int G = a.n_q / a.n_kv, rows = min(n * G, KW_ROWS), d = a.d, groups = d / 32, words = d / 8, base = ctx - n;
   const int tiles = (max(ctx, 0) + KW_THREADS - 1) / KW_THREADS, per = (tiles + a.parts - 1) / a.parts;
   if (n <= 0) return;
-  for (int r0 = 0; r0 < rows; r0 += KW_ROWS) {
-    const int some = min(KW_ROWS, rows - r0);
-    __syncthreads();
-    for (int i = tid; i < KW_ROWS * d; i += KW_THREADS) {
-      const int r = i / d, p = i - r * d, x = p / 8, t = PACKED ? x / groups : 0, at = PACKED ? 32 * (x - t * groups) + 8 * t + p % 8 : p;
-      const int row = r0 + r;
-      qs[r * d + p] = r < some ? to_f32(((const T*)a.q)[(first + row / G) * a.q_stride + (head * G + row % G) * d + at]) : 0.f;
+  for (int i = tid; i < KW_ROWS * d; i += KW_THREADS) {
+    const int r = i / d, p = i - r * d, x = p / 8, t = PACKED ? x / groups : 0, at = PACKED ? 32 * (x - t * groups) + 8 * t + p % 8 : p;
+    qs[r * d + p] = r < rows ? to_f32(((const T*)a.q)[(first + r / G) * a.q_stride + (head * G + r % G) * d + at]) : 0.f;
+  }
+  if (FINAL && tid < rows) {
+    const int h = head * G + tid % G;
+    const long of = (long)(first + tid / G) * a.n_q + h;
+    float v;
+    if (a.lse != nullptr) {
+      v = a.lse[of] * 1.4426950408889634f;
+    } else {
+      const float* part_ml = a.scratch + of * a.parts * 2;
+      float m = a.sinks != nullptr ? a.sinks[h] * 1.4426950408889634f : -INFINITY;
+      const float sink = m;
+      for (int p = 0; p < a.parts; ++p) m = fmaxf(m, part_ml[2 * p]);
+      const float ref = m == -INFINITY ? 0.f : m;
+      float total = a.sinks != nullptr ? exp2f(sink - ref) : 0.f;
+      for (int p = 0; p < a.parts; ++p) {
+        const float pm = part_ml[2 * p], pl = part_ml[2 * p + 1];
+        if (pl != 0.f) total += pl * (pm == -INFINITY ? 1.f : exp2f(pm - ref));
+      }
+      v = total == 0.f ? -INFINITY : ref + log2f(total);
     }
-    if (FINAL && tid < some) {
-      const int row = r0 + tid, h = head * G + row % G;
-      const long of = (long)(first + row / G) * a.n_q + h;
-      float v;
-      if (a.lse != nullptr) {
-        v = a.lse[of] * 1.4426950408889634f;
-      } else {
-        const float* part_ml = a.scratch + of * a.parts * 2;
-        float m = a.sinks != nullptr ? a.sinks[h] * 1.4426950408889634f : -INFINITY;
-        const float sink = m;
-        for (int p = 0; p < a.parts; ++p) m = fmaxf(m, part_ml[2 * p]);
-        const float ref = m == -INFINITY ? 0.f : m;
-        float total = a.sinks != nullptr ? exp2f(sink - ref) : 0.f;
-        for (int p = 0; p < a.parts; ++p) {
-          const float pm = part_ml[2 * p], pl = part_ml[2 * p + 1];
-          if (pl != 0.f) total += pl * (pm == -INFINITY ? 1.f : exp2f(pm - ref));
-        }
-        v = total == 0.f ? -INFINITY : ref + log2f(total);
+    lse_s[tid] = v;
+  }
+  __syncthreads();
+  float m[KW_ROWS], l[KW_ROWS];
+#pragma unroll
+  for (int r = 0; r < KW_ROWS; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
+  for (int tile = part * per; tile < min((part + 1) * per, tiles); ++tile) {
+    const int key = tile * KW_THREADS + tid, pidx = key / a.page_size, slot = key - pidx * a.page_size;
+    int page = -1;
+    if (key < ctx) {
+      page = pidx < a.max_pages ? a.table[(long)seq * a.max_pages + pidx] : -1;
+      if (page < 0 || page >= a.num_pages) {
+        if (FINAL) report_error(a.err, PHOTON_DEV_BAD_PAGE, seq, key, page);
+        page = -1;
       }
-      lse_s[tid] = v;
     }
-    __syncthreads();
-    float m[KW_ROWS], l[KW_ROWS];
+    float s[KW_ROWS];
 #pragma unroll
-    for (int r = 0; r < KW_ROWS; ++r) { m[r] = -INFINITY; l[r] = 0.f; }
-    for (int tile = part * per; tile < min((part + 1) * per, tiles); ++tile) {
-      const int key = tile * KW_THREADS + tid, pidx = key / a.page_size, slot = key - pidx * a.page_size;
-      int page = -1;
-      if (key < ctx) {
-        page = pidx < a.max_pages ? a.table[(long)seq * a.max_pages + pidx] : -1;
-        if (page < 0 || page >= a.num_pages) {
-          if (FINAL && r0 == 0) report_error(a.err, PHOTON_DEV_BAD_PAGE, seq, key, page);
-          page = -1;
-        }
-      }
-      float s[KW_ROWS];
+    for (int r = 0; r < KW_ROWS; ++r) s[r] = 0.f;
+    if (page >= 0) {
+      const uint8_t* at = PACKED ? (const uint8_t*)a.k + ((long)page * a.n_kv + head) * kv4_page_bytes(a.page_size, d) : nullptr;
+      const uint32_t* codes = PACKED ? (const uint32_t*)(at + (long)slot * (d / 2)) : nullptr;
+      const uint8_t* scales = PACKED ? at + (long)a.page_size * (d / 2) + slot * groups : nullptr;
+      const C* row = (const C*)a.k + (((long)page * a.n_kv + head) * a.page_size + slot) * d;
+      for (int x = 0; x < words; ++x) {
+        float c[8];
+        if constexpr (PACKED) {
+          const uint32_t word = codes[x];
+          const float scale = kv4_scale(scales[x % groups]);
 #pragma unroll
-      for (int r = 0; r < KW_ROWS; ++r) s[r] = 0.f;
-      if (page >= 0) {
-        const uint8_t* at = PACKED ? (const uint8_t*)a.k + ((long)page * a.n_kv + head) * kv4_page_bytes(a.page_size, d) : nullptr;
-        const uint32_t* codes = PACKED ? (const uint32_t*)(at + (long)slot * (d / 2)) : nullptr;
-        const uint8_t* scales = PACKED ? at + (long)a.page_size * (d / 2) + slot * groups : nullptr;
-        const C* row = (const C*)a.k + (((long)page * a.n_kv + head) * a.page_size + slot) * d;
-        for (int x = 0; x < words; ++x) {
-          float c[8];
-          if constexpr (PACKED) {
-            const uint32_t word = codes[x];
-            const float scale = kv4_scale(scales[x % groups]);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) c[i] = kv4_code(word, i) * scale;
-          } else {
-            key_numbers<C>(row, x, c);
-          }
-#pragma unroll
-          for (int r = 0; r < KW_ROWS; ++r) {
-            const float4 u = *(const float4*)&qs[r * d + x * 8], v = *(const float4*)&qs[r * d + x * 8 + 4];
-            s[r] += c[0] * u.x + c[1] * u.y + c[2] * u.z + c[3] * u.w + c[4] * v.x + c[5] * v.y + c[6] * v.z + c[7] * v.w;
-          }
-        }
-      }
-      float sum = 0.f;
-#pragma unroll
-      for (int r = 0; r < KW_ROWS; ++r) {
-        const int place = base + (r0 + r) / G;
-        if (page < 0 || r >= some || key > place || (a.window > 0 && key <= place - a.window)) continue;
-        const float x = key_score(s[r], a.scale, a.softcap);
-        if (FINAL) {
-          sum += exp2f(x - lse_s[r]);
+          for (int i = 0; i < 8; ++i) c[i] = kv4_code(word, i) * scale;
         } else {
-          const float top = fmaxf(m[r], x);
-          const float ref = top == -INFINITY ? 0.f : top;
-          l[r] = l[r] * (m[r] == -INFINITY ? 1.f : exp2f(m[r] - ref)) + exp2f(x - ref);
-          m[r] = top;
+          key_numbers<C>(row, x, c);
         }
-      }
-      if (FINAL && page >= 0) {
-        float* w = a.weights + ((long)page * a.n_kv + head) * a.page_size + slot;
-        const bool had = r0 > 0 || (a.held != nullptr ? key < a.held[seq] : key < base);
-        *w = had ? *w + sum : sum;
+#pragma unroll
+        for (int r = 0; r < KW_ROWS; ++r) {
+          const float4 u = *(const float4*)&qs[r * d + x * 8], v = *(const float4*)&qs[r * d + x * 8 + 4];
+          s[r] += c[0] * u.x + c[1] * u.y + c[2] * u.z + c[3] * u.w + c[4] * v.x + c[5] * v.y + c[6] * v.z + c[7] * v.w;
+        }
       }
     }
-    if (!FINAL) {
+    float sum = 0.f;
 #pragma unroll
-      for (int r = 0; r < KW_ROWS; ++r) {
-        __syncthreads();
-        const float top = warp_max(m[r]);
-        if (lane == 0) red[warp] = top;
-        __syncthreads();
-        const float all = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), ref = all == -INFINITY ? 0.f : all;
-        const float total = block_sum(l[r] == 0.f ? 0.f : l[r] * (m[r] == -INFINITY ? 1.f : exp2f(m[r] - ref)), red);
-        if (tid == 0 && r < some) {
-          const int row = r0 + r;
-          float* to = a.scratch + ((long)(first + row / G) * a.n_q + head * G + row % G) * a.parts * 2 + 2 * part;
-          to[0] = all;
-          to[1] = total;
-        }
+    for (int r = 0; r < KW_ROWS; ++r) {
+      const int place = base + r / G;
+      if (page < 0 || r >= rows || key > place || (a.window > 0 && key <= place - a.window)) continue;
+      const float x = key_score(s[r], a.scale, a.softcap);
+      if (FINAL) {
+        sum += exp2f(x - lse_s[r]);
+      } else {
+        const float top = fmaxf(m[r], x);
+        const float ref = top == -INFINITY ? 0.f : top;
+        l[r] = l[r] * (m[r] == -INFINITY ? 1.f : exp2f(m[r] - ref)) + exp2f(x - ref);
+        m[r] = top;
+      }
+    }
+    if (FINAL && page >= 0) {
+      float* w = a.weights + ((long)page * a.n_kv + head) * a.page_size + slot;
+      *w = key < (a.held != nullptr ? a.held[seq] : base) ? *w + sum : sum;
+    }
+  }
+  if (!FINAL) {
+#pragma unroll
+    for (int r = 0; r < KW_ROWS; ++r) {
+      __syncthreads();
+      const float top = warp_max(m[r]);
+      if (lane == 0) red[warp] = top;
+      __syncthreads();
+      const float all = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), ref = all == -INFINITY ? 0.f : all;
+      const float total = block_sum(l[r] == 0.f ? 0.f : l[r] * (m[r] == -INFINITY ? 1.f : exp2f(m[r] - ref)), red);
+      if (tid == 0 && r < rows) {
+        float* to = a.scratch + ((long)(first + r / G) * a.n_q + head * G + r % G) * a.parts * 2 + 2 * part;
+        to[0] = all;
+        to[1] = total;
       }
     }
   }
 }
 
 PHOTON_API int photon_key_weights(const photon_key_weights_call* c, cudaStream_t stream) {
-  if (c->S <= 0 || c->max_keys <= 0) return 0;
+  if (c->S <= 0 || c->max_keys <= 0 || c->max_tokens_per_seq <= 0) return 0;
   if ((c->dtype != PHOTON_F32 && c->dtype != PHOTON_BF16) || c->n_kv <= 0 || c->n_q <= 0 || c->n_q % c->n_kv || c->max_pages <= 0 || c->num_pages < 0) return PHOTON_ERR_ARGUMENT;
   if (c->packed ? !kv4_sizes_ok(c->page_size, c->d) : (c->page_size <= 0 || c->d <= 0 || c->d > 256 || c->d % 8 != 0)) return PHOTON_ERR_UNSUPPORTED;
   if (c->parts < 1 || (c->lse == nullptr && c->scratch == nullptr)) return PHOTON_ERR_ARGUMENT;
-  if (c->S > 65535 || c->n_kv > 65535 || c->scale <= 0.f) return PHOTON_ERR_UNSUPPORTED;
+  if (c->S > 65535 || c->n_kv > 65535 || c->scale <= 0.f || (long)c->max_tokens_per_seq * (c->n_q / c->n_kv) > KW_ROWS) return PHOTON_ERR_UNSUPPORTED;
   const KeyWeightsArgs a = {c->q, c->weights, c->k_cache, c->block_table, c->cu_tokens, c->context_lens, c->held, c->sinks, c->lse, c->scratch, c->err, c->q_stride,
                             c->max_pages, c->n_q, c->n_kv, c->d, c->page_size, c->num_pages, c->window, c->parts, c->scale, c->softcap};
   const dim3 grid(c->parts, c->n_kv, c->S);

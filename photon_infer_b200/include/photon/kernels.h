@@ -673,7 +673,8 @@ PHOTON_EXPORT int photon_kv4_attention_rows(const photon_kv4_attention_call* cal
 PHOTON_EXPORT int photon_kv4_attention_mma(const photon_kv4_attention_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ key_weights.cu */
-/* weights [num_pages][n_kv][page_size]: what the keys below context_lens[s] got of the softmax of request s's rows is added; keys from held[s] on (held null: the call's own tokens)
+/* At most 8 rows (max_tokens_per_seq * n_q / n_kv) a request.
+ * weights [num_pages][n_kv][page_size]: what the keys below context_lens[s] got of the softmax of request s's rows is added; keys from held[s] on (held null: the call's own tokens)
  * are set.  k_cache: of dtype, [num_pages][n_kv][page_size][d], or with packed 4 bits a number.  Rows and masks as in photon_kv4_attention; lse as that leaves it, or null:
  * then scratch has T * n_q * parts * 2 floats. */
 typedef struct {
@@ -690,10 +691,10 @@ PHOTON_EXPORT int photon_key_weights(const photon_key_weights_call* call, cudaSt
 PHOTON_EXPORT int photon_key_weights_rows(const photon_key_weights_call* call, cudaStream_t stream);
 
 /* ------------------------------------------------------------------ key_weights_mma.cu: the same on the tensor cores, bfloat16, d 64 or 128 */
-/* 16-byte aligned rows of q; at most max_tokens_per_seq tokens and max_keys keys a request.  parts: runs of a request's keys.  Without lse, scratch: T * n_q * (2 * parts + 1)
+/* 16-byte aligned rows of q; at most 32 rows (max_tokens_per_seq * n_q / n_kv) and max_keys keys a request.  parts: runs of a request's keys.  Without lse, scratch: T * n_q * (2 * parts + 1)
  * floats, and with keep_scores (at most 16 rows a request: the keys are read once) T * n_q * max_keys more. */
 PHOTON_EXPORT int photon_key_weights_mma(const photon_key_weights_call* call, cudaStream_t stream);
-/* key_weights_tc.cu: the same on tcgen05, for many rows; without keep_scores. */
+/* key_weights_tc.cu: the same on tcgen05, for any number of rows; without keep_scores. */
 PHOTON_EXPORT int photon_key_weights_tc(const photon_key_weights_call* call, cudaStream_t stream);
 /* kv4_attention_mma.cu: with lse, for a cache in 4 bits and at most 8 rows (max_tokens_per_seq * n_q / n_kv), pages of a multiple of 8 tokens, 1,024 requests.  parts: blocks. */
 PHOTON_EXPORT int photon_kv4_key_weights(const photon_key_weights_call* call, cudaStream_t stream);
