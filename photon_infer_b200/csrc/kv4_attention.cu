@@ -28,7 +28,7 @@ kv4_attention_kernel(const Kv4Args a) {
   const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
   const int first = a.cu_tokens[seq], n = a.cu_tokens[seq + 1] - first, ctx = a.context_lens[seq];
   const int G = a.n_q / a.n_kv, all = n * G, row0 = tile * ROWS;
-  if (row0 >= all || all <= a.min_rows || all > a.max_rows) return;
+  if (row0 >= all || all > a.max_rows) return;
   const int rows = min(ROWS, all - row0), d = a.groups * 32, words = d / 8, base = ctx - n;
   const int last_place = base + (row0 + rows - 1) / G, first_place = base + row0 / G;
   const int lo = a.window > 0 ? max(0, first_place - a.window + 1) : 0, hi = max(lo, last_place + 1);
@@ -178,7 +178,7 @@ PHOTON_API int photon_kv4_attention(const photon_kv4_attention_call* c, cudaStre
   if (!kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_UNSUPPORTED;
   if (c->parts < 1 || (c->parts > 1 && c->scratch == nullptr)) return PHOTON_ERR_ARGUMENT;
   Kv4Args a = {c->q, c->out, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->block_table, c->cu_tokens, c->context_lens, c->sinks, c->lse, c->scratch, c->err,
-               c->q_stride, c->out_stride, c->max_pages, c->n_q, c->n_kv, c->d / 32, c->page_size, c->num_pages, c->window, c->parts, c->scale, c->softcap, c->min_rows, c->max_rows};
+               c->q_stride, c->out_stride, c->max_pages, c->n_q, c->n_kv, c->d / 32, c->page_size, c->num_pages, c->window, c->parts, c->scale, c->softcap, c->max_rows};
   const long rows = (long)c->max_tokens_per_seq * (c->n_q / c->n_kv);
   const int R = rows <= 1 ? 1 : rows <= 2 ? 2 : rows <= 4 ? 4 : 8;
   const long y = (rows + R - 1) / R * c->n_kv;

@@ -9,7 +9,7 @@ struct Kv4Args {
   long q_stride, out_stride;
   int max_pages, n_q, n_kv, groups, page_size, num_pages, window, parts;
   float scale, softcap;
-  int min_rows, max_rows;       // requests with other numbers of rows are left to another kernel
+  int max_rows;                 // requests with more are left to another kernel
 };
 
 __device__ __forceinline__ float kv4_bounded(float x, float scale, float softcap) {      // a score in powers of two
@@ -31,7 +31,7 @@ kv4_join_kernel(const Kv4Args a, int S) {
   pdl_wait();
   const int seq = blockIdx.y, d = a.groups * 32, G = a.n_q / a.n_kv, head = blockIdx.x % a.n_q, i = blockIdx.x / a.n_q;
   const int first = a.cu_tokens[seq], n = a.cu_tokens[seq + 1] - first;
-  if (i >= n || n * G <= a.min_rows || n * G > a.max_rows) return;
+  if (i >= n || n * G > a.max_rows) return;
   const long token = first + i, of = token * a.n_q + head;
   const float* part = a.scratch + of * a.parts * (d + 2);
   float m = a.sinks != nullptr ? a.sinks[head] * 1.4426950408889634f : -INFINITY;

@@ -41,7 +41,7 @@ struct Kv4MmaArgs {
   float scale, softcap;
   int page_shift;                // of page_size / 8, or -1
   float* weights; const int* held;      // the second use: what keys got, beside them
-  int min_rows, max_rows, q_vec, out_vec;      // rows of q on 16-byte boundaries, of out on 8-byte ones
+  int max_rows, q_vec, out_vec;      // rows of q on 16-byte boundaries, of out on 8-byte ones
 };
 
 // d += a b: 16 x 16 and 16 x 8 numbers of 16 bits; and d = a b.
@@ -120,7 +120,7 @@ __device__ __forceinline__ KmRequest km_request(const Kv4MmaArgs& a, int s) {
   r.n = a.cu_tokens[s + 1] - r.first;
   r.ctx = a.context_lens[s];
   r.rows = r.n * (a.n_q / a.n_kv);
-  if (r.rows <= a.min_rows || r.rows > a.max_rows) r.rows = 0;
+  if (r.rows > a.max_rows) r.rows = 0;
   r.row_tiles = (r.rows + RT - 1) / RT;
   int lo = a.window > 0 ? max(0, r.ctx - r.n - a.window + 1) : 0;
   if (WEIGH) lo = max(0, min(lo, a.held != nullptr ? a.held[s] : r.ctx - r.n));      // keys without a sum get one
@@ -767,7 +767,7 @@ PHOTON_API int photon_kv4_attention_mma(const photon_kv4_attention_call* c, cuda
   const long words = 8L * c->parts * (most <= 4 ? 4 : 8) * (c->d + 2);
   const Kv4MmaArgs a = {(const bf16*)c->q, (bf16*)c->out, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->block_table, c->cu_tokens, c->context_lens, c->sinks, c->lse,
                         c->scratch, (int*)c->scratch + words, c->err, c->q_stride, c->out_stride, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, shift, nullptr, nullptr,
-                        c->min_rows, c->max_rows, (uintptr_t)c->q % 16 == 0 && c->q_stride % 8 == 0,
+                        c->max_rows, (uintptr_t)c->q % 16 == 0 && c->q_stride % 8 == 0,
                         (uintptr_t)c->out % 8 == 0 && c->out_stride % 4 == 0};
 #define ATTEND(GROUPS, NT) (c->softcap > 0.f ? km_launch<GROUPS, NT, true>(a, c->parts, most, stream) : km_launch<GROUPS, NT, false>(a, c->parts, most, stream))
   if (c->d == 64) return most <= 4 ? ATTEND(2, 1) : ATTEND(2, 2);
@@ -795,7 +795,7 @@ PHOTON_API int photon_kv4_key_weights(const photon_key_weights_call* c, cudaStre
   int shift = -1;
   for (int i = 0; i < 28; ++i) if (c->page_size == 8 << i) shift = i;
   const Kv4MmaArgs a = {(const bf16*)c->q, nullptr, (const uint8_t*)c->k_cache, nullptr, c->block_table, c->cu_tokens, c->context_lens, nullptr, (float*)c->lse, nullptr, nullptr, c->err,
-                        c->q_stride, 0, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, shift, c->weights, c->held, 0, rows,
+                        c->q_stride, 0, c->max_pages, c->S, c->n_q, c->n_kv, c->page_size, c->num_pages, c->window, c->scale, c->softcap, shift, c->weights, c->held, rows,
                         (uintptr_t)c->q % 16 == 0 && c->q_stride % 8 == 0, 0};
 #define WEIGH(GROUPS, NT) (c->softcap > 0.f ? km_weigh<GROUPS, NT, true>(a, c->parts, stream) : km_weigh<GROUPS, NT, false>(a, c->parts, stream))
   if (c->d == 64) return rows <= 4 ? WEIGH(2, 1) : WEIGH(2, 2);

@@ -32,7 +32,7 @@ kv4_attention_rows_kernel(const Kv4Args a) {
   const int seq = blockIdx.z, head = blockIdx.y % a.n_kv, part = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kt = lane & 15, rt = 2 * warp + (lane >> 4);
   const int first = a.cu_tokens[seq], n = a.cu_tokens[seq + 1] - first, ctx = a.context_lens[seq];
   const int G = a.n_q / a.n_kv, all = n * G, row0 = (int)(blockIdx.y / a.n_kv) * KR_ROWS;
-  if (row0 >= all || all <= a.min_rows || all > a.max_rows) return;
+  if (row0 >= all || all > a.max_rows) return;
   const int groups = a.groups, rows = min(KR_ROWS, all - row0), d = groups * 32, base = ctx - n;
   const int last_place = base + (row0 + rows - 1) / G, first_place = base + row0 / G;
   const int lo = a.window > 0 ? max(0, first_place - a.window + 1) : 0, hi = max(lo, last_place + 1);
@@ -266,7 +266,7 @@ PHOTON_API int photon_kv4_attention_rows(const photon_kv4_attention_call* c, cud
   if (!kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_UNSUPPORTED;
   if (c->parts < 1 || (c->parts > 1 && c->scratch == nullptr)) return PHOTON_ERR_ARGUMENT;
   const Kv4Args a = {c->q, c->out, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->block_table, c->cu_tokens, c->context_lens, c->sinks, c->lse, c->scratch, c->err,
-                     c->q_stride, c->out_stride, c->max_pages, c->n_q, c->n_kv, c->d / 32, c->page_size, c->num_pages, c->window, c->parts, c->scale, c->softcap, c->min_rows, c->max_rows};
+                     c->q_stride, c->out_stride, c->max_pages, c->n_q, c->n_kv, c->d / 32, c->page_size, c->num_pages, c->window, c->parts, c->scale, c->softcap, c->max_rows};
   const long rows = (long)c->max_tokens_per_seq * (c->n_q / c->n_kv), y = (rows + KR_ROWS - 1) / KR_ROWS * c->n_kv, x = (long)c->max_tokens_per_seq * c->n_q;
   if (c->S > 65535 || y > 65535 || x > 0x7fffffffL || c->scale <= 0.f) return PHOTON_ERR_UNSUPPORTED;
   const dim3 grid(c->parts, (unsigned)y, c->S);

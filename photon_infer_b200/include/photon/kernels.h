@@ -653,13 +653,13 @@ PHOTON_EXPORT int photon_kv4_spoil(const photon_kv4_unpack_call* call, void* out
 
 /* ------------------------------------------------------------------ kv4_attention.cu */
 /* The tokens cu_tokens[s] .. cu_tokens[s + 1] - 1 of the step are the last of request s's context_lens[s] keys; the one at place p sees keys p - window + 1 .. p (window 0:
- * 0 .. p).  A row that sees nothing is zero.  Requests with rows (tokens x n_q / n_kv) in (min_rows, max_rows] only.  lse (may be null): float [T, n_q], each row's logarithm of the
+ * 0 .. p).  A row that sees nothing is zero.  Requests of at most max_rows rows (tokens x n_q / n_kv) only.  lse (may be null): float [T, n_q], each row's logarithm of the
  * sum of the exponentials of its scores, the sink's among them.  scratch: T * n_q * parts * (d + 2) floats for parts > 1. */
 typedef struct {
   const void* q; void* out; const void* k_cache; const void* v_cache; const int* block_table; const int* cu_tokens; const int* context_lens;
   const float* sinks; float* lse; float* scratch; int* err;
   long q_stride, out_stride;
-  int dtype, max_pages, S, max_tokens_per_seq, n_q, n_kv, d, page_size, num_pages, window, parts, min_rows, max_rows;
+  int dtype, max_pages, S, max_tokens_per_seq, n_q, n_kv, d, page_size, num_pages, window, parts, max_rows;
   float scale, softcap;
 } photon_kv4_attention_call;
 PHOTON_EXPORT int photon_kv4_attention(const photon_kv4_attention_call* call, cudaStream_t stream);

@@ -2854,7 +2854,7 @@ def _sms(index: int, device: torch.device) -> int:
 #: photon_kv4_write_call, photon_kv4_unpack_call, photon_kv4_attention_call, photon_key_weights_call, photon_evict_call
 _KV4_WRITE_CALL = struct.Struct("6q2q6i")
 _KV4_UNPACK_CALL = struct.Struct("11q1q9i4x")
-_KV4_ATTENTION_CALL = struct.Struct("11q2q13i2f4x")
+_KV4_ATTENTION_CALL = struct.Struct("11q2q12i2f")
 _KEY_WEIGHTS_CALL = struct.Struct("11q2q14i2f")
 _EVICT_CALL = struct.Struct("7q13i4x")
 
@@ -2971,7 +2971,7 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
     call = _KV4_ATTENTION_CALL.pack(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(),
                                     0 if sink is None else sink.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
                                     0 if err is None else err.data_ptr(), q_stride, out_stride, _dtype_code(q), pages, num_seqs, tokens, n_q, n_kv, head_dim, page_size, pool,
-                                    window, parts, 0, most, scale, softcap or 0.0)
+                                    window, parts, most, scale, softcap or 0.0)
     _check(_plain_fn(name, "photon_" + name, _CALL_ARGS)(call, _stream()), "kv4_attention")
     if floats:
         _count_launches(1)
