@@ -33,6 +33,7 @@ key_weights_kernel(const KeyWeightsArgs a) {
   const int G = a.n_q / a.n_kv, rows = min(n * G, KW_ROWS), d = a.d, groups = d / 32, words = d / 8, base = ctx - n;
   const int tiles = (max(ctx, 0) + KW_THREADS - 1) / KW_THREADS, per = (tiles + a.parts - 1) / a.parts;
   if (n <= 0) return;
+  const int known = a.held != nullptr ? a.held[seq] : base, low = a.window > 0 ? min(base - a.window + 1, known) : 0;      // keys in front of it no row sees, and they have a sum
   for (int i = tid; i < KW_ROWS * d; i += KW_THREADS) {
     const int r = i / d, p = i - r * d, x = p / 8, t = PACKED ? x / groups : 0, at = PACKED ? 32 * (x - t * groups) + 8 * t + p % 8 : p;
     qs[r * d + p] = r < rows ? to_f32(((const T*)a.q)[(first + r / G) * a.q_stride + (head * G + r % G) * d + at]) : 0.f;
@@ -65,7 +66,7 @@ key_weights_kernel(const KeyWeightsArgs a) {
   for (int tile = part * per; tile < min((part + 1) * per, tiles); ++tile) {
     const int key = tile * KW_THREADS + tid, pidx = key / a.page_size, slot = key - pidx * a.page_size;
     int page = -1;
-    if (key < ctx) {
+    if (key >= low && key < ctx) {
       page = pidx < a.max_pages ? a.table[(long)seq * a.max_pages + pidx] : -1;
       if (page < 0 || page >= a.num_pages) {
         if (FINAL) report_error(a.err, PHOTON_DEV_BAD_PAGE, seq, key, page);
@@ -114,7 +115,7 @@ key_weights_kernel(const KeyWeightsArgs a) {
     }
     if (FINAL && page >= 0) {
       float* w = a.weights + ((long)page * a.n_kv + head) * a.page_size + slot;
-      *w = key < (a.held != nullptr ? a.held[seq] : base) ? *w + sum : sum;
+      *w = key < known ? *w + sum : sum;
     }
   }
   if (!FINAL) {

@@ -59,7 +59,7 @@ key_weights_mma_kernel(const KeyWeightsMmaArgs a) {
   // ---- places: thread `tid` has key `tid` of a tile, and the block table's entry of the next one
   auto entry_of = [&](int tile) {
     const int key = tile * KX_KEYS + tid, pidx = key / a.page_size;
-    return tid < KX_KEYS && tile < tile1 && key < ctx ? (pidx < a.max_pages ? a.table[(long)seq * a.max_pages + pidx] : -1) : -2;      // -2: not asked for
+    return tid < KX_KEYS && tile < tile1 && key >= low && key < ctx ? (pidx < a.max_pages ? a.table[(long)seq * a.max_pages + pidx] : -1) : -2;      // -2: not asked for
   };
   auto settle = [&](int tile, int entry) {             // the tile's places, from its entries
     if (tid < KX_KEYS) {
@@ -296,16 +296,16 @@ key_weights_scores_kernel(const KeyWeightsMmaArgs a) {
   if (threadIdx.x < rows) lse_s[threadIdx.x] = a.lse[(long)(first + threadIdx.x / G) * a.n_q + head * G + threadIdx.x % G] * 1.4426950408889634f;
   __syncthreads();
   if (key >= ctx || key >= a.width) return;
+  const int known = a.held != nullptr ? a.held[seq] : base, low = a.window > 0 ? max(0, base - a.window + 1) : 0;
+  if (key < min(low, known)) return;                  // no row sees it, and it has a sum
   const int pidx = key / a.page_size, page = pidx < a.max_pages ? a.table[(long)seq * a.max_pages + pidx] : -1;
   if (page < 0 || page >= a.num_pages) {
     report_error(a.err, PHOTON_DEV_BAD_PAGE, seq, key, page);
     return;
   }
-  const int known = a.held != nullptr ? a.held[seq] : base, low = a.window > 0 ? max(0, base - a.window + 1) : 0;
-  if (key < low / KX_KEYS * KX_KEYS && key < known) return;      // no row sees it: there are no scores
   float* w = a.weights + ((long)page * a.n_kv + head) * a.page_size + (key - pidx * a.page_size);
   float sum = key < known ? *w : 0.f;
-  if (key >= low / KX_KEYS * KX_KEYS)
+  if (key >= low)                                     // else there are no scores
     for (int r = 0; r < rows; ++r) {
       const float x = a.scores[((long)(first + r / G) * a.n_q + head * G + r % G) * a.width + key];
       if (x != -INFINITY) sum += kx_exp2(x - lse_s[r]);

@@ -33,13 +33,14 @@ key_weights_rows_kernel(const KeyWeightsArgs w) {
   const int seq = blockIdx.z, head = blockIdx.y % a.n_kv, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, kt = lane & 15, rt = 2 * warp + (lane >> 4);
   const int first = a.cu_tokens[seq], n = a.cu_tokens[seq + 1] - first, ctx = a.context_lens[seq];
   const int G = a.n_q / a.n_kv, rows = n * G, d = w.d, groups = d / 32, base = ctx - n, known = a.held != nullptr ? a.held[seq] : base;
+  const int low = a.window > 0 ? min(base - a.window + 1, known) : 0;      // keys in front of it no row sees, and they have a sum
   const int tiles = (max(ctx, 0) + KX_KEYS - 1) / KX_KEYS, per = (tiles + a.parts - 1) / a.parts, tile0 = (int)blockIdx.x * per, tile1 = min(tile0 + per, tiles);
   if (n <= 0) return;
   auto settle = [&](int tile) {                       // thread `tid` finds key `tid` of the tile
     if (tid >= KX_KEYS) return;
     const int key = tile * KX_KEYS + tid, pidx = key / a.page_size, slot = key - pidx * a.page_size;
     int page = -1;
-    if (key < ctx) {
+    if (key >= low && key < ctx) {
       page = pidx < a.max_pages ? a.table[(long)seq * a.max_pages + pidx] : -1;
       if (page < 0 || page >= a.num_pages) {
         if (FINAL) report_error(a.err, PHOTON_DEV_BAD_PAGE, seq, key, page);

@@ -71,7 +71,7 @@ key_weights_tc_kernel(const KeyWeightsMmaArgs a) {
     struct Place { int entry, slot; };                 // entry -2: not asked for
     auto look = [&]() {                                // the tiles one behind the other; what is not there reads some entry of the table, too
       const int entry = a.table[(long)seq * a.max_pages + min(next_page, a.max_pages - 1)];
-      const Place p = {half != 0 || next_key >= min(ctx, tile1 * KX_KEYS) ? -2 : next_page < a.max_pages ? entry : -1, next_slot};
+      const Place p = {half != 0 || next_key < low || next_key >= min(ctx, tile1 * KX_KEYS) ? -2 : next_page < a.max_pages ? entry : -1, next_slot};
       next_key += KX_KEYS;
       next_page += step_pages;
       next_slot += step_slots;

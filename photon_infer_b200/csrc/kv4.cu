@@ -172,14 +172,14 @@ __device__ __forceinline__ void store8(T* p, const float* x) {      // 16-byte a
 }
 
 // Page blockIdx.x of the outputs is page table[i / per * stride + i % per] of the caches; blockIdx.y has a part of its (plane, head, slot, t).  With cu_tokens: i / per is a request, and
-// only the requests with more than min_rows rows (tokens x group) and their pages below context_lens count, and what lies behind their keys is zero; new_table (per wide) gets the
+// only the requests with more than min_rows rows (tokens x group) and their pages below context_lens and, with a window, not wholly in front of the first token's count, and what lies behind their keys is zero; new_table (per wide) gets the
 // outputs' page, or -1; positions gets every token's place in its request.  A value that is not finite is laid out as zero then (a weight of 0 would make it a NaN in rows that
 // do not see it), and flags [S * per * gridDim.y] tells where there was one: kv4_spoil_kernel gives it to the rows that see it.
 template <typename T, int GROUPS>
 __global__ void __launch_bounds__(KV4_THREADS)
 kv4_unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict__ v_cache, const int* __restrict__ table, int per, long stride, T* __restrict__ k_out,
                   T* __restrict__ v_out, int n_kv, int page_size, int page_shift, int num_pages, const int* __restrict__ cu_tokens, const int* __restrict__ context_lens, int group,
-                  int min_rows, int* __restrict__ new_table, int* __restrict__ positions, int* __restrict__ flags, int* err) {
+                  int min_rows, int window, int* __restrict__ new_table, int* __restrict__ positions, int* __restrict__ flags, int* err) {
   constexpr int D = GROUPS * 32;
   pdl_wait();
   pdl_launch_dependents();
@@ -190,7 +190,8 @@ kv4_unpack_kernel(const uint8_t* __restrict__ k_cache, const uint8_t* __restrict
     end = context_lens[s];
     if (positions != nullptr && p == 0 && blockIdx.y == 0)
       for (int x = threadIdx.x; x < n; x += KV4_THREADS) positions[first + x] = end - n + x;
-    if ((long)n * group <= min_rows || (long)p * page_size >= end) {
+    // pages in front of the window are not asked for: they may have been given back
+    if ((long)n * group <= min_rows || (long)p * page_size >= end || (window > 0 && (p + 1L) * page_size <= (long)end - n - window + 1)) {
       if (new_table != nullptr && blockIdx.y == 0 && threadIdx.x == 0) new_table[i] = -1;
       return;
     }
@@ -380,8 +381,8 @@ PHOTON_API int photon_kv4_unpack(const photon_kv4_unpack_call* c, cudaStream_t s
   int shift = -1;
   for (int i = 0; i < 31; ++i) if (c->page_size == 1 << i) shift = i;
 #define UNPACK(T, G) launch_pdl(kv4_unpack_kernel<T, G>, grid, dim3(KV4_THREADS), 0, stream, (const uint8_t*)c->k_cache, (const uint8_t*)c->v_cache, c->table, c->per, c->stride, \
-                                (T*)c->k_out, (T*)c->v_out, c->n_kv, c->page_size, shift, c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, c->new_table, c->positions, \
-                                c->cu_tokens != nullptr ? c->flags : nullptr, c->err)
+                                (T*)c->k_out, (T*)c->v_out, c->n_kv, c->page_size, shift, c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, c->window, c->new_table, \
+                                c->positions, c->cu_tokens != nullptr ? c->flags : nullptr, c->err)
 #define UNPACK_OF(G) (c->dtype == PHOTON_F32 ? UNPACK(float, G) : UNPACK(bf16, G))
   switch (c->d / 32) {
     case 1: return UNPACK_OF(1);
@@ -397,12 +398,12 @@ PHOTON_API int photon_kv4_unpack(const photon_kv4_unpack_call* c, cudaStream_t s
 #undef UNPACK
 }
 
-PHOTON_API int photon_kv4_spoil(const photon_kv4_unpack_call* c, void* out, long out_stride, const void* q, long q_stride, int max_tokens, int window, int bounded, cudaStream_t stream) {
+PHOTON_API int photon_kv4_spoil(const photon_kv4_unpack_call* c, void* out, long out_stride, const void* q, long q_stride, int max_tokens, int bounded, cudaStream_t stream) {
   if (c->S <= 0 || c->per <= 0 || max_tokens <= 0) return 0;
   if (c->dtype != PHOTON_BF16 || c->flags == nullptr || c->cu_tokens == nullptr || c->n_kv <= 0 || c->group <= 0 || !kv4_sizes_ok(c->page_size, c->d)) return PHOTON_ERR_ARGUMENT;
   if (c->S > 65535 || c->group > 128 || ((uintptr_t)out | (uintptr_t)q) % 16 || out_stride % 8 || q_stride % 8) return PHOTON_ERR_UNSUPPORTED;
   const int chunks = (max_tokens + KV4_SPOIL_TOKENS - 1) / KV4_SPOIL_TOKENS;
   return launch_pdl(kv4_spoil_kernel, dim3(c->n_kv, c->S, chunks < 65535 ? chunks : 65535), dim3(KV4_THREADS), 0, stream, (const uint8_t*)c->v_cache, c->table, c->per, c->stride, c->n_kv,
                     c->d / 32, c->page_size, c->num_pages, c->cu_tokens, c->context_lens, c->group, c->min_rows, kv4_unpack_parts(c), (const int*)c->flags, (bf16*)out, out_stride,
-                    (const bf16*)q, q_stride, window, bounded != 0);
+                    (const bf16*)q, q_stride, c->window, bounded != 0);
 }

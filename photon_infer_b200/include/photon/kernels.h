@@ -635,20 +635,20 @@ typedef struct {
 } photon_kv4_write_call;
 PHOTON_EXPORT int photon_kv4_write(const photon_kv4_write_call* call, cudaStream_t stream);
 /* Pages read back, k_out and v_out [S * per][n_kv][page_size][d], 16-byte aligned: page s * per + p is page table[s * stride + p]; one outside the pool is left out.  With cu_tokens
- * (else null): of request s only the pages below context_lens[s], and only where it has more than min_rows rows (tokens x group), with zeros behind the last key; new_table
+ * (else null): of request s only the pages below context_lens[s] and (window > 0) not wholly in front of its first token's window, and only where it has more than min_rows rows (tokens x group), with zeros behind the last key; new_table
  * [S * per] (may be null) gets each output page's own number, or -1, positions [T] (may be null) each token's place in its request;
  * with flags [S * per * ceil(n_kv * page_size / 32)] (may be null) values that are not finite are laid out as zero and marked there for photon_kv4_spoil. */
 typedef struct {
   const void* k_cache; const void* v_cache; const int* table; void* k_out; void* v_out; const int* cu_tokens; const int* context_lens; int* new_table; int* positions;
   int* flags; int* err;
   long stride;
-  int dtype, S, per, n_kv, d, page_size, num_pages, group, min_rows;
+  int dtype, S, per, n_kv, d, page_size, num_pages, group, min_rows, window;
 } photon_kv4_unpack_call;
 PHOTON_EXPORT int photon_kv4_unpack(const photon_kv4_unpack_call* call, cudaStream_t stream);
 /* Behind an attention over what that call laid out: rows of out (bfloat16 [T, n_kv * group * d], 16-byte aligned rows) that see a marked value become NaN in its group's numbers, and
  * rows whose query (q, as out) is not finite and that see a key in all (bounded: the scores were).  At most 128 query heads per key/value head; requests of at most max_tokens tokens in the step, or of more, which
  * take turns. */
-PHOTON_EXPORT int photon_kv4_spoil(const photon_kv4_unpack_call* call, void* out, long out_stride, const void* q, long q_stride, int max_tokens, int window, int bounded,
+PHOTON_EXPORT int photon_kv4_spoil(const photon_kv4_unpack_call* call, void* out, long out_stride, const void* q, long q_stride, int max_tokens, int bounded,
                                    cudaStream_t stream);
 
 /* ------------------------------------------------------------------ kv4_attention.cu */

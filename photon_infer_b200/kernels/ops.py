@@ -2853,7 +2853,7 @@ def _sms(index: int, device: torch.device) -> int:
 
 #: photon_kv4_write_call, photon_kv4_unpack_call, photon_kv4_attention_call, photon_key_weights_call, photon_evict_call
 _KV4_WRITE_CALL = struct.Struct("6q2q6i")
-_KV4_UNPACK_CALL = struct.Struct("11q1q9i4x")
+_KV4_UNPACK_CALL = struct.Struct("11q1q10i")
 _KV4_ATTENTION_CALL = struct.Struct("11q2q12i2f")
 _KEY_WEIGHTS_CALL = struct.Struct("11q2q14i2f")
 _EVICT_CALL = struct.Struct("7q13i4x")
@@ -2893,7 +2893,7 @@ def kv4_unpack(k_cache: torch.Tensor, v_cache: torch.Tensor, pages: torch.Tensor
     if size != page_size:
         raise PhotonError(ErrorCode.SHAPE_MISMATCH, "kv4_unpack: the outputs' pages must be those of the caches")
     call = _KV4_UNPACK_CALL.pack(k_cache.data_ptr(), v_cache.data_ptr(), pages.data_ptr(), k_out.data_ptr(), v_out.data_ptr(), 0, 0, 0, 0, 0,
-                                 0 if err is None else err.data_ptr(), N, _dtype_code(k_out), 1, N, n_kv, head_dim, page_size, pool, 1, 0)
+                                 0 if err is None else err.data_ptr(), N, _dtype_code(k_out), 1, N, n_kv, head_dim, page_size, pool, 1, 0, 0)
     _check(_plain_fn("kv4", "photon_kv4_unpack", _CALL_ARGS)(call, _stream()), "kv4_unpack")
 
 
@@ -2936,7 +2936,8 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
     of request ``s``'s ``context_lens[s]`` keys (at most ``max_keys``); the token at place ``p`` sees keys ``max(0, p - window + 1) .. p``: places in the cache, which are a
     token's position as long as none has left it.  A row that sees nothing is zero.  ``q`` and ``out [T, n_q * d]`` may be views with a row stride; ``sink``, ``softcap``: as in
     ``paged_attention``.  ``lse`` (float32 ``[T, n_q]``): gets the logarithm of the sum of each row's exponentials (the sink's among them; -inf where there is nothing), which
-    ``key_weights`` takes.  A query that is not finite makes its row NaN."""
+    ``key_weights`` takes.  A query that is not finite makes its row NaN.  Pages in front of every row's window may have been given back; one that is missing elsewhere is recorded in
+    ``err``, and its request's rows are not to be used."""
     index = _on_device("kv4_attention", q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, sink, lse, err)
     if sink is not None:
         _check_sink(sink, n_q)
@@ -3010,7 +3011,7 @@ def _kv4_route(dtype: torch.dtype, head_dim: int, page_size: int, page_heads: in
     return "kv4_attention_rows" if many else "kv4_attention", parts, all_rows * parts * (head_dim + 2) if parts > 1 else 0
 
 
-_KV4_SPOIL_ARGS = [c_char_p, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_int, c_void_p]
+_KV4_SPOIL_ARGS = [c_char_p, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c_void_p]
 
 
 def _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, num_seqs, max_tokens, max_keys, n_q, n_kv, head_dim, page_size, window, scale, err,
@@ -3033,10 +3034,10 @@ def _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, 
         n = min(some, num_seqs - s0)
         cu = cu_tokens[s0:s0 + n + 1] if s0 else cu_tokens
         call = _KV4_UNPACK_CALL.pack(k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr() + 4 * s0 * pages, k_at, v_at, cu.data_ptr(), context_lens.data_ptr() + 4 * s0,
-                                     table_at, positions_at, flags_at, _data(err), pages, _dtype_code(q), n, per, n_kv, head_dim, page_size, pool, group, KV4_FEW_ROWS)
+                                     table_at, positions_at, flags_at, _data(err), pages, _dtype_code(q), n, per, n_kv, head_dim, page_size, pool, group, KV4_FEW_ROWS, window)
         _check(unpack(call, _stream()), "kv4_attention")
         attention_tc(q, into, k_numbers, v_numbers, table, cu, positions, n, max_tokens, n_q, n_kv, head_dim, window, scale, err, sink=sink, softcap=softcap, keys=max_keys)
-        _check(spoil(call, into.data_ptr(), into.stride(0), q.data_ptr(), q.stride(0), max_tokens, window, int(bool(softcap)), _stream()), "kv4_attention")
+        _check(spoil(call, into.data_ptr(), into.stride(0), q.data_ptr(), q.stride(0), max_tokens, int(bool(softcap)), _stream()), "kv4_attention")
     if into is not out:
         out.copy_(into)
 
@@ -3050,7 +3051,7 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
     queries may be a step's, or the last ones of a prompt (``cu_tokens`` then counts those).  Keys from ``held[s]`` (int32) on have no sum yet and get this one; without
     ``held`` those are the given tokens' own keys.  ``k_cache``: a plain one of the type of ``q`` (``[pages, n_kv, page_size, d]``, ``d`` a multiple of 8 up to 256) or one in 4 bits.
     ``lse``: as ``kv4_attention`` leaves it for the same queries; without it the keys are read twice.  No page may be two requests' of a call, which would
-    add to one sum at once: requests that share a prefix are given one call after the other."""
+    add to one sum at once: requests that share a prefix are given one call after the other.  Pages of keys that have a sum and that no row's window reaches may have been given back."""
     index = _on_device("key_weights", q, weights, k_cache, block_table, cu_tokens, context_lens, held, sink, lse, err)
     if sink is not None:
         _check_sink(sink, n_q)
