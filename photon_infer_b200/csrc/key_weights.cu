@@ -36,7 +36,7 @@ key_weights_kernel(const KeyWeightsArgs a) {
   const int known = a.held != nullptr ? a.held[seq] : base, low = a.window > 0 ? min(base - a.window + 1, known) : 0;      // keys in front of it no row sees, and they have a sum
   for (int i = tid; i < KW_ROWS * d; i += KW_THREADS) {
     const int r = i / d, p = i - r * d, x = p / 8, t = PACKED ? x / groups : 0, at = PACKED ? 32 * (x - t * groups) + 8 * t + p % 8 : p;
-    qs[r * d + p] = r < rows ? to_f32(((const T*)a.q)[(first + r / G) * a.q_stride + (head * G + r % G) * d + at]) : 0.f;
+    qs[r * d + p] = r < rows ? kv4_query(((const T*)a.q)[(first + r / G) * a.q_stride + (head * G + r % G) * d + at]) : 0.f;
   }
   if (FINAL && tid < rows) {
     const int h = head * G + tid % G;

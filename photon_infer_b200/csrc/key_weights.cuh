@@ -33,6 +33,8 @@ __device__ __forceinline__ float key_score(float x, float scale, float softcap) 
   return softcap > 0.f ? softcap * tanhf(x * scale / softcap) * LOG2E : x * (scale * LOG2E);
 }
 
+__device__ __forceinline__ uint4 kx_queries(uint4 x) { return make_uint4(kv4_query2(x.x), kv4_query2(x.y), kv4_query2(x.z), kv4_query2(x.w)); }
+
 // Numbers 8 x .. 8 x + 7 of a key's row in its own order.
 template <typename C>
 __device__ __forceinline__ void key_numbers(const C* row, int x, float* c) {

@@ -121,7 +121,7 @@ key_weights_mma_kernel(const KeyWeightsMmaArgs a) {
   for (int x = tid; x < wr * 16 * (D / 8); x += KX_THREADS) {
     const int r = x / (D / 8), piece = x - r * (D / 8);
     uint4 v = make_uint4(0u, 0u, 0u, 0u);
-    if (r < rows) v = *(const uint4*)(a.q + (first + r / G) * a.q_stride + (long)(head * G + r % G) * D + 8 * piece);
+    if (r < rows) v = kx_queries(*(const uint4*)(a.q + (first + r / G) * a.q_stride + (long)(head * G + r % G) * D + 8 * piece));
     *(uint4*)(q_s + r * PITCH + 16 * piece) = v;
   }
   if (FINAL && tid < KX_ROWS) lse_s[tid] = tid < rows ? a.lse[(long)(first + tid / G) * a.n_q + head * G + tid % G] * 1.4426950408889634f : INFINITY;

@@ -87,7 +87,7 @@ key_weights_rows_kernel(const KeyWeightsArgs w) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int row = r0 + PER * warp + i, at = KW_PIECE * c + lane;
-        x[i] = row < rows && at < d ? to_f32(((const T*)w.q)[(first + row / G) * a.q_stride + (long)(head * G + row % G) * d + at]) : 0.f;
+        x[i] = row < rows && at < d ? kv4_query(((const T*)w.q)[(first + row / G) * a.q_stride + (long)(head * G + row % G) * d + at]) : 0.f;
       }
     };
 #pragma unroll

@@ -143,7 +143,7 @@ key_weights_tc_kernel(const KeyWeightsMmaArgs a) {
 #pragma unroll
       for (int i = 0; i < EACH; ++i) {
         const int x = i * KT_THREADS + tid, r = x / (D / 8), piece = x - r * (D / 8);
-        *(uint4*)piece_at(q_s, r, piece) = v[i];
+        *(uint4*)piece_at(q_s, r, piece) = kx_queries(v[i]);
       }
       if (half != 0) return;
       place_s[tid] = row < rows ? base + token : -1;

@@ -13,6 +13,7 @@
 #include "common.cuh"
 #include "limits.cuh"
 #include <cuda_fp16.h>
+#include <math.h>
 
 __host__ __device__ __forceinline__ long kv4_page_bytes(int page_size, int d) { return (long)page_size * (d / 32) * 17; }
 static inline bool kv4_sizes_ok(int page_size, int d) { return d > 0 && d % 32 == 0 && d <= 256 && page_size > 0 && (long)page_size * d % 512 == 0; }
@@ -20,3 +21,12 @@ static inline bool kv4_sizes_ok(int page_size, int d) { return d > 0 && d % 32 =
 __device__ __forceinline__ float kv4_scale(uint32_t byte) { return __half2float(__ushort_as_half((unsigned short)(byte << 7))); }
 // Nibble i of a word, less 8: 2^23 + code is exact, and so is what is left.
 __device__ __forceinline__ float kv4_code(uint32_t word, int i) { return __uint_as_float(((word >> (4 * i)) & 15u) | 0x4B000000u) - 8388616.f; }
+
+// A query's number.  One that is not finite makes every score of its row NaN: infinity and keys of one sign give scores of minus infinity, as if the row saw nothing.
+template <typename T>
+__device__ __forceinline__ float kv4_query(T x) {
+  const float y = to_f32(x);
+  return isfinite(y) ? y : NAN;
+}
+// Two bfloat16 numbers likewise: where all bits of the exponent are set, one more of them carries into the bit in front of them, which gives the NaN's.
+__device__ __forceinline__ uint32_t kv4_query2(uint32_t x) { return x | (((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 9; }

@@ -17,13 +17,6 @@ __device__ __forceinline__ float kv4_bounded(float x, float scale, float softcap
   return softcap > 0.f ? softcap * tanhf(x * scale / softcap) * LOG2E : x * (scale * LOG2E);
 }
 
-// A query's number.  One that is not finite makes every score of its row NaN: infinity and keys of one sign give scores of minus infinity, as if the row saw nothing.
-template <typename T>
-__device__ __forceinline__ float kv4_query(T x) {
-  const float y = to_f32(x);
-  return isfinite(y) ? y : NAN;
-}
-
 // One (token, head): the shares' results in ascending order.
 template <typename T>
 static __global__ void __launch_bounds__(256)

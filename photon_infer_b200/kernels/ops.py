@@ -3050,7 +3050,8 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
     gets, for its key/value head, the sum over the request's rows of ``exp(score - lse)``.  Tokens, keys, masks, ``sink`` and ``softcap`` as in ``kv4_attention``; the
     queries may be a step's, or the last ones of a prompt (``cu_tokens`` then counts those).  Keys from ``held[s]`` (int32) on have no sum yet and get this one; without
     ``held`` those are the given tokens' own keys.  ``k_cache``: a plain one of the type of ``q`` (``[pages, n_kv, page_size, d]``, ``d`` a multiple of 8 up to 256) or one in 4 bits.
-    ``lse``: as ``kv4_attention`` leaves it for the same queries; without it the keys are read twice.  No page may be two requests' of a call, which would
+    ``lse``: as ``kv4_attention`` leaves it for the same queries; without it the keys are read twice.  A
+    query that is not finite makes the weights of the keys that its row sees NaN.  No page may be two requests' of a call, which would
     add to one sum at once: requests that share a prefix are given one call after the other.  Pages of keys that have a sum and that no row's window reaches may have been given back."""
     index = _on_device("key_weights", q, weights, k_cache, block_table, cu_tokens, context_lens, held, sink, lse, err)
     if sink is not None:
