@@ -323,7 +323,8 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       const bool odd = top >= 0x7f800000u;
       const int e = top == 0 || odd ? 0 : max((int)(top >> 23), 1) - 127;
       const float up1 = km_power((14 - e) / 2), up2 = km_power(14 - e - (14 - e) / 2);      // the largest number to [2^14, 2^15)
-      const float f = fmaxf(km_scaled(a.scale * (CAP ? 1.f : 1.4426950408889634f), e - 14 + 24), 1e-37f);
+      // where no 32 bits hold it, the largest that they do: scores stay as far apart as a softmax can tell
+      const float f = fminf(fmaxf(km_scaled(a.scale * (CAP ? 1.f : 1.4426950408889634f), e - 14 + 24), 1e-37f), 3e38f);
 #pragma unroll
       for (int j = 0; j < GROUPS; ++j) {
         float sum = 0.f, y[8];
@@ -419,7 +420,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       }
       // ---- the softmax
       const bool masked = here != 15u || key0 < clear_from || key0 + 31 > clear_to;
-      if constexpr (CAP) {                              // tanh y = 1 - 2 / (1 + e^2y); the factor is in it then
+      if constexpr (CAP) {                              // tanh y = 1 - 2 / (1 + e^2y), off by some 2^-22 of the bound; the factor is in it then
 #pragma unroll
         for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -471,7 +472,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
             if (!(here >> o & 1u) || key > last_place || key < low) vs[u][b] = GROUPS == 4 ? 0x78787878u : 0x7878u;      // 1, whatever lies there: its weight is 0
           }
       }
-      float alpha[NT], ref[NT];
+      float alpha[NT], ref[NT], times[NT];
       bool grown = false;
 #pragma unroll
       for (int x = 0; x < NT; ++x) {
@@ -485,11 +486,15 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         grown |= top > m[x];
         m[x] = top;
         ref[x] = top == -INFINITY ? 0.f : top - 15.f;
+        times[x] = factor[x];
       }
       // scales that call for another power of two (a byte of 48 is 2^-9, one of 128 is 2), or no numbers
       constexpr uint32_t FIRST = GROUPS == 4 ? 0x80808080u : 0x8080u, UP = GROUPS == 4 ? 0x50505050u : 0x5050u;
       const uint32_t some = vs[0][0] | vs[0][1] | vs[1][0] | vs[1][1], all = (vs[0][0] + UP) & (vs[0][1] + UP) & (vs[1][0] + UP) & (vs[1][1] + UP);
-      const bool rare = __any_sync(0xffffffffu, ((some | ~all) & FIRST) != 0 || held != 0);
+      bool far = false;                                // a maximum beyond 2^20: the bits that rounding it takes are no small part of a weight's 15 powers of two
+#pragma unroll
+      for (int x = 0; x < NT; ++x) far |= (__float_as_uint(m[x]) & 0x7fffffffu) - 0x49800001u < 0x7f800000u - 0x49800001u;
+      const bool rare = __any_sync(0xffffffffu, ((some | ~all) & FIRST) != 0 || held != 0 || far);
       uint32_t bands = 2;
       bool odd_scales = false;
       if (rare) {
@@ -505,6 +510,16 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         odd_scales = bands & 16u;
         bands &= 15u;
         if (bands == 0) bands = 2;
+        if (__any_sync(0xffffffffu, far)) {            // scores as far below the maximum as they are, from products rounded as it was; then as if it were 0
+#pragma unroll
+          for (int x = 0; x < NT; ++x) {
+            const float back = m[x] == -INFINITY ? 0.f : m[x];
+#pragma unroll
+            for (int o = 0; o < 4; ++o) sc[x][o] = (CAP ? sc[x][o] : __fmul_rn(sc[x][o], factor[x])) - back;
+            ref[x] = -15.f;
+            times[x] = 1.f;
+          }
+        }
       }
       if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -523,7 +538,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
         float p[4];
 #pragma unroll
         for (int o = 0; o < 4; ++o) {
-          p[o] = km_exp2(CAP ? sc[x][o] - ref[x] : fmaf(sc[x][o], factor[x], -ref[x]));
+          p[o] = km_exp2(CAP ? sc[x][o] - ref[x] : fmaf(sc[x][o], times[x], -ref[x]));
           l[x] += p[o];
         }
         p2[x][0] = km_half2(p[0], p[1]);
