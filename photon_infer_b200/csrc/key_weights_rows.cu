@@ -60,7 +60,8 @@ key_weights_rows_kernel(const KeyWeightsArgs w) {
   float acc[R][8];                                    // of rows rt R .. and keys 4 kt .., 64 + 4 kt ..
   auto products = [&](int r0) {
     const int p = tid & 7, g = tid >> 3;              // numbers 4 p .. of keys 4 g ..; number `lane` of rows PER warp ..
-    float k[4][4], x[PER];
+    float k[4][4];
+    T x[PER];                                         // as they come: whoever looks at one waits for it
     auto load = [&](int c) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -87,7 +88,7 @@ key_weights_rows_kernel(const KeyWeightsArgs w) {
 #pragma unroll
       for (int i = 0; i < PER; ++i) {
         const int row = r0 + PER * warp + i, at = KW_PIECE * c + lane;
-        x[i] = row < rows && at < d ? kv4_query(((const T*)w.q)[(first + row / G) * a.q_stride + (long)(head * G + row % G) * d + at]) : 0.f;
+        x[i] = row < rows && at < d ? ((const T*)w.q)[(first + row / G) * a.q_stride + (long)(head * G + row % G) * d + at] : from_f32<T>(0.f);
       }
     };
 #pragma unroll
@@ -101,9 +102,9 @@ key_weights_rows_kernel(const KeyWeightsArgs w) {
       for (int j = 0; j < 4; ++j) *(float4*)&k_s[(4 * p + j) * KW_KEY_PITCH + 4 * g] = make_float4(k[0][j], k[1][j], k[2][j], k[3][j]);
       if constexpr (R == 4) {
 #pragma unroll
-        for (int i = 0; i < PER; i += 4) *(float4*)&q_s[lane * PITCH + PER * warp + i] = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        for (int i = 0; i < PER; i += 4) *(float4*)&q_s[lane * PITCH + PER * warp + i] = make_float4(kv4_query(x[i]), kv4_query(x[i + 1]), kv4_query(x[i + 2]), kv4_query(x[i + 3]));
       } else {
-        *(float2*)&q_s[lane * PITCH + PER * warp] = make_float2(x[0], x[1]);
+        *(float2*)&q_s[lane * PITCH + PER * warp] = make_float2(kv4_query(x[0]), kv4_query(x[1]));
       }
       __syncthreads();
       if ((c + 1) * KW_PIECE < d) load(c + 1);

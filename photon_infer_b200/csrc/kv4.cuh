@@ -23,10 +23,13 @@ __device__ __forceinline__ float kv4_scale(uint32_t byte) { return __half2float(
 __device__ __forceinline__ float kv4_code(uint32_t word, int i) { return __uint_as_float(((word >> (4 * i)) & 15u) | 0x4B000000u) - 8388616.f; }
 
 // A query's number.  One that is not finite makes every score of its row NaN: infinity and keys of one sign give scores of minus infinity, as if the row saw nothing.
+// x + 0 x is x or NaN.
 template <typename T>
 __device__ __forceinline__ float kv4_query(T x) {
   const float y = to_f32(x);
-  return isfinite(y) ? y : NAN;
+  return __fmaf_rn(y, 0.f, y);
 }
-// Two bfloat16 numbers likewise: where all bits of the exponent are set, one more of them carries into the bit in front of them, which gives the NaN's.
-__device__ __forceinline__ uint32_t kv4_query2(uint32_t x) { return x | (((x & 0x7f807f80u) + 0x00800080u) & 0x80008000u) >> 9; }
+__device__ __forceinline__ uint32_t kv4_query2(uint32_t x) {      // two bfloat16 numbers likewise
+  const __nv_bfloat162 v = *(const __nv_bfloat162*)&x, y = __hfma2(v, __float2bfloat162_rn(0.f), v);
+  return *(const uint32_t*)&y;
+}

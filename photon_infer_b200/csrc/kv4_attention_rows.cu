@@ -71,7 +71,8 @@ kv4_attention_rows_kernel(const Kv4Args a) {
     float acc[4][8];
     {
       const int p = tid & 7, g = tid >> 3;            // numbers 4 p .. of keys 4 g ..; number `lane` of rows 8 warp ..
-      float k[4][4], x[8];
+      float k[4][4];
+      T x[8];                                         // as they come: whoever looks at one waits for it
       auto load = [&](int c) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -89,7 +90,7 @@ kv4_attention_rows_kernel(const Kv4Args a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const int r = 8 * warp + i, row = row0 + min(r, rows - 1), token = row / G;
-          x[i] = r < rows ? kv4_query(((const T*)a.q)[(first + token) * a.q_stride + (long)(head * G + row - token * G) * d + KR_PIECE * c + lane]) : 0.f;
+          x[i] = r < rows ? ((const T*)a.q)[(first + token) * a.q_stride + (long)(head * G + row - token * G) * d + KR_PIECE * c + lane] : from_f32<T>(0.f);
         }
       };
 #pragma unroll
@@ -102,7 +103,7 @@ kv4_attention_rows_kernel(const Kv4Args a) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) *(float4*)&k_s[(4 * p + j) * KR_KEY_PITCH + 4 * g] = make_float4(k[0][j], k[1][j], k[2][j], k[3][j]);
 #pragma unroll
-        for (int i = 0; i < 8; i += 4) *(float4*)&q_s[lane * KR_PITCH + 8 * warp + i] = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+        for (int i = 0; i < 8; i += 4) *(float4*)&q_s[lane * KR_PITCH + 8 * warp + i] = make_float4(kv4_query(x[i]), kv4_query(x[i + 1]), kv4_query(x[i + 2]), kv4_query(x[i + 3]));
         __syncthreads();
         if (c + 1 < groups) load(c + 1);
 #pragma unroll 8
