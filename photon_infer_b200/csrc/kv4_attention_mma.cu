@@ -157,7 +157,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       uint32_t x = 0;
       if (s0 + lane < a.S) {
         const KmRequest r = km_request<RT, WEIGH>(a, s0 + lane);
-        x = (uint32_t)min((unsigned long long)r.steps * r.row_tiles * a.n_kv, (unsigned long long)KM_MOST);
+        x = (uint32_t)min((unsigned long long)r.steps * (uint32_t)(r.row_tiles * a.n_kv), (unsigned long long)KM_MOST);
       }
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
@@ -493,29 +493,34 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
       const uint32_t some = vs[0][0] | vs[0][1] | vs[1][0] | vs[1][1], all = (vs[0][0] + UP) & (vs[0][1] + UP) & (vs[1][0] + UP) & (vs[1][1] + UP);
       bool far = false;                                // a maximum beyond 2^20: the bits that rounding it takes are no small part of a weight's 15 powers of two
 #pragma unroll
-      for (int x = 0; x < NT; ++x) far |= (__float_as_uint(m[x]) & 0x7fffffffu) - 0x49800001u < 0x7f800000u - 0x49800001u;
+      for (int x = 0; x < NT; ++x) far |= fabsf(m[x]) > 1048576.f;
       const bool rare = __any_sync(0xffffffffu, ((some | ~all) & FIRST) != 0 || held != 0 || far);
       uint32_t bands = 2;
-      bool odd_scales = false;
+      bool odd_scales = false, several = false;        // no numbers; more than one band, or such
       if (rare) {
-        uint32_t mine = 0;
+        // four bytes at a time, what is found in a byte's first bit: which bands there are (0 is in none), and whether a byte is 248 or more
+        uint32_t in0 = 0, in1 = 0, in2 = 0, in3 = 0, none = 0;
 #pragma unroll
-        for (int j = 0; j < GROUPS; ++j)
-#pragma unroll
-          for (int w = 0; w < 4; ++w) {
-            const uint32_t byte = vs[w >> 1][w & 1] >> (8 * j) & 255u;
-            mine |= byte == 0 ? 0u : byte < 48 ? 1u : byte < 128 ? 2u : byte < 192 ? 4u : byte < 248 ? 8u : 16u;
-          }
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t v = vs[w >> 1][w & 1], low = v & 0x7f7f7f7fu, above = low + 0x50505050u, some = (low + 0x7f7f7f7fu) & ~v, no = v & ((v & 0x78787878u) + 0x08080808u);
+          in0 |= some & ~above;
+          in1 |= above & ~v;
+          in2 |= v & ~(v << 1);
+          in3 |= v & (v << 1) & ~no;
+          none |= no;
+        }
+        const uint32_t mine = (in0 & FIRST ? 1u : 0u) | (in1 & FIRST ? 2u : 0u) | (in2 & FIRST ? 4u : 0u) | (in3 & FIRST ? 8u : 0u) | (none & FIRST ? 16u : 0u);
         bands = __reduce_or_sync(0xffffffffu, mine);
         odd_scales = bands & 16u;
+        several = (bands & (bands - 1)) != 0;
         bands &= 15u;
         if (bands == 0) bands = 2;
         if (__any_sync(0xffffffffu, far)) {            // scores as far below the maximum as they are, from products rounded as it was; then as if it were 0
 #pragma unroll
           for (int x = 0; x < NT; ++x) {
-            const float back = m[x] == -INFINITY ? 0.f : m[x];
+            if (fabsf(m[x]) <= 1048576.f || m[x] == -INFINITY) continue;
 #pragma unroll
-            for (int o = 0; o < 4; ++o) sc[x][o] = (CAP ? sc[x][o] : __fmul_rn(sc[x][o], factor[x])) - back;
+            for (int o = 0; o < 4; ++o) sc[x][o] = (CAP ? sc[x][o] : __fmul_rn(sc[x][o], factor[x])) - m[x];
             ref[x] = -15.f;
             times[x] = 1.f;
           }
@@ -602,7 +607,7 @@ kv4_mma_kernel(const Kv4MmaArgs a) {
                     }
                   }
               }
-              s2[j] &= ((s2[j] & 0xffffu) - from < size ? 0x0000ffffu : 0u) | ((s2[j] >> 16) - from < size ? 0xffff0000u : 0u);
+              if (several) s2[j] &= ((s2[j] & 0xffffu) - from < size ? 0x0000ffffu : 0u) | ((s2[j] >> 16) - from < size ? 0xffff0000u : 0u);
               s2[j] = km_mul2(s2[j], lift2);
             }
           }
