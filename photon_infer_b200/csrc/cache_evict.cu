@@ -6,9 +6,9 @@
 // evict_move: a block moves a slice of the rows of one (entry, request, head, plane) as they are.  Row j comes from place kept[j] >= j, so a run of rows
 // is read as a whole before it is written, and what a later run reads lies behind all that an earlier one wrote.
 //
-// What bounds it: memory, where there is much to move: 8 requests of up to 6,001 keys that keep 2,048, 28 layers, 8 heads of 128 in 16 bits, 445 us, 0.97 of the copy rate by the
-// rows that may move.  With little to move two chains of latencies: one request, 1,152 to 1,024, 16 layers, 8 heads of 64 in 4 bits, 17.5 us.  Sums that stay in shared memory and places
-// found once for a batch of rows: 684 to 445 us.
+// What bounds it: memory, where there is much to move: 8 requests of up to 6,001 keys that keep 2,048, 28 layers, 8 heads of 128 in 16 bits, 520 us on caches that hold their keys as they came, 0.83 of
+// the copy rate by the rows that may move.  Rows that lie where they belong are not moved: calls in a row on the same caches take 370 to 440.  With little to move two chains of latencies: one
+// request, 1,152 to 1,024, 16 layers, 8 heads of 64 in 4 bits, 17.5 us.  Sums that stay in shared memory and places found once for a batch of rows: 684 to 445 us in a row.
 #include "common.cuh"
 #include "limits.cuh"
 

@@ -7,8 +7,8 @@
 // Without the rows' logarithms a first kernel leaves each run's maxima and sums and a second one joins them.  Up to 16 rows' scores are kept as well, 4 bytes for 2 d of a key's
 // row, and a third kernel turns them into weights; for more rows the keys are read again.
 //
-// What bounds it: a token of 32 requests beside 8,000 keys, 32 query heads on 8, heads of 128: 161 us, 524 MB of keys, 0.5 of the copy rate (runs end at different times, scores are written and
-// read once); of 8 beside 4,000: 30 us.  With the keys read twice and no scores kept the 32 requests took twice the bytes.  More than 32 rows are key_weights_tc.cu's, which is the faster.
+// What bounds it: a token of 32 requests beside 8,000 keys, 32 query heads on 8, heads of 128: 160 us, 524 MB of keys, 0.5 of the copy rate (runs end at different times, scores are written and
+// read once); of 8 beside 4,000: 29 us.  With the keys read twice and no scores kept the 32 requests took twice the bytes.  More than 32 rows are key_weights_tc.cu's, which is the faster.
 #include "key_weights.cuh"
 #include <type_traits>
 

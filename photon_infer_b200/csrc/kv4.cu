@@ -6,8 +6,9 @@
 // step, where 2^-6 is the least).  For 32 bits the multiple from that product is put right by what is left over, x - n scale, which is exact.
 // kv4_unpack: a thread reads a quarter of a row, 8 numbers of every group, and writes them where they belong.
 //
-// What bounds it: the instructions of the rounding.  8,191 rows of keys and values, 8 heads of 128, written, and their pages read back: 21 us, 85 MB, 0.6 of the copy rate; one row of 8 heads of 64 and
-// its page: 3.0 us, launches and rounds of latencies.  With one thread for a group and quotients by division it was 57 us.  Pages of 6,144 keys laid out for the tcgen05 kernel: 12 us of a portion's 185.
+// What bounds it: the instructions of the rounding.  8,191 rows of keys and values, 8 heads of 128, written, and their pages read back: 21 us, 85 MB, 0.6 of the copy rate (in 32 bits 42 us); one row of 8
+// heads of 64 and its page: 3.2 us, launches and rounds of latencies.  With one thread for a group and quotients by division it was 57 us.  Pages of 6,144 keys laid out for the tcgen05 kernel: 12 us
+// of a portion's 187.
 #include "kv4.cuh"
 
 #define KV4_THREADS 256

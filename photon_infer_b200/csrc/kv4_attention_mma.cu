@@ -1,8 +1,8 @@
 // Attention of decoded tokens over a paged cache in 4 bits (the format: kv4.cuh): bfloat16, heads of 64 or 128 numbers.
 //
 // The codes go to the tensor cores as they are: a byte under a mask, two codes c0 + 16 c1, is the 16-bit float (c0 + 16 c1) 2^-24, and its upper half under a mask is 16 c1
-// 2^-24, both below the normal numbers and exact.  Four instructions make eight numbers of an operand so (four ANDs and a shift, with every code by itself: five), and what
-// those cost bounds the kernel: they run at half the rate of others.  The pairs are taken apart where it costs nothing: a key's by the queries they meet,
+// 2^-24, both below the normal numbers and exact.  Four instructions make eight numbers of an operand so (four ANDs and a shift, with every code by itself: five), which
+// run at half the rate of others.  The pairs are taken apart where it costs nothing: a key's by the queries they meet,
 //   c0 q0 + c1 q1 = (c0 + 16 c1) q0 + 16 c1 (q1 / 16 - q0),
 // where the last factor has two parts, two 16-bit floats, in neighbouring columns of the second operand, so that four rows (tokens x query heads of a key/value head) fill its
 // eight columns; a value's behind the sum, since two rows of the result are the sums over c0 + 16 c1 and 16 c1.
@@ -10,16 +10,20 @@
 // the last sum known beforehand.  The weights, as 16-bit floats, are turned over in registers and multiplied by the values' scales,
 //   out[number][row] = sum over keys  (c - 8) (p scale)[key][group(number)][row],
 // where pairs of codes under the mask get the exponent of 1,024 with it and 1,024 and the eights are taken off by an addition, which is exact.  Weights are lifted by 2^15, and scales of 2
-// or more, or below 2^-9, meet them by themselves, lifted by a power of two.  All sums and the softmax are in 32 bits; the first number of a pair is the difference of two sums and so off
+// or more, or below 2^-9, meet them by themselves, lifted by a power of two.  All sums and the softmax are in 32 bits (an exponential is off by 2^-22).
+// A query has 22 bits, a weight and its product with a scale 11 each, since they meet the values as 16-bit floats: a row is off by 0.0017 of its size, which the result's own rounding to 8 bits
+// gives with weights in 32 bits, too.  The first number of a pair is the difference of two sums and so off
 // by some 2^-20 of the second one's, where its own rounding to 4 bits was off by half a scale.
 //
 // All warps have equal runs of the requests' tiles of 32 keys, wherever units (a request, a head, 4 or 8 rows) begin and end, and nothing to do with one another: a tile's
 // bytes come through three stages of the warp's own in shared memory, two of them on their way.  Results of a unit that lies in one warp are written, the others' parts are joined by a
 // second kernel, in the same order every time.
 //
-// What bounds it: instructions.  A warp's tile of 32 keys and values, heads of 128, has some 620, of which 290 run at half rate: 47 us of the 68 that 64 requests of up to 6,000 keys take (24
-// query heads on 8; 253 MB, 0.57 of the copy rate); 20 us are begin, end and join.  Two requests of 100,003 keys, 32 on 8: 63 us, 0.53.  One of 640, heads of 64: 7.5 us, a chain of
-// latencies.  Equal runs instead of a block for each share of a request: 94 to 79 us for the 64.  8-bit products were slower.
+// What bounds it: latency, with three warps a scheduler.  64 requests of up to 6,000 keys (24 query heads on 8 of 128; 253 MB) take 69 us, 0.56 of the copy rate: 68,000 instructions a scheduler are
+// 36 us of them if each cycle had one, and neither the issue slots (61 %) nor a pipe (54 % of the one that takes codes apart, 22 % of the tensor cores) is full; for each instruction issued a warp waits
+// one for the last one's result, 0.6 for that pipe and 0.7 for the others' turn.  A sum's registers (160 a thread) leave room for no fourth warp.  20 us of the 69 are begin, end and join.  Two requests of
+// 100,003 keys, 32 on 8: 63 us, 0.52.  One of 640, heads of 64: 7.7 us, a chain of latencies.  Equal runs instead of a block for each share of a request: 94 to 79 us for the 64.  8-bit
+// products were slower.  Values' scales all in another band take 86 us instead of the 69, one in 100 in another 119.
 #include "kv4.cuh"
 #include <math.h>
 

@@ -7,7 +7,7 @@
 // is looked through once more for the rows that do.
 //
 // What bounds it: the products, at 0.3 of the rate of 32-bit sums: three 16-byte reads of shared memory for 32 of them, barriers between pieces, and blocks of which some SMs have two and
-// some one.  32 query heads on 8, 32 bits: 200 tokens behind 4,000, heads of 128, 737 us (kv4_attention.cu 1,004; the framework's kernel for plain caches, with pages laid out, 1,094);
+// some one.  32 query heads on 8, 32 bits: 200 tokens behind 4,000, heads of 128, 733 us (kv4_attention.cu 1,004; the framework's kernel for plain caches, with pages laid out, 1,094);
 // 256 of 2 requests behind 8,192, heads of 64, 1,648 (2,890; 1,503).
 #include "kv4_attention.cuh"
 

@@ -2924,7 +2924,7 @@ def _rows_on_16_bytes(x: torch.Tensor) -> torch.Tensor:
 
 #: Rows (tokens x query heads per key/value head) up to which ``attention_tc`` leaves a request to other kernels.
 KV4_FEW_ROWS = 16
-#: Bytes of a prompt portion's keys and values in bfloat16 that are laid out at a time.
+#: Bytes of prompt portions' keys and values in bfloat16 that are laid out at a time: as many requests as fit, and one as a whole, however long it is.
 KV4_PROMPT_BYTES = 2 << 30
 
 
@@ -2981,14 +2981,14 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
 def _kv4_few(head_dim: int, page_size: int, num_seqs: int, n_kv: int, rows: int, keys: int) -> bool:
     """Whether requests of up to ``rows`` rows go to the kernel that reads the codes, eight rows at a time, rather than have their pages laid out for the tcgen05 kernel, whose blocks
     walk a request's keys one tile behind the other.  In us, the two sides of the comparison and 9 to 12 each.  Measured (pages laid out, codes), 32/8 heads of 128, 1 request of 8
-    tokens behind 1,500 39 and 23, behind 6,000 99 and 28; of 64 39 and 36, 109 and 81; of 128 40 and 51, 111 and 141; 4 of 16 44 and 36, 123 and 81; 4 of 33 45 and 53, 132 and 148; 16 of 8
-    75 and 51, 193 and 142; 16 of 16 75 and 85, 193 and 266; of 64, 1 of 33 30 and 21, 82 and 33; 4 of 64 33 and 54, 95 and 160; 16 of 8 44 and 33, 145 and 87."""
+    tokens behind 1,500 40 and 21, behind 6,000 100 and 25; of 64 41 and 32, 111 and 79; of 128 42 and 48, 112 and 141; 4 of 16 46 and 32, 124 and 80; 4 of 33 46 and 50, 133 and 149; 16 of 8
+    75 and 48, 195 and 142; 16 of 16 75 and 82, 195 and 269; of 64, 1 of 33 31 and 20, 83 and 33; 4 of 64 35 and 54, 97 and 166; 16 of 8 46 and 33, 146 and 89."""
     if head_dim not in (64, 128) or page_size % 8 or num_seqs > 1024:
         return False
     codes = num_seqs * n_kv * -(-rows // 8) * -(-keys // 32) * (1.33e-3 if head_dim == 128 else 0.78e-3) + 3
     laid_out = keys * (15.5e-3 if head_dim == 128 else 11.8e-3) + num_seqs * n_kv * keys * head_dim * 1.37e-6
-    # Short prompts are bound by the host, since the framework launches prompt portions from Python: the five launches with laid out pages take it 77 to 88 us, the two with the codes 18
-    # to 28.  128 tokens behind 500: 87 and 42 us a call (captured in a graph 21 and 40), heads of 64 80 and 23 (17 and 21); 64 behind 200: 89 and 28 (17 and 21).
+    # Short prompts are bound by the host, since the framework launches prompt portions from Python: the five launches with laid out pages take it 75 to 80 us, the two with the codes about
+    # 20.  128 tokens behind 500: 80 and 41 us a call (captured in a graph 22 and 37), heads of 64 78 and 24 (18 and 21); 64 behind 200: 78 and 21 (18 and 19).
     return codes <= max(laid_out, 15)
 
 
@@ -3017,7 +3017,8 @@ _KV4_SPOIL_ARGS = [c_char_p, c_void_p, c_long, c_void_p, c_long, c_int, c_int, c
 def _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, num_seqs, max_tokens, max_keys, n_q, n_kv, head_dim, page_size, window, scale, err,
                 sink, softcap) -> None:
     """The requests with more than ``KV4_FEW_ROWS`` rows: their pages are laid out in bfloat16, which holds them exactly, and the tcgen05 kernel attends to them.  Their
-    products are many times the bytes: 2,048 tokens of 32/8 heads of 128 behind 4,096 keys are 86 GFLOP and 25 MB laid out."""
+    products are many times the bytes: 2,048 tokens of 32/8 heads of 128 behind 4,096 keys are 172 GFLOP and 25 MB laid out.  The rows' weights are bfloat16 there, as everywhere in that kernel
+    (8 bits: with them a row is off by 0.0023 of its size, with weights in 32 bits by 0.0017, most of which is the result's own rounding)."""
     per = min(-(-max_keys // page_size), block_table.shape[1])
     device, (T, width) = q.device, q.shape
     q = _rows_on_16_bytes(q)
