@@ -2924,6 +2924,8 @@ def _rows_on_16_bytes(x: torch.Tensor) -> torch.Tensor:
 
 #: Rows (tokens x query heads per key/value head) up to which ``attention_tc`` leaves a request to other kernels.
 KV4_FEW_ROWS = 16
+#: Bounds of scores up to which the tensor-core kernels bound them, by an exponential and a quotient that leave a score off by 2^-22 of its bound; above it the general kernels call tanh.
+KV4_MOST_SOFTCAP = 256.0
 #: Bytes of prompt portions' keys and values in bfloat16 that are laid out at a time: as many requests as fit, and one as a whole, however long it is.
 KV4_PROMPT_BYTES = 2 << 30
 
@@ -2960,14 +2962,15 @@ def kv4_attention(q: torch.Tensor, out: torch.Tensor, k_cache: torch.Tensor, v_c
         return
     group, window = n_q // n_kv, min(window or 0, 0x7fffffff)
     most = max_tokens_per_seq * group                   # rows of a request
-    if most > KV4_FEW_ROWS and lse is None and attention_tc_supported(dtype, head_dim, group, page_size) \
+    general = softcap is not None and softcap > KV4_MOST_SOFTCAP
+    if most > KV4_FEW_ROWS and lse is None and not general and attention_tc_supported(dtype, head_dim, group, page_size) \
             and not _kv4_few(head_dim, page_size, num_seqs, n_kv, most, min(max_keys, window + max_tokens_per_seq) if window else max_keys):
         _kv4_prompt(q, out, k_cache, v_cache, block_table, cu_tokens, context_lens, num_seqs, max_tokens_per_seq, max_keys, n_q, n_kv, head_dim, page_size, window,
                     scale, err, sink, softcap)
         most = KV4_FEW_ROWS
     tokens = -(-most // group)
     keys = min(max_keys, window + tokens) if window else max_keys
-    name, parts, floats = _kv4_route(dtype, head_dim, page_size, pool * n_kv, num_seqs, n_kv, most, keys, T * n_q, _sms(index, q.device))
+    name, parts, floats = _kv4_route(torch.float32 if general else dtype, head_dim, page_size, pool * n_kv, num_seqs, n_kv, most, keys, T * n_q, _sms(index, q.device))
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if floats else None
     call = _KV4_ATTENTION_CALL.pack(q.data_ptr(), out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(),
                                     0 if sink is None else sink.data_ptr(), 0 if lse is None else lse.data_ptr(), 0 if scratch is None else scratch.data_ptr(),
@@ -3083,7 +3086,8 @@ def key_weights(q: torch.Tensor, weights: torch.Tensor, k_cache: torch.Tensor, b
         return
     if q.dtype == torch.bfloat16 and head_dim in (64, 128) and (q.stride(0) % 8 or q.data_ptr() % 16):
         q = _rows_on_16_bytes(q)                        # a copy of the queries is little beside the keys
-    name, parts, floats, keep = _key_weights_route(q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, packed, lse is not None, num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv),
+    general = softcap is not None and softcap > KV4_MOST_SOFTCAP
+    name, parts, floats, keep = _key_weights_route(torch.float32 if general else q.dtype, head_dim, page_size, k_cache.shape[0] * n_kv, packed, lse is not None, num_seqs, n_kv, max_tokens_per_seq * (n_q // n_kv),
                                                    max_keys, T * n_q, _sms(index, q.device))
     scratch = torch.empty(floats, dtype=torch.float32, device=q.device) if lse is None else None
     call = _KEY_WEIGHTS_CALL.pack(q.data_ptr(), weights.data_ptr(), k_cache.data_ptr(), block_table.data_ptr(), cu_tokens.data_ptr(), context_lens.data_ptr(), _data(held),
